@@ -1,0 +1,247 @@
+"""The attention side of a decoder layer (ctypes mirror of the gevva_attn_* entry points): norms around the attention block, per-head
+norms and rotation with the append to a paged cache, and causal attention over packed prompts or over the cache.  They stand where the
+reference's layer loop has them (src/cuda/runtime/prefill.cuh:924-1199, src/cuda/kernels/qkv_transform.cuh)."""
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from .runtime import GevvaMoeError, _address, _check, _enqueue, library
+
+HEAD_DIMS = (64, 128, 256, 512)
+
+
+class _Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = ([("keys", ctypes.c_void_p), ("values", ctypes.c_void_p)] +
+                [(n, ctypes.c_longlong) for n in ("key_page_stride", "key_slot_stride", "key_head_stride", "value_page_stride",
+                                                  "value_slot_stride", "value_head_stride")] +
+                [("pages", ctypes.c_int), ("page_size", ctypes.c_int)])
+
+
+class _Batch(ctypes.Structure):
+    _fields_ = [("token_offsets", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("sequences", ctypes.c_int), ("table_width", ctypes.c_int), ("table_stride", ctypes.c_int)]
+
+
+def _lib():
+    lib = library()
+    if getattr(lib, "_gv_attn_ready", False):
+        return lib
+    vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+    rows, cache, batch = ctypes.POINTER(_Rows), ctypes.POINTER(_Cache), ctypes.POINTER(_Batch)
+    lib.gevva_attn_norm.argtypes = [vp, vp, vp, i32, i32, f32, vp]
+    lib.gevva_attn_norm_add.argtypes = [vp] * 8 + [i32, i32, f32, vp]
+    lib.gevva_attn_append.argtypes = [rows, rows, rows, cache, batch, i32, i32, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, vp, vp, vp]
+    lib.gevva_attn_prompt.argtypes = [rows, rows, rows, vp, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp]
+    lib.gevva_attn_chunk_workspace_bytes.argtypes = [i32]
+    lib.gevva_attn_chunk_workspace_bytes.restype = ctypes.c_size_t
+    lib.gevva_attn_chunk.argtypes = [rows, cache, batch, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp]
+    lib._gv_attn_ready = True
+    return lib
+
+
+def _status(status, where):
+    if status != 0:
+        raise GevvaMoeError(status, where)
+
+
+def _device(tensor, device, name):
+    if tensor.device != device:
+        raise ValueError(f"{name}: expected on {device}, got {tensor.device}")
+
+
+def _heads(tensor, name, device=None, shape=None):
+    """bf16 [tokens, heads, dim] on the GPU, its last dimension contiguous."""
+    if (tensor.dtype is not torch.bfloat16 or tensor.dim() != 3 or not tensor.is_cuda or tensor.shape[2] not in HEAD_DIMS or
+            tensor.stride(2) != 1 or (shape is not None and tensor.shape != shape) or (device is not None and tensor.device != device)):
+        want = "(tokens, heads, 64|128|256|512)" if shape is None else tuple(shape)
+        raise ValueError(f"{name}: expected CUDA bfloat16 {want} with contiguous heads, got {tensor.dtype} {tuple(tensor.shape)} "
+                         f"strides {tensor.stride()} on {tensor.device}")
+    return _Rows(tensor.data_ptr(), tensor.stride(0), tensor.stride(1))
+
+
+def _out(out, like_shape, device, name="out"):
+    if out is None:
+        return torch.empty(like_shape, dtype=torch.bfloat16, device=device)
+    _check(out, torch.bfloat16, like_shape, name)
+    _device(out, device, name)
+    return out
+
+
+def _status_word(status, device):
+    if status is not None:
+        _check(status, torch.int32, (1,), "status")
+        _device(status, device, "status")
+    return _address(status)
+
+
+def block_norm(x, weight, eps=1e-6, out=None, stream=None):
+    """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768."""
+    rows, width = x.shape
+    _check(x, torch.bfloat16, (rows, width), "input")
+    _check(weight, torch.bfloat16, (width,), "weight")
+    _device(weight, x.device, "weight")
+    out = _out(out, x.shape, x.device)
+    _status(_enqueue(_lib().gevva_attn_norm, x.device, stream, x.data_ptr(), weight.data_ptr(), out.data_ptr(), rows, width, eps),
+            "block_norm")
+    return out
+
+
+def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None, eps=1e-6, out=None, stream=None):
+    """(residual + gate * norm(x) * weight) * scale, the norm behind a block; with `next_weight` also the next block's norm of
+    the result, returned as (out, next).  gate bf16 [width] and scale bf16 [1] are optional; out may be residual."""
+    rows, width = x.shape
+    _check(x, torch.bfloat16, (rows, width), "input")
+    _check(residual, torch.bfloat16, (rows, width), "residual")
+    _device(residual, x.device, "residual")
+    for tensor, size, name in ((weight, width, "weight"), (gate, width, "gate"), (scale, 1, "scale"), (next_weight, width, "next_weight")):
+        if tensor is not None:
+            _check(tensor, torch.bfloat16, (size,), name)
+            _device(tensor, x.device, name)
+    out = _out(out, x.shape, x.device)
+    following = torch.empty_like(x) if next_weight is not None else None
+    _status(_enqueue(_lib().gevva_attn_norm_add, x.device, stream, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), _address(gate),
+                     _address(scale), _address(next_weight), out.data_ptr(), _address(following), rows, width, eps), "block_norm_add")
+    return out if following is None else (out, following)
+
+
+class KvCache:
+    """Keys and values in pages: two bf16 tensors [pages, page_size, kv_heads, dim] (any strides, the last dimension contiguous).
+    page_size is a power of two, at least 16.  `status` is the int32 word that calls on this cache report into."""
+
+    def __init__(self, k, v):
+        if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.dim() != 4 or v.shape != k.shape or not k.is_cuda or
+                v.device != k.device or k.stride(3) != 1 or v.stride(3) != 1 or k.shape[3] not in HEAD_DIMS):
+            raise ValueError(f"cache: expected two CUDA bfloat16 tensors (pages, page_size, kv_heads, 64|128|256|512), got {k.dtype} "
+                             f"{tuple(k.shape)} and {v.dtype} {tuple(v.shape)} on {k.device} and {v.device}")
+        pages, page_size = k.shape[:2]
+        if pages < 1 or page_size < 16 or page_size & (page_size - 1):
+            raise ValueError(f"cache: page_size has to be a power of two, at least 16, and there has to be a page; got {tuple(k.shape)}")
+        self.k, self.v = k, v
+        self.page_size, self.kv_heads, self.head_dim = page_size, k.shape[2], k.shape[3]
+        self.device = k.device
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self._packed = _Cache(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
+                              pages, page_size)
+
+    @classmethod
+    def empty(cls, pages, page_size, kv_heads, head_dim, device="cuda:0"):
+        shape = (pages, page_size, kv_heads, head_dim)
+        return cls(*(torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(2)))
+
+    def last_status(self):
+        """Synchronises, then returns and clears the status of the calls on this cache (0 = ok)."""
+        status = -int(self.status.item())
+        if status:
+            self.status.zero_()
+        return status
+
+    def check(self):
+        _status(self.last_status(), "device status")
+
+
+class PagedBatch:
+    """The sequences of a call, int32 on the GPU: new tokens token_offsets[s] .. token_offsets[s + 1] - 1 (rows of the call's
+    tensors), lengths[s] keys with the new ones counted, and table [sequences, pages a sequence], whose entry x / page_size is the page of position x.
+    The tensors are read when the calls run, so a captured call can be replayed with other contents; rows outside the offsets are left as they were."""
+
+    def __init__(self, token_offsets, lengths, table):
+        sequences = lengths.shape[0] if lengths.dim() == 1 else -1
+        for tensor, shape, name in ((token_offsets, (sequences + 1,), "token_offsets"), (lengths, (sequences,), "lengths")):
+            _check(tensor, torch.int32, shape, name)
+            _device(tensor, table.device, name)
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != sequences or table.shape[1] < 1 or sequences < 1 or (
+                table.stride(1) != 1 and table.shape[1] > 1):
+            raise ValueError(f"table: expected int32 ({sequences}, pages a sequence), got {table.dtype} {tuple(table.shape)}")
+        self.token_offsets, self.lengths, self.table = token_offsets, lengths, table
+        self.device = table.device
+        stride = table.stride(0) if sequences > 1 else table.shape[1]
+        self._packed = _Batch(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
+
+
+@dataclass
+class Appended:
+    """What kv_append leaves beside the cache: rotated queries and, packed, rotated keys and values."""
+    q: torch.Tensor
+    k: torch.Tensor
+    v: torch.Tensor
+
+    def __iter__(self):
+        return iter((self.q, self.k, self.v))
+
+
+def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, normalize_v=False, eps=1e-6, packed=False, out=None,
+              stream=None):
+    """Norms q and k over their heads (weights bf16 [dim], None: no norm) and, with normalize_v, v without a weight; turns the pairs
+    (j, len(frequencies) + j) of q and k by position * frequencies[j] (float64 on the GPU, None: no rotation); stores k and v at their
+    positions in the cache.  q, k, v are [tokens, heads, dim], views of one projection's rows for instance.  Returns the queries, with
+    `packed` also keys and values as [tokens, kv_heads, dim] for prompt_attention.  `out` takes the queries.  A token
+    without a page is not stored; cache.check() reports it."""
+    q_rows = _heads(q, "q")
+    tokens, heads, dim = q.shape
+    kv_heads = cache.kv_heads
+    device = q.device
+    if cache.head_dim != dim or cache.device != device or batch.device != device:
+        raise ValueError(f"kv_append: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
+    k_rows, v_rows = _heads(k, "k", device, (tokens, kv_heads, dim)), _heads(v, "v", device, (tokens, kv_heads, dim))
+    for tensor, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if tensor is not None:
+            _check(tensor, torch.bfloat16, (dim,), name)
+            _device(tensor, device, name)
+    if frequencies is not None:
+        _check(frequencies, torch.float64, (frequencies.numel(),), "frequencies")
+        _device(frequencies, device, "frequencies")
+    rotated = 0 if frequencies is None else 2 * frequencies.numel()
+    out = _out(out, q.shape, device)
+    k_out, v_out = (torch.empty(k.shape, dtype=torch.bfloat16, device=device) for _ in range(2)) if packed else (None, None)
+    _status(_enqueue(_lib().gevva_attn_append, device, stream, q_rows, k_rows, v_rows, cache._packed, batch._packed, tokens, heads, kv_heads,
+                     dim, _address(frequencies), rotated, _address(q_weight), _address(k_weight), normalize_v, eps, out.data_ptr(),
+                     _address(k_out), _address(v_out), cache.status.data_ptr()), "kv_append")
+    return Appended(out, k_out, v_out) if packed else out
+
+
+def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=None, stream=None):
+    """Causal attention of packed prompts: rows token_offsets[s] .. token_offsets[s + 1] - 1 (int32 on the GPU) are sequence s, and
+    each sees its sequence's rows up to itself, the last `window` of them where that is not zero.  q [tokens, heads, dim], k and v
+    [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`.  `status` is an optional int32 [1] device word."""
+    q_rows = _heads(q, "q")
+    tokens, heads, dim = q.shape
+    device = q.device
+    if k.dim() != 3:
+        raise ValueError(f"k: expected (tokens, kv_heads, dim), got {tuple(k.shape)}")
+    shape = (tokens, k.shape[1], dim)
+    k_rows, v_rows = _heads(k, "k", device, shape), _heads(v, "v", device, shape)
+    _check(token_offsets, torch.int32, (token_offsets.numel(),), "token_offsets")
+    _device(token_offsets, device, "token_offsets")
+    out = _out(out, q.shape, device)
+    _status(_enqueue(_lib().gevva_attn_prompt, device, stream, q_rows, k_rows, v_rows, token_offsets.data_ptr(), token_offsets.numel() - 1,
+                     tokens, heads, shape[1], dim, scale, window, out.data_ptr(), _status_word(status, device)), "prompt_attention")
+    return out
+
+
+def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
+    """Causal attention of new tokens over the pages of their sequences, which hold their keys and values already (kv_append):
+    one token a sequence when decoding, several for verification and chunked prefill.  A row that sees no key is zero; rows outside the offsets
+    are left as they were in `out`."""
+    q_rows = _heads(q, "q")
+    tokens, heads, dim = q.shape
+    device = q.device
+    if cache.head_dim != dim or cache.device != device or batch.device != device:
+        raise ValueError(f"chunk_attention: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
+    lib = _lib()
+    out = _out(out, q.shape, device)
+
+    def launch(*args):
+        # (the workspace's size goes by the device, which is the current one in here)
+        workspace = torch.empty(lib.gevva_attn_chunk_workspace_bytes(dim), dtype=torch.uint8, device=device)
+        if stream is not None:  # not the stream that the workspace belongs to
+            workspace.record_stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
+        return lib.gevva_attn_chunk(q_rows, cache._packed, batch._packed, tokens, heads, cache.kv_heads, dim, scale, window, out.data_ptr(),
+                                    workspace.data_ptr(), cache.status.data_ptr(), *args)
+
+    _status(_enqueue(launch, device, stream), "chunk_attention")
+    return out

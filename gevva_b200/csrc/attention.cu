@@ -1,0 +1,1043 @@
+// Causal attention with grouped heads: whole prompts over packed keys, or new tokens over a paged cache (declared in
+// include/gevva_moe.h as gevva_attn_prompt and gevva_attn_chunk).
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale * q_i.k_j - m_i),   i - window < j <= i
+//
+// in one pass over the keys: a row keeps a reference m_i, the sum of its p and the sum of p * v.  The sums may be taken against any
+// reference, so m_i follows the row's maximum only when that has grown by more than 8 binary orders (p stays below 256); only then is what
+// has been summed scaled down.  p is rounded to bf16 for its product with v (2^-9 of each term, as v itself is); its sum is of the unrounded values.
+//
+// A query tile is 128 rows: floor(128 / group) tokens times the query heads of one key head, so that a key tile of 128 keys is read
+// once for all of them, with one token as with many.  Scores and outputs are products of the tensor pipe (tcgen05.mma, M = 128): S = Q K^T with both operands
+// in shared memory, O += P V with P in tensor memory, where the softmax threads leave it over the scores it came from.
+//   warp 0    fetches Q, K and V by TMA, a page's slots at a time where the keys are paged
+//   warp 1    issues the MMAs
+//   warp 2    works out the pieces of work, a step ahead of the others
+//   warps 4+  softmax and epilogue, a row per thread
+// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile, whose
+// scores for the next keys are computed while the softmax of these runs; a key tile takes the tensor pipe 2048 cycles and the exponentials 1024.
+// Heads of 64 and 128: two query tiles in turn, each with a softmax warpgroup of its own, since there both take as long.
+//
+// Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the items
+// longest first within a sequence, further ones by cancelling launches that have not started (clusterlaunchcontrol).  Chunks: a CTA takes an equal run of key tiles, whatever
+// the sequences' lengths, which only the device knows; an item that a run's end cuts leaves sums in the workspace, and
+// attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
+#include <cuda.h>
+#include <math_constants.h>
+
+#include "gv_attention.h"
+#include "gv_attention_plan.h"
+#include "gv_common.cuh"
+#include "gv_gemm_parts.cuh"
+#include "gv_launchers.h"
+
+namespace gv {
+namespace {
+
+constexpr int kRows = 128;         // rows of a query tile
+constexpr int kKeys = kAttnKeys;   // keys of a key tile
+constexpr int kPieceSlots = 2;     // pieces worked on: this one, and the next, whose first operands are fetched meanwhile
+constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
+constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
+constexpr int kLeastRun = 4;       // key tiles of the shortest run that a CTA is given
+
+// One run of key tiles of one item.
+struct Piece {
+  int tiles;       // 0: there are no more pieces
+  int first_tile;
+  int query0;      // row in q of the query tile's first token
+  int tokens;      // its tokens
+  int position0;   // of the first token
+  int key_origin;  // prompt: row in k of the sequence's first key
+  int sequence;
+  int kv_head, half;
+  int slot;        // where its sums go; -1: the whole item, which goes to the output
+};
+
+// Keys of a piece's j-th tile that some row of its item sees: [from, to) within the tile.  What stands elsewhere is other sequences' or
+// stale (behind the sequence's end, in front of the window), and zero times a value need not be zero: those rows of V are cleared.
+struct Seen {
+  int from, to;
+  __device__ bool all() const { return from <= 0 && to >= kKeys; }
+};
+__device__ __forceinline__ Seen seen_keys(const Piece& piece, int j, int window) {
+  const int key0 = (piece.first_tile + j) * kKeys;
+  return Seen{(window > 0 ? max(piece.position0 - window + 1, 0) : 0) - key0, max(piece.position0 + piece.tokens, 0) - key0};
+}
+
+template <int kDim, int kTiles>
+struct Shape {
+  static constexpr int kValueDim = kDim < 256 ? kDim : 256;
+  static constexpr int kHalves = kDim / kValueDim;
+  static constexpr int kStageDim = kDim < 128 ? kDim : 128;
+  static constexpr int kStageBytes = kKeys * kStageDim * 2;
+  static constexpr int kKeyStages = kDim / kStageDim;
+  static constexpr int kValueStages = kValueDim / kStageDim;
+  static constexpr int kQueryTileBytes = kRows * kDim * 2;
+  static constexpr int kControlBytes = 2048;
+  static constexpr int kRoom = (232448 - kControlBytes - kTiles * kQueryTileBytes) / kStageBytes;
+  static constexpr int kStages = kRoom < 8 ? kRoom : 8;
+  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kThreads = 128 + 32 * kSoftmaxWarps;
+  static_assert(kStages > kValueStages, "the values of a tile are in shared memory at the same time");
+  static_assert(kTiles == 1 || kDim <= 128, "two query tiles need 2 * (128 + dim) columns of tensor memory");
+};
+
+template <int kDim, int kTiles>
+struct AttnSmem {
+  using S = Shape<kDim, kTiles>;
+  uint8_t queries[kTiles][S::kQueryTileBytes];
+  uint8_t stage[S::kStages][S::kStageBytes];
+  uint64_t full[S::kStages], empty[S::kStages];
+  uint64_t q_full, q_empty;
+  uint64_t acc_full[2];       // scores: by key tile in turn (one query tile) or by query tile (two)
+  uint64_t p_ready[2];
+  uint64_t pv_done[kTiles];   // completes once a key tile
+  uint64_t o_free[kTiles];    // the outputs of the last piece have been read
+  uint64_t piece_full[kPieceSlots], piece_empty[kPieceSlots];
+  uint64_t v_landed;          // values of a tile that has rows to be cleared
+  uint64_t next_full;
+  alignas(16) uint4 next_item;  // answer to a request for another item
+  Piece pieces[kPieceSlots];
+  long long warp_work[S::kThreads / 32];
+  long long start_offset;
+  int start_sequence;
+  uint32_t tmem_base;
+  volatile int abort;
+};
+
+struct AttnParams {
+  const int* token_offsets;
+  const int* lengths;
+  const int* table;
+  int table_width, table_stride, page_shift;
+  int sequences, tokens;
+  int group, kv_heads;
+  int step;        // tokens of one 128-row tile: 128 / group
+  int window;
+  float scale_log2;
+  __nv_bfloat16* out;
+  long long out_token_stride, out_head_stride;
+  float* partial;  // [2 * CTAs][kTiles * 128][value columns]
+  float* partial_stats;  // [2 * CTAs][kTiles * 128][2]: reference (binary orders), sum
+  int* records;    // [CTAs][8]
+  int* status;
+};
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tensor_map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(tensor_map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_32x32(uint32_t tmem_address, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(tmem_address),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D (+)= A B^T, bf16 operands, fp32 sums, K = 16; A from shared memory or from tensor memory.
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+               "l"(a), "l"(b), "r"(descriptor), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t descriptor, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+               "r"(a), "l"(b), "r"(descriptor), "r"(accumulate)
+               : "memory");
+}
+
+// Instruction descriptors: fp32 sums (bit 4), bf16 operands (1 at [7,10) and [10,13)), B with its rows (keys) along K instead of N for the values
+// (bit 16), N at [17,23) in units of 8, M at [24,29) in units of 16.
+constexpr uint32_t kIdescScores = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+template <int kColumns>
+constexpr uint32_t kIdescValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((kColumns >> 3) << 17) | ((kRows >> 4) << 24);
+
+// With two query tiles a softmax thread holds more registers than the launch gives every thread: 168 a thread at launch, and
+// 128 x 88 + 256 x 208 = 384 x 168.  (At the top of each role: that is what the compiler goes by.)
+template <int kTiles>
+__device__ __forceinline__ void fewer_registers() {
+  if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+}
+template <int kTiles>
+__device__ __forceinline__ void more_registers() {
+  if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+}
+
+template <int kDim, int kTiles, bool kPaged>
+__global__ void __launch_bounds__(Shape<kDim, kTiles>::kThreads, 1)
+attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
+  using S = Shape<kDim, kTiles>;
+  using Smem = AttnSmem<kDim, kTiles>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem* smem = reinterpret_cast<Smem*>(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(&smem->full[s], 1);
+      mbar_init(&smem->empty[s], 1);
+    }
+    mbar_init(&smem->q_full, 1);
+    mbar_init(&smem->q_empty, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&smem->acc_full[s], 1);
+      mbar_init(&smem->p_ready[s], 4);
+    }
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(&smem->pv_done[t], 1);
+      mbar_init(&smem->o_free[t], 4);
+    }
+    for (int s = 0; s < kPieceSlots; ++s) {
+      mbar_init(&smem->piece_full[s], 1);
+      mbar_init(&smem->piece_empty[s], 2 + S::kSoftmaxWarps);  // fetching warp, MMA warp, softmax warps
+    }
+    mbar_init(&smem->v_landed, 1);
+    mbar_init(&smem->next_full, 1);
+    // shared memory that is not where the swizzle wants it: nothing is computed, and the status word says so
+    smem->abort = (smem_u32(smem_raw) & 1023u) != 0;
+    if (smem->abort && p.status) atomicExch(p.status, static_cast<int>(kCudaError));
+    fence_barrier_init();
+    prefetch_tensor_map(&map_q);
+    prefetch_tensor_map(&map_k);
+    prefetch_tensor_map(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(&smem->tmem_base, 512);
+    tmem_relinquish();
+  }
+  grid_launch_dependents();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = smem->tmem_base;
+  grid_dependency_wait();
+
+  const int step = p.step * kTiles;  // tokens of an item
+  long long run_begin = 0, run_end = 0;
+  long long work = 0;
+  int parts = 0;
+  if constexpr (kPaged) {
+    // Where this CTA's run begins: every CTA adds up all sequences' work, a few of them a thread.
+    const int heads = p.kv_heads * S::kHalves;
+    const int capacity = p.table_width << p.page_shift;
+    const int each = (p.sequences + S::kThreads - 1) / S::kThreads;
+    const int first = static_cast<int>(threadIdx.x) * each;
+    const auto work_of = [&](int s) -> long long {
+      const int from = max(p.token_offsets[s], 0), news = min(p.token_offsets[s + 1], p.tokens) - from;
+      if (news <= 0) return 0;
+      const AttnSequence q = attn_sequence(news, min(max(p.lengths[s], 0), capacity), step);
+      return heads * attn_tiles_before(q, q.query_tiles, step, p.window);
+    };
+    long long mine = 0;
+    for (int s = first; s < min(first + each, p.sequences); ++s) mine += work_of(s);
+    long long upto = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += other;
+    }
+    if (lane == 31) smem->warp_work[warp] = upto;
+    __syncthreads();
+    long long before = 0;
+    for (int w = 0; w < S::kThreads / 32; ++w) {
+      if (w < warp) before += smem->warp_work[w];
+      work += smem->warp_work[w];
+    }
+    upto += before;
+    parts = attn_parts(work, static_cast<int>(gridDim.x), kLeastRun);
+    if (static_cast<int>(blockIdx.x) < parts) {
+      run_begin = attn_part_begin(work, parts, blockIdx.x);
+      run_end = attn_part_begin(work, parts, blockIdx.x + 1);
+      if (upto - mine <= run_begin && run_begin < upto) {
+        long long at = upto - mine;
+        int s = first;
+        for (long long w = work_of(s); at + w <= run_begin; w = work_of(s)) {
+          at += w;
+          ++s;
+        }
+        smem->start_sequence = s;
+        smem->start_offset = run_begin - at;
+      }
+    }
+    __syncthreads();
+  }
+
+  if (warp < 4) {
+  fewer_registers<kTiles>();  // (a warpgroup's four warps at the same place)
+  if (warp == 2) {
+    // ---------------- what to do next ----------------
+    uint32_t count = 0;  // pieces handed out
+    bool ok = true;
+    const auto room = [&] {  // waits until the next piece's slot is free
+      return __all_sync(0xffffffffu, wait_or_abort(&smem->piece_empty[count % kPieceSlots], ((count / kPieceSlots) & 1u) ^ 1u, smem, p.status));
+    };
+    const auto hand_out = [&](const Piece& piece) {
+      if (lane == 0) {
+        smem->pieces[count % kPieceSlots] = piece;
+        mbar_arrive(&smem->piece_full[count % kPieceSlots]);
+      }
+      __syncwarp();
+      ++count;
+    };
+    if constexpr (kPaged) {
+      int record[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (run_end > run_begin) {
+        const int capacity = p.table_width << p.page_shift;
+        int s = smem->start_sequence;
+        long long offset = smem->start_offset, at = run_begin;
+        while (ok && at < run_end) {
+          const int from = max(p.token_offsets[s], 0), news = min(p.token_offsets[s + 1], p.tokens) - from;
+          if (news > 0) {
+            const AttnSequence q = attn_sequence(news, min(max(p.lengths[s], 0), capacity), step);
+            const long long of_head = attn_tiles_before(q, q.query_tiles, step, p.window);
+            int head = static_cast<int>(offset / of_head);
+            offset -= head * of_head;
+            int tile = attn_find_query_tile(q, offset, step, p.window);
+            offset -= attn_tiles_before(q, tile, step, p.window);
+            for (; ok && head < p.kv_heads * S::kHalves && at < run_end; ++head) {
+              for (; ok && tile < q.query_tiles && at < run_end; ++tile) {
+                const int tiles = attn_tiles(q, tile, step, p.window);
+                const int skip = static_cast<int>(offset);
+                const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), run_end - at));
+                Piece piece;
+                piece.tiles = take;
+                piece.first_tile = attn_first_tile(q, tile, step, p.window) + skip;
+                piece.query0 = from + tile * step;
+                piece.tokens = min(step, news - tile * step);
+                piece.position0 = q.past + tile * step;
+                piece.key_origin = 0;
+                piece.sequence = s;
+                piece.kv_head = head / S::kHalves;
+                piece.half = head % S::kHalves;
+                piece.slot = take == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (skip == 0 ? 1 : 0);
+                if (skip == 0 && take < tiles) {
+                  // the item goes on in the next CTAs' runs: what attention_join_kernel has to add up
+                  int last = blockIdx.x + 1;
+                  while (attn_part_begin(work, parts, last + 1) < at + tiles) ++last;
+                  record[0] = last - static_cast<int>(blockIdx.x);
+                  record[1] = piece.query0;
+                  record[2] = piece.tokens;
+                  record[3] = piece.kv_head;
+                  record[4] = piece.half;
+                }
+                at += take;
+                offset = 0;
+                ok = room();
+                if (ok) hand_out(piece);
+              }
+              tile = 0;
+            }
+          }
+          ++s;
+          offset = 0;
+        }
+      }
+      if (lane == 0) {
+        int4* slot = reinterpret_cast<int4*>(p.records + 8 * static_cast<size_t>(blockIdx.x));
+        slot[0] = make_int4(record[0], record[1], record[2], record[3]);
+        slot[1] = make_int4(record[4], 0, 0, 0);
+      }
+    } else {
+      const int heads = p.kv_heads * S::kHalves;
+      uint32_t asked = 0;
+      int item = blockIdx.x;
+      for (;;) {
+        // The item's sequence and query tile: rank in the list of all query tiles, each sequence's last one first.
+        int rank = item / heads;
+        Piece piece;
+        piece.tiles = 0;
+        for (int base = 0; base < p.sequences; base += 32) {
+          const int s = base + lane;
+          int from = 0, news = 0;
+          if (s < p.sequences) {
+            from = max(p.token_offsets[s], 0);
+            news = max(min(p.token_offsets[s + 1], p.tokens) - from, 0);
+          }
+          const int mine = (news + step - 1) / step;
+          int upto = mine;
+#pragma unroll
+          for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += other;
+          }
+          const uint32_t holds = __ballot_sync(0xffffffffu, upto > rank);
+          if (holds == 0) {
+            rank -= __shfl_sync(0xffffffffu, upto, 31);
+            continue;
+          }
+          const int owner = __ffs(holds) - 1;
+          rank -= __shfl_sync(0xffffffffu, upto - mine, owner);
+          from = __shfl_sync(0xffffffffu, from, owner);
+          news = __shfl_sync(0xffffffffu, news, owner);
+          const AttnSequence q = attn_sequence(news, news, step);
+          const int tile = q.query_tiles - 1 - rank;
+          const int head = item % heads;
+          piece.tiles = attn_tiles(q, tile, step, p.window);
+          piece.first_tile = attn_first_tile(q, tile, step, p.window);
+          piece.query0 = from + tile * step;
+          piece.tokens = min(step, news - tile * step);
+          piece.position0 = tile * step;
+          piece.key_origin = from;
+          piece.sequence = base + owner;
+          piece.kv_head = head / S::kHalves;
+          piece.half = head % S::kHalves;
+          piece.slot = -1;
+          break;
+        }
+        if (piece.tiles > 0) {
+          ok = room();
+          if (!ok) break;
+          hand_out(piece);
+        }
+        // Another item is asked for once its slot is free, so that no CTA holds more than one that it does not work on.
+        ok = room();
+        if (!ok) break;
+        if (lane == 0) {
+          fence_proxy_async_smem();  // (the last answer has been read)
+          mbar_arrive_expect_tx(&smem->next_full, 16);
+          asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                           smem_u32(&smem->next_item)),
+                       "r"(smem_u32(&smem->next_full))
+                       : "memory");
+        }
+        __syncwarp();
+        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->next_full, asked & 1u, smem, p.status));
+        if (!ok) {
+          if (lane == 0) mbar_wait_bounded(&smem->next_full, asked & 1u, 40000000ll);  // shared memory is given up only behind the answer
+          break;
+        }
+        ++asked;
+        uint32_t granted, next;
+        asm volatile(
+            "{\n\t.reg .b128 answer;\n\t.reg .pred p;\n\t.reg .b32 y, z, w;\n\t"
+            "ld.shared.b128 answer, [%2];\n\t"
+            "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, answer;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+            "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, answer;\n\t}"
+            : "=r"(granted), "=r"(next)
+            : "r"(smem_u32(&smem->next_item))
+            : "memory");
+        __syncwarp();
+        if (!granted) break;
+        item = static_cast<int>(next);
+      }
+    }
+    if (ok && room()) {
+      Piece none;
+      none.tiles = 0;
+      none.first_tile = none.query0 = none.tokens = none.position0 = none.key_origin = none.sequence = 0;
+      none.kv_head = none.half = 0;
+      none.slot = -1;
+      hand_out(none);
+    }
+  } else if (warp == 0) {
+    // ---------------- operands ----------------
+    uint32_t stage = 0, phase = 0, issued = 0;
+    bool ok = true;
+    const int page_boxes = kPaged && p.page_shift < 7 ? kKeys >> p.page_shift : 1;  // boxes of one tile's 64 columns
+    const int box_rows = kKeys / page_boxes;
+    const int box = lane & (page_boxes - 1), column = lane / page_boxes;
+    uint32_t q_issued = 0;
+    for (uint32_t count = 0;; ++count) {
+      const int slot = count % kPieceSlots;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      if (!ok) break;
+      const Piece piece = smem->pieces[slot];
+      if (piece.tiles == 0) break;
+      const int* table = kPaged ? p.table + static_cast<size_t>(piece.sequence) * p.table_stride : nullptr;
+      const auto page_of = [&](int tile) {  // of this lane's box
+        if constexpr (!kPaged) return 0;
+        const int index = (tile * kKeys + box * box_rows) >> p.page_shift;
+        return __ldg(table + min(index, p.table_width - 1));
+      };
+      const auto fetch = [&](const CUtensorMap* map, int x, int tile, int page) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->empty[stage], phase ^ 1u, smem, p.status));
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(&smem->full[stage], S::kStageBytes);
+        __syncwarp();
+        if (column < S::kStageDim / 64) {
+          uint8_t* to = smem->stage[stage] + column * kColumnBytes + box * box_rows * 128;
+          const int row = kPaged ? (tile * kKeys + box * box_rows) & ((1 << p.page_shift) - 1) : piece.key_origin + tile * kKeys;
+          tma_load_4d(to, map, &smem->full[stage], x + 64 * column, row, piece.kv_head, page);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      };
+      const auto fetch_keys = [&](int tile, int page) {
+#pragma unroll
+        for (int i = 0; i < S::kKeyStages; ++i)
+          if (ok) fetch(&map_k, i * S::kStageDim, tile, page);
+      };
+      const auto fetch_values = [&](int tile, int page) {
+#pragma unroll
+        for (int i = 0; i < S::kValueStages; ++i)
+          if (ok) fetch(&map_v, piece.half * S::kValueDim + i * S::kStageDim, tile, page);
+      };
+      int page = page_of(piece.first_tile), next_page = page_of(piece.first_tile + 1);
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->q_empty, (count & 1u) ^ 1u, smem, p.status));
+      if (!ok) break;
+      if (lane == 0) {
+        constexpr int kBoxes = kTiles * kDim / 64;
+        mbar_arrive_expect_tx(&smem->q_full, kBoxes * 128 * p.step * p.group);
+#pragma unroll
+        for (int i = 0; i < kBoxes; ++i) {
+          const int t = i / (kDim / 64), c = i % (kDim / 64);
+          tma_load_3d(smem->queries[t] + c * kColumnBytes, &map_q, &smem->q_full, 64 * c, piece.kv_head * p.group, piece.query0 + t * p.step);
+        }
+      }
+      __syncwarp();
+      ++q_issued;
+      if constexpr (kTiles == 1) fetch_keys(piece.first_tile, page);
+      for (int j = 0; ok && j < piece.tiles; ++j) {
+        const int tile = piece.first_tile + j;
+        const int page_after = page_of(tile + 2);
+        if constexpr (kTiles == 1) {
+          if (j + 1 < piece.tiles) fetch_keys(tile + 1, next_page);
+        } else {
+          fetch_keys(tile, page);
+        }
+        if (ok) fetch_values(tile, page);
+        page = next_page;
+        next_page = page_after;
+      }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&smem->piece_empty[slot]);
+      __syncwarp();
+    }
+    if (!ok && lane == 0) {
+      // let the copies already issued land before shared memory is given up
+      const uint32_t pending = issued < static_cast<uint32_t>(S::kStages) ? issued : S::kStages;
+      uint32_t s = stage, ph = phase;
+      for (uint32_t i = 0; i < pending; ++i) {
+        if (s == 0) {
+          s = S::kStages;
+          ph ^= 1u;
+        }
+        --s;
+        mbar_wait_bounded(&smem->full[s], ph, 40000000ll);
+      }
+      if (q_issued) mbar_wait_bounded(&smem->q_full, (q_issued - 1) & 1u, 40000000ll);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    uint32_t stage = 0, phase = 0;
+    const bool leader = elect_one();
+    const uint64_t q_desc = make_smem_desc(smem_u32(smem->queries[0]), 1024, 2);
+    const uint64_t k_desc = make_smem_desc(smem_u32(smem->stage[0]), 1024, 2);
+    // values: 64 columns a swizzle row, the next 64 a column block further (leading offset), keys eight rows a group (stride offset)
+    const uint64_t v_desc = k_desc | (static_cast<uint64_t>(kColumnBytes >> 4) << 16);
+    bool ok = true;
+    uint32_t done = 0;  // key tiles of the pieces before
+    const auto stage_ready = [&] { return wait_or_abort(&smem->full[stage], phase, smem, p.status); };
+    const auto next_stage = [&] {
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    };
+    // The products of one stage: 128 (64) of the columns that scores sum over, or of the outputs' columns.
+    const auto scores_of_stage = [&](uint32_t d, int tile, int part) {
+#pragma unroll
+      for (int i = 0; i < S::kStageDim / 16; ++i) {
+        const uint32_t at = (i / 4) * kColumnBytes + (i % 4) * 32;
+        mma_shared(d, q_desc + ((tile * S::kQueryTileBytes + part * 2 * kColumnBytes + at) >> 4),
+                   k_desc + ((stage * S::kStageBytes + at) >> 4), kIdescScores, part > 0 || i > 0);
+      }
+    };
+    const auto values_of_stage = [&](uint32_t d, uint32_t a, bool fresh) {
+#pragma unroll
+      for (int i = 0; i < kKeys / 16; ++i)
+        mma_tensor(d, a + 8 * i, v_desc + ((stage * S::kStageBytes + i * 2048) >> 4), kIdescValues<S::kStageDim>, !fresh || i > 0);
+    };
+    for (uint32_t count = 0; ok; ++count) {
+      const int slot = count % kPieceSlots;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      if (!ok) break;
+      const Piece piece = smem->pieces[slot];
+      const int tiles = piece.tiles;
+      if (tiles == 0) break;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->q_full, count & 1u, smem, p.status));
+      if (!ok) break;
+      if constexpr (kTiles == 1) {
+        const auto scores = [&](uint32_t n) {
+          for (int i = 0; ok && i < S::kKeyStages; ++i) {
+            ok = __all_sync(0xffffffffu, stage_ready());
+            if (ok && leader) {
+              scores_of_stage(tmem_base + (n & 1u) * kKeys, 0, i);
+              tc_commit(&smem->empty[stage]);
+            }
+            next_stage();
+          }
+          if (ok && leader) tc_commit(&smem->acc_full[n & 1u]);
+        };
+        scores(done);
+        for (int j = 0; ok && j < tiles; ++j) {
+          const uint32_t n = done + j;
+          if (j + 1 < tiles) scores(n + 1);
+          if (ok && j + 1 == tiles && leader) tc_commit(&smem->q_empty);
+          if (j == 0) ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->o_free[0], (count & 1u) ^ 1u, smem, p.status));
+          if (!seen_keys(piece, j, p.window).all()) {
+            // the softmax warps clear rows of these values before they say that P is there
+            const uint32_t first_stage = stage, first_phase = phase;
+            for (int i = 0; ok && i < S::kValueStages; ++i) {
+              ok = __all_sync(0xffffffffu, stage_ready());
+              next_stage();
+            }
+            stage = first_stage;
+            phase = first_phase;
+            if (ok && lane == 0) mbar_arrive(&smem->v_landed);
+          }
+          ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->p_ready[n & 1u], (n >> 1) & 1u, smem, p.status));
+          if (!ok) break;
+          tc_fence_after_sync();
+          for (int i = 0; ok && i < S::kValueStages; ++i) {
+            ok = __all_sync(0xffffffffu, stage_ready());
+            if (ok && leader) {
+              values_of_stage(tmem_base + 256 + i * S::kStageDim, tmem_base + (n & 1u) * kKeys, j == 0);
+              tc_commit(&smem->empty[stage]);
+            }
+            next_stage();
+          }
+          if (ok && leader) tc_commit(&smem->pv_done[0]);
+        }
+      } else {
+        // one stage holds a tile's keys, another its values
+        ok = __all_sync(0xffffffffu, stage_ready());
+        if (!ok) break;
+        if (leader) {
+          for (int t = 0; t < kTiles; ++t) {
+            scores_of_stage(tmem_base + t * kKeys, t, 0);
+            tc_commit(&smem->acc_full[t]);
+          }
+          tc_commit(&smem->empty[stage]);
+        }
+        next_stage();
+        for (int j = 0; ok && j < tiles; ++j) {
+          const uint32_t n = done + j;
+          const uint32_t value_stage = stage, value_phase = phase;
+          next_stage();
+          const uint32_t key_stage = stage, key_phase = phase;
+          const bool more = j + 1 < tiles;
+          for (int t = 0; ok && t < kTiles; ++t) {
+            if (j == 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->o_free[t], (count & 1u) ^ 1u, smem, p.status));
+            stage = value_stage;
+            phase = value_phase;
+            ok = ok && __all_sync(0xffffffffu, stage_ready());
+            if (ok && t == 0 && lane == 0 && !seen_keys(piece, j, p.window).all()) mbar_arrive(&smem->v_landed);
+            ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->p_ready[t], n & 1u, smem, p.status));
+            if (!ok) break;
+            tc_fence_after_sync();
+            if (leader) {
+              values_of_stage(tmem_base + 256 + t * kDim, tmem_base + t * kKeys, j == 0);
+              tc_commit(&smem->pv_done[t]);
+              if (t + 1 == kTiles) tc_commit(&smem->empty[value_stage]);
+            }
+            stage = key_stage;
+            phase = key_phase;
+            if (more) {
+              ok = __all_sync(0xffffffffu, stage_ready());
+              if (ok && leader) {
+                scores_of_stage(tmem_base + t * kKeys, t, 0);
+                tc_commit(&smem->acc_full[t]);
+                if (t + 1 == kTiles) tc_commit(&smem->empty[key_stage]);
+              }
+            }
+          }
+          if (more) next_stage();
+          else if (ok && leader) tc_commit(&smem->q_empty);
+        }
+      }
+      done += tiles;
+      if (ok && lane == 0) mbar_arrive(&smem->piece_empty[slot]);
+      __syncwarp();
+    }
+  }
+  } else {
+    // ---------------- softmax and epilogue ----------------
+    more_registers<kTiles>();
+    const int own = (warp - 4) / 4;            // query tile of this warpgroup
+    const int quarter = warp & 3;              // the tensor-memory lanes this warp may read
+    const int row = quarter * 32 + lane;
+    const int row_token = row / p.group, row_head = row - row_token * p.group;
+    const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+    const uint32_t outputs = lanes + 256 + own * kDim;
+    const float c = p.scale_log2;
+    uint32_t done = 0, ring = 0;  // key tiles and operand stages of the pieces before
+    uint32_t cleared = 0;         // tiles with cleared values
+    bool ok = true;
+    for (uint32_t count = 0; ok; ++count) {
+      const int slot = count % kPieceSlots;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      if (!ok) break;
+      const Piece piece = smem->pieces[slot];
+      if (piece.tiles == 0) break;
+      const int token = own * p.step + row_token;
+      const bool valid = row_token < p.step && token < piece.tokens;
+      // keys that the row sees: [row_begin, row_end)
+      const int position = piece.position0 + token;
+      const int row_end = valid && position >= 0 ? position + 1 : 0;
+      const int row_begin = p.window > 0 && position - p.window + 1 > 0 ? position - p.window + 1 : 0;
+      const bool active = __any_sync(0xffffffffu, valid);
+      const int least_end = __reduce_min_sync(0xffffffffu, valid ? row_end : 0x7fffffff);
+      const int most_begin = __reduce_max_sync(0xffffffffu, valid ? row_begin : 0);
+      float reference = -CUDART_INF_F, sum = 0.0f;
+#pragma unroll 1
+      for (int j = 0; j < piece.tiles; ++j) {
+        const uint32_t n = done + j;
+        const uint32_t scores_slot = kTiles == 2 ? own : n & 1u;
+        const uint32_t scores_parity = kTiles == 2 ? n & 1u : (n >> 1) & 1u;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->acc_full[scores_slot], scores_parity, smem, p.status));
+        if (!ok) break;
+        tc_fence_after_sync();
+        const uint32_t scores = lanes + scores_slot * kKeys;
+        const int key0 = (piece.first_tile + j) * kKeys;
+        if (active) {
+          uint32_t s0[32], s1[32], s2[32], s3[32];
+          tmem_load_32x32(scores, s0);
+          tmem_load_32x32(scores + 32, s1);
+          tmem_load_32x32(scores + 64, s2);
+          tmem_load_32x32(scores + 96, s3);
+          tmem_load_wait(s0, s1, s2, s3);
+          if (key0 + kKeys > least_end || key0 < most_begin) {
+            const int from = row_begin - key0, to = row_end - key0;
+            const auto hide = [&](uint32_t (&s)[32], int first) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (first + i < from || first + i >= to) s[i] = 0xff800000u;  // -inf
+            };
+            hide(s0, 0);
+            hide(s1, 32);
+            hide(s2, 64);
+            hide(s3, 96);
+          }
+          float top0 = -CUDART_INF_F, top1 = top0, top2 = top0, top3 = top0;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            top0 = fmaxf(top0, __uint_as_float(s0[i]));
+            top1 = fmaxf(top1, __uint_as_float(s1[i]));
+            top2 = fmaxf(top2, __uint_as_float(s2[i]));
+            top3 = fmaxf(top3, __uint_as_float(s3[i]));
+          }
+          const float top = fmaxf(fmaxf(top0, top1), fmaxf(top2, top3));
+          // (false where nothing has been seen yet: the difference of two infinities is no number)
+          const bool grow = (top - reference) * c > kGrowth;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float factor = grow ? exp2_approx((reference - top) * c) : 1.0f;
+            if (grow) reference = top;
+            sum *= factor;
+            if (j > 0) {
+              ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (n - 1) & 1u, smem, p.status));
+              if (!ok) break;
+              tc_fence_after_sync();
+#pragma unroll 1
+              for (int i = 0; i < S::kValueDim; i += 32) {
+                uint32_t o[32];
+                tmem_load_32x32(outputs + i, o);
+                tmem_load_wait(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                tmem_store_32x32(outputs + i, o);
+              }
+            }
+          }
+          const float shift = reference == -CUDART_INF_F ? 0.0f : -reference * c;
+          const unsigned long long c2 = two(c, c), shift2 = two(shift, shift);
+          unsigned long long total = two(0.0f, 0.0f);
+          uint32_t packed[32];
+          const auto exponentials = [&](const uint32_t (&s)[32], int first) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const unsigned long long v = fma2(two(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, shift2);
+              const float a = exp2_approx(low_of(v)), b = exp2_approx(high_of(v));
+              total = add2(total, two(a, b));
+              packed[first + i] = pack_bf16x2(a, b);
+            }
+          };
+          exponentials(s0, 0);
+          exponentials(s1, 16);
+          tmem_store_32x32(scores, packed);
+          exponentials(s2, 0);
+          exponentials(s3, 16);
+          tmem_store_32x32(scores + 32, packed);
+          sum += low_of(total) + high_of(total);
+          tmem_store_wait();
+        }
+        tc_fence_before_sync();
+        const Seen seen = seen_keys(piece, j, p.window);
+        if (own == 0 && !seen.all()) {
+          // (the MMA warp says when they have landed: these threads do not follow the stages' phases)
+          ok = __all_sync(0xffffffffu, wait_or_abort(&smem->v_landed, cleared & 1u, smem, p.status));
+          if (!ok) break;
+          ++cleared;
+          // K0 K1 V0 K2 V1 .. with one query tile, K0 V0 K1 V1 .. with two
+          const uint32_t at = ring + (kTiles == 2 ? j * (S::kKeyStages + S::kValueStages) + S::kKeyStages
+                                                  : min(j + 2, piece.tiles) * S::kKeyStages + j * S::kValueStages);
+          if (row < seen.from || row >= seen.to)
+            for (int i = 0; i < S::kValueStages; ++i)
+              for (int x = 0; x < S::kStageDim / 64; ++x)
+#pragma unroll
+                for (int y = 0; y < 8; ++y)  // (a row of the tile is 128 bytes in a row, whatever the swizzle does within them)
+                  *reinterpret_cast<uint4*>(smem->stage[(at + i) % S::kStages] + x * kColumnBytes + row * 128 + ((y ^ (row & 7)) << 4)) =
+                      make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&smem->p_ready[scores_slot]);
+      }
+      if (!ok) break;
+      done += piece.tiles;
+      ring += piece.tiles * (S::kKeyStages + S::kValueStages);
+      // (The last scores say that the outputs of the tile two before are there: a phase is waited for only when it is the next to complete.)
+      if (piece.tiles > 1) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (done - 2) & 1u, smem, p.status));
+      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (done - 1) & 1u, smem, p.status));
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (active) {
+        const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;  // a row that sees nothing: zeros
+        const int column0 = piece.half * S::kValueDim;
+        __nv_bfloat16* out = p.out + static_cast<long long>(piece.query0 + token) * p.out_token_stride +
+                             static_cast<long long>(piece.kv_head * p.group + row_head) * p.out_head_stride + column0;
+        const size_t partial_row = (static_cast<size_t>(piece.slot < 0 ? 0 : piece.slot) * kTiles + own) * kRows + row;
+#pragma unroll 1
+        for (int i = 0; i < S::kValueDim; i += 32) {
+          uint32_t o[32];
+          tmem_load_32x32(outputs + i, o);
+          tmem_load_wait(o);
+          if (valid && piece.slot < 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 v;
+              v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inverse, __uint_as_float(o[8 * k + 1]) * inverse);
+              v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inverse, __uint_as_float(o[8 * k + 3]) * inverse);
+              v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inverse, __uint_as_float(o[8 * k + 5]) * inverse);
+              v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inverse, __uint_as_float(o[8 * k + 7]) * inverse);
+              *reinterpret_cast<uint4*>(out + i + 8 * k) = v;
+            }
+          } else if (valid) {
+            uint4* to = reinterpret_cast<uint4*>(p.partial + partial_row * S::kValueDim + i);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+          __syncwarp();
+        }
+        if (valid && piece.slot >= 0) {
+          float2* stats = reinterpret_cast<float2*>(p.partial_stats) + partial_row;
+          *stats = make_float2(reference == -CUDART_INF_F ? -CUDART_INF_F : reference * c, sum);
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&smem->o_free[own]);
+        mbar_arrive(&smem->piece_empty[slot]);
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    __syncwarp();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Adds up the sums of the items that the ends of runs have cut: CTA x takes the item that begins in run x and does not end there, its
+// rows dealt out over the warps of gridDim.y CTAs.
+template <int kValueDim>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p, int tiles) {
+  grid_dependency_wait();
+  const int4 first = *reinterpret_cast<const int4*>(p.records + 8 * static_cast<size_t>(blockIdx.x));
+  const int more = first.x;
+  if (more == 0) return;
+  const int half = p.records[8 * static_cast<size_t>(blockIdx.x) + 4];
+  const int lane = threadIdx.x & 31;
+  const int query0 = first.y, tokens = first.z, kv_head = first.w;
+  const size_t slot_rows = static_cast<size_t>(tiles) * kRows;
+  const auto row_of = [&](int part) {  // first row of the item's part
+    return static_cast<size_t>(2 * (static_cast<int>(blockIdx.x) + part) + (part == 0 ? 1 : 0)) * slot_rows;
+  };
+  const int rows = tokens * p.group;
+  for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
+    const int token = r / p.group, head = r - token * p.group;
+    const int row = (token / p.step) * kRows + (token % p.step) * p.group + head;
+    float top = -CUDART_INF_F;
+    for (int i = lane; i <= more; i += 32) top = fmaxf(top, p.partial_stats[2 * (row_of(i) + row)]);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (top == -CUDART_INF_F) top = 0.0f;  // every weight is zero then
+    constexpr int kEach = kValueDim / 32;
+    float acc[kEach] = {};
+    float sum = 0.0f;
+    for (int i = 0; i <= more; ++i) {
+      const float2 stats = reinterpret_cast<const float2*>(p.partial_stats)[row_of(i) + row];
+      const float weight = exp2_approx(stats.x - top);
+      sum = fmaf(stats.y, weight, sum);
+      const float* from = p.partial + (row_of(i) + row) * kValueDim + lane * kEach;
+      if constexpr (kEach == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(from);
+        acc[0] = fmaf(v.x, weight, acc[0]);
+        acc[1] = fmaf(v.y, weight, acc[1]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kEach; k += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(from + k);
+          acc[k] = fmaf(v.x, weight, acc[k]);
+          acc[k + 1] = fmaf(v.y, weight, acc[k + 1]);
+          acc[k + 2] = fmaf(v.z, weight, acc[k + 2]);
+          acc[k + 3] = fmaf(v.w, weight, acc[k + 3]);
+        }
+      }
+    }
+    const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
+    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + static_cast<long long>(query0 + token) * p.out_token_stride +
+                                                static_cast<long long>(kv_head * p.group + head) * p.out_head_stride +
+                                                half * kValueDim + lane * kEach);
+    if constexpr (kEach == 2) {
+      out[0] = pack_bf16x2(acc[0] * inverse, acc[1] * inverse);
+    } else if constexpr (kEach == 4) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(acc[0] * inverse, acc[1] * inverse), pack_bf16x2(acc[2] * inverse, acc[3] * inverse));
+    } else {
+      *reinterpret_cast<uint4*>(out) =
+          make_uint4(pack_bf16x2(acc[0] * inverse, acc[1] * inverse), pack_bf16x2(acc[2] * inverse, acc[3] * inverse),
+                     pack_bf16x2(acc[4] * inverse, acc[5] * inverse), pack_bf16x2(acc[6] * inverse, acc[7] * inverse));
+    }
+  }
+}
+
+constexpr int kJoinColumns = 8;  // CTAs that share an item's rows
+
+bool make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const long long* strides, const uint32_t* box) {
+  uint64_t bytes[3];
+  for (int i = 0; i + 1 < rank; ++i) bytes[i] = static_cast<uint64_t>(strides[i]) * 2;
+  return make_bf16_tensor_map(map, base, rank, dims, bytes, box);
+}
+
+template <int kDim, int kTiles, bool kPaged>
+cudaError_t launch_shape(const AttnCall& call, cudaStream_t stream) {
+  using S = Shape<kDim, kTiles>;
+  const auto kernel = attention_kernel<kDim, kTiles, kPaged>;
+  constexpr int kSmemBytes = static_cast<int>(sizeof(AttnSmem<kDim, kTiles>));
+  static_assert(kSmemBytes <= 232448, "shared memory of an SM");
+  static bool prepared[64] = {};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 0 || device >= 64 || !prepared[device]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    if (device >= 0 && device < 64) prepared[device] = true;
+  }
+  const int group = call.heads / call.kv_heads;
+  AttnParams p{};
+  p.token_offsets = call.token_offsets;
+  p.sequences = call.sequences;
+  p.tokens = call.tokens;
+  p.group = group;
+  p.kv_heads = call.kv_heads;
+  p.step = kRows / group;
+  p.window = call.window;
+  p.scale_log2 = call.scale * 1.4426950408889634f;
+  p.out = static_cast<__nv_bfloat16*>(call.out);
+  p.out_token_stride = call.out_token_stride;
+  p.out_head_stride = call.out_head_stride;
+  p.status = call.status;
+  CUtensorMap map_q, map_k, map_v;
+  {
+    const uint64_t dims[3] = {kDim, static_cast<uint64_t>(call.heads), static_cast<uint64_t>(call.tokens)};
+    const long long strides[2] = {call.q.head_stride, call.q.token_stride};
+    const uint32_t box[3] = {64, static_cast<uint32_t>(group), static_cast<uint32_t>(p.step)};
+    if (!make_map(&map_q, call.q.data, 3, dims, strides, box)) return cudaErrorInvalidValue;
+  }
+  long long items;
+  if constexpr (kPaged) {
+    const AttnPages& c = call.pages;
+    p.lengths = c.lengths;
+    p.table = c.table;
+    p.table_width = c.table_width;
+    p.table_stride = c.table_stride;
+    while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
+    const uint64_t dims[4] = {kDim, static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(call.kv_heads), static_cast<uint64_t>(c.page_count)};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(c.page_size < kKeys ? c.page_size : kKeys), 1, 1};
+    const long long key_strides[3] = {c.key_slot_stride, c.key_head_stride, c.key_page_stride};
+    const long long value_strides[3] = {c.value_slot_stride, c.value_head_stride, c.value_page_stride};
+    if (!make_map(&map_k, c.keys, 4, dims, key_strides, box) || !make_map(&map_v, c.values, 4, dims, value_strides, box))
+      return cudaErrorInvalidValue;
+    items = call.sm_count;
+    const size_t rows = 2 * static_cast<size_t>(call.sm_count) * kTiles * kRows;
+    p.partial = static_cast<float*>(call.workspace);
+    p.partial_stats = p.partial + rows * S::kValueDim;
+    p.records = reinterpret_cast<int*>(p.partial_stats + 2 * rows);
+  } else {
+    const uint64_t dims[4] = {kDim, static_cast<uint64_t>(call.tokens), static_cast<uint64_t>(call.kv_heads), 1};
+    const uint32_t box[4] = {64, kKeys, 1, 1};
+    const long long whole = call.k.token_stride * call.tokens, whole_v = call.v.token_stride * call.tokens;
+    const long long key_strides[3] = {call.k.token_stride, call.k.head_stride, whole};
+    const long long value_strides[3] = {call.v.token_stride, call.v.head_stride, whole_v};
+    if (!make_map(&map_k, call.k.data, 4, dims, key_strides, box) || !make_map(&map_v, call.v.data, 4, dims, value_strides, box))
+      return cudaErrorInvalidValue;
+    // as many query tiles as sequences of any lengths can have
+    const long long step = static_cast<long long>(p.step) * kTiles;
+    items = (call.tokens + call.sequences * (step - 1)) / step * call.kv_heads * S::kHalves;
+    if (items > 0x7fffffff) return cudaErrorInvalidConfiguration;
+  }
+  e = launch_chained(kernel, dim3(static_cast<unsigned>(items)), dim3(S::kThreads), kSmemBytes, stream, map_q, map_k, map_v, p);
+  if (e != cudaSuccess) return e;
+  if constexpr (kPaged)
+    e = launch_chained(attention_join_kernel<S::kValueDim>, dim3(static_cast<unsigned>(items), kJoinColumns), dim3(256), 0, stream, p, kTiles);
+  return e;
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(int dim, int sm_count) {
+  const size_t tiles = dim <= 128 ? 2 : 1;
+  const size_t rows = 2 * static_cast<size_t>(sm_count) * tiles * kRows;
+  return rows * ((dim < 256 ? dim : 256) + 2) * sizeof(float) + static_cast<size_t>(sm_count) * 8 * sizeof(int);
+}
+
+cudaError_t launch_attention(const AttnCall& call, cudaStream_t stream) {
+  // Two query tiles where there are rows for them: below, half of the products and exponentials would be of rows that do not exist.
+  const long long rows = static_cast<long long>(call.tokens) * (call.heads / call.kv_heads);
+  const bool two_tiles = rows > static_cast<long long>(call.sequences) * kRows;
+  if (call.paged) {
+    switch (call.dim) {
+      case 64: return two_tiles ? launch_shape<64, 2, true>(call, stream) : launch_shape<64, 1, true>(call, stream);
+      case 128: return two_tiles ? launch_shape<128, 2, true>(call, stream) : launch_shape<128, 1, true>(call, stream);
+      case 256: return launch_shape<256, 1, true>(call, stream);
+      default: return launch_shape<512, 1, true>(call, stream);
+    }
+  }
+  switch (call.dim) {
+    case 64: return two_tiles ? launch_shape<64, 2, false>(call, stream) : launch_shape<64, 1, false>(call, stream);
+    case 128: return two_tiles ? launch_shape<128, 2, false>(call, stream) : launch_shape<128, 1, false>(call, stream);
+    case 256: return launch_shape<256, 1, false>(call, stream);
+    default: return launch_shape<512, 1, false>(call, stream);
+  }
+}
+
+}  // namespace gv

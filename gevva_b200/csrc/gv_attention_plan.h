@@ -1,0 +1,116 @@
+// How attention work is counted and cut into pieces.  Plain integer arithmetic for host and device: the kernel walks it, and a
+// host program plays it through (tests/attention_plan_probe.cpp).
+//
+// A sequence of `news` new tokens over `length` keys (the new ones included) has its token i at position length - news + i, which sees
+// the keys up to that position, the last `window` of them only where a window is set.  Tokens are taken `step` at a time (a query
+// tile) and keys 128 at a time (a key tile, counted from the sequence's first key).  An item is one query tile of one key head (and of one half
+// of the value columns, for heads of 512); its work is its number of key tiles, at least one, so that rows that see nothing are written too.
+#pragma once
+
+#ifdef __CUDACC__
+#define GV_HD __host__ __device__ __forceinline__
+#else
+#define GV_HD inline
+#endif
+
+namespace gv {
+
+constexpr int kAttnKeys = 128;  // keys of a tile
+
+struct AttnSequence {
+  int news, past;    // past = length - news; below zero where there are fewer keys than new tokens
+  int query_tiles;   // ceil(news / step)
+};
+
+GV_HD AttnSequence attn_sequence(int news, int length, int step) {
+  AttnSequence s;
+  s.news = news;
+  s.past = length - news;
+  s.query_tiles = (news + step - 1) / step;
+  return s;
+}
+
+// One past the last key that any token of query tile q sees, and the first key that any of them does.
+GV_HD int attn_key_end(const AttnSequence& s, int q, int step) {
+  const int tokens = (q + 1) * step < s.news ? (q + 1) * step : s.news;
+  return s.past + tokens > 0 ? s.past + tokens : 0;
+}
+GV_HD int attn_key_begin(const AttnSequence& s, int q, int step, int window) {
+  const int first = s.past + q * step - window + 1;
+  return window > 0 && first > 0 ? first : 0;
+}
+GV_HD int attn_first_tile(const AttnSequence& s, int q, int step, int window) { return attn_key_begin(s, q, step, window) / kAttnKeys; }
+GV_HD int attn_tiles(const AttnSequence& s, int q, int step, int window) {
+  const int tiles = (attn_key_end(s, q, step) + kAttnKeys - 1) / kAttnKeys - attn_first_tile(s, q, step, window);
+  return tiles > 0 ? tiles : 1;
+}
+
+// Sum over i < n of floor((a * i + b) / m) for a, b >= 0 and m > 0, in as many rounds as Euclid's algorithm takes for (a, m).
+GV_HD long long attn_floor_sum(long long n, long long m, long long a, long long b) {
+  long long sum = 0;
+  while (n > 0) {
+    if (a >= m) {
+      sum += n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      sum += n * (b / m);
+      b %= m;
+    }
+    const long long top = a * n + b;
+    if (top < m) break;
+    n = top / m;
+    b = top % m;
+    const long long t = m;
+    m = a;
+    a = t;
+  }
+  return sum;
+}
+
+// Key tiles of the first `count` query tiles of a sequence (for one head).
+GV_HD long long attn_tiles_before(const AttnSequence& s, int count, int step, int window) {
+  if (count <= 4) {
+    long long sum = 0;
+    for (int q = 0; q < count; ++q) sum += attn_tiles(s, q, step, window);
+    return sum;
+  }
+  // query tiles in front of the first key see nothing and count one each
+  int blind = s.past < 0 ? -s.past / step : 0;
+  if (blind > s.query_tiles - 1) blind = s.query_tiles - 1;
+  if (s.past + s.news <= 0) blind = s.query_tiles;
+  if (count <= blind) return count;
+  long long sum = blind;
+  const int full = count < s.query_tiles - 1 ? count : s.query_tiles - 1;  // tiles of whole `step` tokens
+  if (full > blind)
+    sum += attn_floor_sum(full - blind, kAttnKeys, step, static_cast<long long>(s.past) + static_cast<long long>(blind + 1) * step + kAttnKeys - 1);
+  if (count == s.query_tiles) sum += (s.past + s.news + kAttnKeys - 1) / kAttnKeys;
+  if (window > 0) {
+    const int lead = window - 1 - s.past;
+    int from = lead > 0 ? (lead + step - 1) / step : 0;
+    if (from < blind) from = blind;
+    if (count > from)
+      sum -= attn_floor_sum(count - from, kAttnKeys, step, static_cast<long long>(s.past) + static_cast<long long>(from) * step - window + 1);
+  }
+  return sum;
+}
+
+// The query tile that holds key tile `at` (0 <= at < attn_tiles_before(all)) of a head's work, counted from its first.
+GV_HD int attn_find_query_tile(const AttnSequence& s, long long at, int step, int window) {
+  int low = 0, high = s.query_tiles - 1;
+  while (low < high) {
+    const int mid = (low + high) / 2;
+    if (attn_tiles_before(s, mid + 1, step, window) > at) high = mid;
+    else low = mid + 1;
+  }
+  return low;
+}
+
+// Work is dealt out to `parts` CTAs in runs of equal length; fewer CTAs where a run would be shorter than `least` key tiles.
+GV_HD int attn_parts(long long work, int parts, int least) {
+  const long long useful = (work + least - 1) / least;
+  return useful < parts ? static_cast<int>(useful) : parts;
+}
+GV_HD long long attn_part_begin(long long work, int parts, int part) { return work * part / parts; }
+
+}  // namespace gv

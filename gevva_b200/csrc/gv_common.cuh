@@ -27,6 +27,7 @@ enum Status : int {
   kCudaError = 4,
   kNoDevice = 5,
   kTooLarge = 6,
+  kBadPage = 7,         // a new token's position has no page of the cache
 };
 
 // Tile geometry of the grouped GEMM (tokens on MMA-M, weight rows on MMA-N).
@@ -498,6 +499,9 @@ __device__ __forceinline__ void tmem_load_wait(uint32_t (&a)[16], uint32_t (&b)[
 }
 __device__ __forceinline__ void tmem_load_wait(uint32_t (&a)[32]) { GV_LOAD_WAIT(GV_LOADED32(a)); }
 __device__ __forceinline__ void tmem_load_wait(uint32_t (&a)[32], uint32_t (&b)[32]) { GV_LOAD_WAIT(GV_LOADED32(a), GV_LOADED32(b)); }
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&a)[32], uint32_t (&b)[32], uint32_t (&c)[32], uint32_t (&d)[32]) {
+  GV_LOAD_WAIT(GV_LOADED32(a), GV_LOADED32(b), GV_LOADED32(c), GV_LOADED32(d));
+}
 __device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[4][8]) {
   GV_LOAD_WAIT(GV_LOADED8(r[0], 0), GV_LOADED8(r[1], 0), GV_LOADED8(r[2], 0), GV_LOADED8(r[3], 0));
 }

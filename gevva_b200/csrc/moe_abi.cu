@@ -266,6 +266,21 @@ bool make_w2_down_tensor_map(CUtensorMap* map, const void* base, uint64_t expert
 bool make_piece_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes) {
   return make_column_order_map(map, base, rows, row_bytes, 0);
 }
+bool make_bf16_tensor_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* stride_bytes, const uint32_t* box) {
+  cuuint64_t extents[4], strides[3];
+  cuuint32_t boxes[4];
+  const cuuint32_t element_strides[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    extents[i] = dims[i];
+    boxes[i] = box[i];
+    if (i + 1 < rank) strides[i] = stride_bytes[i];
+  }
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, static_cast<cuuint32_t>(rank), const_cast<void*>(base), extents, strides, boxes,
+            element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 bool make_operand_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes,
                              int box_rows) {
   return make_operand_map(map, base, rows, row_bytes, box_rows);
@@ -443,6 +458,7 @@ const char* gevva_moe_strerror(int status) {
     case GEVVA_MOE_OK: return "ok";
     case GEVVA_MOE_BAD_EXPERT_ID: return "expert id outside [0,128)";
     case GEVVA_MOE_WAIT_TIMEOUT: return "bounded device wait expired";
+    case GEVVA_MOE_BAD_PAGE: return "position without a page of the cache";
     case GEVVA_MOE_BAD_ARGUMENT: return "bad argument";
     case GEVVA_MOE_CUDA_ERROR: return g_error_text[0] ? g_error_text : "CUDA error";
     case GEVVA_MOE_NO_DEVICE: return "no sm_100 device or driver entry point";

@@ -37,7 +37,8 @@ enum gevva_moe_status {
   GEVVA_MOE_BAD_ARGUMENT = -3,
   GEVVA_MOE_CUDA_ERROR = -4,
   GEVVA_MOE_NO_DEVICE = -5,     /* no sm_100 device / driver entry point missing */
-  GEVVA_MOE_TOO_LARGE = -6
+  GEVVA_MOE_TOO_LARGE = -6,
+  GEVVA_MOE_BAD_PAGE = -7 /* device: a new token's position has no page of the cache (gevva_attn_append) */
 };
 
 /* The eight sidecar tensors of one layer that the reference's constructor resolves
@@ -358,6 +359,83 @@ typedef struct {
 size_t gevva_ff_layer_workspace_bytes(int tokens);
 int gevva_ff_layer_launch(const gevva_ff_layer* layer, const void* hidden, void* out, void* workspace,
                           int tokens, gevva_stream_t stream, gevva_stream_t aux_stream);
+
+/* ---- the attention side of a decoder layer --------------------------------------------------
+ * What stands in front of the feed-forward calls in the reference's layer loop
+ * (src/cuda/runtime/prefill.cuh:924-1199): norms around the attention block, per-head norms and rotation of
+ * queries and keys with the append to the cache (src/cuda/kernels/qkv_transform.cuh), and causal attention.  The projections
+ * between them are the caller's.  Tensors are bf16; heads have 64, 128, 256 or 512 values; query head h reads key head
+ * h / (heads / kv_heads), where kv_heads divides heads and a key head has at most 128 query heads.  Sums, norms and softmax statistics
+ * are held in 32 bits, rotation angles in 64.  All pointers are 16-byte aligned, strides are in elements, positive and multiples of 8.
+ * The calls keep no state; `device_status` is an optional device status word that receives
+ * GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do. */
+
+/* bf16 [tokens, heads, dim], the last dimension contiguous: a view of a fused projection's rows, for instance. */
+typedef struct {
+  const void* data;
+  long long token_stride, head_stride;
+} gevva_attn_rows;
+
+/* A paged cache: keys and values are bf16 [pages, page_size, kv_heads, dim] with strides of their own; page_size is a power of two,
+ * at least 16. */
+typedef struct {
+  void* keys;
+  void* values;
+  long long key_page_stride, key_slot_stride, key_head_stride;
+  long long value_page_stride, value_slot_stride, value_head_stride;
+  int pages, page_size;
+} gevva_attn_cache;
+
+/* The sequences of a call, all on the device.  Sequence s has the new tokens (rows) token_offsets[s] .. token_offsets[s + 1] - 1;
+ * lengths[s] is its number of keys with the new ones counted, so its last new token is at position lengths[s] - 1;
+ * position x lives in slot x % page_size of page table[s * table_stride + x / page_size], where x / page_size < table_width
+ * (table_width * page_size is at most 2^30).
+ * Rows in front of token_offsets[0] and from token_offsets[sequences] on (a padded batch) are left as they were.  Offsets ascend. */
+typedef struct {
+  const int* token_offsets; /* [sequences + 1] */
+  const int* lengths;       /* [sequences] */
+  const int* table;         /* [sequences, table_stride] */
+  int sequences, table_width, table_stride;
+} gevva_attn_batch;
+
+/* out = x / sqrt(mean(x^2) + eps) * weight, rows of `width` values, a multiple of 8 up to 32768.  The norm in front of a block. */
+int gevva_attn_norm(const void* x, const void* weight, void* out, int rows, int width, float eps, gevva_stream_t stream);
+
+/* out = (residual + gate * norm(x) * weight) * scale: the norm behind a block with its residual (rmsnorm_add_2816_kernel,
+ * src/cuda/runtime/prefill.cuh:1197-1199).  gate [width] and scale [1] are optional (NULL: one).  With next_weight (and next; both or none)
+ * next = norm(out) * next_weight as well, of the values of `out` before they are rounded.  `out` may be `residual` or `x`. */
+int gevva_attn_norm_add(const void* x, const void* weight, const void* residual, const void* gate, const void* scale,
+                        const void* next_weight, void* out, void* next, int rows, int width, float eps,
+                        gevva_stream_t stream);
+
+/* Queries and keys: norm over the head with q_weight and k_weight ([dim]; NULL: none); values: norm without a weight where normalize_v
+ * is not zero.  Then the rotation: pair (j, rotated / 2 + j) turns by position * frequencies[j] (f64 [rotated / 2]; rotated is
+ * a multiple of 16 up to dim, zero for none; values from `rotated` on stay).  Queries go to q_out [tokens, heads, dim], keys and
+ * values to the cache and, where k_out and v_out are given (both or none), to [tokens, kv_heads, dim], which gevva_attn_prompt
+ * reads.  A token without a page (position outside the table, page outside the cache) is not stored and reported as
+ * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot. */
+int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v,
+                      const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads, int kv_heads,
+                      int dim, const double* frequencies, int rotated, const void* q_weight, const void* k_weight,
+                      int normalize_v, float eps, void* q_out, void* k_out, void* v_out, int* device_status,
+                      gevva_stream_t stream);
+
+/* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
+ * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  scale > 0.  No row sees another sequence's keys,
+ * whatever their values are; within a sequence, keys and values that a row does not see have to be finite. */
+int gevva_attn_prompt(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v, const int* token_offsets,
+                      int sequences, int tokens, int heads, int kv_heads, int dim, float scale, int window, void* out,
+                      int* device_status, gevva_stream_t stream);
+
+/* The same for new tokens over a paged cache that already holds their keys and values (gevva_attn_append): one token a sequence when
+ * decoding, several in verification and chunked prefill.  Lengths are read on the device, so a captured call can be replayed with
+ * others.  Row i of n sees the keys up to lengths[s] - n + i; a row that sees none is zero.  Slots that no row of a
+ * sequence sees may hold anything.  `workspace` is device memory of gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed
+ * the call; calls that may run at the same time need one each. */
+size_t gevva_attn_chunk_workspace_bytes(int dim);
+int gevva_attn_chunk(const gevva_attn_rows* q, const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens,
+                     int heads, int kv_heads, int dim, float scale, int window, void* out, void* workspace,
+                     int* device_status, gevva_stream_t stream);
 
 /* Per-tensor FP8 quantiser (tools/pack_fp8_dense.py:64-70): scale = amax/448, q = e4m3(w/scale). */
 int gevva_pack_fp8(const float* weights, size_t count, void* out, float* scale, gevva_stream_t stream);

@@ -1,0 +1,393 @@
+"""The attention operators on a GPU against plain forms in 64 bits."""
+import pytest
+import torch
+
+from tests import attention_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def attn():
+    from gevva_b200 import attention
+    return attention
+
+
+def randn(shape, device, seed, std=1.0, mean=0.0):
+    gen = torch.Generator(device=device)
+    gen.manual_seed(seed)
+    return (torch.randn(shape, generator=gen, device=device) * std + mean).to(torch.bfloat16)
+
+
+def offsets_of(news, device):
+    return torch.tensor([0] + torch.tensor(news).cumsum(0).tolist(), dtype=torch.int32, device=device)
+
+
+def make_batch(attn, news, lengths, page, device, seed, spare=2, width=None):
+    """Sequences over pages in random order; table entries that no position needs name no page at all."""
+    gen = torch.Generator().manual_seed(seed)
+    needed = [-(-n // page) for n in lengths]
+    pages = sum(needed) + spare
+    order = torch.randperm(pages, generator=gen).to(torch.int32)
+    table = torch.full((len(news), max([width or 1] + needed)), -7, dtype=torch.int32)
+    at = 0
+    for s, n in enumerate(needed):
+        table[s, :n] = order[at:at + n]
+        at += n
+    return attn.PagedBatch(offsets_of(news, device), torch.tensor(lengths, dtype=torch.int32, device=device), table.to(device)), pages
+
+
+def gathered(cache, batch, s, length):
+    rows = batch.table[s, :-(-length // cache.page_size)].long()
+    return [c[rows].flatten(0, 1)[:length] for c in (cache.k, cache.v)]
+
+
+# ---- prompts ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("news,heads,kv_heads,window", [
+    ([1], 1, 1, 0), ([128], 2, 2, 0), ([17, 1, 130], 4, 2, 0), ([129, 0, 300], 8, 1, 0), ([700], 6, 2, 100),
+    ([64, 1000, 5], 5, 1, 128), ([1, 1, 1, 1], 7, 1, 3), ([257, 255], 3, 1, 1)])
+def test_prompt(attn, cuda_device, dim, news, heads, kv_heads, window):
+    tokens = sum(news)
+    q, k, v = (randn((tokens, h, dim), cuda_device, i) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    scale = dim ** -0.5
+    got = attn.prompt_attention(q, k, v, offsets_of(news, cuda_device), scale, window=window)
+    at = 0
+    for n in news:
+        want, bound = ref.attention(q[at:at + n], k[at:at + n], v[at:at + n], 0, scale, window)
+        ref.within(got[at:at + n], want, bound, f"rows {at}..{at + n}")
+        at += n
+
+
+def test_prompt_reads_views_and_leaves_padding(attn, cuda_device):
+    """Operands as views of one projection's rows; rows outside the offsets stay; other sequences' and padding rows are never seen, whatever they hold."""
+    news, heads, kv_heads, dim = [100, 190], 4, 2, 128
+    first, tokens = 3, 3 + 290 + 9
+    qkv = randn((tokens, heads + 2 * kv_heads, dim), cuda_device, 1)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    at = torch.tensor([3, 103, 293], dtype=torch.int32, device=cuda_device)
+    for bad in (float("nan"), float("inf")):
+        qkv[:first] = bad
+        qkv[first + 290:] = bad
+        out = torch.full((tokens, heads, dim), 5.0, dtype=torch.bfloat16, device=cuda_device)
+        assert attn.prompt_attention(q, k, v, at, 0.1, out=out) is out
+        assert (out[:first] == 5).all() and (out[first + 290:] == 5).all()
+        for a, b in ((3, 103), (103, 293)):
+            want, bound = ref.attention(q[a:b], k[a:b], v[a:b], 0, 0.1, 0)
+            ref.within(out[a:b], want, bound)
+    # a sequence of nothing but infinities leaves its neighbours alone
+    qkv[:first] = 0
+    qkv[103:293] = float("inf")
+    got = attn.prompt_attention(q, k, v, at, 0.1)
+    want, bound = ref.attention(q[3:103], k[3:103], v[3:103], 0, 0.1, 0)
+    ref.within(got[3:103], want, bound)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_prompt_of_large_scores_and_growing_maxima(attn, cuda_device, dim):
+    """Rows whose maximum grows with every key tile, so that what has been summed is scaled down again and again."""
+    n, heads = 600, 2
+    q, k, v = (randn((n, heads, dim), cuda_device, 10 + i) for i in range(3))
+    k = (k.float() * torch.linspace(0.1, 12.0, n, device=cuda_device)[:, None, None]).to(torch.bfloat16)
+    got = attn.prompt_attention(q, k, v, offsets_of([n], cuda_device), dim ** -0.5)
+    want, bound = ref.attention(q, k, v, 0, dim ** -0.5, 0)
+    ref.within(got, want, bound)
+
+
+# ---- chunks over the cache ----------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("news,lengths,heads,kv_heads,page,window", [
+    ([1], [1], 1, 1, 16, 0), ([1], [700], 4, 2, 16, 0), ([1, 1, 1], [129, 5, 2000], 8, 1, 32, 0), ([5, 0, 5], [300, 40, 5], 6, 2, 64, 0),
+    ([200, 1], [1500, 900], 4, 1, 128, 0), ([3, 1], [5000, 64], 5, 1, 256, 1000), ([130], [130], 3, 1, 16, 17),
+    ([9, 4], [4, 0], 2, 1, 16, 0), ([1] * 40, [37 * i + 1 for i in range(40)], 2, 2, 32, 50), ([1], [20000], 7, 1, 16, 0)])
+def test_chunk(attn, cuda_device, dim, news, lengths, heads, kv_heads, page, window):
+    batch, pages = make_batch(attn, news, lengths, page, cuda_device, 3)
+    cache = attn.KvCache(randn((pages, page, kv_heads, dim), cuda_device, 1), randn((pages, page, kv_heads, dim), cuda_device, 2))
+    # slots that nobody sees hold anything
+    for s, n in enumerate(lengths):
+        if n % page:
+            last = int(batch.table[s, n // page])
+            cache.k[last, n % page:] = float("nan")
+            cache.v[last, n % page:] = float("inf")
+    q = randn((sum(news), heads, dim), cuda_device, 4)
+    scale = dim ** -0.5
+    got = attn.chunk_attention(q, cache, batch, scale, window=window)
+    cache.check()
+    at = 0
+    for s, (n, length) in enumerate(zip(news, lengths)):
+        k, v = gathered(cache, batch, s, length)
+        want, bound = ref.attention(q[at:at + n], k, v, length - n, scale, window)
+        ref.within(got[at:at + n], want, bound, f"sequence {s}")
+        at += n
+
+
+def test_chunk_of_strided_cache_and_padded_batch(attn, cuda_device):
+    """Heads in front of slots, keys and values side by side in one tensor; a batch padded with rows behind the last sequence."""
+    page, kv_heads, dim, heads = 32, 2, 128, 4
+    batch, pages = make_batch(attn, [1, 2], [100, 333], page, cuda_device, 8, width=40)
+    both = randn((pages, kv_heads, page, 2, dim), cuda_device, 1)
+    cache = attn.KvCache(both[:, :, :, 0].transpose(1, 2), both[:, :, :, 1].transpose(1, 2))
+    q = randn((6, heads, 2 * dim), cuda_device, 2)[:, :, dim:]
+    out = torch.full((6, heads, dim), -3.0, dtype=torch.bfloat16, device=cuda_device)
+    attn.chunk_attention(q, cache, batch, 0.09, out=out)
+    assert (out[3:] == -3).all()
+    for s, (a, b, length) in enumerate(((0, 1, 100), (1, 3, 333))):
+        k, v = gathered(cache, batch, s, length)
+        want, bound = ref.attention(q[a:b], k, v, length - (b - a), 0.09, 0)
+        ref.within(out[a:b], want, bound)
+
+
+def test_chunk_ignores_pages_in_front_of_the_window(attn, cuda_device):
+    """A window's old pages may have been given to others already: what stands there is not seen."""
+    page, dim, length, window = 16, 256, 1000, 200
+    batch, pages = make_batch(attn, [3], [length], page, cuda_device, 2)
+    cache = attn.KvCache(randn((pages, page, 1, dim), cuda_device, 1), randn((pages, page, 1, dim), cuda_device, 2))
+    q = randn((3, 2, dim), cuda_device, 3)
+    k, v = gathered(cache, batch, 0, length)
+    want, bound = ref.attention(q, k, v, length - 3, 0.05, window)
+    first = length - 3 - window + 1
+    rows = batch.table[0, :first // page].long()
+    cache.k[rows] = float("nan")
+    cache.v[rows] = float("nan")
+    part = int(batch.table[0, first // page])
+    cache.v[part, :first % page] = float("inf")
+    batch.table[0, :first // page] = 1 << 30  # no page at all
+    ref.within(attn.chunk_attention(q, cache, batch, 0.05, window=window), want, bound)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (256, 16, 8), (512, 16, 2)])
+def test_chunk_repeats_its_bits_and_equals_the_prompt_form(attn, cuda_device, dim, heads, kv_heads):
+    n, page = 900, 64
+    batch, pages = make_batch(attn, [n], [n], page, cuda_device, 5)
+    k, v = (randn((n, kv_heads, dim), cuda_device, i) for i in (1, 2))
+    cache = attn.KvCache.empty(pages, page, kv_heads, dim, cuda_device)
+    rows = batch.table[0].long()
+    for store, x in ((cache.k, k), (cache.v, v)):
+        padded = torch.zeros(len(rows) * page, kv_heads, dim, dtype=torch.bfloat16, device=cuda_device)
+        padded[:n] = x
+        store[rows] = padded.view(len(rows), page, kv_heads, dim)
+    q = randn((n, heads, dim), cuda_device, 3)
+    first = attn.chunk_attention(q, cache, batch, 0.06)
+    for _ in range(5):
+        assert torch.equal(first, attn.chunk_attention(q, cache, batch, 0.06))
+    prompt = attn.prompt_attention(q, k, v, batch.token_offsets, 0.06)
+    assert torch.equal(prompt, attn.prompt_attention(q, k, v, batch.token_offsets, 0.06))
+    want, bound = ref.attention(q, k, v, 0, 0.06, 0)
+    ref.within(first, want, bound)
+    ref.within(prompt, want, bound)
+
+
+def test_chunk_with_offsets_past_32_bits(attn, cuda_device):
+    """A cache of more than 2^32 bytes a tensor: the last page lies behind 32-bit offsets."""
+    page, kv_heads, dim = 128, 8, 256
+    pages = (1 << 32) // (page * kv_heads * dim * 2) + 9
+    cache = attn.KvCache(*(torch.empty((pages, page, kv_heads, dim), dtype=torch.bfloat16, device=cuda_device) for _ in range(2)))
+    batch = attn.PagedBatch(offsets_of([2], cuda_device), torch.tensor([250], dtype=torch.int32, device=cuda_device),
+                            torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device=cuda_device))
+    for i, store in enumerate((cache.k, cache.v)):
+        store[pages - 2:] = randn((2, page, kv_heads, dim), cuda_device, i)
+    q = randn((2, 16, dim), cuda_device, 7)
+    k, v = gathered(cache, batch, 0, 250)
+    want, bound = ref.attention(q, k, v, 248, 0.0625, 0)
+    ref.within(attn.chunk_attention(q, cache, batch, 0.0625), want, bound)
+    # and the append stores there
+    new = randn((2, 2 * kv_heads + 16, dim), cuda_device, 9)
+    attn.kv_append(new[:, :16], new[:, 16:24], new[:, 24:], cache, batch, None)
+    cache.check()
+    for c, x in ((cache.k, new[:, 16:24]), (cache.v, new[:, 24:])):
+        assert torch.equal(c[pages - 2, 248 - page:250 - page], x)
+
+
+# ---- append -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("news,lengths,heads,kv_heads,page,rotated,normed,packed", [
+    ([1], [1], 1, 1, 16, 1.0, True, False), ([1, 1, 1], [5, 100000, 17], 16, 8, 16, 1.0, True, False),
+    ([7, 0, 20], [7, 30, 4000], 6, 3, 64, 0.5, True, True), ([33], [33], 5, 1, 32, 0.25, False, True), ([3, 4], [900, 4], 2, 2, 128, 0, True, False)])
+def test_append(attn, cuda_device, dim, news, lengths, heads, kv_heads, page, rotated, normed, packed):
+    batch, pages = make_batch(attn, news, lengths, page, cuda_device, 3)
+    cache = attn.KvCache(randn((pages, page, kv_heads, dim), cuda_device, 1), randn((pages, page, kv_heads, dim), cuda_device, 2))
+    before = cache.k.clone(), cache.v.clone()
+    tokens = sum(news)
+    qkv = randn((tokens, heads + 2 * kv_heads, dim), cuda_device, 4, std=3.0)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:]
+    qw, kw = (randn((dim,), cuda_device, 5 + i, 0.2, 1.0) if normed else None for i in range(2))
+    half = int(dim * rotated) // 2
+    freq = (1e4 ** (-torch.arange(half, dtype=torch.float64, device=cuda_device) / max(half, 1))) if half else None
+    eps = 1e-6
+    got = attn.kv_append(q, k, v, cache, batch, freq, q_weight=qw, k_weight=kw, normalize_v=normed, eps=eps, packed=packed)
+    cache.check()
+    position = torch.cat([torch.arange(length - n, length, device=cuda_device) for n, length in zip(news, lengths)])
+    sequence = torch.repeat_interleave(torch.arange(len(news), device=cuda_device), torch.tensor(news, device=cuda_device))
+    at = (batch.table[sequence, position // page].long(), position % page)
+
+    def check(x, weight, turn, result, what):
+        y = ref.norm(x, weight, eps) if (weight is not None or (not turn and normed)) else x.double()
+        want, size = ref.rotate(y, position, freq) if turn else (y, y.abs())
+        # norm: a sum of dim squares, a square root and three products; angle: 2^-20 of a radian at most
+        ref.within(result, want, ref.BF16 * want.abs() + size * ((dim / 2 + 16) * ref.FP32 + 2.0 ** -20) + 1e-30, what)
+
+    check(q, qw, True, got.q if packed else got, "q")
+    check(k, kw, True, cache.k[at], "k")
+    check(v, None, False, cache.v[at], "v")
+    if packed:
+        assert torch.equal(got.k, cache.k[at]) and torch.equal(got.v, cache.v[at])
+    for now, old in zip((cache.k, cache.v), before):
+        old[at] = now[at]
+        assert torch.equal(now, old)  # nothing else has been written
+
+
+def test_append_without_pages_and_behind_the_last_sequence(attn, cuda_device):
+    page, dim = 16, 64
+    cache = attn.KvCache.empty(3, page, 1, dim, cuda_device)
+    x = randn((8, 3, dim), cuda_device, 1)
+    # sequence 0: position 16 is in a page that does not exist; sequence 1: position 40 is outside the table; rows 5.. are padding
+    batch = attn.PagedBatch(torch.tensor([0, 3, 5], dtype=torch.int32, device=cuda_device), torch.tensor([17, 41], dtype=torch.int32, device=cuda_device),
+                            torch.tensor([[1, 3], [2, -1]], dtype=torch.int32, device=cuda_device))
+    out = torch.full((8, 1, dim), 9.0, dtype=torch.bfloat16, device=cuda_device)
+    attn.kv_append(x[:, :1], x[:, 1:2], x[:, 2:], cache, batch, None, out=out)
+    from gevva_b200 import GevvaMoeError
+    with pytest.raises(GevvaMoeError, match="page"):
+        cache.check()
+    cache.check()  # cleared
+    assert torch.equal(out[:5], x[:5, :1]) and (out[5:] == 9).all()
+    want = torch.zeros_like(cache.k)
+    want[1, 14:16] = x[:2, 1:2]
+    assert torch.equal(cache.k, want)
+
+
+def test_append_turns_far_positions_as_exactly_as_near_ones(attn, cuda_device):
+    page, dim, far = 256, 128, 262143
+    width = (far + page) // page
+    cache = attn.KvCache.empty(1, page, 1, dim, cuda_device)
+    table = torch.zeros((1, width), dtype=torch.int32, device=cuda_device)
+    batch = attn.PagedBatch(offsets_of([1], cuda_device), torch.tensor([far + 1], dtype=torch.int32, device=cuda_device), table)
+    x = randn((1, 3, dim), cuda_device, 1)
+    freq = 1e6 ** (-torch.arange(dim // 2, dtype=torch.float64, device=cuda_device) / (dim // 2))
+    got = attn.kv_append(x[:, :1], x[:, 1:2], x[:, 2:], cache, batch, freq)
+    want, size = ref.rotate(x[:, :1].double(), torch.tensor([far], device=cuda_device), freq)
+    ref.within(got, want, ref.BF16 * want.abs() + size * 2.0 ** -20)
+
+
+# ---- norms --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 3, 64, 777])
+@pytest.mark.parametrize("width", [8, 64, 264, 512, 520, 2816, 4104, 8200, 32768])
+def test_norms(attn, cuda_device, rows, width):
+    x, residual = randn((rows, width), cuda_device, 1, 3.0), randn((rows, width), cuda_device, 2, 2.0)
+    weight, gate, following = (randn((width,), cuda_device, 3 + i, 0.3, 1.0) for i in range(3))
+    scale = randn((1,), cuda_device, 6, 0.1, 0.8)
+    if rows > 2:
+        x[1] = 0
+        residual[2] = 0
+    eps = 1e-5
+    small = (width / 2 + 16) * ref.FP32  # a sum of `width` squares under a square root, and a few products
+    y = ref.norm(x, weight, eps)
+    ref.within(attn.block_norm(x, weight, eps=eps), y, y.abs() * (ref.BF16 + small) + 1e-30, "norm")
+    for g, s, f in ((None, None, None), (gate, None, None), (gate, scale, following), (None, scale, following)):
+        part = y if g is None else y * g.double()
+        want = residual.double() + part
+        size = residual.double().abs() + part.abs()
+        if s is not None:
+            want, size = want * s.double(), size * s.double().abs()
+        got = attn.block_norm_add(x, weight, residual, gate=g, scale=s, next_weight=f, eps=eps)
+        if f is not None:
+            got, after = got
+            # each value is off by small * size before the second norm, its statistic by no more than the largest of them relative to the row's size
+            second = ref.norm(want, f, eps)
+            rms = torch.sqrt((want * want).mean(-1, keepdim=True) + eps)
+            off = 2 * small * size
+            bound = ref.BF16 * second.abs() + (off / rms + (want.abs() / rms) * (off.amax(-1, keepdim=True) / rms + small)) * f.double().abs()
+            ref.within(after, second, bound + 1e-30, "next")
+        ref.within(got, want, want.abs() * ref.BF16 + 2 * small * size + 1e-30, "add")
+
+
+def test_norm_add_in_place(attn, cuda_device):
+    x, residual, weight = randn((50, 2816), cuda_device, 1), randn((50, 2816), cuda_device, 2), randn((2816,), cuda_device, 3)
+    want = attn.block_norm_add(x, weight, residual)
+    hidden = residual.clone()
+    assert attn.block_norm_add(x, weight, hidden, out=hidden) is hidden and torch.equal(hidden, want)
+
+
+# ---- together, streams and graphs ---------------------------------------------------------------
+def test_append_then_attention_as_one_graph_of_growing_lengths(attn, cuda_device):
+    """A decode step captured once and replayed while lengths, positions and pages move on; checked against the prompt form of the same tokens."""
+    heads, kv_heads, dim, page, steps, sequences = 4, 2, 256, 16, 40, 3
+    starts = [0, 5, 130]
+    width = 16
+    gen = torch.Generator().manual_seed(2)
+    table = torch.randperm(sequences * width, generator=gen).to(torch.int32).view(sequences, width).to(cuda_device)
+    cache = attn.KvCache.empty(sequences * width, page, kv_heads, dim, cuda_device)
+    freq = 1e4 ** (-torch.arange(dim // 2, dtype=torch.float64, device=cuda_device) / (dim // 2))
+    total = [s + steps for s in starts]
+    qkv = [randn((n, heads + 2 * kv_heads, dim), cuda_device, 20 + i) for i, n in enumerate(total)]
+
+    def split(x):
+        return x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
+
+    # the prompts' share, all at once
+    if sum(starts):
+        batch = attn.PagedBatch(offsets_of(starts, cuda_device), torch.tensor(starts, dtype=torch.int32, device=cuda_device), table)
+        attn.kv_append(*split(torch.cat([x[:n] for x, n in zip(qkv, starts)])), cache, batch, freq)
+    static = torch.empty((sequences, heads + 2 * kv_heads, dim), dtype=torch.bfloat16, device=cuda_device)
+    lengths = torch.tensor(starts, dtype=torch.int32, device=cuda_device)
+    batch = attn.PagedBatch(offsets_of([1] * sequences, cuda_device), lengths, table)
+    lengths += 1
+    static.copy_(torch.stack([x[n] for x, n in zip(qkv, starts)]))
+
+    def step():
+        return attn.chunk_attention(attn.kv_append(*split(static), cache, batch, freq), cache, batch, 0.0625)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    got = [[] for _ in range(sequences)]
+    for i in range(steps):
+        static.copy_(torch.stack([x[n + i] for x, n in zip(qkv, starts)]))
+        lengths.copy_(torch.tensor([n + i + 1 for n in starts], dtype=torch.int32))
+        graph.replay()
+        for s in range(sequences):
+            got[s].append(out[s].clone())
+    cache.check()
+    for s, n in enumerate(total):
+        own = attn.KvCache.empty(width, page, kv_heads, dim, cuda_device)
+        whole = attn.PagedBatch(offsets_of([n], cuda_device), torch.tensor([n], dtype=torch.int32, device=cuda_device),
+                                torch.arange(width, dtype=torch.int32, device=cuda_device)[None])
+        q, k, v = attn.kv_append(*split(qkv[s]), own, whole, freq, packed=True)
+        want, bound = ref.attention(q, k, v, 0, 0.0625, 0)
+        ref.within(torch.stack(got[s]), want[starts[s]:], bound[starts[s]:], f"sequence {s}")
+
+
+def test_two_streams_at_once(attn, cuda_device):
+    """Chunk calls on streams of their own overlap, each with a workspace of its own."""
+    cases = []
+    for i in range(2):
+        batch, pages = make_batch(attn, [1] * 20, [400 + 111 * j for j in range(20)], 32, cuda_device, i)
+        cache = attn.KvCache(randn((pages, 32, 2, 128), cuda_device, i), randn((pages, 32, 2, 128), cuda_device, 10 + i))
+        cases.append((randn((20, 8, 128), cuda_device, 20 + i), cache, batch, 0.09))
+    want = [attn.chunk_attention(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(cases, streams)):
+            out = torch.empty_like(want[i])
+            got[i].append(attn.chunk_attention(*c, out=out, stream=s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert torch.equal(g, want[i])
+
+
+def test_nothing_to_do(attn, cuda_device):
+    x = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=cuda_device)
+    zero = torch.zeros(2, dtype=torch.int32, device=cuda_device)
+    assert attn.prompt_attention(x, x, x, zero, 1.0).shape == (0, 2, 64)
+    cache = attn.KvCache.empty(1, 16, 2, 64, cuda_device)
+    batch = attn.PagedBatch(zero, zero[:1], torch.zeros((1, 1), dtype=torch.int32, device=cuda_device))
+    assert attn.chunk_attention(x, cache, batch, 1.0).shape == (0, 2, 64)
+    assert attn.kv_append(x, x, x, cache, batch, None).shape == (0, 2, 64)
+    assert attn.block_norm(torch.empty((0, 64), dtype=torch.bfloat16, device=cuda_device), torch.ones(64, dtype=torch.bfloat16, device=cuda_device)).shape == (0, 64)
