@@ -36,7 +36,7 @@ namespace {
 
 constexpr int kRows = 128;         // rows of a query tile
 constexpr int kKeys = kAttnKeys;   // keys of a key tile
-constexpr int kPieceSlots = 2;     // pieces worked on: this one, and the next, whose first operands are fetched meanwhile
+constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, and one whose operands are fetched
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
 constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
 constexpr int kLeastRun = 4;       // key tiles of the shortest run that a CTA is given
@@ -74,11 +74,13 @@ struct Shape {
   static constexpr int kKeyStages = kDim / kStageDim;
   static constexpr int kValueStages = kValueDim / kStageDim;
   static constexpr int kQueryTileBytes = kRows * kDim * 2;
-  static constexpr int kControlBytes = 2048;
+  static constexpr int kControlBytes = 3072;
   static constexpr int kRoom = (232448 - kControlBytes - kTiles * kQueryTileBytes) / kStageBytes;
   static constexpr int kStages = kRoom < 8 ? kRoom : 8;
-  static constexpr int kSoftmaxWarps = 4 * kTiles;
+  static constexpr int kSoftmaxWarps = 8;
   static constexpr int kThreads = 128 + 32 * kSoftmaxWarps;
+  // Whether a tile's values and the next one's keys fit side by side: scores of the next piece may then be asked for before this one's end.
+  static constexpr bool kAhead = kTiles == 1 && kStages >= kKeyStages + kValueStages;
   static_assert(kStages > kValueStages, "the values of a tile are in shared memory at the same time");
   static_assert(kTiles == 1 || kDim <= 128, "two query tiles need 2 * (128 + dim) columns of tensor memory");
 };
@@ -92,10 +94,12 @@ struct AttnSmem {
   uint64_t q_full, q_empty;
   uint64_t acc_full[2];       // scores: by key tile in turn (one query tile) or by query tile (two)
   uint64_t p_ready[2];
-  uint64_t pv_done[kTiles];   // completes once a key tile
+  uint64_t pv_done[2];        // outputs of a key tile are summed up; by key tile in turn or by query tile, like the scores
   uint64_t o_free[kTiles];    // the outputs of the last piece have been read
   uint64_t piece_full[kPieceSlots], piece_empty[kPieceSlots];
-  uint64_t v_landed;          // values of a tile that has rows to be cleared
+  uint64_t v_landed[2];       // values of a tile that has rows to be cleared, by softmax warpgroup
+  // One query tile: the warpgroups take the key tiles in turn, and hand each row's reference and sum on (a barrier for each quarter's warps).
+  uint64_t reference_ready[2][4], sum_ready[2][4];
   uint64_t next_full;
   alignas(16) uint4 next_item;  // answer to a request for another item
   Piece pieces[kPieceSlots];
@@ -104,6 +108,7 @@ struct AttnSmem {
   int start_sequence;
   uint32_t tmem_base;
   volatile int abort;
+  float references[kTiles == 1 ? 2 : 1][kTiles == 1 ? kRows : 1], sums[kTiles == 1 ? 2 : 1][kTiles == 1 ? kRows : 1];
 };
 
 struct AttnParams {
@@ -169,15 +174,13 @@ constexpr uint32_t kIdescScores = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeys >
 template <int kColumns>
 constexpr uint32_t kIdescValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((kColumns >> 3) << 17) | ((kRows >> 4) << 24);
 
-// With two query tiles a softmax thread holds more registers than the launch gives every thread: 168 a thread at launch, and
+// A softmax thread holds more registers than the launch gives every thread: 168 a thread at launch, and
 // 128 x 88 + 256 x 208 = 384 x 168.  (At the top of each role: that is what the compiler goes by.)
-template <int kTiles>
 __device__ __forceinline__ void fewer_registers() {
-  if constexpr (kTiles == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
 }
-template <int kTiles>
 __device__ __forceinline__ void more_registers() {
-  if constexpr (kTiles == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
 }
 
 template <int kDim, int kTiles, bool kPaged>
@@ -201,16 +204,20 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     for (int s = 0; s < 2; ++s) {
       mbar_init(&smem->acc_full[s], 1);
       mbar_init(&smem->p_ready[s], 4);
+      mbar_init(&smem->pv_done[s], 1);
     }
-    for (int t = 0; t < kTiles; ++t) {
-      mbar_init(&smem->pv_done[t], 1);
-      mbar_init(&smem->o_free[t], 4);
-    }
+    for (int t = 0; t < kTiles; ++t) mbar_init(&smem->o_free[t], 4);
     for (int s = 0; s < kPieceSlots; ++s) {
       mbar_init(&smem->piece_full[s], 1);
       mbar_init(&smem->piece_empty[s], 2 + S::kSoftmaxWarps);  // fetching warp, MMA warp, softmax warps
     }
-    mbar_init(&smem->v_landed, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&smem->v_landed[w], 1);
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&smem->reference_ready[w][i], 1);
+        mbar_init(&smem->sum_ready[w][i], 1);
+      }
+    }
     mbar_init(&smem->next_full, 1);
     // shared memory that is not where the swizzle wants it: nothing is computed, and the status word says so
     smem->abort = (smem_u32(smem_raw) & 1023u) != 0;
@@ -282,7 +289,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
 
   if (warp < 4) {
-  fewer_registers<kTiles>();  // (a warpgroup's four warps at the same place)
+  fewer_registers();  // (a warpgroup's four warps at the same place)
   if (warp == 2) {
     // ---------------- what to do next ----------------
     uint32_t count = 0;  // pieces handed out
@@ -543,131 +550,211 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    uint32_t stage = 0, phase = 0;
+    // The tensor pipe holds few instructions ahead, so what lies between two batches of products is time that it stands still: one wait for all that a
+    // batch needs (a lane for each barrier), and few, wide products.
     const bool leader = elect_one();
     const uint64_t q_desc = make_smem_desc(smem_u32(smem->queries[0]), 1024, 2);
     const uint64_t k_desc = make_smem_desc(smem_u32(smem->stage[0]), 1024, 2);
     // values: 64 columns a swizzle row, the next 64 a column block further (leading offset), keys eight rows a group (stride offset)
     const uint64_t v_desc = k_desc | (static_cast<uint64_t>(kColumnBytes >> 4) << 16);
+    constexpr int kTogether = S::kStages > 3 ? 2 : 1;  // stages of a batch: of three, one has to be free for the next
+    uint32_t stage = 0, phase = 0;
     bool ok = true;
-    uint32_t done = 0;  // key tiles of the pieces before
-    const auto stage_ready = [&] { return wait_or_abort(&smem->full[stage], phase, smem, p.status); };
-    const auto next_stage = [&] {
-      if (++stage == S::kStages) {
-        stage = 0;
+    const auto skip_stages = [&](uint32_t count) {
+      stage += count;
+      if (stage >= S::kStages) {
+        stage -= S::kStages;
         phase ^= 1u;
       }
     };
-    // The products of one stage: 128 (64) of the columns that scores sum over, or of the outputs' columns.
+    // Waits until the next `count` stages are there, and `other`'s phase is over (lanes from 16 on; null: nothing else).
+    const auto ready = [&](uint32_t count, uint64_t* other, uint32_t other_parity) {
+      uint32_t s = stage + min(static_cast<uint32_t>(lane & 15), count - 1), parity = phase;
+      if (s >= S::kStages) {
+        s -= S::kStages;
+        parity ^= 1u;
+      }
+      uint64_t* bar = &smem->full[s];
+      if (lane >= 16 && other) {
+        bar = other;
+        parity = other_parity;
+      }
+      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, smem, p.status));
+    };
+    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_or_abort(bar, parity, smem, p.status)); };
+    // The products of one stage: 128 (64) of the columns that scores sum over; or of the outputs' columns, of one stage or of two that lie side by side.
     const auto scores_of_stage = [&](uint32_t d, int tile, int part) {
+      const uint64_t b = k_desc + stage * (S::kStageBytes >> 4);
 #pragma unroll
       for (int i = 0; i < S::kStageDim / 16; ++i) {
         const uint32_t at = (i / 4) * kColumnBytes + (i % 4) * 32;
-        mma_shared(d, q_desc + ((tile * S::kQueryTileBytes + part * 2 * kColumnBytes + at) >> 4),
-                   k_desc + ((stage * S::kStageBytes + at) >> 4), kIdescScores, part > 0 || i > 0);
+        mma_shared(d, q_desc + ((tile * S::kQueryTileBytes + part * 2 * kColumnBytes + at) >> 4), b + (at >> 4), kIdescScores, part > 0 || i > 0 ? 1u : 0u);
       }
     };
-    const auto values_of_stage = [&](uint32_t d, uint32_t a, bool fresh) {
+    const auto values_of_stage = [&](uint32_t d, uint32_t at_stage, uint32_t a, uint32_t accumulate, uint32_t descriptor) {
+      const uint64_t b = v_desc + at_stage * (S::kStageBytes >> 4);
 #pragma unroll
-      for (int i = 0; i < kKeys / 16; ++i)
-        mma_tensor(d, a + 8 * i, v_desc + ((stage * S::kStageBytes + i * 2048) >> 4), kIdescValues<S::kStageDim>, !fresh || i > 0);
+      for (int i = 0; i < kKeys / 16; ++i) mma_tensor(d, a + 8 * i, b + ((i * 2048) >> 4), descriptor, i > 0 ? 1u : accumulate);
     };
+    uint32_t done = 0;    // key tiles of the pieces before
+    bool scored = false;  // the piece's first scores have been asked for at the end of the one before
     for (uint32_t count = 0; ok; ++count) {
       const int slot = count % kPieceSlots;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      ok = wait_for(&smem->piece_full[slot], (count / kPieceSlots) & 1u);
       if (!ok) break;
       const Piece piece = smem->pieces[slot];
       const int tiles = piece.tiles;
       if (tiles == 0) break;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->q_full, count & 1u, smem, p.status));
+      if (!scored) ok = wait_for(&smem->q_full, count & 1u);
       if (!ok) break;
       if constexpr (kTiles == 1) {
-        const auto scores = [&](uint32_t n) {
-          for (int i = 0; ok && i < S::kKeyStages; ++i) {
-            ok = __all_sync(0xffffffffu, stage_ready());
-            if (ok && leader) {
-              scores_of_stage(tmem_base + (n & 1u) * kKeys, 0, i);
-              tc_commit(&smem->empty[stage]);
+        // Of key tile n, the piece's last one or not: its queries may be replaced behind the last one's.
+        const auto scores = [&](uint32_t n, bool last) {
+#pragma unroll
+          for (int i = 0; i < S::kKeyStages; i += kTogether) {
+            constexpr int kBatch = kTogether < S::kKeyStages ? kTogether : S::kKeyStages;
+            ok = ok && ready(kBatch, nullptr, 0);
+            if (!ok) break;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+              if (leader) {
+                scores_of_stage(tmem_base + (n & 1u) * kKeys, 0, i + k);
+                tc_commit(&smem->empty[stage]);
+                if (i + k + 1 == S::kKeyStages) {
+                  tc_commit(&smem->acc_full[n & 1u]);
+                  if (last) tc_commit(&smem->q_empty);
+                }
+              }
+              __syncwarp();
+              skip_stages(1);
             }
-            next_stage();
           }
-          if (ok && leader) tc_commit(&smem->acc_full[n & 1u]);
         };
-        scores(done);
+        if (!scored) scores(done, tiles == 1);
+        scored = false;
         for (int j = 0; ok && j < tiles; ++j) {
           const uint32_t n = done + j;
-          if (j + 1 < tiles) scores(n + 1);
-          if (ok && j + 1 == tiles && leader) tc_commit(&smem->q_empty);
-          if (j == 0) ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->o_free[0], (count & 1u) ^ 1u, smem, p.status));
-          if (!seen_keys(piece, j, p.window).all()) {
+          if (j + 1 < tiles) scores(n + 1, j + 2 == tiles);
+          if (j == 0) ok = ok && wait_for(&smem->o_free[0], (count & 1u) ^ 1u);
+          if (ok && !seen_keys(piece, j, p.window).all()) {
             // the softmax warps clear rows of these values before they say that P is there
-            const uint32_t first_stage = stage, first_phase = phase;
-            for (int i = 0; ok && i < S::kValueStages; ++i) {
-              ok = __all_sync(0xffffffffu, stage_ready());
-              next_stage();
-            }
-            stage = first_stage;
-            phase = first_phase;
-            if (ok && lane == 0) mbar_arrive(&smem->v_landed);
+            ok = ready(S::kValueStages, nullptr, 0);
+            if (ok && lane == 0) mbar_arrive(&smem->v_landed[n & 1u]);
           }
-          ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->p_ready[n & 1u], (n >> 1) & 1u, smem, p.status));
+          if (S::kAhead && ok && j + 1 == tiles) {
+            // While the last softmax runs: the first scores of the next piece, if its operands are there before P is.
+            const uint32_t value_stage = stage, value_phase = phase;
+            const int next_slot = (count + 1) % kPieceSlots;
+            const uint32_t next_parity = ((count + 1) / kPieceSlots) & 1u;
+            const long long start = clock64();
+            skip_stages(S::kValueStages);
+            while (!scored && !__all_sync(0xffffffffu, mbar_try_wait(&smem->p_ready[n & 1u], (n >> 1) & 1u))) {
+              bool there = mbar_try_wait(&smem->piece_full[next_slot], next_parity);
+              if (there) there = smem->pieces[next_slot].tiles > 0 && mbar_try_wait(&smem->q_full, (count + 1) & 1u);
+              if (there) {
+                uint32_t s = stage + min(lane, S::kKeyStages - 1), parity = phase;
+                if (s >= S::kStages) {
+                  s -= S::kStages;
+                  parity ^= 1u;
+                }
+                there = mbar_try_wait(&smem->full[s], parity);
+              }
+              if (__all_sync(0xffffffffu, there)) {
+                scores(n + 1, __all_sync(0xffffffffu, smem->pieces[next_slot].tiles == 1));
+                scored = true;
+              }
+              // (the wait below says that P does not come; this loop only has to end)
+              if (__any_sync(0xffffffffu, smem->abort || clock64() - start > kWaitLimitCycles)) break;
+            }
+            stage = value_stage;
+            phase = value_phase;
+          }
+          constexpr int kBatch = kTogether < S::kValueStages ? kTogether : S::kValueStages;
+          ok = ok && ready(kBatch, &smem->p_ready[n & 1u], (n >> 1) & 1u);
           if (!ok) break;
           tc_fence_after_sync();
-          for (int i = 0; ok && i < S::kValueStages; ++i) {
-            ok = __all_sync(0xffffffffu, stage_ready());
-            if (ok && leader) {
-              values_of_stage(tmem_base + 256 + i * S::kStageDim, tmem_base + (n & 1u) * kKeys, j == 0);
+          const uint32_t weights = tmem_base + (n & 1u) * kKeys, accumulate = j > 0 ? 1u : 0u;
+          if (kBatch == 2 && stage + 1 < S::kStages) {
+            if (leader) {
+              values_of_stage(tmem_base + 256, stage, weights, accumulate, kIdescValues<2 * S::kStageDim>);
               tc_commit(&smem->empty[stage]);
+              tc_commit(&smem->empty[stage + 1]);
+              tc_commit(&smem->pv_done[n & 1u]);
             }
-            next_stage();
+            __syncwarp();
+            skip_stages(2);
+          } else {
+#pragma unroll
+            for (int i = 0; i < S::kValueStages; ++i) {
+              if (i >= kBatch) ok = ok && ready(1, nullptr, 0);
+              if (!ok) break;
+              if (leader) {
+                values_of_stage(tmem_base + 256 + i * S::kStageDim, stage, weights, accumulate, kIdescValues<S::kStageDim>);
+                tc_commit(&smem->empty[stage]);
+                if (i + 1 == S::kValueStages) tc_commit(&smem->pv_done[n & 1u]);
+              }
+              __syncwarp();
+              skip_stages(1);
+            }
+            if (!ok) break;
           }
-          if (ok && leader) tc_commit(&smem->pv_done[0]);
+          if (scored) skip_stages(S::kKeyStages);  // the next piece's keys stand behind these values, and have been used
         }
       } else {
         // one stage holds a tile's keys, another its values
-        ok = __all_sync(0xffffffffu, stage_ready());
+        ok = ready(1, nullptr, 0);
         if (!ok) break;
         if (leader) {
+#pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             scores_of_stage(tmem_base + t * kKeys, t, 0);
             tc_commit(&smem->acc_full[t]);
           }
           tc_commit(&smem->empty[stage]);
         }
-        next_stage();
+        __syncwarp();
+        skip_stages(1);
         for (int j = 0; ok && j < tiles; ++j) {
           const uint32_t n = done + j;
-          const uint32_t value_stage = stage, value_phase = phase;
-          next_stage();
-          const uint32_t key_stage = stage, key_phase = phase;
+          const uint32_t accumulate = j > 0 ? 1u : 0u;
           const bool more = j + 1 < tiles;
-          for (int t = 0; ok && t < kTiles; ++t) {
-            if (j == 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->o_free[t], (count & 1u) ^ 1u, smem, p.status));
-            stage = value_stage;
-            phase = value_phase;
-            ok = ok && __all_sync(0xffffffffu, stage_ready());
-            if (ok && t == 0 && lane == 0 && !seen_keys(piece, j, p.window).all()) mbar_arrive(&smem->v_landed);
-            ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->p_ready[t], n & 1u, smem, p.status));
-            if (!ok) break;
-            tc_fence_after_sync();
-            if (leader) {
-              values_of_stage(tmem_base + 256 + t * kDim, tmem_base + t * kKeys, j == 0);
-              tc_commit(&smem->pv_done[t]);
-              if (t + 1 == kTiles) tc_commit(&smem->empty[value_stage]);
-            }
-            stage = key_stage;
-            phase = key_phase;
+          if (j == 0) ok = wait_for(&smem->o_free[0], (count & 1u) ^ 1u) && wait_for(&smem->o_free[1], (count & 1u) ^ 1u);
+          if (ok && !seen_keys(piece, j, p.window).all()) {
+            ok = ready(1, nullptr, 0);
+            if (ok && lane == 0) mbar_arrive(&smem->v_landed[0]);
+          }
+          // P of the first tile, the values and the next keys; then P of the second
+          ok = ok && ready(more ? 2 : 1, &smem->p_ready[0], n & 1u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t value_stage = stage;
+          skip_stages(1);
+          if (leader) {
+            values_of_stage(tmem_base + 256, value_stage, tmem_base, accumulate, kIdescValues<S::kStageDim>);
+            tc_commit(&smem->pv_done[0]);
             if (more) {
-              ok = __all_sync(0xffffffffu, stage_ready());
-              if (ok && leader) {
-                scores_of_stage(tmem_base + t * kKeys, t, 0);
-                tc_commit(&smem->acc_full[t]);
-                if (t + 1 == kTiles) tc_commit(&smem->empty[key_stage]);
-              }
+              scores_of_stage(tmem_base, 0, 0);
+              tc_commit(&smem->acc_full[0]);
             }
           }
-          if (more) next_stage();
-          else if (ok && leader) tc_commit(&smem->q_empty);
+          __syncwarp();
+          ok = wait_for(&smem->p_ready[1], n & 1u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          if (leader) {
+            values_of_stage(tmem_base + 256 + kDim, value_stage, tmem_base + kKeys, accumulate, kIdescValues<S::kStageDim>);
+            tc_commit(&smem->pv_done[1]);
+            tc_commit(&smem->empty[value_stage]);
+            if (more) {
+              scores_of_stage(tmem_base + kKeys, 1, 0);
+              tc_commit(&smem->acc_full[1]);
+              tc_commit(&smem->empty[stage]);
+            } else {
+              tc_commit(&smem->q_empty);
+            }
+          }
+          __syncwarp();
+          if (more) skip_stages(1);
         }
       }
       done += tiles;
@@ -677,16 +764,20 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
   } else {
     // ---------------- softmax and epilogue ----------------
-    more_registers<kTiles>();
-    const int own = (warp - 4) / 4;            // query tile of this warpgroup
+    more_registers();
+    // This warpgroup's query tile; or, of the one query tile there is, the key tiles that are its turn: those whose scores stand in its half
+    // of the score columns.
+    const int own = (warp - 4) / 4;
+    const int tile_of_rows = kTiles == 2 ? own : 0;
     const int quarter = warp & 3;              // the tensor-memory lanes this warp may read
     const int row = quarter * 32 + lane;
     const int row_token = row / p.group, row_head = row - row_token * p.group;
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t outputs = lanes + 256 + own * kDim;
+    const uint32_t scores = lanes + own * kKeys;
+    const uint32_t outputs = lanes + 256 + tile_of_rows * kDim;
     const float c = p.scale_log2;
     uint32_t done = 0, ring = 0;  // key tiles and operand stages of the pieces before
-    uint32_t cleared = 0;         // tiles with cleared values
+    uint32_t cleared = 0;         // tiles with values that this warpgroup has cleared
     bool ok = true;
     for (uint32_t count = 0; ok; ++count) {
       const int slot = count % kPieceSlots;
@@ -694,7 +785,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (!ok) break;
       const Piece piece = smem->pieces[slot];
       if (piece.tiles == 0) break;
-      const int token = own * p.step + row_token;
+      const int token = tile_of_rows * p.step + row_token;
       const bool valid = row_token < p.step && token < piece.tokens;
       // keys that the row sees: [row_begin, row_end)
       const int position = piece.position0 + token;
@@ -704,16 +795,22 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int least_end = __reduce_min_sync(0xffffffffu, valid ? row_end : 0x7fffffff);
       const int most_begin = __reduce_max_sync(0xffffffffu, valid ? row_begin : 0);
       float reference = -CUDART_INF_F, sum = 0.0f;
+      const int first = kTiles == 2 ? 0 : static_cast<int>((done & 1u) ^ static_cast<uint32_t>(own));
 #pragma unroll 1
-      for (int j = 0; j < piece.tiles; ++j) {
+      for (int j = first; j < piece.tiles; j += kTiles == 2 ? 1 : 2) {
         const uint32_t n = done + j;
-        const uint32_t scores_slot = kTiles == 2 ? own : n & 1u;
-        const uint32_t scores_parity = kTiles == 2 ? n & 1u : (n >> 1) & 1u;
-        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->acc_full[scores_slot], scores_parity, smem, p.status));
+        const uint32_t turn = kTiles == 2 ? n : n >> 1;  // of this warpgroup
+        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->acc_full[own], turn & 1u, smem, p.status));
         if (!ok) break;
         tc_fence_after_sync();
-        const uint32_t scores = lanes + scores_slot * kKeys;
         const int key0 = (piece.first_tile + j) * kKeys;
+        float factor = 1.0f, tile_sum = 0.0f;
+        const uint32_t turn_before = ((n - 1) >> 1) & 1u;  // of the other warpgroup, for the tile before
+        if (!active && kTiles == 1) {
+          if (n > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->reference_ready[own ^ 1][quarter], turn_before, smem, p.status));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(&smem->reference_ready[own][quarter]);
+        }
         if (active) {
           uint32_t s0[32], s1[32], s2[32], s3[32];
           tmem_load_32x32(scores, s0);
@@ -723,10 +820,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tmem_load_wait(s0, s1, s2, s3);
           if (key0 + kKeys > least_end || key0 < most_begin) {
             const int from = row_begin - key0, to = row_end - key0;
-            const auto hide = [&](uint32_t (&s)[32], int first) {
+            const auto hide = [&](uint32_t (&s)[32], int base) {
 #pragma unroll
               for (int i = 0; i < 32; ++i)
-                if (first + i < from || first + i >= to) s[i] = 0xff800000u;  // -inf
+                if (base + i < from || base + i >= to) s[i] = 0xff800000u;  // -inf
             };
             hide(s0, 0);
             hide(s1, 32);
@@ -742,25 +839,39 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             top3 = fmaxf(top3, __uint_as_float(s3[i]));
           }
           const float top = fmaxf(fmaxf(top0, top1), fmaxf(top2, top3));
+          if constexpr (kTiles == 1) {
+            // (waited for at a piece's first tile too: then nothing is read, but what this warp writes next has been read)
+            if (n > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->reference_ready[own ^ 1][quarter], turn_before, smem, p.status));
+            if (!ok) break;
+            reference = j > 0 ? smem->references[own ^ 1][row] : -CUDART_INF_F;
+          }
           // (false where nothing has been seen yet: the difference of two infinities is no number)
           const bool grow = (top - reference) * c > kGrowth;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float factor = grow ? exp2_approx((reference - top) * c) : 1.0f;
-            if (grow) reference = top;
-            sum *= factor;
-            if (j > 0) {
-              ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (n - 1) & 1u, smem, p.status));
-              if (!ok) break;
-              tc_fence_after_sync();
+          const bool any_grow = __any_sync(0xffffffffu, grow);
+          if (grow) {
+            factor = exp2_approx((reference - top) * c);
+            reference = top;
+          }
+          if constexpr (kTiles == 1) {
+            smem->references[own][row] = reference;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&smem->reference_ready[own][quarter]);
+          }
+          if (any_grow && j > 0) {
+            // (A wait can tell a phase from the one before it, not from the one after the next: each of these barriers is one phase behind at most, since
+            // the scores at hand were asked for behind the outputs of two tiles before, and one ahead at most.)
+            const uint32_t before = kTiles == 2 ? n - 1 : (n - 1) >> 1;
+            ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[kTiles == 2 ? own : own ^ 1], before & 1u, smem, p.status));
+            if (!ok) break;
+            tc_fence_after_sync();
 #pragma unroll 1
-              for (int i = 0; i < S::kValueDim; i += 32) {
-                uint32_t o[32];
-                tmem_load_32x32(outputs + i, o);
-                tmem_load_wait(o);
+            for (int i = 0; i < S::kValueDim; i += 32) {
+              uint32_t o[32];
+              tmem_load_32x32(outputs + i, o);
+              tmem_load_wait(o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                tmem_store_32x32(outputs + i, o);
-              }
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+              tmem_store_32x32(outputs + i, o);
             }
           }
           const float shift = reference == -CUDART_INF_F ? 0.0f : -reference * c;
@@ -782,14 +893,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           exponentials(s2, 0);
           exponentials(s3, 16);
           tmem_store_32x32(scores + 32, packed);
-          sum += low_of(total) + high_of(total);
+          tile_sum = low_of(total) + high_of(total);
           tmem_store_wait();
         }
         tc_fence_before_sync();
         const Seen seen = seen_keys(piece, j, p.window);
-        if (own == 0 && !seen.all()) {
+        if ((kTiles == 1 || own == 0) && !seen.all()) {
           // (the MMA warp says when they have landed: these threads do not follow the stages' phases)
-          ok = __all_sync(0xffffffffu, wait_or_abort(&smem->v_landed, cleared & 1u, smem, p.status));
+          ok = __all_sync(0xffffffffu, wait_or_abort(&smem->v_landed[own], cleared & 1u, smem, p.status));
           if (!ok) break;
           ++cleared;
           // K0 K1 V0 K2 V1 .. with one query tile, K0 V0 K1 V1 .. with two
@@ -805,14 +916,27 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           fence_proxy_async_smem();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&smem->p_ready[scores_slot]);
+        if (lane == 0) mbar_arrive(&smem->p_ready[own]);
+        if constexpr (kTiles == 1) {
+          if (n > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->sum_ready[own ^ 1][quarter], turn_before, smem, p.status));
+          if (!ok) break;
+          sum = j > 0 ? fmaf(smem->sums[own ^ 1][row], factor, tile_sum) : tile_sum;
+          smem->sums[own][row] = sum;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&smem->sum_ready[own][quarter]);
+        } else {
+          sum = fmaf(sum, factor, tile_sum);
+        }
       }
       if (!ok) break;
+      const bool finishes = kTiles == 2 || ((done + piece.tiles - 1) & 1u) == static_cast<uint32_t>(own);
       done += piece.tiles;
       ring += piece.tiles * (S::kKeyStages + S::kValueStages);
-      // (The last scores say that the outputs of the tile two before are there: a phase is waited for only when it is the next to complete.)
-      if (piece.tiles > 1) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (done - 2) & 1u, smem, p.status));
-      ok = ok && __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (done - 1) & 1u, smem, p.status));
+      if (!finishes) {  // the other warpgroup has the last tile, and so the outputs
+        if (lane == 0) mbar_arrive(&smem->piece_empty[slot]);
+        continue;
+      }
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (kTiles == 2 ? done - 1 : (done - 1) >> 1) & 1u, smem, p.status));
       if (!ok) break;
       tc_fence_after_sync();
       if (active) {
@@ -820,7 +944,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int column0 = piece.half * S::kValueDim;
         __nv_bfloat16* out = p.out + static_cast<long long>(piece.query0 + token) * p.out_token_stride +
                              static_cast<long long>(piece.kv_head * p.group + row_head) * p.out_head_stride + column0;
-        const size_t partial_row = (static_cast<size_t>(piece.slot < 0 ? 0 : piece.slot) * kTiles + own) * kRows + row;
+        const size_t partial_row = (static_cast<size_t>(piece.slot < 0 ? 0 : piece.slot) * kTiles + tile_of_rows) * kRows + row;
 #pragma unroll 1
         for (int i = 0; i < S::kValueDim; i += 32) {
           uint32_t o[32];
@@ -851,7 +975,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&smem->o_free[own]);
+        mbar_arrive(&smem->o_free[tile_of_rows]);
         mbar_arrive(&smem->piece_empty[slot]);
       }
     }
