@@ -126,7 +126,7 @@ int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const 
   call.k_out = k_out;
   call.v_out = v_out;
   call.status = device_status;
-  return launched(gv::launch_kv_append(call, stream));
+  return launched(gv::launch_kv_append(call, gv::current_sm_count(), stream));
 }
 
 int gevva_attn_prompt(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v, const int* token_offsets,

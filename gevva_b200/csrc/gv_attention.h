@@ -61,7 +61,7 @@ struct AppendCall {
   void* v_out;
   int* status;
 };
-cudaError_t launch_kv_append(const AppendCall& call, cudaStream_t stream);
+cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t stream);
 
 // out = rms_norm(x) * weight, or (residual + gate * rms_norm(x) * weight) * scale where there is a residual; next = rms_norm(out) *
 // next_weight of the values before their rounding.
