@@ -6,13 +6,10 @@ from dataclasses import dataclass
 
 import torch
 
-from .runtime import GevvaMoeError, _address, _check, _enqueue, library
+from .runtime import GevvaMoeError, _address, _enqueue, library
 
 HEAD_DIMS = (64, 128, 256, 512)
-
-
-class _Rows(ctypes.Structure):
-    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+_empty = torch.empty
 
 
 class _Cache(ctypes.Structure):
@@ -32,14 +29,15 @@ def _lib():
     if getattr(lib, "_gv_attn_ready", False):
         return lib
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
-    rows, cache, batch = ctypes.POINTER(_Rows), ctypes.POINTER(_Cache), ctypes.POINTER(_Batch)
+    i64 = ctypes.c_longlong
+    rows = [vp, i64, i64]  # address, strides of a token and of a head
     lib.gevva_attn_norm.argtypes = [vp, vp, vp, i32, i32, f32, vp]
     lib.gevva_attn_norm_add.argtypes = [vp] * 8 + [i32, i32, f32, vp]
-    lib.gevva_attn_append.argtypes = [rows, rows, rows, cache, batch, i32, i32, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, vp, vp, vp]
-    lib.gevva_attn_prompt.argtypes = [rows, rows, rows, vp, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp]
+    lib.gevva_attn_append.argtypes = rows * 3 + [vp, vp, i32, i32, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, vp, vp, vp]
+    lib.gevva_attn_prompt.argtypes = rows * 3 + [vp, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp]
     lib.gevva_attn_chunk_workspace_bytes.argtypes = [i32]
     lib.gevva_attn_chunk_workspace_bytes.restype = ctypes.c_size_t
-    lib.gevva_attn_chunk.argtypes = [rows, cache, batch, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp]
+    lib.gevva_attn_chunk.argtypes = rows + [vp, vp, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp]
     lib._gv_attn_ready = True
     return lib
 
@@ -49,63 +47,69 @@ def _status(status, where):
         raise GevvaMoeError(status, where)
 
 
-def _device(tensor, device, name):
-    if tensor.device != device:
-        raise ValueError(f"{name}: expected on {device}, got {tensor.device}")
+def _at(tensor, dtype, shape, device, name):
+    """Address of a contiguous tensor on `device`; None stays None."""
+    if tensor is None:
+        return None
+    if tensor.dtype is dtype and tensor.shape == shape and tensor.device == device and tensor.is_contiguous():
+        return tensor.data_ptr()
+    raise ValueError(f"{name}: expected contiguous {dtype} {tuple(shape)} on {device}, got {tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
 
 
-def _heads(tensor, name, device=None, shape=None):
-    """bf16 [tokens, heads, dim] on the GPU, its last dimension contiguous."""
-    if (tensor.dtype is not torch.bfloat16 or tensor.dim() != 3 or not tensor.is_cuda or tensor.shape[2] not in HEAD_DIMS or
-            tensor.stride(2) != 1 or (shape is not None and tensor.shape != shape) or (device is not None and tensor.device != device)):
-        want = "(tokens, heads, 64|128|256|512)" if shape is None else tuple(shape)
-        raise ValueError(f"{name}: expected CUDA bfloat16 {want} with contiguous heads, got {tensor.dtype} {tuple(tensor.shape)} "
-                         f"strides {tensor.stride()} on {tensor.device}")
-    return _Rows(tensor.data_ptr(), tensor.stride(0), tensor.stride(1))
+def _heads(tensor, name, device, shape):
+    """(address, strides of a token and of a head) of a bf16 [tokens, heads, dim] on the GPU, its last dimension contiguous."""
+    if tensor.dtype is torch.bfloat16 and tensor.shape == shape and tensor.device == device:
+        token_stride, head_stride, one = tensor.stride()
+        if one == 1:
+            return tensor.data_ptr(), token_stride, head_stride
+    raise ValueError(f"{name}: expected bfloat16 {tuple(shape)} on {device} with contiguous heads, got {tensor.dtype} {tuple(tensor.shape)} "
+                     f"strides {tensor.stride()} on {tensor.device}")
+
+
+def _queries(q):
+    device = q.device
+    if q.dim() != 3 or q.shape[2] not in HEAD_DIMS or device.type != "cuda":
+        raise ValueError(f"q: expected CUDA bfloat16 (tokens, heads, 64|128|256|512), got {q.dtype} {tuple(q.shape)} on {device}")
+    return device, q.shape, _heads(q, "q", device, q.shape)
 
 
 def _out(out, like_shape, device, name="out"):
     if out is None:
-        return torch.empty(like_shape, dtype=torch.bfloat16, device=device)
-    _check(out, torch.bfloat16, like_shape, name)
-    _device(out, device, name)
+        return _empty(like_shape, dtype=torch.bfloat16, device=device)
+    _at(out, torch.bfloat16, like_shape, device, name)
     return out
 
 
-def _status_word(status, device):
-    if status is not None:
-        _check(status, torch.int32, (1,), "status")
-        _device(status, device, "status")
-    return _address(status)
+def _rows(x, name="input"):
+    if x.dtype is not torch.bfloat16 or x.dim() != 2 or not x.is_contiguous() or not x.is_cuda:
+        raise ValueError(f"{name}: expected contiguous CUDA bfloat16 (rows, width), got {x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.device, x.shape
 
 
 def block_norm(x, weight, eps=1e-6, out=None, stream=None):
     """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768."""
-    rows, width = x.shape
-    _check(x, torch.bfloat16, (rows, width), "input")
-    _check(weight, torch.bfloat16, (width,), "weight")
-    _device(weight, x.device, "weight")
-    out = _out(out, x.shape, x.device)
-    _status(_enqueue(_lib().gevva_attn_norm, x.device, stream, x.data_ptr(), weight.data_ptr(), out.data_ptr(), rows, width, eps),
-            "block_norm")
+    device, shape = _rows(x)
+    rows, width = shape
+    out = _out(out, shape, device)
+    _status(_enqueue(_lib().gevva_attn_norm, device, stream, x.data_ptr(), _at(weight, torch.bfloat16, (width,), device, "weight"),
+                     out.data_ptr(), rows, width, eps), "block_norm")
     return out
 
 
 def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None, eps=1e-6, out=None, stream=None):
     """(residual + gate * norm(x) * weight) * scale, the norm behind a block; with `next_weight` also the next block's norm of
     the result, returned as (out, next).  gate bf16 [width] and scale bf16 [1] are optional; out may be residual."""
-    rows, width = x.shape
-    _check(x, torch.bfloat16, (rows, width), "input")
-    _check(residual, torch.bfloat16, (rows, width), "residual")
-    _device(residual, x.device, "residual")
-    for tensor, size, name in ((weight, width, "weight"), (gate, width, "gate"), (scale, 1, "scale"), (next_weight, width, "next_weight")):
-        if tensor is not None:
-            _check(tensor, torch.bfloat16, (size,), name)
-            _device(tensor, x.device, name)
-    out = _out(out, x.shape, x.device)
-    following = torch.empty_like(x) if next_weight is not None else None
-    _status(_enqueue(_lib().gevva_attn_norm_add, x.device, stream, x.data_ptr(), weight.data_ptr(), residual.data_ptr(), _address(gate),
-                     _address(scale), _address(next_weight), out.data_ptr(), _address(following), rows, width, eps), "block_norm_add")
+    device, shape = _rows(x)
+    rows, width = shape
+    bf16 = torch.bfloat16
+    following = None
+    out = _out(out, shape, device)
+    if next_weight is not None:
+        following = _empty(shape, dtype=bf16, device=device)
+    _status(_enqueue(_lib().gevva_attn_norm_add, device, stream, x.data_ptr(), _at(weight, bf16, (width,), device, "weight"),
+                     _at(residual, bf16, shape, device, "residual"), _at(gate, bf16, (width,), device, "gate"),
+                     _at(scale, bf16, (1,), device, "scale"), _at(next_weight, bf16, (width,), device, "next_weight"), out.data_ptr(),
+                     _address(following), rows, width, eps), "block_norm_add")
     return out if following is None else (out, following)
 
 
@@ -127,6 +131,7 @@ class KvCache:
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
         self._packed = _Cache(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
                               pages, page_size)
+        self._address = ctypes.addressof(self._packed)
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, device="cuda:0"):
@@ -152,8 +157,9 @@ class PagedBatch:
     def __init__(self, token_offsets, lengths, table):
         sequences = lengths.shape[0] if lengths.dim() == 1 else -1
         for tensor, shape, name in ((token_offsets, (sequences + 1,), "token_offsets"), (lengths, (sequences,), "lengths")):
-            _check(tensor, torch.int32, shape, name)
-            _device(tensor, table.device, name)
+            if not tensor.is_cuda:
+                raise ValueError(f"{name}: expected a CUDA tensor, got {tensor.device}")
+            _at(tensor, torch.int32, shape, table.device, name)
         if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != sequences or table.shape[1] < 1 or sequences < 1 or (
                 table.stride(1) != 1 and table.shape[1] > 1):
             raise ValueError(f"table: expected int32 ({sequences}, pages a sequence), got {table.dtype} {tuple(table.shape)}")
@@ -161,6 +167,7 @@ class PagedBatch:
         self.device = table.device
         stride = table.stride(0) if sequences > 1 else table.shape[1]
         self._packed = _Batch(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
+        self._address = ctypes.addressof(self._packed)
 
 
 @dataclass
@@ -181,25 +188,18 @@ def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, 
     positions in the cache.  q, k, v are [tokens, heads, dim], views of one projection's rows for instance.  Returns the queries, with
     `packed` also keys and values as [tokens, kv_heads, dim] for prompt_attention.  `out` takes the queries.  A token
     without a page is not stored; cache.check() reports it."""
-    q_rows = _heads(q, "q")
-    tokens, heads, dim = q.shape
+    device, shape, q_rows = _queries(q)
+    tokens, heads, dim = shape
     kv_heads = cache.kv_heads
-    device = q.device
     if cache.head_dim != dim or cache.device != device or batch.device != device:
         raise ValueError(f"kv_append: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
     k_rows, v_rows = _heads(k, "k", device, (tokens, kv_heads, dim)), _heads(v, "v", device, (tokens, kv_heads, dim))
-    for tensor, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if tensor is not None:
-            _check(tensor, torch.bfloat16, (dim,), name)
-            _device(tensor, device, name)
-    if frequencies is not None:
-        _check(frequencies, torch.float64, (frequencies.numel(),), "frequencies")
-        _device(frequencies, device, "frequencies")
     rotated = 0 if frequencies is None else 2 * frequencies.numel()
-    out = _out(out, q.shape, device)
-    k_out, v_out = (torch.empty(k.shape, dtype=torch.bfloat16, device=device) for _ in range(2)) if packed else (None, None)
-    _status(_enqueue(_lib().gevva_attn_append, device, stream, q_rows, k_rows, v_rows, cache._packed, batch._packed, tokens, heads, kv_heads,
-                     dim, _address(frequencies), rotated, _address(q_weight), _address(k_weight), normalize_v, eps, out.data_ptr(),
+    out = _out(out, shape, device)
+    k_out, v_out = (_empty(k.shape, dtype=torch.bfloat16, device=device) for _ in range(2)) if packed else (None, None)
+    _status(_enqueue(_lib().gevva_attn_append, device, stream, *q_rows, *k_rows, *v_rows, cache._address, batch._address, tokens, heads, kv_heads,
+                     dim, frequencies if frequencies is None else _at(frequencies, torch.float64, frequencies.shape, device, "frequencies"), rotated,
+                     _at(q_weight, torch.bfloat16, (dim,), device, "q_weight"), _at(k_weight, torch.bfloat16, (dim,), device, "k_weight"), normalize_v, eps, out.data_ptr(),
                      _address(k_out), _address(v_out), cache.status.data_ptr()), "kv_append")
     return Appended(out, k_out, v_out) if packed else out
 
@@ -208,18 +208,16 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
     """Causal attention of packed prompts: rows token_offsets[s] .. token_offsets[s + 1] - 1 (int32 on the GPU) are sequence s, and
     each sees its sequence's rows up to itself, the last `window` of them where that is not zero.  q [tokens, heads, dim], k and v
     [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`.  `status` is an optional int32 [1] device word."""
-    q_rows = _heads(q, "q")
-    tokens, heads, dim = q.shape
-    device = q.device
+    device, shape, q_rows = _queries(q)
+    tokens, heads, dim = shape
     if k.dim() != 3:
         raise ValueError(f"k: expected (tokens, kv_heads, dim), got {tuple(k.shape)}")
-    shape = (tokens, k.shape[1], dim)
-    k_rows, v_rows = _heads(k, "k", device, shape), _heads(v, "v", device, shape)
-    _check(token_offsets, torch.int32, (token_offsets.numel(),), "token_offsets")
-    _device(token_offsets, device, "token_offsets")
-    out = _out(out, q.shape, device)
-    _status(_enqueue(_lib().gevva_attn_prompt, device, stream, q_rows, k_rows, v_rows, token_offsets.data_ptr(), token_offsets.numel() - 1,
-                     tokens, heads, shape[1], dim, scale, window, out.data_ptr(), _status_word(status, device)), "prompt_attention")
+    kv_heads = k.shape[1]
+    k_rows, v_rows = (_heads(x, name, device, (tokens, kv_heads, dim)) for x, name in ((k, "k"), (v, "v")))
+    sequences = token_offsets.numel() - 1
+    out = _out(out, shape, device)
+    _status(_enqueue(_lib().gevva_attn_prompt, device, stream, *q_rows, *k_rows, *v_rows, _at(token_offsets, torch.int32, (sequences + 1,), device, "token_offsets"), sequences,
+                     tokens, heads, kv_heads, dim, scale, window, out.data_ptr(), _at(status, torch.int32, (1,), device, "status")), "prompt_attention")
     return out
 
 
@@ -227,20 +225,19 @@ def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
     """Causal attention of new tokens over the pages of their sequences, which hold their keys and values already (kv_append):
     one token a sequence when decoding, several for verification and chunked prefill.  A row that sees no key is zero; rows outside the offsets
     are left as they were in `out`."""
-    q_rows = _heads(q, "q")
-    tokens, heads, dim = q.shape
-    device = q.device
+    device, shape, q_rows = _queries(q)
+    tokens, heads, dim = shape
     if cache.head_dim != dim or cache.device != device or batch.device != device:
         raise ValueError(f"chunk_attention: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
     lib = _lib()
-    out = _out(out, q.shape, device)
+    out = _out(out, shape, device)
 
     def launch(*args):
         # (the workspace's size goes by the device, which is the current one in here)
-        workspace = torch.empty(lib.gevva_attn_chunk_workspace_bytes(dim), dtype=torch.uint8, device=device)
+        workspace = _empty(lib.gevva_attn_chunk_workspace_bytes(dim), dtype=torch.uint8, device=device)
         if stream is not None:  # not the stream that the workspace belongs to
             workspace.record_stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
-        return lib.gevva_attn_chunk(q_rows, cache._packed, batch._packed, tokens, heads, cache.kv_heads, dim, scale, window, out.data_ptr(),
+        return lib.gevva_attn_chunk(*q_rows, cache._address, batch._address, tokens, heads, cache.kv_heads, dim, scale, window, out.data_ptr(),
                                     workspace.data_ptr(), cache.status.data_ptr(), *args)
 
     _status(_enqueue(launch, device, stream), "chunk_attention")

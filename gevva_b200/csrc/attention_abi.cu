@@ -31,9 +31,9 @@ bool heads_ok(int tokens, int heads, int kv_heads, int dim) {
          (dim == 64 || dim == 128 || dim == 256 || dim == 512);
 }
 
-bool rows_ok(gv::AttnRows* out, const gevva_attn_rows* in, int tokens, int heads, int dim) {
-  if (!in || !aligned_for(in->data, tokens)) return false;
-  *out = gv::AttnRows{in->data, in->token_stride, in->head_stride};
+bool rows_ok(gv::AttnRows* out, const void* data, long long token_stride, long long head_stride, int tokens, int heads, int dim) {
+  if (!aligned_for(data, tokens)) return false;
+  *out = gv::AttnRows{data, token_stride, head_stride};
   return stride_ok(out->head_stride, heads, dim) && stride_ok(out->token_stride, tokens, static_cast<long long>(heads) * dim);
 }
 
@@ -99,13 +99,16 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
   return launched(gv::launch_block_norm(call, gv::current_sm_count(), stream));
 }
 
-int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v, const gevva_attn_cache* cache,
+int gevva_attn_append(const void* q, long long q_token_stride, long long q_head_stride,
+                      const void* k, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_token_stride, long long v_head_stride,
+                      const gevva_attn_cache* cache,
                       const gevva_attn_batch* batch, int tokens, int heads, int kv_heads, int dim, const double* frequencies,
                       int rotated, const void* q_weight, const void* k_weight, int normalize_v, float eps, void* q_out, void* k_out,
                       void* v_out, int* device_status, gevva_stream_t stream) {
   gv::AppendCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, tokens, heads, dim) || !rows_ok(&call.k, k, tokens, kv_heads, dim) ||
-      !rows_ok(&call.v, v, tokens, kv_heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) || rotated < 0 || rotated > dim ||
+  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !rows_ok(&call.k, k, k_token_stride, k_head_stride, tokens, kv_heads, dim) ||
+      !rows_ok(&call.v, v, v_token_stride, v_head_stride, tokens, kv_heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) || rotated < 0 || rotated > dim ||
       rotated % 16 || (rotated > 0 && (!frequencies || (reinterpret_cast<uintptr_t>(frequencies) & 7))) || !aligned_or_null(q_weight) ||
       !aligned_or_null(k_weight) || !(eps >= 0.0f) || !aligned_for(q_out, tokens) || !aligned_or_null(k_out) || !aligned_or_null(v_out) || (tokens > 0 && !k_out != !v_out))
     return GEVVA_MOE_BAD_ARGUMENT;
@@ -129,12 +132,15 @@ int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const 
   return launched(gv::launch_kv_append(call, gv::current_sm_count(), stream));
 }
 
-int gevva_attn_prompt(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v, const int* token_offsets,
+int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_stride,
+                      const void* k, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_token_stride, long long v_head_stride,
+                      const int* token_offsets,
                       int sequences, int tokens, int heads, int kv_heads, int dim, float scale, int window, void* out,
                       int* device_status, gevva_stream_t stream) {
   gv::AttnCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, tokens, heads, dim) || !rows_ok(&call.k, k, tokens, kv_heads, dim) ||
-      !rows_ok(&call.v, v, tokens, kv_heads, dim) || !token_offsets || sequences < 1 || tokens > kMaxPositions || !attention_ok(scale, window) ||
+  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !rows_ok(&call.k, k, k_token_stride, k_head_stride, tokens, kv_heads, dim) ||
+      !rows_ok(&call.v, v, v_token_stride, v_head_stride, tokens, kv_heads, dim) || !token_offsets || sequences < 1 || tokens > kMaxPositions || !attention_ok(scale, window) ||
       !aligned_for(out, tokens))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (tokens == 0) return GEVVA_MOE_OK;
@@ -158,11 +164,12 @@ size_t gevva_attn_chunk_workspace_bytes(int dim) {
   return dim == 64 || dim == 128 || dim == 256 || dim == 512 ? gv::attention_workspace_bytes(dim, gv::current_sm_count()) : 0;
 }
 
-int gevva_attn_chunk(const gevva_attn_rows* q, const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads,
+int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_stride,
+                     const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads,
                      int kv_heads, int dim, float scale, int window, void* out, void* workspace, int* device_status,
                      gevva_stream_t stream) {
   gv::AttnCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, tokens, heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) ||
+  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) ||
       tokens > kMaxPositions || !attention_ok(scale, window) || !aligned_for(out, tokens) || !aligned(workspace))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (tokens == 0) return GEVVA_MOE_OK;

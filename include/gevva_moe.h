@@ -367,14 +367,9 @@ int gevva_ff_layer_launch(const gevva_ff_layer* layer, const void* hidden, void*
  * between them are the caller's.  Tensors are bf16; heads have 64, 128, 256 or 512 values; query head h reads key head
  * h / (heads / kv_heads), where kv_heads divides heads and a key head has at most 128 query heads.  Sums, norms and softmax statistics
  * are held in 32 bits, rotation angles in 64.  All pointers are 16-byte aligned, strides are in elements, positive and multiples of 8.
- * The calls keep no state; `device_status` is an optional device status word that receives
+ * Queries, keys and values are [tokens, heads, dim] with the last dimension contiguous, given as an address and two strides (of a token and
+ * of a head): views of a fused projection's rows, for instance.  The calls keep no state; `device_status` is an optional device status word that receives
  * GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do. */
-
-/* bf16 [tokens, heads, dim], the last dimension contiguous: a view of a fused projection's rows, for instance. */
-typedef struct {
-  const void* data;
-  long long token_stride, head_stride;
-} gevva_attn_rows;
 
 /* A paged cache: keys and values are bf16 [pages, page_size, kv_heads, dim] with strides of their own; page_size is a power of two,
  * at least 16. */
@@ -414,7 +409,9 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
  * values to the cache and, where k_out and v_out are given (both or none), to [tokens, kv_heads, dim], which gevva_attn_prompt
  * reads.  A token without a page (position outside the table, page outside the cache) is not stored and reported as
  * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot. */
-int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v,
+int gevva_attn_append(const void* q, long long q_token_stride, long long q_head_stride,
+                      const void* k, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_token_stride, long long v_head_stride,
                       const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads, int kv_heads,
                       int dim, const double* frequencies, int rotated, const void* q_weight, const void* k_weight,
                       int normalize_v, float eps, void* q_out, void* k_out, void* v_out, int* device_status,
@@ -423,7 +420,10 @@ int gevva_attn_append(const gevva_attn_rows* q, const gevva_attn_rows* k, const 
 /* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
  * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  scale > 0.  No row sees another sequence's keys,
  * whatever their values are; within a sequence, keys and values that a row does not see have to be finite. */
-int gevva_attn_prompt(const gevva_attn_rows* q, const gevva_attn_rows* k, const gevva_attn_rows* v, const int* token_offsets,
+int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_stride,
+                      const void* k, long long k_token_stride, long long k_head_stride,
+                      const void* v, long long v_token_stride, long long v_head_stride,
+                      const int* token_offsets,
                       int sequences, int tokens, int heads, int kv_heads, int dim, float scale, int window, void* out,
                       int* device_status, gevva_stream_t stream);
 
@@ -433,7 +433,8 @@ int gevva_attn_prompt(const gevva_attn_rows* q, const gevva_attn_rows* k, const 
  * sequence sees may hold anything.  `workspace` is device memory of gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed
  * the call; calls that may run at the same time need one each. */
 size_t gevva_attn_chunk_workspace_bytes(int dim);
-int gevva_attn_chunk(const gevva_attn_rows* q, const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens,
+int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_stride,
+                     const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens,
                      int heads, int kv_heads, int dim, float scale, int window, void* out, void* workspace,
                      int* device_status, gevva_stream_t stream);
 

@@ -18,7 +18,7 @@ def lib():
 
 
 def rows(data=A, token=512, head=64):
-    return attn._Rows(data, token, head)
+    return data, token, head
 
 
 def cache(**change):
@@ -32,16 +32,19 @@ def batch(**change):
     return attn._Batch(*dict(fields, **change).values())
 
 
+CACHE, BATCH = cache(), batch()
+
+
 def chunk(lib, q=None, c=None, b=None, tokens=3, heads=4, kv_heads=2, dim=64, scale=0.1, window=0, out=A, workspace=A):
-    return lib.gevva_attn_chunk(q or rows(), c or cache(), b or batch(), tokens, heads, kv_heads, dim, scale, window, out, workspace, None, None)
+    return lib.gevva_attn_chunk(*(q or rows()), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), tokens, heads, kv_heads, dim, scale, window, out, workspace, None, None)
 
 
 def prompt(lib, q=None, k=None, v=None, offsets=A, sequences=2, tokens=3, heads=4, kv_heads=2, dim=64, scale=0.1, window=0, out=A):
-    return lib.gevva_attn_prompt(q or rows(), k or rows(), v or rows(), offsets, sequences, tokens, heads, kv_heads, dim, scale, window, out, None, None)
+    return lib.gevva_attn_prompt(*(q or rows()), *(k or rows()), *(v or rows()), offsets, sequences, tokens, heads, kv_heads, dim, scale, window, out, None, None)
 
 
 def append(lib, q=None, c=None, b=None, tokens=3, heads=4, kv_heads=2, dim=64, freq=A, rotated=64, eps=1e-6, q_out=A, k_out=None, v_out=None, qw=None):
-    return lib.gevva_attn_append(q or rows(), rows(), rows(), c or cache(), b or batch(), tokens, heads, kv_heads, dim, freq, rotated, qw, None, 0, eps,
+    return lib.gevva_attn_append(*(q or rows()), *rows(), *rows(), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), tokens, heads, kv_heads, dim, freq, rotated, qw, None, 0, eps,
                                  q_out, k_out, v_out, None, None)
 
 
