@@ -39,7 +39,7 @@ constexpr int kKeys = kAttnKeys;   // keys of a key tile
 constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, and one whose operands are fetched
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
 constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
-constexpr int kLeastRun = 4;       // key tiles of the shortest run that a CTA is given
+constexpr int kLeastRun = 1;    // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256: 16.0 us, with 2 16.4, with 4 20.8)
 
 // One run of key tiles of one item.
 struct Piece {
@@ -103,9 +103,6 @@ struct AttnSmem {
   uint64_t next_full;
   alignas(16) uint4 next_item;  // answer to a request for another item
   Piece pieces[kPieceSlots];
-  long long warp_work[S::kThreads / 32];
-  long long start_offset;
-  int start_sequence;
   uint32_t tmem_base;
   volatile int abort;
   float references[kTiles == 1 ? 2 : 1][kTiles == 1 ? kRows : 1], sums[kTiles == 1 ? 2 : 1][kTiles == 1 ? kRows : 1];
@@ -239,55 +236,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   grid_dependency_wait();
 
   const int step = p.step * kTiles;  // tokens of an item
-  long long run_begin = 0, run_end = 0;
-  long long work = 0;
-  int parts = 0;
-  if constexpr (kPaged) {
-    // Where this CTA's run begins: every CTA adds up all sequences' work, a few of them a thread.
-    const int heads = p.kv_heads * S::kHalves;
-    const int capacity = p.table_width << p.page_shift;
-    const int each = (p.sequences + S::kThreads - 1) / S::kThreads;
-    const int first = static_cast<int>(threadIdx.x) * each;
-    const auto work_of = [&](int s) -> long long {
-      const int from = max(p.token_offsets[s], 0), news = min(p.token_offsets[s + 1], p.tokens) - from;
-      if (news <= 0) return 0;
-      const AttnSequence q = attn_sequence(news, min(max(p.lengths[s], 0), capacity), step);
-      return heads * attn_tiles_before(q, q.query_tiles, step, p.window);
-    };
-    long long mine = 0;
-    for (int s = first; s < min(first + each, p.sequences); ++s) mine += work_of(s);
-    long long upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const long long other = __shfl_up_sync(0xffffffffu, upto, d);
-      if (lane >= d) upto += other;
-    }
-    if (lane == 31) smem->warp_work[warp] = upto;
-    __syncthreads();
-    long long before = 0;
-    for (int w = 0; w < S::kThreads / 32; ++w) {
-      if (w < warp) before += smem->warp_work[w];
-      work += smem->warp_work[w];
-    }
-    upto += before;
-    parts = attn_parts(work, static_cast<int>(gridDim.x), kLeastRun);
-    if (static_cast<int>(blockIdx.x) < parts) {
-      run_begin = attn_part_begin(work, parts, blockIdx.x);
-      run_end = attn_part_begin(work, parts, blockIdx.x + 1);
-      if (upto - mine <= run_begin && run_begin < upto) {
-        long long at = upto - mine;
-        int s = first;
-        for (long long w = work_of(s); at + w <= run_begin; w = work_of(s)) {
-          at += w;
-          ++s;
-        }
-        smem->start_sequence = s;
-        smem->start_offset = run_begin - at;
-      }
-    }
-    __syncthreads();
-  }
-
   if (warp < 4) {
   fewer_registers();  // (a warpgroup's four warps at the same place)
   if (warp == 2) {
@@ -307,20 +255,69 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     };
     if constexpr (kPaged) {
       int record[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (run_end > run_begin) {
-        const int capacity = p.table_width << p.page_shift;
-        int s = smem->start_sequence;
-        long long offset = smem->start_offset, at = run_begin;
+      // All sequences' work, 32 at a time, a lane each; then the sequence that this CTA's run begins in.
+      const int heads = p.kv_heads * S::kHalves;
+      const int capacity = p.table_width << p.page_shift;
+      int lane_from = 0, lane_news = 0, lane_length = 0, loaded = -1;  // of the 32 sequences from `loaded` on
+      const auto load_sequences = [&](int first) {
+        if (first == loaded) return;
+        loaded = first;
+        lane_from = lane_news = lane_length = 0;
+        if (first + lane < p.sequences) {
+          lane_from = max(p.token_offsets[first + lane], 0);
+          lane_news = max(min(p.token_offsets[first + lane + 1], p.tokens) - lane_from, 0);
+          lane_length = min(max(p.lengths[first + lane], 0), capacity);
+        }
+      };
+      const auto upto_lane = [&] {  // work of the loaded sequences up to the lane's
+        long long upto = 0;
+        if (lane_news > 0) {
+          const AttnSequence q = attn_sequence(lane_news, lane_length, step);
+          upto = heads * attn_tiles_before(q, q.query_tiles, step, p.window);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+          const long long other = __shfl_up_sync(0xffffffffu, upto, d);
+          if (lane >= d) upto += other;
+        }
+        return upto;
+      };
+      long long work = 0, upto = 0;
+      for (int first = 0; first < p.sequences; first += 32) {
+        load_sequences(first);
+        upto = upto_lane();
+        work += __shfl_sync(0xffffffffu, upto, 31);
+      }
+      const int parts = attn_parts(work, static_cast<int>(gridDim.x), kLeastRun);
+      if (static_cast<int>(blockIdx.x) < parts) {
+        const long long run_begin = attn_part_begin(work, parts, blockIdx.x), run_end = attn_part_begin(work, parts, blockIdx.x + 1);
+        long long at = run_begin, before = 0;
+        int s = 0;
+        for (;; s += 32) {
+          if (loaded != s) {
+            load_sequences(s);
+            upto = upto_lane();
+          }
+          const long long all = __shfl_sync(0xffffffffu, upto, 31);
+          if (before + all > run_begin) break;
+          before += all;
+        }
+        const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > run_begin)) - 1;
+        const long long in_front = __shfl_sync(0xffffffffu, upto, (owner + 31) & 31);
+        long long offset = run_begin - before - (owner > 0 ? in_front : 0);
+        s += owner;
         while (ok && at < run_end) {
-          const int from = max(p.token_offsets[s], 0), news = min(p.token_offsets[s + 1], p.tokens) - from;
+          load_sequences(s & ~31);
+          const int from = __shfl_sync(0xffffffffu, lane_from, s & 31), news = __shfl_sync(0xffffffffu, lane_news, s & 31);
+          const int length = __shfl_sync(0xffffffffu, lane_length, s & 31);
           if (news > 0) {
-            const AttnSequence q = attn_sequence(news, min(max(p.lengths[s], 0), capacity), step);
+            const AttnSequence q = attn_sequence(news, length, step);
             const long long of_head = attn_tiles_before(q, q.query_tiles, step, p.window);
-            int head = static_cast<int>(offset / of_head);
+            int head = attn_quotient(offset, of_head);
             offset -= head * of_head;
             int tile = attn_find_query_tile(q, offset, step, p.window);
             offset -= attn_tiles_before(q, tile, step, p.window);
-            for (; ok && head < p.kv_heads * S::kHalves && at < run_end; ++head) {
+            for (; ok && head < heads && at < run_end; ++head) {
               for (; ok && tile < q.query_tiles && at < run_end; ++tile) {
                 const int tiles = attn_tiles(q, tile, step, p.window);
                 const int skip = static_cast<int>(offset);
@@ -991,14 +988,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // Adds up the sums of the items that the ends of runs have cut: CTA x takes the item that begins in run x and does not end there, its
-// rows dealt out over the warps of gridDim.y CTAs.
+// rows dealt out over the warps of gridDim.y CTAs.  Bound by latency: the record says where the parts are, and what of them is asked for, four
+// at a time, waits for nothing else.
 template <int kValueDim>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p, int tiles) {
   grid_dependency_wait();
   const int4 first = *reinterpret_cast<const int4*>(p.records + 8 * static_cast<size_t>(blockIdx.x));
-  const int more = first.x;
-  if (more == 0) return;
   const int half = p.records[8 * static_cast<size_t>(blockIdx.x) + 4];
+  const int parts = first.x + 1;
+  if (parts == 1) return;
   const int lane = threadIdx.x & 31;
   const int query0 = first.y, tokens = first.z, kv_head = first.w;
   const size_t slot_rows = static_cast<size_t>(tiles) * kRows;
@@ -1006,49 +1004,61 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p,
     return static_cast<size_t>(2 * (static_cast<int>(blockIdx.x) + part) + (part == 0 ? 1 : 0)) * slot_rows;
   };
   const int rows = tokens * p.group;
+  constexpr int kEach = kValueDim / 32, kVector = kEach < 4 ? kEach : 4, kVectors = kEach / kVector;
   for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < rows; r += gridDim.y * 8) {
     const int token = r / p.group, head = r - token * p.group;
     const int row = (token / p.step) * kRows + (token % p.step) * p.group + head;
-    float top = -CUDART_INF_F;
-    for (int i = lane; i <= more; i += 32) top = fmaxf(top, p.partial_stats[2 * (row_of(i) + row)]);
+    float top = -CUDART_INF_F, sum = 0.0f, acc[kEach] = {};
+    for (int part = 0; part < parts; part += 4) {
+      float2 stats[4];
+      float v[4][kEach];
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (top == -CUDART_INF_F) top = 0.0f;  // every weight is zero then
-    constexpr int kEach = kValueDim / 32;
-    float acc[kEach] = {};
-    float sum = 0.0f;
-    for (int i = 0; i <= more; ++i) {
-      const float2 stats = reinterpret_cast<const float2*>(p.partial_stats)[row_of(i) + row];
-      const float weight = exp2_approx(stats.x - top);
-      sum = fmaf(stats.y, weight, sum);
-      const float* from = p.partial + (row_of(i) + row) * kValueDim + lane * kEach;
-      if constexpr (kEach == 2) {
-        const float2 v = *reinterpret_cast<const float2*>(from);
-        acc[0] = fmaf(v.x, weight, acc[0]);
-        acc[1] = fmaf(v.y, weight, acc[1]);
-      } else {
+      for (int i = 0; i < 4; ++i) {
+        const size_t at = row_of(min(part + i, parts - 1)) + row;
+        stats[i] = reinterpret_cast<const float2*>(p.partial_stats)[at];
+        if (part + i >= parts) stats[i] = make_float2(-CUDART_INF_F, 0.0f);
+        const float* from = p.partial + at * kValueDim;
 #pragma unroll
-        for (int k = 0; k < kEach; k += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(from + k);
-          acc[k] = fmaf(v.x, weight, acc[k]);
-          acc[k + 1] = fmaf(v.y, weight, acc[k + 1]);
-          acc[k + 2] = fmaf(v.z, weight, acc[k + 2]);
-          acc[k + 3] = fmaf(v.w, weight, acc[k + 3]);
+        for (int k = 0; k < kVectors; ++k) {
+          if constexpr (kVector == 2) {
+            const float2 x = reinterpret_cast<const float2*>(from)[lane];
+            v[i][0] = x.x;
+            v[i][1] = x.y;
+          } else {
+            const float4 x = reinterpret_cast<const float4*>(from)[k * 32 + lane];
+            v[i][4 * k] = x.x;
+            v[i][4 * k + 1] = x.y;
+            v[i][4 * k + 2] = x.z;
+            v[i][4 * k + 3] = x.w;
+          }
         }
       }
+      const float now = fmaxf(fmaxf(fmaxf(stats[0].x, stats[1].x), fmaxf(stats[2].x, stats[3].x)), top);
+      const float shift = now == -CUDART_INF_F ? 0.0f : now;  // (nothing seen: every weight is zero)
+      const float keep = exp2_approx(top - shift);
+      sum *= keep;
+#pragma unroll
+      for (int k = 0; k < kEach; ++k) acc[k] *= keep;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float weight = exp2_approx(stats[i].x - shift);
+        sum = fmaf(stats[i].y, weight, sum);
+        // (a part that is not there, or has seen nothing, adds nothing, whatever its sums hold)
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) acc[k] = weight > 0.0f || weight != weight ? fmaf(v[i][k], weight, acc[k]) : acc[k];
+      }
+      top = now;
     }
     const float inverse = sum != 0.0f ? 1.0f / sum : 0.0f;
-    uint32_t* out = reinterpret_cast<uint32_t*>(p.out + static_cast<long long>(query0 + token) * p.out_token_stride +
-                                                static_cast<long long>(kv_head * p.group + head) * p.out_head_stride +
-                                                half * kValueDim + lane * kEach);
-    if constexpr (kEach == 2) {
-      out[0] = pack_bf16x2(acc[0] * inverse, acc[1] * inverse);
-    } else if constexpr (kEach == 4) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16x2(acc[0] * inverse, acc[1] * inverse), pack_bf16x2(acc[2] * inverse, acc[3] * inverse));
-    } else {
-      *reinterpret_cast<uint4*>(out) =
-          make_uint4(pack_bf16x2(acc[0] * inverse, acc[1] * inverse), pack_bf16x2(acc[2] * inverse, acc[3] * inverse),
-                     pack_bf16x2(acc[4] * inverse, acc[5] * inverse), pack_bf16x2(acc[6] * inverse, acc[7] * inverse));
+    __nv_bfloat16* out = p.out + static_cast<long long>(query0 + token) * p.out_token_stride +
+                         static_cast<long long>(kv_head * p.group + head) * p.out_head_stride + half * kValueDim;
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+      if constexpr (kVector == 2)
+        reinterpret_cast<uint32_t*>(out)[lane] = pack_bf16x2(acc[0] * inverse, acc[1] * inverse);
+      else
+        reinterpret_cast<uint2*>(out)[k * 32 + lane] = make_uint2(pack_bf16x2(acc[4 * k] * inverse, acc[4 * k + 1] * inverse),
+                                                                  pack_bf16x2(acc[4 * k + 2] * inverse, acc[4 * k + 3] * inverse));
     }
   }
 }

@@ -108,9 +108,16 @@ GV_HD int attn_find_query_tile(const AttnSequence& s, long long at, int step, in
 
 // Work is dealt out to `parts` CTAs in runs of equal length; fewer CTAs where a run would be shorter than `least` key tiles.
 GV_HD int attn_parts(long long work, int parts, int least) {
-  const long long useful = (work + least - 1) / least;
-  return useful < parts ? static_cast<int>(useful) : parts;
+  return work < static_cast<long long>(parts) * least ? static_cast<int>(work + least - 1) / least : parts;
 }
-GV_HD long long attn_part_begin(long long work, int parts, int part) { return work * part / parts; }
+// (Divisions in 32 bits where they do, up to 1023 parts of fewer than 2^22 key tiles: in 64 they are a hundred instructions.)
+GV_HD long long attn_part_begin(long long work, int parts, int part) {
+  if (work < (1ll << 22) && parts < 1024) return static_cast<unsigned>(work) * static_cast<unsigned>(part) / static_cast<unsigned>(parts);
+  return work * part / parts;
+}
+GV_HD int attn_quotient(long long a, long long b) {
+  if (a < (1ll << 32) && b < (1ll << 32)) return static_cast<int>(static_cast<unsigned>(a) / static_cast<unsigned>(b));
+  return static_cast<int>(a / b);
+}
 
 }  // namespace gv
