@@ -1,4 +1,4 @@
-"""B200-native NVFP4 mixture-of-experts path of Gemma-4 26B-A4B.
+"""B200-native NVFP4 mixture-of-experts path of Gemma-4 26B-A4B, and the attention in front of it.
 
 Python mirror of the reference's operator interface for this path
 (``gevva::Nvfp4ExpertRunner``, include/gevva/gpu.hpp:217-247, and the inline
@@ -7,6 +7,16 @@ router launch ``route_128_top8_kernel``) on top of the C ABI in
 computation happens in ``libgevva_moe.so``.  There is no CPU fallback: loading
 fails loudly when the library has not been built.
 """
+from .attention import (  # noqa: F401
+    AttentionLayer,
+    KvCache,
+    PagedBatch,
+    block_norm,
+    block_norm_add,
+    chunk_attention,
+    kv_append,
+    prompt_attention,
+)
 from .runtime import (  # noqa: F401
     ExpertWeights,
     GevvaMoeError,
@@ -18,6 +28,14 @@ from .runtime import (  # noqa: F401
 )
 
 __all__ = [
+    "AttentionLayer",
+    "KvCache",
+    "PagedBatch",
+    "block_norm",
+    "block_norm_add",
+    "chunk_attention",
+    "kv_append",
+    "prompt_attention",
     "ExpertWeights",
     "GevvaMoeError",
     "Nvfp4ExpertRunner",

@@ -242,3 +242,39 @@ def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
 
     _status(_enqueue(launch, device, stream), "chunk_attention")
     return out
+
+
+@dataclass
+class AttentionLayer:
+    """The attention half of one decoder layer, in front of a FeedForwardLayer (the wiring of
+    src/cuda/runtime/prefill.cuh:924-1199): norm, projection, per-head norms with rotation and append, attention, output projection,
+    and the norm behind it with the residual.  The two projections are plain products of a library (torch.mm)."""
+    pre: torch.Tensor            # bf16 [hidden] norm in front
+    post: torch.Tensor           # bf16 [hidden] norm behind
+    qkv_w: torch.Tensor          # bf16 [(heads + 2 * kv_heads) * dim, hidden]: queries, keys, values
+    out_w: torch.Tensor          # bf16 [hidden, heads * dim]
+    q_norm: torch.Tensor         # bf16 [dim], or None
+    k_norm: torch.Tensor
+    frequencies: torch.Tensor    # f64 [pairs that turn]
+    cache: KvCache
+    heads: int
+    scale: float
+    window: int = 0              # 0: the whole context
+    normalize_v: bool = True
+    eps: float = 1e-6
+
+    def forward(self, hidden, batch, prompt=False):
+        """The layer's output, a new tensor [tokens, hidden]; appends the tokens' keys and values to the cache.  With `prompt` every
+        sequence is new, a whole prompt of its own, and attention reads the packed keys; otherwise it reads the pages.  Every row of `hidden`
+        is a token of a sequence."""
+        tokens, kv_heads, dim = hidden.shape[0], self.cache.kv_heads, self.cache.head_dim
+        x = block_norm(hidden, self.pre, self.eps)
+        qkv = torch.mm(x, self.qkv_w.t()).view(tokens, self.heads + 2 * kv_heads, dim)
+        q, k, v = qkv.split((self.heads, kv_heads, kv_heads), 1)
+        got = kv_append(q, k, v, self.cache, batch, self.frequencies, self.q_norm, self.k_norm, self.normalize_v, self.eps, packed=prompt)
+        if prompt:
+            seen = prompt_attention(got.q, got.k, got.v, batch.token_offsets, self.scale, self.window, status=self.cache.status)
+        else:
+            seen = chunk_attention(got, self.cache, batch, self.scale, self.window)
+        y = torch.mm(seen.view(tokens, self.heads * dim), self.out_w.t())
+        return block_norm_add(y, self.post, hidden, eps=self.eps)

@@ -10,6 +10,7 @@ w13 rows are [up; gate], block scales are interleaved per expert, and one alpha
 per expert per GEMM is input_scale * weight_global.
 """
 import math
+from dataclasses import dataclass
 
 import torch
 
@@ -142,13 +143,28 @@ class SyntheticLayer:
         return out
 
 
+@dataclass
+class SyntheticAttention:
+    """Shape of the attention in a SyntheticStack: every `whole_every`-th layer sees the whole context, the others the last
+    `window` positions (1024 in 25 of 30 layers, src/runtime.cpp:358-368).  Heads are generic."""
+    heads: int = 16
+    kv_heads: int = 8
+    head_dim: int = 256
+    window: int = 1024
+    whole_every: int = 6
+    theta: float = 1e4
+    pages: int = 64
+    page_size: int = 64
+
+
 class SyntheticStack:
     """Random-init FFN stack in the shape of Gemma-4 26B-A4B with attention replaced by
     identity: per layer the MoE above plus a dense FP8 GeGLU MLP of width 2112 (weights
     ~N(0, 0.02), per-tensor scale amax/448), norm weights 1, layer scalar 1.  With
-    `distinct_experts=False` every layer shares one packed expert set (tests)."""
+    `distinct_experts=False` every layer shares one packed expert set (tests).  With `attention` (a SyntheticAttention)
+    every layer has an attention half in front, with weights and a cache of its own, and `forward` takes the batch."""
 
-    def __init__(self, layers, max_tokens, device="cuda:0", seed=0, distinct_experts=True, s1=None, s2=None):
+    def __init__(self, layers, max_tokens, device="cuda:0", seed=0, distinct_experts=True, s1=None, s2=None, attention=None):
         from .feedforward import DENSE, DenseMlp, FeedForwardLayer, pack_fp8
         self.device = torch.device(device)
         gen = torch.Generator(device=self.device)
@@ -180,9 +196,29 @@ class SyntheticStack:
                 layer_scalar=torch.ones(1, dtype=torch.bfloat16, device=self.device),
                 experts=base.runner, dense=dense))
             self._keep = getattr(self, "_keep", []) + [base]
+        self.attention = [self._attention_layer(index, attention, seed) for index in range(layers)] if attention else None
         self.aux = torch.cuda.Stream(device=self.device)
 
-    def forward(self, hidden, concurrent=True):
-        for layer in self.layers:
+    def _attention_layer(self, index, shape, seed):
+        from .attention import AttentionLayer, KvCache
+        gen = torch.Generator(device=self.device)
+        gen.manual_seed(seed * 31 + index + 99)
+        rows, half = (shape.heads + 2 * shape.kv_heads) * shape.head_dim, shape.head_dim // 2
+        ones = torch.ones(HIDDEN, dtype=torch.bfloat16, device=self.device)
+        head_ones = torch.ones(shape.head_dim, dtype=torch.bfloat16, device=self.device)
+        return AttentionLayer(
+            pre=ones, post=ones, qkv_w=_randn((rows, HIDDEN), 0.02, gen, self.device).to(torch.bfloat16),
+            out_w=_randn((HIDDEN, shape.heads * shape.head_dim), 0.02, gen, self.device).to(torch.bfloat16), q_norm=head_ones,
+            k_norm=head_ones, frequencies=shape.theta ** (-torch.arange(half, dtype=torch.float64, device=self.device) / half),
+            cache=KvCache.empty(shape.pages, shape.page_size, shape.kv_heads, shape.head_dim, self.device), heads=shape.heads,
+            scale=shape.head_dim ** -0.5, window=0 if (index + 1) % shape.whole_every == 0 else shape.window)
+
+    def forward(self, hidden, concurrent=True, batch=None, prompt=False):
+        """`batch` (an attention.PagedBatch) and `prompt` (every sequence is a whole prompt) go with a stack that has attention."""
+        if (batch is not None) != (self.attention is not None):
+            raise ValueError("a stack with attention takes a batch, one without takes none")
+        for index, layer in enumerate(self.layers):
+            if self.attention is not None:
+                hidden = self.attention[index].forward(hidden, batch, prompt)
             hidden = layer.forward(hidden, self.aux if concurrent else None)
         return hidden

@@ -391,3 +391,45 @@ def test_nothing_to_do(attn, cuda_device):
     assert attn.chunk_attention(x, cache, batch, 1.0).shape == (0, 2, 64)
     assert attn.kv_append(x, x, x, cache, batch, None).shape == (0, 2, 64)
     assert attn.block_norm(torch.empty((0, 64), dtype=torch.bfloat16, device=cuda_device), torch.ones(64, dtype=torch.bfloat16, device=cuda_device)).shape == (0, 64)
+
+
+def test_layers_of_a_stack(attn, cuda_device):
+    """A stack with attention: prompts, then a chunk and single tokens over the same cache.  Each layer's call is the sequence of its parts, and
+    both forms of attention see the same context."""
+    from gevva_b200.synthetic import SyntheticAttention, SyntheticStack
+    shape = SyntheticAttention(heads=4, kv_heads=2, head_dim=256, window=100, whole_every=2, pages=40, page_size=16)
+    stack = SyntheticStack(2, 512, cuda_device, distinct_experts=False, attention=shape)
+    assert [a.window for a in stack.attention] == [100, 0]
+    news = [130, 7]
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(2, 20).to(cuda_device)
+
+    def batch_of(news, lengths):
+        return attn.PagedBatch(offsets_of(news, cuda_device), torch.tensor(lengths, dtype=torch.int32, device=cuda_device), table)
+
+    hidden = randn((sum(news), 2816), cuda_device, 5)
+    with pytest.raises(ValueError, match="batch"):
+        stack.forward(hidden)
+    out = stack.forward(hidden, batch=batch_of(news, news), prompt=True)
+    assert torch.isfinite(out).all()
+    # the parts of the first layer, one by one; its cache holds these tokens
+    layer, batch = stack.attention[0], batch_of(news, news)
+    x = attn.block_norm(hidden, layer.pre)
+    qkv = torch.mm(x, layer.qkv_w.t()).view(-1, 8, 256)
+    q, k, v = attn.kv_append(qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], layer.cache, batch, layer.frequencies, layer.q_norm, layer.k_norm, True, packed=True)
+    seen = attn.prompt_attention(q, k, v, batch.token_offsets, layer.scale, 100)
+    paged = attn.chunk_attention(q, layer.cache, batch, layer.scale, 100)
+    at = 0
+    for n in news:
+        want, bound = ref.attention(q[at:at + n], k[at:at + n], v[at:at + n], 0, layer.scale, 100)
+        ref.within(seen[at:at + n], want, bound)
+        ref.within(paged[at:at + n], want, bound)
+        at += n
+    y = attn.block_norm_add(torch.mm(seen.view(-1, 1024), layer.out_w.t()), layer.post, hidden)
+    assert torch.equal(y, layer.forward(hidden, batch, prompt=True))
+    # a chunk, then tokens one by one
+    for news, lengths in (([5, 3], [135, 10]), ([1, 1], [136, 11]), ([1, 1], [137, 12])):
+        out = stack.forward(randn((sum(news), 2816), cuda_device, lengths[0]), batch=batch_of(news, lengths))
+        assert torch.isfinite(out).all()
+    for a, f in zip(stack.attention, stack.layers):
+        a.cache.check()
+        f.experts.check()
