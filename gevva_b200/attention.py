@@ -9,7 +9,7 @@ import torch
 from .runtime import GevvaMoeError, _address, _enqueue, library
 
 HEAD_DIMS = (64, 128, 256, 512)
-_empty = torch.empty
+_empty, _empty_like, _contiguous = torch.empty, torch.empty_like, torch.contiguous_format  # (empty_like: half the host's time of empty)
 
 
 class _Cache(ctypes.Structure):
@@ -73,10 +73,11 @@ def _queries(q):
     return device, q.shape, _heads(q, "q", device, q.shape)
 
 
-def _out(out, like_shape, device, name="out"):
+def _out(out, like, device, name="out"):
+    """`out`, or a contiguous tensor of the shape and type of `like`."""
     if out is None:
-        return _empty(like_shape, dtype=torch.bfloat16, device=device)
-    _at(out, torch.bfloat16, like_shape, device, name)
+        return _empty_like(like, memory_format=_contiguous)
+    _at(out, torch.bfloat16, like.shape, device, name)
     return out
 
 
@@ -90,7 +91,7 @@ def block_norm(x, weight, eps=1e-6, out=None, stream=None):
     """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768."""
     device, shape = _rows(x)
     rows, width = shape
-    out = _out(out, shape, device)
+    out = _out(out, x, device)
     _status(_enqueue(_lib().gevva_attn_norm, device, stream, x.data_ptr(), _at(weight, torch.bfloat16, (width,), device, "weight"),
                      out.data_ptr(), rows, width, eps), "block_norm")
     return out
@@ -103,9 +104,9 @@ def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None,
     rows, width = shape
     bf16 = torch.bfloat16
     following = None
-    out = _out(out, shape, device)
+    out = _out(out, x, device)
     if next_weight is not None:
-        following = _empty(shape, dtype=bf16, device=device)
+        following = _empty_like(x)
     _status(_enqueue(_lib().gevva_attn_norm_add, device, stream, x.data_ptr(), _at(weight, bf16, (width,), device, "weight"),
                      _at(residual, bf16, shape, device, "residual"), _at(gate, bf16, (width,), device, "gate"),
                      _at(scale, bf16, (1,), device, "scale"), _at(next_weight, bf16, (width,), device, "next_weight"), out.data_ptr(),
@@ -195,8 +196,8 @@ def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, 
         raise ValueError(f"kv_append: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
     k_rows, v_rows = _heads(k, "k", device, (tokens, kv_heads, dim)), _heads(v, "v", device, (tokens, kv_heads, dim))
     rotated = 0 if frequencies is None else 2 * frequencies.numel()
-    out = _out(out, shape, device)
-    k_out, v_out = (_empty(k.shape, dtype=torch.bfloat16, device=device) for _ in range(2)) if packed else (None, None)
+    out = _out(out, q, device)
+    k_out, v_out = (_out(None, k, device), _out(None, v, device)) if packed else (None, None)
     _status(_enqueue(_lib().gevva_attn_append, device, stream, *q_rows, *k_rows, *v_rows, cache._address, batch._address, tokens, heads, kv_heads,
                      dim, frequencies if frequencies is None else _at(frequencies, torch.float64, frequencies.shape, device, "frequencies"), rotated,
                      _at(q_weight, torch.bfloat16, (dim,), device, "q_weight"), _at(k_weight, torch.bfloat16, (dim,), device, "k_weight"), normalize_v, eps, out.data_ptr(),
@@ -215,7 +216,7 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
     kv_heads = k.shape[1]
     k_rows, v_rows = (_heads(x, name, device, (tokens, kv_heads, dim)) for x, name in ((k, "k"), (v, "v")))
     sequences = token_offsets.numel() - 1
-    out = _out(out, shape, device)
+    out = _out(out, q, device)
     _status(_enqueue(_lib().gevva_attn_prompt, device, stream, *q_rows, *k_rows, *v_rows, _at(token_offsets, torch.int32, (sequences + 1,), device, "token_offsets"), sequences,
                      tokens, heads, kv_heads, dim, scale, window, out.data_ptr(), _at(status, torch.int32, (1,), device, "status")), "prompt_attention")
     return out
@@ -230,7 +231,7 @@ def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
     if cache.head_dim != dim or cache.device != device or batch.device != device:
         raise ValueError(f"chunk_attention: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
     lib = _lib()
-    out = _out(out, shape, device)
+    out = _out(out, q, device)
 
     def launch(*args):
         # (the workspace's size goes by the device, which is the current one in here)
