@@ -153,6 +153,12 @@ __device__ __forceinline__ void tmem_store_32x32(uint32_t tmem_address, const ui
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// 32 bytes, to an address that is a multiple of that.
+__device__ __forceinline__ void store_32(void* to, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
+}
 // D (+)= A B^T, bf16 operands, fp32 sums, K = 16; A from shared memory or from tensor memory.
 __device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
@@ -942,27 +948,47 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         __nv_bfloat16* out = p.out + static_cast<long long>(piece.query0 + token) * p.out_token_stride +
                              static_cast<long long>(piece.kv_head * p.group + row_head) * p.out_head_stride + column0;
         const size_t partial_row = (static_cast<size_t>(piece.slot < 0 ? 0 : piece.slot) * kTiles + tile_of_rows) * kRows + row;
-#pragma unroll 1
-        for (int i = 0; i < S::kValueDim; i += 32) {
-          uint32_t o[32];
-          tmem_load_32x32(outputs + i, o);
-          tmem_load_wait(o);
-          if (valid && piece.slot < 0) {
+        // A store of a row per lane keeps the store unit busy for 32 lines whatever it stores.  So lanes work in pairs: each has 64 bytes of a row, and they
+        // store first the one's, then the other's, 32 bytes each.
+        const bool odd = lane & 1;
+        __nv_bfloat16* other_out = reinterpret_cast<__nv_bfloat16*>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 1));
+        const bool other_valid = __shfl_xor_sync(0xffffffffu, valid ? 1 : 0, 1) != 0;
+        __nv_bfloat16* const first_out = odd ? other_out + 16 : out;
+        __nv_bfloat16* const second_out = odd ? out + 16 : other_out;
+        const bool first_valid = odd ? other_valid : valid, second_valid = odd ? valid : other_valid;
+        const auto finish = [&](const uint32_t (&o)[32], int i) {
+          if (piece.slot < 0) {
+            uint32_t mine[16], theirs[8];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) mine[k] = pack_bf16x2(__uint_as_float(o[2 * k]) * inverse, __uint_as_float(o[2 * k + 1]) * inverse);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) theirs[k] = __shfl_xor_sync(0xffffffffu, odd ? mine[k] : mine[8 + k], 1);
+            uint32_t first[8], second[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              first[k] = odd ? theirs[k] : mine[k];
+              second[k] = odd ? mine[8 + k] : theirs[k];
+            }
+            if (first_valid) store_32(first_out + i, first);
+            if (second_valid) store_32(second_out + i, second);
+          } else if (valid) {
+            float* to = p.partial + partial_row * S::kValueDim + i;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              uint4 v;
-              v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inverse, __uint_as_float(o[8 * k + 1]) * inverse);
-              v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inverse, __uint_as_float(o[8 * k + 3]) * inverse);
-              v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inverse, __uint_as_float(o[8 * k + 5]) * inverse);
-              v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inverse, __uint_as_float(o[8 * k + 7]) * inverse);
-              *reinterpret_cast<uint4*>(out + i + 8 * k) = v;
+              const uint32_t v[8] = {o[8 * k], o[8 * k + 1], o[8 * k + 2], o[8 * k + 3], o[8 * k + 4], o[8 * k + 5], o[8 * k + 6], o[8 * k + 7]};
+              store_32(to + 8 * k, v);
             }
-          } else if (valid) {
-            uint4* to = reinterpret_cast<uint4*>(p.partial + partial_row * S::kValueDim + i);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
           __syncwarp();
+        };
+#pragma unroll 1
+        for (int i = 0; i < S::kValueDim; i += 64) {
+          uint32_t o0[32], o1[32];
+          tmem_load_32x32(outputs + i, o0);
+          tmem_load_32x32(outputs + i + 32, o1);
+          tmem_load_wait(o0, o1);
+          finish(o0, i);
+          finish(o1, i + 32);
         }
         if (valid && piece.slot >= 0) {
           float2* stats = reinterpret_cast<float2*>(p.partial_stats) + partial_row;

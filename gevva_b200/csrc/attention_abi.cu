@@ -14,6 +14,8 @@ constexpr int kMaxGroup = 128;
 bool aligned(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned_or_null(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// (attention stores 32 bytes at a time)
+bool aligned_32(const void* p, int rows) { return (rows == 0 || p) && (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 // Rows of a call without any may be nowhere.
 bool aligned_for(const void* p, int rows) { return rows > 0 ? aligned(p) : aligned_or_null(p); }
 
@@ -141,7 +143,7 @@ int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_
   gv::AttnCall call{};
   if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !rows_ok(&call.k, k, k_token_stride, k_head_stride, tokens, kv_heads, dim) ||
       !rows_ok(&call.v, v, v_token_stride, v_head_stride, tokens, kv_heads, dim) || !token_offsets || sequences < 1 || tokens > kMaxPositions || !attention_ok(scale, window) ||
-      !aligned_for(out, tokens))
+      !aligned_32(out, tokens))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (tokens == 0) return GEVVA_MOE_OK;
   call.token_offsets = token_offsets;
@@ -170,7 +172,7 @@ int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_s
                      gevva_stream_t stream) {
   gv::AttnCall call{};
   if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) ||
-      tokens > kMaxPositions || !attention_ok(scale, window) || !aligned_for(out, tokens) || !aligned(workspace))
+      tokens > kMaxPositions || !attention_ok(scale, window) || !aligned_32(out, tokens) || !workspace || !aligned_32(workspace, 1))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (tokens == 0) return GEVVA_MOE_OK;
   call.paged = true;

@@ -366,7 +366,8 @@ int gevva_ff_layer_launch(const gevva_ff_layer* layer, const void* hidden, void*
  * queries and keys with the append to the cache (src/cuda/kernels/qkv_transform.cuh), and causal attention.  The projections
  * between them are the caller's.  Tensors are bf16; heads have 64, 128, 256 or 512 values; query head h reads key head
  * h / (heads / kv_heads), where kv_heads divides heads and a key head has at most 128 query heads.  Sums, norms and softmax statistics
- * are held in 32 bits, rotation angles in 64.  All pointers are 16-byte aligned, strides are in elements, positive and multiples of 8.
+ * are held in 32 bits, rotation angles in 64.  All pointers are 16-byte aligned (32-byte: `out` and `workspace` of the two
+ * attention calls), strides are in elements, positive and multiples of 8.
  * Queries, keys and values are [tokens, heads, dim] with the last dimension contiguous, given as an address and two strides (of a token and
  * of a head): views of a fused projection's rows, for instance.  The calls keep no state; `device_status` is an optional device status word that receives
  * GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do. */
