@@ -553,9 +553,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
+    if (elect_one()) {
     // The tensor pipe holds few instructions ahead, so what lies between two batches of products is time that it stands still: one wait for all that a
     // batch needs (a lane for each barrier), and few, wide products.
-    const bool leader = elect_one();
     const uint64_t q_desc = make_smem_desc(smem_u32(smem->queries[0]), 1024, 2);
     const uint64_t k_desc = make_smem_desc(smem_u32(smem->stage[0]), 1024, 2);
     // values: 64 columns a swizzle row, the next 64 a column block further (leading offset), keys eight rows a group (stride offset)
@@ -570,21 +570,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         phase ^= 1u;
       }
     };
-    // Waits until the next `count` stages are there, and `other`'s phase is over (lanes from 16 on; null: nothing else).
+    // Waits until the next `count` stages are there, and `other`'s phase is over (null: nothing else); all are looked at before any is waited for.
     const auto ready = [&](uint32_t count, uint64_t* other, uint32_t other_parity) {
-      uint32_t s = stage + min(static_cast<uint32_t>(lane & 15), count - 1), parity = phase;
-      if (s >= S::kStages) {
-        s -= S::kStages;
-        parity ^= 1u;
-      }
-      uint64_t* bar = &smem->full[s];
-      if (lane >= 16 && other) {
-        bar = other;
-        parity = other_parity;
-      }
-      return __all_sync(0xffffffffu, wait_or_abort(bar, parity, smem, p.status));
+      const uint32_t behind = stage + 1 == S::kStages ? 0 : stage + 1, behind_phase = stage + 1 == S::kStages ? phase ^ 1u : phase;
+      const bool first = mbar_try_wait(&smem->full[stage], phase);
+      const bool second = count < 2 || mbar_try_wait(&smem->full[behind], behind_phase);
+      const bool third = !other || mbar_try_wait(other, other_parity);
+      if (first && second && third) return true;
+      return wait_or_abort(&smem->full[stage], phase, smem, p.status) && (count < 2 || wait_or_abort(&smem->full[behind], behind_phase, smem, p.status)) &&
+             (!other || wait_or_abort(other, other_parity, smem, p.status));
     };
-    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_or_abort(bar, parity, smem, p.status)); };
+    const auto wait_for = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, smem, p.status); };
     // The products of one stage: 128 (64) of the columns that scores sum over; or of the outputs' columns, of one stage or of two that lie side by side.
     const auto scores_of_stage = [&](uint32_t d, int tile, int part) {
       const uint64_t b = k_desc + stage * (S::kStageBytes >> 4);
@@ -620,7 +616,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (!ok) break;
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
-              if (leader) {
+              {
                 scores_of_stage(tmem_base + (n & 1u) * kKeys, 0, i + k);
                 tc_commit(&smem->empty[stage]);
                 if (i + k + 1 == S::kKeyStages) {
@@ -628,7 +624,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                   if (last) tc_commit(&smem->q_empty);
                 }
               }
-              __syncwarp();
               skip_stages(1);
             }
           }
@@ -642,7 +637,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (ok && !seen_keys(piece, j, p.window).all()) {
             // the softmax warps clear rows of these values before they say that P is there
             ok = ready(S::kValueStages, nullptr, 0);
-            if (ok && lane == 0) mbar_arrive(&smem->v_landed[n & 1u]);
+            if (ok) mbar_arrive(&smem->v_landed[n & 1u]);
           }
           if (S::kAhead && ok && j + 1 == tiles) {
             // While the last softmax runs: the first scores of the next piece, if its operands are there before P is.
@@ -651,23 +646,25 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const uint32_t next_parity = ((count + 1) / kPieceSlots) & 1u;
             const long long start = clock64();
             skip_stages(S::kValueStages);
-            while (!scored && !__all_sync(0xffffffffu, mbar_try_wait(&smem->p_ready[n & 1u], (n >> 1) & 1u))) {
-              bool there = mbar_try_wait(&smem->piece_full[next_slot], next_parity);
-              if (there) there = smem->pieces[next_slot].tiles > 0 && mbar_try_wait(&smem->q_full, (count + 1) & 1u);
-              if (there) {
-                uint32_t s = stage + min(lane, S::kKeyStages - 1), parity = phase;
-                if (s >= S::kStages) {
-                  s -= S::kStages;
-                  parity ^= 1u;
+            while (!scored && !mbar_try_wait(&smem->p_ready[n & 1u], (n >> 1) & 1u)) {
+              if (mbar_try_wait(&smem->piece_full[next_slot], next_parity) && smem->pieces[next_slot].tiles > 0 &&
+                  mbar_try_wait(&smem->q_full, (count + 1) & 1u)) {
+                bool there = true;
+                uint32_t s = stage, parity = phase;
+                for (int i = 0; i < S::kKeyStages; ++i) {
+                  there = there && mbar_try_wait(&smem->full[s], parity);
+                  if (++s == S::kStages) {
+                    s = 0;
+                    parity ^= 1u;
+                  }
                 }
-                there = mbar_try_wait(&smem->full[s], parity);
-              }
-              if (__all_sync(0xffffffffu, there)) {
-                scores(n + 1, __all_sync(0xffffffffu, smem->pieces[next_slot].tiles == 1));
-                scored = true;
+                if (there) {
+                  scores(n + 1, smem->pieces[next_slot].tiles == 1);
+                  scored = true;
+                }
               }
               // (the wait below says that P does not come; this loop only has to end)
-              if (__any_sync(0xffffffffu, smem->abort || clock64() - start > kWaitLimitCycles)) break;
+              if (smem->abort || clock64() - start > kWaitLimitCycles) break;
             }
             stage = value_stage;
             phase = value_phase;
@@ -678,25 +675,23 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc_fence_after_sync();
           const uint32_t weights = tmem_base + (n & 1u) * kKeys, accumulate = j > 0 ? 1u : 0u;
           if (kBatch == 2 && stage + 1 < S::kStages) {
-            if (leader) {
+            {
               values_of_stage(tmem_base + 256, stage, weights, accumulate, kIdescValues<2 * S::kStageDim>);
               tc_commit(&smem->empty[stage]);
               tc_commit(&smem->empty[stage + 1]);
               tc_commit(&smem->pv_done[n & 1u]);
             }
-            __syncwarp();
             skip_stages(2);
           } else {
 #pragma unroll
             for (int i = 0; i < S::kValueStages; ++i) {
               if (i >= kBatch) ok = ok && ready(1, nullptr, 0);
               if (!ok) break;
-              if (leader) {
+              {
                 values_of_stage(tmem_base + 256 + i * S::kStageDim, stage, weights, accumulate, kIdescValues<S::kStageDim>);
                 tc_commit(&smem->empty[stage]);
                 if (i + 1 == S::kValueStages) tc_commit(&smem->pv_done[n & 1u]);
               }
-              __syncwarp();
               skip_stages(1);
             }
             if (!ok) break;
@@ -707,7 +702,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // one stage holds a tile's keys, another its values
         ok = ready(1, nullptr, 0);
         if (!ok) break;
-        if (leader) {
+        {
 #pragma unroll
           for (int t = 0; t < kTiles; ++t) {
             scores_of_stage(tmem_base + t * kKeys, t, 0);
@@ -715,7 +710,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
           tc_commit(&smem->empty[stage]);
         }
-        __syncwarp();
         skip_stages(1);
         for (int j = 0; ok && j < tiles; ++j) {
           const uint32_t n = done + j;
@@ -724,7 +718,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (j == 0) ok = wait_for(&smem->o_free[0], (count & 1u) ^ 1u) && wait_for(&smem->o_free[1], (count & 1u) ^ 1u);
           if (ok && !seen_keys(piece, j, p.window).all()) {
             ok = ready(1, nullptr, 0);
-            if (ok && lane == 0) mbar_arrive(&smem->v_landed[0]);
+            if (ok) mbar_arrive(&smem->v_landed[0]);
           }
           // P of the first tile, the values and the next keys; then P of the second
           ok = ok && ready(more ? 2 : 1, &smem->p_ready[0], n & 1u);
@@ -732,7 +726,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           tc_fence_after_sync();
           const uint32_t value_stage = stage;
           skip_stages(1);
-          if (leader) {
+          {
             values_of_stage(tmem_base + 256, value_stage, tmem_base, accumulate, kIdescValues<S::kStageDim>);
             tc_commit(&smem->pv_done[0]);
             if (more) {
@@ -740,11 +734,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               tc_commit(&smem->acc_full[0]);
             }
           }
-          __syncwarp();
           ok = wait_for(&smem->p_ready[1], n & 1u);
           if (!ok) break;
           tc_fence_after_sync();
-          if (leader) {
+          {
             values_of_stage(tmem_base + 256 + kDim, value_stage, tmem_base + kKeys, accumulate, kIdescValues<S::kStageDim>);
             tc_commit(&smem->pv_done[1]);
             tc_commit(&smem->empty[value_stage]);
@@ -756,14 +749,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               tc_commit(&smem->q_empty);
             }
           }
-          __syncwarp();
           if (more) skip_stages(1);
         }
       }
       done += tiles;
-      if (ok && lane == 0) mbar_arrive(&smem->piece_empty[slot]);
-      __syncwarp();
+      if (ok) mbar_arrive(&smem->piece_empty[slot]);
     }
+    }
+    __syncwarp();
   }
   } else {
     // ---------------- softmax and epilogue ----------------
