@@ -11,17 +11,24 @@
 // once for all of them, with one token as with many.  Scores and outputs are products of the tensor pipe (tcgen05.mma, M = 128): S = Q K^T with both operands
 // in shared memory, O += P V with P in tensor memory, where the softmax threads leave it over the scores it came from.
 //   warp 0    fetches Q, K and V by TMA, a page's slots at a time where the keys are paged
-//   warp 1    issues the MMAs
+//   warp 1    issues the products, by one thread: the tensor pipe holds few of them ahead, so an issuer's votes and branches are time that it
+//             stands still (heads of 512: 1190 -> 1068 us; with a second issuer for the outputs 1295, since the two kinds of product then alternate)
 //   warp 2    works out the pieces of work, a step ahead of the others
-//   warps 4+  softmax and epilogue, a row per thread
-// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile, whose
-// scores for the next keys are computed while the softmax of these runs; a key tile takes the tensor pipe 2048 cycles and the exponentials 1024.
-// Heads of 64 and 128: two query tiles in turn, each with a softmax warpgroup of its own, since there both take as long.
+//   warps 4+  softmax and epilogue, a row per thread, by two warpgroups
+// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile. Its key tiles are
+// taken by the warpgroups in turn, and the scores of the next are worked out while the softmax of this one runs, over the end of a piece too; a key
+// tile takes the tensor pipe 2048 cycles, and half as much again for 512, whose scores both items work out.
+// Heads of 64 and 128: two query tiles, a warpgroup each, since there a tile's exponentials take as long as its products or longer.
 //
-// Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the items
-// longest first within a sequence, further ones by cancelling launches that have not started (clusterlaunchcontrol).  Chunks: a CTA takes an equal run of key tiles, whatever
-// the sequences' lengths, which only the device knows; an item that a run's end cuts leaves sums in the workspace, and
-// attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
+// Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the items, a sequence's
+// last and longest first, further ones by cancelling launches that have not started (clusterlaunchcontrol).  Chunks: a CTA takes an equal
+// run of key tiles, whatever the sequences' lengths, which only the device knows; an item that a run's end cuts leaves sums in the
+// workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
+//
+// What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: the pace at which products are issued beside the softmax warps, some 80 to 95 cycles
+// one instead of the tensor pipe's 64: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128 1216, 32 of 64 718 (exponentials), 16 of 512 1050 (1575 with the
+// scores that are worked out twice).  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
+// latencies, 15 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -39,7 +46,8 @@ constexpr int kKeys = kAttnKeys;   // keys of a key tile
 constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, and one whose operands are fetched
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
 constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
-constexpr int kLeastRun = 1;    // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256: 16.0 us, with 2 16.4, with 4 20.8)
+constexpr int kLeastRun = 1;       // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256: 16.0 us,
+                                   // with 2 16.4, with 4 20.8)
 
 // One run of key tiles of one item.
 struct Piece {
@@ -289,7 +297,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (first + lane < p.sequences) {
           lane_from = max(p.token_offsets[first + lane], 0);
           lane_news = max(min(p.token_offsets[first + lane + 1], p.tokens) - lane_from, 0);
-          lane_length = min(max(p.lengths[first + lane], 0), capacity);
+          const int length = p.lengths[first + lane];
+          if (length > capacity && blockIdx.x == 0 && p.status) atomicExch(p.status, static_cast<int>(kBadPage));
+          lane_length = min(max(length, 0), capacity);
         }
       };
       const auto upto_lane = [&] {  // work of the loaded sequences up to the lane's
@@ -1173,9 +1183,8 @@ cudaError_t launch_shape(const AttnCall& call, cudaStream_t stream) {
   } else {
     const uint64_t dims[4] = {kDim, static_cast<uint64_t>(call.tokens), static_cast<uint64_t>(call.kv_heads), 1};
     const uint32_t box[4] = {64, kKeys, 1, 1};
-    const long long whole = call.k.token_stride * call.tokens, whole_v = call.v.token_stride * call.tokens;
-    const long long key_strides[3] = {call.k.token_stride, call.k.head_stride, whole};
-    const long long value_strides[3] = {call.v.token_stride, call.v.head_stride, whole_v};
+    const long long key_strides[3] = {call.k.token_stride, call.k.head_stride, kDim};  // (the last is of one page that there is)
+    const long long value_strides[3] = {call.v.token_stride, call.v.head_stride, kDim};
     if (!make_map(&map_k, call.k.data, 4, dims, key_strides, box) || !make_map(&map_v, call.v.data, 4, dims, value_strides, box))
       return cudaErrorInvalidValue;
     // as many query tiles as sequences of any lengths can have

@@ -59,7 +59,7 @@ int launched(cudaError_t e) {
   return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
 }
 
-bool attention_ok(float scale, int window) { return scale > 0.0f && isfinite(scale) && window >= 0; }
+bool attention_ok(float scale, int window) { return scale > 0.0f && scale <= 1e30f && window >= 0; }
 
 }  // namespace
 

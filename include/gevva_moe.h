@@ -419,7 +419,7 @@ int gevva_attn_append(const void* q, long long q_token_stride, long long q_head_
                       gevva_stream_t stream);
 
 /* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
- * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  scale > 0.  No row sees another sequence's keys,
+ * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  0 < scale <= 1e30.  No row sees another sequence's keys,
  * whatever their values are; within a sequence, keys and values that a row does not see have to be finite. */
 int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_stride,
                       const void* k, long long k_token_stride, long long k_head_stride,
@@ -431,7 +431,7 @@ int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_
 /* The same for new tokens over a paged cache that already holds their keys and values (gevva_attn_append): one token a sequence when
  * decoding, several in verification and chunked prefill.  Lengths are read on the device, so a captured call can be replayed with
  * others.  Row i of n sees the keys up to lengths[s] - n + i; a row that sees none is zero.  Slots that no row of a
- * sequence sees may hold anything.  `workspace` is device memory of gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed
+ * sequence sees may hold anything, others have to be finite.  A length beyond the table is cut to it and reported as GEVVA_MOE_BAD_PAGE.  `workspace` is device memory of gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed
  * the call; calls that may run at the same time need one each. */
 size_t gevva_attn_chunk_workspace_bytes(int dim);
 int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_stride,

@@ -55,10 +55,10 @@ PAGES = [dict(c=cache(keys=None)), dict(c=cache(values=A + 4)), dict(c=cache(pag
          dict(c=cache(key_slot_stride=100)), dict(c=cache(value_page_stride=0)), dict(c=cache(key_head_stride=-64)), dict(b=batch(token_offsets=None)),
          dict(b=batch(lengths=None)), dict(b=batch(table=None)), dict(b=batch(sequences=0)), dict(b=batch(table_width=0)), dict(b=batch(table_stride=2)),
          dict(b=batch(table_width=1 << 27, table_stride=1 << 27))]
-SOFTMAX = [dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(window=-1), dict(out=None), dict(out=A + 2)]
+SOFTMAX = [dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e31), dict(window=-1), dict(out=None), dict(out=A + 16)]
 
 
-@pytest.mark.parametrize("change", SHAPES + PAGES + SOFTMAX + [dict(workspace=None), dict(workspace=A + 8)])
+@pytest.mark.parametrize("change", SHAPES + PAGES + SOFTMAX + [dict(workspace=None), dict(workspace=A + 16)])
 def test_chunk(lib, change):
     assert chunk(lib, **change) == BAD
 

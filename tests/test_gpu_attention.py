@@ -155,6 +155,21 @@ def test_chunk_ignores_pages_in_front_of_the_window(attn, cuda_device):
     ref.within(attn.chunk_attention(q, cache, batch, 0.05, window=window), want, bound)
 
 
+def test_chunk_reports_lengths_beyond_the_table(attn, cuda_device):
+    from gevva_b200 import GevvaMoeError
+    cache = attn.KvCache(randn((4, 16, 1, 64), cuda_device, 1), randn((4, 16, 1, 64), cuda_device, 2))
+    batch = attn.PagedBatch(offsets_of([1, 1], cuda_device), torch.tensor([20, 33], dtype=torch.int32, device=cuda_device),
+                            torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=cuda_device))
+    q = randn((2, 1, 64), cuda_device, 3)
+    got = attn.chunk_attention(q, cache, batch, 0.125)
+    with pytest.raises(GevvaMoeError, match="page"):
+        cache.check()
+    k, v = gathered(cache, batch, 0, 20)
+    want, bound = ref.attention(q[:1], k, v, 19, 0.125, 0)
+    ref.within(got[:1], want, bound)
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (256, 16, 8), (512, 16, 2)])
 def test_chunk_repeats_its_bits_and_equals_the_prompt_form(attn, cuda_device, dim, heads, kv_heads):
     n, page = 900, 64
