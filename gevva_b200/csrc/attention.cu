@@ -43,7 +43,11 @@ namespace {
 
 constexpr int kRows = 128;         // rows of a query tile
 constexpr int kKeys = kAttnKeys;   // keys of a key tile
-constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, and one whose operands are fetched
+constexpr int kPieceSlots = 3;     // pieces in work at most: one whose outputs are read, one whose scores are, and one whose operands are fetched
+// Items that CTAs take from one another are better not taken far ahead (1500, 1, 2049 and 1058 tokens through a window of 1024: 67.7 -> 65.7 us), but with heads of
+// 64 the time to the next counts more (8192 tokens: 383 and 391 us).
+template <int kTiles, bool kPaged>
+constexpr uint32_t kSlotsOf = kPaged || kTiles == 2 ? kPieceSlots : 2;
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
 constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
 constexpr int kLeastRun = 1;       // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256: 16.0 us,
@@ -216,6 +220,7 @@ __global__ void __launch_bounds__(Shape<kDim, kTiles>::kThreads, 1)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
   using S = Shape<kDim, kTiles>;
+  constexpr uint32_t kSlots = kSlotsOf<kTiles, kPaged>;
   using Smem = AttnSmem<kDim, kTiles>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem* smem = reinterpret_cast<Smem*>(smem_raw);
@@ -235,7 +240,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&smem->pv_done[s], 1);
     }
     for (int t = 0; t < kTiles; ++t) mbar_init(&smem->o_free[t], 4);
-    for (int s = 0; s < kPieceSlots; ++s) {
+    for (uint32_t s = 0; s < kSlots; ++s) {
       mbar_init(&smem->piece_full[s], 1);
       mbar_init(&smem->piece_empty[s], 2 + S::kSoftmaxWarps);  // fetching warp, MMA warp, softmax warps
     }
@@ -274,12 +279,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     uint32_t count = 0;  // pieces handed out
     bool ok = true;
     const auto room = [&] {  // waits until the next piece's slot is free
-      return __all_sync(0xffffffffu, wait_or_abort(&smem->piece_empty[count % kPieceSlots], ((count / kPieceSlots) & 1u) ^ 1u, smem, p.status));
+      return __all_sync(0xffffffffu, wait_or_abort(&smem->piece_empty[count % kSlots], ((count / kSlots) & 1u) ^ 1u, smem, p.status));
     };
     const auto hand_out = [&](const Piece& piece) {
       if (lane == 0) {
-        smem->pieces[count % kPieceSlots] = piece;
-        mbar_arrive(&smem->piece_full[count % kPieceSlots]);
+        smem->pieces[count % kSlots] = piece;
+        mbar_arrive(&smem->piece_full[count % kSlots]);
       }
       __syncwarp();
       ++count;
@@ -495,8 +500,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int box = lane & (page_boxes - 1), column = lane / page_boxes;
     uint32_t q_issued = 0;
     for (uint32_t count = 0;; ++count) {
-      const int slot = count % kPieceSlots;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      const int slot = count % kSlots;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kSlots) & 1u, smem, p.status));
       if (!ok) break;
       const Piece piece = smem->pieces[slot];
       if (piece.tiles == 0) break;
@@ -625,8 +630,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     uint32_t done = 0;    // key tiles of the pieces before
     bool scored = false;  // the piece's first scores have been asked for at the end of the one before
     for (uint32_t count = 0; ok; ++count) {
-      const int slot = count % kPieceSlots;
-      ok = wait_for(&smem->piece_full[slot], (count / kPieceSlots) & 1u);
+      const int slot = count % kSlots;
+      ok = wait_for(&smem->piece_full[slot], (count / kSlots) & 1u);
       if (!ok) break;
       const Piece piece = smem->pieces[slot];
       const int tiles = piece.tiles;
@@ -669,8 +674,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (S::kAhead && ok && j + 1 == tiles) {
             // While the last softmax runs: the first scores of the next piece, if its operands are there before P is.
             const uint32_t value_stage = stage, value_phase = phase;
-            const int next_slot = (count + 1) % kPieceSlots;
-            const uint32_t next_parity = ((count + 1) / kPieceSlots) & 1u;
+            const int next_slot = (count + 1) % kSlots;
+            const uint32_t next_parity = ((count + 1) / kSlots) & 1u;
             const long long start = clock64();
             skip_stages(S::kValueStages);
             while (!scored && !mbar_try_wait(&smem->p_ready[n & 1u], (n >> 1) & 1u)) {
@@ -803,8 +808,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     uint32_t cleared = 0;         // tiles with values that this warpgroup has cleared
     bool ok = true;
     for (uint32_t count = 0; ok; ++count) {
-      const int slot = count % kPieceSlots;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kPieceSlots) & 1u, smem, p.status));
+      const int slot = count % kSlots;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->piece_full[slot], (count / kSlots) & 1u, smem, p.status));
       if (!ok) break;
       const Piece piece = smem->pieces[slot];
       if (piece.tiles == 0) break;
