@@ -307,11 +307,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           lane_length = min(max(length, 0), capacity);
         }
       };
-      const auto upto_lane = [&] {  // work of the loaded sequences up to the lane's
+      const auto upto_lane = [&] {  // key tiles of one head in the loaded sequences up to the lane's
         long long upto = 0;
         if (lane_news > 0) {
           const AttnSequence q = attn_sequence(lane_news, lane_length, step);
-          upto = heads * attn_tiles_before(q, q.query_tiles, step, p.window);
+          upto = attn_tiles_before(q, q.query_tiles, step, p.window);
         }
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
@@ -320,15 +320,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         return upto;
       };
-      long long work = 0, upto = 0;
+      long long of_head = 0, upto = 0;
       for (int first = 0; first < p.sequences; first += 32) {
         load_sequences(first);
         upto = upto_lane();
-        work += __shfl_sync(0xffffffffu, upto, 31);
+        of_head += __shfl_sync(0xffffffffu, upto, 31);
       }
-      const int parts = attn_parts(work, static_cast<int>(gridDim.x), kLeastRun);
+      // Head after head, each through all sequences: with as many runs for each head, the heads of a page are read at the same time.
+      const long long work = heads * of_head;
+      const int parts = attn_parts(work, static_cast<int>(gridDim.x), heads, kLeastRun);
       if (static_cast<int>(blockIdx.x) < parts) {
         const long long run_begin = attn_part_begin(work, parts, blockIdx.x), run_end = attn_part_begin(work, parts, blockIdx.x + 1);
+        int head = attn_quotient(run_begin, of_head);
+        const long long in_head = run_begin - head * of_head;
         long long at = run_begin, before = 0;
         int s = 0;
         for (;; s += 32) {
@@ -337,12 +341,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             upto = upto_lane();
           }
           const long long all = __shfl_sync(0xffffffffu, upto, 31);
-          if (before + all > run_begin) break;
+          if (before + all > in_head) break;
           before += all;
         }
-        const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > run_begin)) - 1;
+        const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > in_head)) - 1;
         const long long in_front = __shfl_sync(0xffffffffu, upto, (owner + 31) & 31);
-        long long offset = run_begin - before - (owner > 0 ? in_front : 0);
+        long long offset = in_head - before - (owner > 0 ? in_front : 0);
         s += owner;
         while (ok && at < run_end) {
           load_sequences(s & ~31);
@@ -350,47 +354,44 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const int length = __shfl_sync(0xffffffffu, lane_length, s & 31);
           if (news > 0) {
             const AttnSequence q = attn_sequence(news, length, step);
-            const long long of_head = attn_tiles_before(q, q.query_tiles, step, p.window);
-            int head = attn_quotient(offset, of_head);
-            offset -= head * of_head;
             int tile = attn_find_query_tile(q, offset, step, p.window);
             offset -= attn_tiles_before(q, tile, step, p.window);
-            for (; ok && head < heads && at < run_end; ++head) {
-              for (; ok && tile < q.query_tiles && at < run_end; ++tile) {
-                const int tiles = attn_tiles(q, tile, step, p.window);
-                const int skip = static_cast<int>(offset);
-                const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), run_end - at));
-                Piece piece;
-                piece.tiles = take;
-                piece.first_tile = attn_first_tile(q, tile, step, p.window) + skip;
-                piece.query0 = from + tile * step;
-                piece.tokens = min(step, news - tile * step);
-                piece.position0 = q.past + tile * step;
-                piece.key_origin = 0;
-                piece.sequence = s;
-                piece.kv_head = head / S::kHalves;
-                piece.half = head % S::kHalves;
-                piece.slot = take == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (skip == 0 ? 1 : 0);
-                if (skip == 0 && take < tiles) {
-                  // the item goes on in the next CTAs' runs: what attention_join_kernel has to add up
-                  int last = blockIdx.x + 1;
-                  while (attn_part_begin(work, parts, last + 1) < at + tiles) ++last;
-                  record[0] = last - static_cast<int>(blockIdx.x);
-                  record[1] = piece.query0;
-                  record[2] = piece.tokens;
-                  record[3] = piece.kv_head;
-                  record[4] = piece.half;
-                }
-                at += take;
-                offset = 0;
-                ok = room();
-                if (ok) hand_out(piece);
+            for (; ok && tile < q.query_tiles && at < run_end; ++tile) {
+              const int tiles = attn_tiles(q, tile, step, p.window);
+              const int skip = static_cast<int>(offset);
+              const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), run_end - at));
+              Piece piece;
+              piece.tiles = take;
+              piece.first_tile = attn_first_tile(q, tile, step, p.window) + skip;
+              piece.query0 = from + tile * step;
+              piece.tokens = min(step, news - tile * step);
+              piece.position0 = q.past + tile * step;
+              piece.key_origin = 0;
+              piece.sequence = s;
+              piece.kv_head = head / S::kHalves;
+              piece.half = head % S::kHalves;
+              piece.slot = take == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (skip == 0 ? 1 : 0);
+              if (skip == 0 && take < tiles) {
+                // the item goes on in the next CTAs' runs: what attention_join_kernel has to add up
+                int last = blockIdx.x + 1;
+                while (attn_part_begin(work, parts, last + 1) < at + tiles) ++last;
+                record[0] = last - static_cast<int>(blockIdx.x);
+                record[1] = piece.query0;
+                record[2] = piece.tokens;
+                record[3] = piece.kv_head;
+                record[4] = piece.half;
               }
-              tile = 0;
+              at += take;
+              offset = 0;
+              ok = room();
+              if (ok) hand_out(piece);
             }
           }
-          ++s;
           offset = 0;
+          if (++s == p.sequences) {
+            s = 0;
+            ++head;
+          }
         }
       }
       if (lane == 0) {

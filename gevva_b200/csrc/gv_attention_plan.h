@@ -106,8 +106,11 @@ GV_HD int attn_find_query_tile(const AttnSequence& s, long long at, int step, in
   return low;
 }
 
-// Work is dealt out to `parts` CTAs in runs of equal length; fewer CTAs where a run would be shorter than `least` key tiles.
-GV_HD int attn_parts(long long work, int parts, int least) {
+// Work, `heads` times the same, is dealt out to at most `parts` CTAs in runs of equal length: to as many for each head where that leaves no more than a
+// sixteenth of them without, to fewer where a run would be shorter than `least` key tiles.
+GV_HD int attn_parts(long long work, int parts, int heads, int least) {
+  const int even = heads <= parts ? parts / heads * heads : parts;
+  if (16 * even >= 15 * parts) parts = even;
   return work < static_cast<long long>(parts) * least ? static_cast<int>(work + least - 1) / least : parts;
 }
 // (Divisions in 32 bits where they do, up to 1023 parts of fewer than 2^22 key tiles: in 64 they are a hundred instructions.)

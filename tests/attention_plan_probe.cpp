@@ -41,15 +41,17 @@ static bool play(int window, int step, int heads, int parts_most, int least, con
       before += want;
     }
     if (attn_tiles_before(q, q.query_tiles, step, window) != before) return fail("all", attn_tiles_before(q, q.query_tiles, step, window), before);
-    for (int h = 0; h < heads; ++h)
+  }
+  for (int h = 0; h < heads; ++h)
+    for (const AttnSequence& q : all)
       for (int t = 0; t < q.query_tiles; ++t) {
         item_begin.push_back(work);
         item_tiles.push_back(attn_tiles(q, t, step, window));
         work += item_tiles.back();
       }
-  }
-  const int parts = attn_parts(work, parts_most, least);
-  if (parts > parts_most || (work > 0 && parts < 1)) return fail("parts", parts, work);
+  const int parts = attn_parts(work, parts_most, heads, least);
+  if (parts > parts_most || (work > 0 && parts < 1) || (work >= 2ll * parts_most * least && 16 * parts < 15 * parts_most)) return fail("parts", parts, work);
+  if (work > 0 && attn_quotient(work - 1, work / heads) != heads - 1) return fail("quotient", work, heads);
   long long at = 0;
   for (int c = 0; c < parts; ++c) {
     const long long begin = attn_part_begin(work, parts, c), end = attn_part_begin(work, parts, c + 1);
