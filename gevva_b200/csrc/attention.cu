@@ -124,7 +124,7 @@ struct AttnParams {
   const int* token_offsets;
   const int* lengths;
   const int* table;
-  int table_width, table_stride, page_shift;
+  int table_width, table_stride, page_shift, page_count;
   int sequences, tokens;
   int group, kv_heads;
   int step;        // tokens of one 128-row tile: 128 / group
@@ -530,6 +530,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
       };
       const auto fetch_keys = [&](int tile, int page) {
+        if (kPaged && static_cast<unsigned>(page) >= static_cast<unsigned>(p.page_count)) {
+          // (read as zeros, wherever that is; reported where some row sees it)
+          const Seen seen = seen_keys(piece, tile - piece.first_tile, p.window);
+          if (seen.to > box * box_rows && seen.from < (box + 1) * box_rows && p.status) atomicExch(p.status, static_cast<int>(kBadPage));
+        }
 #pragma unroll
         for (int i = 0; i < S::kKeyStages; ++i)
           if (ok) fetch(&map_k, i * S::kStageDim, tile, page);
@@ -1174,6 +1179,7 @@ cudaError_t launch_shape(const AttnCall& call, cudaStream_t stream) {
     p.table = c.table;
     p.table_width = c.table_width;
     p.table_stride = c.table_stride;
+    p.page_count = c.page_count;
     while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
     const uint64_t dims[4] = {kDim, static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(call.kv_heads), static_cast<uint64_t>(c.page_count)};
     const uint32_t box[4] = {64, static_cast<uint32_t>(c.page_size < kKeys ? c.page_size : kKeys), 1, 1};

@@ -170,6 +170,28 @@ def test_chunk_reports_lengths_beyond_the_table(attn, cuda_device):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 256), (512, 32)])
+def test_chunk_reports_pages_outside_the_cache(attn, cuda_device, dim, page):
+    """One that a row sees reads as zeros and is reported; those in front of a window and behind the last key are nobody's."""
+    from gevva_b200 import GevvaMoeError
+    batch, pages = make_batch(attn, [2, 3], [500, 1000], page, cuda_device, 2)
+    cache = attn.KvCache(randn((pages, page, 1, dim), cuda_device, 1), randn((pages, page, 1, dim), cuda_device, 2))
+    q = randn((5, 2, dim), cuda_device, 3)
+    batch.table[1, :(1000 - 3 - 200 + 1) // page] = pages
+    batch.table[:, -(-1000 // page):] = -1
+    attn.chunk_attention(q, cache, batch, 0.05, window=200)
+    cache.check()
+    for wrong in (-1, pages, -2 ** 31, 2 ** 31 - 1):
+        batch.table[1, 900 // page] = wrong
+        got = attn.chunk_attention(q, cache, batch, 0.05, window=200)
+        with pytest.raises(GevvaMoeError, match="page"):
+            cache.check()
+        cache.check()  # (reported once)
+        (k, v), seen = gathered(cache, batch, 0, 500), slice(0, 2)
+        ref.within(got[seen], *ref.attention(q[seen], k, v, 498, 0.05, 200))
+        assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 4), (256, 16, 8), (512, 16, 2)])
 def test_chunk_repeats_its_bits_and_equals_the_prompt_form(attn, cuda_device, dim, heads, kv_heads):
     n, page = 900, 64
