@@ -1,7 +1,11 @@
 """The attention side of a decoder layer (ctypes mirror of the gevva_attn_* entry points): norms around the attention block, per-head
 norms and rotation with the append to a paged cache, and causal attention over packed prompts or over the cache.  They stand where the
-reference's layer loop has them (src/cuda/runtime/prefill.cuh:924-1199, src/cuda/kernels/qkv_transform.cuh)."""
+reference's layer loop has them (src/cuda/runtime/prefill.cuh:924-1199, src/cuda/kernels/qkv_transform.cuh).
+
+Calls run on the current stream of their tensors' device, or on `stream`, whose work the caller orders behind what made the inputs; the
+tensors that a call makes belong to the stream that it runs on."""
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -24,20 +28,24 @@ class _Batch(ctypes.Structure):
                 ("sequences", ctypes.c_int), ("table_width", ctypes.c_int), ("table_stride", ctypes.c_int)]
 
 
+# gevva_attn_append_args, gevva_attn_prompt_args, gevva_attn_chunk_args: packed in one go, since the conversion of two dozen
+# single arguments took the host longer than the launch.
+_APPEND = struct.Struct("@" + "Pqq" * 3 + "P" * 9 + "6ifi")
+_PROMPT = struct.Struct("@" + "Pqq" * 3 + "P" * 3 + "6ifi")
+_CHUNK = struct.Struct("@Pqq" + "P" * 5 + "5if")
+
+
 def _lib():
     lib = library()
     if getattr(lib, "_gv_attn_ready", False):
         return lib
     vp, i32, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
-    i64 = ctypes.c_longlong
-    rows = [vp, i64, i64]  # address, strides of a token and of a head
     lib.gevva_attn_norm.argtypes = [vp, vp, vp, i32, i32, f32, vp]
     lib.gevva_attn_norm_add.argtypes = [vp] * 8 + [i32, i32, f32, vp]
-    lib.gevva_attn_append.argtypes = rows * 3 + [vp, vp, i32, i32, i32, i32, vp, i32, vp, vp, i32, f32, vp, vp, vp, vp, vp]
-    lib.gevva_attn_prompt.argtypes = rows * 3 + [vp, i32, i32, i32, i32, i32, f32, i32, vp, vp, vp]
+    for function in (lib.gevva_attn_append, lib.gevva_attn_prompt, lib.gevva_attn_chunk):
+        function.argtypes = [ctypes.c_char_p, vp]  # the packed arguments, the stream
     lib.gevva_attn_chunk_workspace_bytes.argtypes = [i32]
     lib.gevva_attn_chunk_workspace_bytes.restype = ctypes.c_size_t
-    lib.gevva_attn_chunk.argtypes = rows + [vp, vp, i32, i32, i32, i32, f32, i32, vp, vp, vp, vp]
     lib._gv_attn_ready = True
     return lib
 
@@ -48,12 +56,28 @@ def _status(status, where):
 
 
 def _at(tensor, dtype, shape, device, name):
-    """Address of a contiguous tensor on `device`; None stays None."""
+    """Address of a contiguous tensor on `device`; 0 for None."""
     if tensor is None:
-        return None
+        return 0
     if tensor.dtype is dtype and tensor.shape == shape and tensor.device == device and tensor.is_contiguous():
         return tensor.data_ptr()
     raise ValueError(f"{name}: expected contiguous {dtype} {tuple(shape)} on {device}, got {tensor.dtype} {tuple(tensor.shape)} on {tensor.device}")
+
+
+def _on(stream, device):
+    """Makes `stream` (a torch.cuda.Stream or a raw handle) the current one: what a call makes then belongs to it, as on the current stream."""
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    if stream.device != device:
+        raise ValueError(f"stream: expected one of {device}, got one of {stream.device}")
+    return torch.cuda.stream(stream)
+
+
+def _pack(layout, *values):
+    try:
+        return layout.pack(*values)
+    except struct.error as error:
+        raise ValueError(f"argument out of range: {error}") from None
 
 
 def _heads(tensor, name, device, shape):
@@ -90,9 +114,12 @@ def _rows(x, name="input"):
 def block_norm(x, weight, eps=1e-6, out=None, stream=None):
     """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768."""
     device, shape = _rows(x)
+    if stream is not None:
+        with _on(stream, device):
+            return block_norm(x, weight, eps, out)
     rows, width = shape
     out = _out(out, x, device)
-    _status(_enqueue(_lib().gevva_attn_norm, device, stream, x.data_ptr(), _at(weight, torch.bfloat16, (width,), device, "weight"),
+    _status(_enqueue(_lib().gevva_attn_norm, device, None, x.data_ptr(), _at(weight, torch.bfloat16, (width,), device, "weight"),
                      out.data_ptr(), rows, width, eps), "block_norm")
     return out
 
@@ -101,13 +128,16 @@ def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None,
     """(residual + gate * norm(x) * weight) * scale, the norm behind a block; with `next_weight` also the next block's norm of
     the result, returned as (out, next).  gate bf16 [width] and scale bf16 [1] are optional; out may be residual."""
     device, shape = _rows(x)
+    if stream is not None:
+        with _on(stream, device):
+            return block_norm_add(x, weight, residual, gate, scale, next_weight, eps, out)
     rows, width = shape
     bf16 = torch.bfloat16
     following = None
     out = _out(out, x, device)
     if next_weight is not None:
         following = _empty_like(x)
-    _status(_enqueue(_lib().gevva_attn_norm_add, device, stream, x.data_ptr(), _at(weight, bf16, (width,), device, "weight"),
+    _status(_enqueue(_lib().gevva_attn_norm_add, device, None, x.data_ptr(), _at(weight, bf16, (width,), device, "weight"),
                      _at(residual, bf16, shape, device, "residual"), _at(gate, bf16, (width,), device, "gate"),
                      _at(scale, bf16, (1,), device, "scale"), _at(next_weight, bf16, (width,), device, "next_weight"), out.data_ptr(),
                      _address(following), rows, width, eps), "block_norm_add")
@@ -140,7 +170,8 @@ class KvCache:
         return cls(*(torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(2)))
 
     def last_status(self):
-        """Synchronises, then returns and clears the status of the calls on this cache (0 = ok)."""
+        """Waits for the device, then returns and clears the status of the calls on this cache (0 = ok)."""
+        torch.cuda.synchronize(self.device)
         status = -int(self.status.item())
         if status:
             self.status.zero_()
@@ -152,8 +183,9 @@ class KvCache:
 
 class PagedBatch:
     """The sequences of a call, int32 on the GPU: new tokens token_offsets[s] .. token_offsets[s + 1] - 1 (rows of the call's
-    tensors), lengths[s] keys with the new ones counted, and table [sequences, pages a sequence], whose entry x / page_size is the page of position x.
-    The tensors are read when the calls run, so a captured call can be replayed with other contents; rows outside the offsets are left as they were."""
+    tensors), lengths[s] keys with the new ones counted, and table [sequences, pages a sequence], whose entry x / page_size is the page of
+    position x.  The tensors are read when the calls run, so a captured call can be replayed with other contents; rows outside the offsets
+    are left as they were."""
 
     def __init__(self, token_offsets, lengths, table):
         sequences = lengths.shape[0] if lengths.dim() == 1 else -1
@@ -190,6 +222,9 @@ def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, 
     `packed` also keys and values as [tokens, kv_heads, dim] for prompt_attention.  `out` takes the queries.  A token
     without a page is not stored; cache.check() reports it."""
     device, shape, q_rows = _queries(q)
+    if stream is not None:
+        with _on(stream, device):
+            return kv_append(q, k, v, cache, batch, frequencies, q_weight, k_weight, normalize_v, eps, packed, out)
     tokens, heads, dim = shape
     kv_heads = cache.kv_heads
     if cache.head_dim != dim or cache.device != device or batch.device != device:
@@ -198,18 +233,25 @@ def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, 
     rotated = 0 if frequencies is None else 2 * frequencies.numel()
     out = _out(out, q, device)
     k_out, v_out = (_out(None, k, device), _out(None, v, device)) if packed else (None, None)
-    _status(_enqueue(_lib().gevva_attn_append, device, stream, *q_rows, *k_rows, *v_rows, cache._address, batch._address, tokens, heads, kv_heads,
-                     dim, frequencies if frequencies is None else _at(frequencies, torch.float64, frequencies.shape, device, "frequencies"), rotated,
-                     _at(q_weight, torch.bfloat16, (dim,), device, "q_weight"), _at(k_weight, torch.bfloat16, (dim,), device, "k_weight"), normalize_v, eps, out.data_ptr(),
-                     _address(k_out), _address(v_out), cache.status.data_ptr()), "kv_append")
+    bf16 = torch.bfloat16
+    args = _pack(_APPEND, *q_rows, *k_rows, *v_rows, cache._address, batch._address,
+                        0 if frequencies is None else _at(frequencies, torch.float64, frequencies.shape, device, "frequencies"),
+                        _at(q_weight, bf16, (dim,), device, "q_weight"), _at(k_weight, bf16, (dim,), device, "k_weight"), out.data_ptr(),
+                        k_out.data_ptr() if packed else 0, v_out.data_ptr() if packed else 0, cache.status.data_ptr(), tokens, heads, kv_heads, dim,
+                        rotated, normalize_v, eps, 0)
+    _status(_enqueue(_lib().gevva_attn_append, device, None, args), "kv_append")
     return Appended(out, k_out, v_out) if packed else out
 
 
 def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=None, stream=None):
     """Causal attention of packed prompts: rows token_offsets[s] .. token_offsets[s + 1] - 1 (int32 on the GPU) are sequence s, and
     each sees its sequence's rows up to itself, the last `window` of them where that is not zero.  q [tokens, heads, dim], k and v
-    [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`.  `status` is an optional int32 [1] device word."""
+    [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`.  `status` is an optional
+    int32 [1] device word."""
     device, shape, q_rows = _queries(q)
+    if stream is not None:
+        with _on(stream, device):
+            return prompt_attention(q, k, v, token_offsets, scale, window, out, status)
     tokens, heads, dim = shape
     if k.dim() != 3:
         raise ValueError(f"k: expected (tokens, kv_heads, dim), got {tuple(k.shape)}")
@@ -217,31 +259,33 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
     k_rows, v_rows = (_heads(x, name, device, (tokens, kv_heads, dim)) for x, name in ((k, "k"), (v, "v")))
     sequences = token_offsets.numel() - 1
     out = _out(out, q, device)
-    _status(_enqueue(_lib().gevva_attn_prompt, device, stream, *q_rows, *k_rows, *v_rows, _at(token_offsets, torch.int32, (sequences + 1,), device, "token_offsets"), sequences,
-                     tokens, heads, kv_heads, dim, scale, window, out.data_ptr(), _at(status, torch.int32, (1,), device, "status")), "prompt_attention")
+    args = _pack(_PROMPT, *q_rows, *k_rows, *v_rows, _at(token_offsets, torch.int32, (sequences + 1,), device, "token_offsets"), out.data_ptr(),
+                        _at(status, torch.int32, (1,), device, "status"), sequences, tokens, heads, kv_heads, dim, window, scale, 0)
+    _status(_enqueue(_lib().gevva_attn_prompt, device, None, args), "prompt_attention")
     return out
 
 
 def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
     """Causal attention of new tokens over the pages of their sequences, which hold their keys and values already (kv_append):
-    one token a sequence when decoding, several for verification and chunked prefill.  A row that sees no key is zero; rows outside the offsets
-    are left as they were in `out`."""
+    one token a sequence when decoding, several for verification and chunked prefill.  A row that sees no key is zero; rows outside the
+    offsets are left as they were in `out`.  cache.check() reports lengths beyond the table and pages outside the cache."""
     device, shape, q_rows = _queries(q)
+    if stream is not None:
+        with _on(stream, device):
+            return chunk_attention(q, cache, batch, scale, window, out)
     tokens, heads, dim = shape
     if cache.head_dim != dim or cache.device != device or batch.device != device:
         raise ValueError(f"chunk_attention: queries of {dim} on {device}, cache of {cache.head_dim} on {cache.device}, batch on {batch.device}")
     lib = _lib()
     out = _out(out, q, device)
 
-    def launch(*args):
+    def launch(handle):
         # (the workspace's size goes by the device, which is the current one in here)
         workspace = _empty(lib.gevva_attn_chunk_workspace_bytes(dim), dtype=torch.uint8, device=device)
-        if stream is not None:  # not the stream that the workspace belongs to
-            workspace.record_stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
-        return lib.gevva_attn_chunk(*q_rows, cache._address, batch._address, tokens, heads, cache.kv_heads, dim, scale, window, out.data_ptr(),
-                                    workspace.data_ptr(), cache.status.data_ptr(), *args)
+        return lib.gevva_attn_chunk(_pack(_CHUNK, *q_rows, cache._address, batch._address, out.data_ptr(), workspace.data_ptr(),
+                                                cache.status.data_ptr(), tokens, heads, cache.kv_heads, dim, window, scale), handle)
 
-    _status(_enqueue(launch, device, stream), "chunk_attention")
+    _status(_enqueue(launch, device, None), "chunk_attention")
     return out
 
 

@@ -59,7 +59,25 @@ int launched(cudaError_t e) {
   return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
 }
 
-bool attention_ok(float scale, int window) { return scale > 0.0f && scale <= 1e30f && window >= 0; }
+bool attention_ok(int tokens, float scale, int window) {
+  return tokens <= kMaxPositions && scale > 0.0f && scale <= 1e30f && window >= 0;
+}
+
+// What both attention calls have.
+template <class Args>
+void fill_attention(gv::AttnCall* call, const Args& a) {
+  call->tokens = a.tokens;
+  call->heads = a.heads;
+  call->kv_heads = a.kv_heads;
+  call->dim = a.dim;
+  call->window = a.window < kMaxPositions ? a.window : 0;  // (a window that no sequence is longer than)
+  call->scale = a.scale;
+  call->out = a.out;
+  call->out_token_stride = static_cast<long long>(a.heads) * a.dim;
+  call->out_head_stride = a.dim;
+  call->status = a.device_status;
+  call->sm_count = gv::current_sm_count();
+}
 
 }  // namespace
 
@@ -101,64 +119,49 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
   return launched(gv::launch_block_norm(call, gv::current_sm_count(), stream));
 }
 
-int gevva_attn_append(const void* q, long long q_token_stride, long long q_head_stride,
-                      const void* k, long long k_token_stride, long long k_head_stride,
-                      const void* v, long long v_token_stride, long long v_head_stride,
-                      const gevva_attn_cache* cache,
-                      const gevva_attn_batch* batch, int tokens, int heads, int kv_heads, int dim, const double* frequencies,
-                      int rotated, const void* q_weight, const void* k_weight, int normalize_v, float eps, void* q_out, void* k_out,
-                      void* v_out, int* device_status, gevva_stream_t stream) {
+int gevva_attn_append(const gevva_attn_append_args* a, gevva_stream_t stream) {
   gv::AppendCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !rows_ok(&call.k, k, k_token_stride, k_head_stride, tokens, kv_heads, dim) ||
-      !rows_ok(&call.v, v, v_token_stride, v_head_stride, tokens, kv_heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) || rotated < 0 || rotated > dim ||
-      rotated % 16 || (rotated > 0 && (!frequencies || (reinterpret_cast<uintptr_t>(frequencies) & 7))) || !aligned_or_null(q_weight) ||
-      !aligned_or_null(k_weight) || !(eps >= 0.0f) || !aligned_for(q_out, tokens) || !aligned_or_null(k_out) || !aligned_or_null(v_out) || (tokens > 0 && !k_out != !v_out))
+  if (!a || !heads_ok(a->tokens, a->heads, a->kv_heads, a->dim) ||
+      !rows_ok(&call.q, a->q, a->q_token_stride, a->q_head_stride, a->tokens, a->heads, a->dim) ||
+      !rows_ok(&call.k, a->k, a->k_token_stride, a->k_head_stride, a->tokens, a->kv_heads, a->dim) ||
+      !rows_ok(&call.v, a->v, a->v_token_stride, a->v_head_stride, a->tokens, a->kv_heads, a->dim) ||
+      !pages_ok(&call.pages, a->cache, a->batch, a->kv_heads, a->dim) || a->rotated < 0 || a->rotated > a->dim || a->rotated % 16 ||
+      (a->rotated > 0 && (!a->frequencies || (reinterpret_cast<uintptr_t>(a->frequencies) & 7))) || !aligned_or_null(a->q_weight) ||
+      !aligned_or_null(a->k_weight) || !(a->eps >= 0.0f) || !aligned_for(a->q_out, a->tokens) || !aligned_or_null(a->k_out) ||
+      !aligned_or_null(a->v_out) || (a->tokens > 0 && !a->k_out != !a->v_out) || a->reserved)
     return GEVVA_MOE_BAD_ARGUMENT;
-  if (tokens == 0) return GEVVA_MOE_OK;
-  call.token_offsets = batch->token_offsets;
-  call.sequences = batch->sequences;
-  call.tokens = tokens;
-  call.heads = heads;
-  call.kv_heads = kv_heads;
-  call.dim = dim;
-  call.frequencies = frequencies;
-  call.rotated = rotated;
-  call.q_weight = q_weight;
-  call.k_weight = k_weight;
-  call.normalize_v = normalize_v != 0;
-  call.eps = eps;
-  call.q_out = q_out;
-  call.k_out = k_out;
-  call.v_out = v_out;
-  call.status = device_status;
+  if (a->tokens == 0) return GEVVA_MOE_OK;
+  call.token_offsets = a->batch->token_offsets;
+  call.sequences = a->batch->sequences;
+  call.tokens = a->tokens;
+  call.heads = a->heads;
+  call.kv_heads = a->kv_heads;
+  call.dim = a->dim;
+  call.frequencies = a->frequencies;
+  call.rotated = a->rotated;
+  call.q_weight = a->q_weight;
+  call.k_weight = a->k_weight;
+  call.normalize_v = a->normalize_v != 0;
+  call.eps = a->eps;
+  call.q_out = a->q_out;
+  call.k_out = a->k_out;
+  call.v_out = a->v_out;
+  call.status = a->device_status;
   return launched(gv::launch_kv_append(call, gv::current_sm_count(), stream));
 }
 
-int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_stride,
-                      const void* k, long long k_token_stride, long long k_head_stride,
-                      const void* v, long long v_token_stride, long long v_head_stride,
-                      const int* token_offsets,
-                      int sequences, int tokens, int heads, int kv_heads, int dim, float scale, int window, void* out,
-                      int* device_status, gevva_stream_t stream) {
+int gevva_attn_prompt(const gevva_attn_prompt_args* a, gevva_stream_t stream) {
   gv::AttnCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !rows_ok(&call.k, k, k_token_stride, k_head_stride, tokens, kv_heads, dim) ||
-      !rows_ok(&call.v, v, v_token_stride, v_head_stride, tokens, kv_heads, dim) || !token_offsets || sequences < 1 || tokens > kMaxPositions || !attention_ok(scale, window) ||
-      !aligned_32(out, tokens))
+  if (!a || !heads_ok(a->tokens, a->heads, a->kv_heads, a->dim) ||
+      !rows_ok(&call.q, a->q, a->q_token_stride, a->q_head_stride, a->tokens, a->heads, a->dim) ||
+      !rows_ok(&call.k, a->k, a->k_token_stride, a->k_head_stride, a->tokens, a->kv_heads, a->dim) ||
+      !rows_ok(&call.v, a->v, a->v_token_stride, a->v_head_stride, a->tokens, a->kv_heads, a->dim) || !a->token_offsets || a->sequences < 1 ||
+      !attention_ok(a->tokens, a->scale, a->window) || !aligned_32(a->out, a->tokens) || a->reserved)
     return GEVVA_MOE_BAD_ARGUMENT;
-  if (tokens == 0) return GEVVA_MOE_OK;
-  call.token_offsets = token_offsets;
-  call.sequences = sequences;
-  call.tokens = tokens;
-  call.heads = heads;
-  call.kv_heads = kv_heads;
-  call.dim = dim;
-  call.window = window < kMaxPositions ? window : 0;  // (a window that no sequence is longer than)
-  call.scale = scale;
-  call.out = out;
-  call.out_token_stride = static_cast<long long>(heads) * dim;
-  call.out_head_stride = dim;
-  call.status = device_status;
-  call.sm_count = gv::current_sm_count();
+  if (a->tokens == 0) return GEVVA_MOE_OK;
+  call.token_offsets = a->token_offsets;
+  call.sequences = a->sequences;
+  fill_attention(&call, *a);
   return launched(gv::launch_attention(call, stream));
 }
 
@@ -166,30 +169,19 @@ size_t gevva_attn_chunk_workspace_bytes(int dim) {
   return dim == 64 || dim == 128 || dim == 256 || dim == 512 ? gv::attention_workspace_bytes(dim, gv::current_sm_count()) : 0;
 }
 
-int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_stride,
-                     const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads,
-                     int kv_heads, int dim, float scale, int window, void* out, void* workspace, int* device_status,
-                     gevva_stream_t stream) {
+int gevva_attn_chunk(const gevva_attn_chunk_args* a, gevva_stream_t stream) {
   gv::AttnCall call{};
-  if (!heads_ok(tokens, heads, kv_heads, dim) || !rows_ok(&call.q, q, q_token_stride, q_head_stride, tokens, heads, dim) || !pages_ok(&call.pages, cache, batch, kv_heads, dim) ||
-      tokens > kMaxPositions || !attention_ok(scale, window) || !aligned_32(out, tokens) || !workspace || !aligned_32(workspace, 1))
+  if (!a || !heads_ok(a->tokens, a->heads, a->kv_heads, a->dim) ||
+      !rows_ok(&call.q, a->q, a->q_token_stride, a->q_head_stride, a->tokens, a->heads, a->dim) ||
+      !pages_ok(&call.pages, a->cache, a->batch, a->kv_heads, a->dim) || !attention_ok(a->tokens, a->scale, a->window) ||
+      !aligned_32(a->out, a->tokens) || !aligned_32(a->workspace, 1))
     return GEVVA_MOE_BAD_ARGUMENT;
-  if (tokens == 0) return GEVVA_MOE_OK;
+  if (a->tokens == 0) return GEVVA_MOE_OK;
   call.paged = true;
-  call.token_offsets = batch->token_offsets;
-  call.sequences = batch->sequences;
-  call.tokens = tokens;
-  call.heads = heads;
-  call.kv_heads = kv_heads;
-  call.dim = dim;
-  call.window = window < kMaxPositions ? window : 0;
-  call.scale = scale;
-  call.out = out;
-  call.out_token_stride = static_cast<long long>(heads) * dim;
-  call.out_head_stride = dim;
-  call.workspace = workspace;
-  call.status = device_status;
-  call.sm_count = gv::current_sm_count();
+  call.token_offsets = a->batch->token_offsets;
+  call.sequences = a->batch->sequences;
+  call.workspace = a->workspace;
+  fill_attention(&call, *a);
   if (call.sm_count < 1) return GEVVA_MOE_NO_DEVICE;
   return launched(gv::launch_attention(call, stream));
 }

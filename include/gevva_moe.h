@@ -38,7 +38,7 @@ enum gevva_moe_status {
   GEVVA_MOE_CUDA_ERROR = -4,
   GEVVA_MOE_NO_DEVICE = -5,     /* no sm_100 device / driver entry point missing */
   GEVVA_MOE_TOO_LARGE = -6,
-  GEVVA_MOE_BAD_PAGE = -7 /* device: a new token's position has no page of the cache (gevva_attn_append) */
+  GEVVA_MOE_BAD_PAGE = -7 /* device: a position has no page of the cache (gevva_attn_append, gevva_attn_chunk) */
 };
 
 /* The eight sidecar tensors of one layer that the reference's constructor resolves
@@ -409,35 +409,69 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
  * a multiple of 16 up to dim, zero for none; values from `rotated` on stay).  Queries go to q_out [tokens, heads, dim], keys and
  * values to the cache and, where k_out and v_out are given (both or none), to [tokens, kv_heads, dim], which gevva_attn_prompt
  * reads.  A token without a page (position outside the table, page outside the cache) is not stored and reported as
- * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot. */
-int gevva_attn_append(const void* q, long long q_token_stride, long long q_head_stride,
-                      const void* k, long long k_token_stride, long long k_head_stride,
-                      const void* v, long long v_token_stride, long long v_head_stride,
-                      const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens, int heads, int kv_heads,
-                      int dim, const double* frequencies, int rotated, const void* q_weight, const void* k_weight,
-                      int normalize_v, float eps, void* q_out, void* k_out, void* v_out, int* device_status,
-                      gevva_stream_t stream);
+ * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot.  q_out may be q. */
+typedef struct {
+  const void* q;
+  long long q_token_stride, q_head_stride;
+  const void* k;
+  long long k_token_stride, k_head_stride;
+  const void* v;
+  long long v_token_stride, v_head_stride;
+  const gevva_attn_cache* cache;
+  const gevva_attn_batch* batch;
+  const double* frequencies;
+  const void* q_weight;
+  const void* k_weight;
+  void* q_out;
+  void* k_out;
+  void* v_out;
+  int* device_status;
+  int tokens, heads, kv_heads, dim, rotated, normalize_v;
+  float eps;
+  int reserved; /* 0 */
+} gevva_attn_append_args;
+int gevva_attn_append(const gevva_attn_append_args* args, gevva_stream_t stream);
 
 /* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
- * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  0 < scale <= 1e30.  No row sees another sequence's keys,
- * whatever their values are; within a sequence, keys and values that a row does not see have to be finite. */
-int gevva_attn_prompt(const void* q, long long q_token_stride, long long q_head_stride,
-                      const void* k, long long k_token_stride, long long k_head_stride,
-                      const void* v, long long v_token_stride, long long v_head_stride,
-                      const int* token_offsets,
-                      int sequences, int tokens, int heads, int kv_heads, int dim, float scale, int window, void* out,
-                      int* device_status, gevva_stream_t stream);
+ * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  0 < scale <= 1e30.  No row sees another sequence's
+ * keys, whatever their values are; within a sequence, keys and values that a row does not see have to be finite.  out may not
+ * overlap what the call reads. */
+typedef struct {
+  const void* q;
+  long long q_token_stride, q_head_stride;
+  const void* k;
+  long long k_token_stride, k_head_stride;
+  const void* v;
+  long long v_token_stride, v_head_stride;
+  const int* token_offsets; /* [sequences + 1] */
+  void* out;
+  int* device_status;
+  int sequences, tokens, heads, kv_heads, dim, window;
+  float scale;
+  int reserved; /* 0 */
+} gevva_attn_prompt_args;
+int gevva_attn_prompt(const gevva_attn_prompt_args* args, gevva_stream_t stream);
 
 /* The same for new tokens over a paged cache that already holds their keys and values (gevva_attn_append): one token a sequence when
  * decoding, several in verification and chunked prefill.  Lengths are read on the device, so a captured call can be replayed with
- * others.  Row i of n sees the keys up to lengths[s] - n + i; a row that sees none is zero.  Slots that no row of a
- * sequence sees may hold anything, others have to be finite.  A length beyond the table is cut to it and reported as GEVVA_MOE_BAD_PAGE.  `workspace` is device memory of gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed
- * the call; calls that may run at the same time need one each. */
+ * others.  Row i of n sees the keys up to lengths[s] - n + i; a row that sees none is zero.  Slots that no row of a sequence sees
+ * may hold anything, others have to be finite.  A length beyond the table is cut to it, a page outside the cache is read as zeros,
+ * and both are reported as GEVVA_MOE_BAD_PAGE.  out may not overlap what the call reads.  `workspace` is device memory of
+ * gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed the call; calls that may run at the same time need
+ * one each. */
 size_t gevva_attn_chunk_workspace_bytes(int dim);
-int gevva_attn_chunk(const void* q, long long q_token_stride, long long q_head_stride,
-                     const gevva_attn_cache* cache, const gevva_attn_batch* batch, int tokens,
-                     int heads, int kv_heads, int dim, float scale, int window, void* out, void* workspace,
-                     int* device_status, gevva_stream_t stream);
+typedef struct {
+  const void* q;
+  long long q_token_stride, q_head_stride;
+  const gevva_attn_cache* cache;
+  const gevva_attn_batch* batch;
+  void* out;
+  void* workspace;
+  int* device_status;
+  int tokens, heads, kv_heads, dim, window;
+  float scale;
+} gevva_attn_chunk_args;
+int gevva_attn_chunk(const gevva_attn_chunk_args* args, gevva_stream_t stream);
 
 /* Per-tensor FP8 quantiser (tools/pack_fp8_dense.py:64-70): scale = amax/448, q = e4m3(w/scale). */
 int gevva_pack_fp8(const float* weights, size_t count, void* out, float* scale, gevva_stream_t stream);

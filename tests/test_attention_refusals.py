@@ -18,7 +18,7 @@ def lib():
 
 
 def rows(data=A, token=512, head=64):
-    return data, token, head
+    return data or 0, token, head
 
 
 def cache(**change):
@@ -36,16 +36,20 @@ CACHE, BATCH = cache(), batch()
 
 
 def chunk(lib, q=None, c=None, b=None, tokens=3, heads=4, kv_heads=2, dim=64, scale=0.1, window=0, out=A, workspace=A):
-    return lib.gevva_attn_chunk(*(q or rows()), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), tokens, heads, kv_heads, dim, scale, window, out, workspace, None, None)
+    return lib.gevva_attn_chunk(attn._CHUNK.pack(*(q or rows()), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), out or 0, workspace or 0, 0,
+                                                 tokens, heads, kv_heads, dim, window, scale), None)
 
 
-def prompt(lib, q=None, k=None, v=None, offsets=A, sequences=2, tokens=3, heads=4, kv_heads=2, dim=64, scale=0.1, window=0, out=A):
-    return lib.gevva_attn_prompt(*(q or rows()), *(k or rows()), *(v or rows()), offsets, sequences, tokens, heads, kv_heads, dim, scale, window, out, None, None)
+def prompt(lib, q=None, k=None, v=None, offsets=A, sequences=2, tokens=3, heads=4, kv_heads=2, dim=64, scale=0.1, window=0, out=A, reserved=0):
+    return lib.gevva_attn_prompt(attn._PROMPT.pack(*(q or rows()), *(k or rows()), *(v or rows()), offsets or 0, out or 0, 0, sequences, tokens, heads,
+                                                   kv_heads, dim, window, scale, reserved), None)
 
 
-def append(lib, q=None, c=None, b=None, tokens=3, heads=4, kv_heads=2, dim=64, freq=A, rotated=64, eps=1e-6, q_out=A, k_out=None, v_out=None, qw=None):
-    return lib.gevva_attn_append(*(q or rows()), *rows(), *rows(), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), tokens, heads, kv_heads, dim, freq, rotated, qw, None, 0, eps,
-                                 q_out, k_out, v_out, None, None)
+def append(lib, q=None, c=None, b=None, tokens=3, heads=4, kv_heads=2, dim=64, freq=A, rotated=64, eps=1e-6, q_out=A, k_out=None, v_out=None, qw=None,
+           reserved=0):
+    return lib.gevva_attn_append(attn._APPEND.pack(*(q or rows()), *rows(), *rows(), ctypes.addressof(c or CACHE), ctypes.addressof(b or BATCH), freq or 0,
+                                                   qw or 0, 0, q_out or 0, k_out or 0, v_out or 0, 0, tokens, heads, kv_heads, dim, rotated, 0, eps,
+                                                   reserved), None)
 
 
 SHAPES = [dict(tokens=-1), dict(heads=0), dict(kv_heads=0), dict(heads=5), dict(heads=258, kv_heads=2), dict(dim=96), dict(dim=0), dict(dim=1024),
@@ -63,14 +67,14 @@ def test_chunk(lib, change):
     assert chunk(lib, **change) == BAD
 
 
-@pytest.mark.parametrize("change", SHAPES + SOFTMAX + [dict(k=rows(A + 2)), dict(v=rows(head=4)), dict(offsets=None), dict(sequences=0)])
+@pytest.mark.parametrize("change", SHAPES + SOFTMAX + [dict(k=rows(A + 2)), dict(v=rows(head=4)), dict(offsets=None), dict(sequences=0), dict(reserved=1)])
 def test_prompt(lib, change):
     assert prompt(lib, **change) == BAD
 
 
 @pytest.mark.parametrize("change", SHAPES + PAGES + [dict(rotated=-16), dict(rotated=80), dict(rotated=8), dict(freq=None), dict(freq=A + 4),
                                                      dict(eps=-1.0), dict(eps=float("nan")), dict(q_out=None), dict(k_out=A), dict(v_out=A),
-                                                     dict(qw=A + 2)])
+                                                     dict(qw=A + 2), dict(reserved=1)])
 def test_append(lib, change):
     assert append(lib, **change) == BAD
 
@@ -87,6 +91,22 @@ def test_norms(lib):
         assert norm(**change) == BAD and add(**change) == BAD, change
     for change in (dict(r=None), dict(gate=A + 2), dict(scale=A + 1), dict(nw=A), dict(nxt=A), dict(nw=A + 2, nxt=A)):
         assert add(**change) == BAD, change
+
+
+def test_packed_arguments_have_the_layout_of_the_header(lib, tmp_path):
+    import shutil
+    import subprocess
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    source = tmp_path / "sizes.c"
+    names = ("append", "prompt", "chunk")
+    source.write_text('#include <stdio.h>\n#include "gevva_moe.h"\nint main(void) {' + "".join(
+        f'printf("%zu\\n", sizeof(gevva_attn_{n}_args));' for n in names) + "return 0; }")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), "-o", str(tmp_path / "sizes"), str(source)], check=True)
+    sizes = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], capture_output=True, text=True, check=True).stdout.split()]
+    assert sizes == [attn._APPEND.size, attn._PROMPT.size, attn._CHUNK.size]
+    for function in (lib.gevva_attn_append, lib.gevva_attn_prompt, lib.gevva_attn_chunk):
+        assert function(None, None) == BAD
 
 
 def test_calls_without_rows_do_nothing(lib):
@@ -121,3 +141,9 @@ def test_python_mirror_refuses():
         attn.block_norm_add(x[:, 0], w, x[:, 0])
     fields = [n for n, _ in attn._Cache._fields_]
     assert fields[-2:] == ["pages", "page_size"] and ctypes.sizeof(attn._Cache) == 72 and ctypes.sizeof(attn._Batch) == 40
+
+
+def test_numbers_that_an_argument_cannot_hold():
+    for window, scale in ((1 << 31, 0.1), (-(1 << 31) - 1, 0.1), (0, None)):
+        with pytest.raises(ValueError, match="out of range"):
+            attn._pack(attn._CHUNK, A, 8, 8, A, A, A, A, 0, 1, 1, 1, 64, window, scale)

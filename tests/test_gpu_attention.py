@@ -419,6 +419,34 @@ def test_two_streams_at_once(attn, cuda_device):
             assert torch.equal(g, want[i])
 
 
+def test_what_a_call_makes_belongs_to_its_stream(attn, cuda_device):
+    """On a stream other than the current one: what the call gives back to the allocator may still be in use there, and here it is not handed out."""
+    x = randn((200, 2, 64), cuda_device, 1)
+    offsets = offsets_of([200], cuda_device)
+    batch, pages = make_batch(attn, [200], [200], 16, cuda_device, 2)
+    cache = attn.KvCache(randn((pages, 16, 2, 64), cuda_device, 1), randn((pages, 16, 2, 64), cuda_device, 2))
+    rows = x.view(200, 128)
+    weight = torch.ones(128, dtype=torch.bfloat16, device=cuda_device)
+    calls = [lambda s: attn.block_norm(rows, weight, stream=s), lambda s: attn.block_norm_add(rows, weight, rows, stream=s),
+             lambda s: attn.kv_append(x, x, x, cache, batch, None, stream=s), lambda s: attn.prompt_attention(x, x, x, offsets, 0.125, stream=s),
+             lambda s: attn.chunk_attention(x, cache, batch, 0.125, stream=s)]
+    for i, call in enumerate(calls):
+        side = torch.cuda.Stream(cuda_device)
+        torch.cuda.synchronize()
+        want = call(None)
+        for stream in (side, side.cuda_stream, 0):
+            torch.cuda.synchronize()
+            got = call(stream)
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), i
+            if stream:
+                at = got.data_ptr()
+                del got
+                held = [torch.empty_like(x) for _ in range(8)]
+                assert all(h.data_ptr() != at for h in held), i
+    cache.check()
+
+
 def test_nothing_to_do(attn, cuda_device):
     x = torch.empty((0, 2, 64), dtype=torch.bfloat16, device=cuda_device)
     zero = torch.zeros(2, dtype=torch.int32, device=cuda_device)
