@@ -355,11 +355,32 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (news > 0) {
             const AttnSequence q = attn_sequence(news, length, step);
             int tile = attn_find_query_tile(q, offset, step, p.window);
+            // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as when a
+            // chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of each
+            // one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 535 us).
+            int last = -1;
+            long long end = run_end;
+            const long long ends_at = offset + run_end - at;
+            if (offset > 0 && tile + 1 < q.query_tiles && ends_at <= attn_tiles_before(q, q.query_tiles, step, p.window)) {
+              const int ends_in = attn_find_query_tile(q, ends_at - 1, step, p.window);
+              if (ends_in > tile) {
+                last = ends_in;
+                end = run_end - (ends_at - attn_tiles_before(q, last, step, p.window));
+              }
+            }
             offset -= attn_tiles_before(q, tile, step, p.window);
-            for (; ok && tile < q.query_tiles && at < run_end; ++tile) {
+            const int first = tile;
+            const long long first_offset = offset, first_at = at;
+            bool ahead = last >= 0;
+            if (ahead) {
+              tile = last;
+              offset = 0;
+              at = end;
+            }
+            for (; ok && tile < q.query_tiles && (ahead || at < end); ++tile) {
               const int tiles = attn_tiles(q, tile, step, p.window);
               const int skip = static_cast<int>(offset);
-              const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), run_end - at));
+              const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), (ahead ? run_end : end) - at));
               Piece piece;
               piece.tiles = take;
               piece.first_tile = attn_first_tile(q, tile, step, p.window) + skip;
@@ -373,9 +394,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               piece.slot = take == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (skip == 0 ? 1 : 0);
               if (skip == 0 && take < tiles) {
                 // the item goes on in the next CTAs' runs: what attention_join_kernel has to add up
-                int last = blockIdx.x + 1;
-                while (attn_part_begin(work, parts, last + 1) < at + tiles) ++last;
-                record[0] = last - static_cast<int>(blockIdx.x);
+                int upto_part = blockIdx.x + 1;
+                while (attn_part_begin(work, parts, upto_part + 1) < at + tiles) ++upto_part;
+                record[0] = upto_part - static_cast<int>(blockIdx.x);
                 record[1] = piece.query0;
                 record[2] = piece.tokens;
                 record[3] = piece.kv_head;
@@ -385,7 +406,14 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               offset = 0;
               ok = room();
               if (ok) hand_out(piece);
+              if (ahead) {
+                ahead = false;
+                tile = first - 1;
+                offset = first_offset;
+                at = first_at;
+              }
             }
+            if (last >= 0) at = run_end;
           }
           offset = 0;
           if (++s == p.sequences) {

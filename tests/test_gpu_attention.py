@@ -170,6 +170,19 @@ def test_chunk_reports_lengths_beyond_the_table(attn, cuda_device):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("dim,news,past,window", [(64, 4096, 0, 100), (256, 4096, 37, 300), (256, 1000, 9000, 0), (512, 700, 5000, 0)])
+def test_chunk_of_many_query_tiles(attn, cuda_device, dim, news, past, window):
+    """Runs of key tiles inside one sequence, longer and shorter than a query tile's, that begin and end inside them."""
+    page, heads = 64, 16
+    batch, pages = make_batch(attn, [news], [news + past], page, cuda_device, 2)
+    cache = attn.KvCache(randn((pages, page, 1, dim), cuda_device, 1), randn((pages, page, 1, dim), cuda_device, 2))
+    q = randn((news, heads, dim), cuda_device, 3)
+    k, v = gathered(cache, batch, 0, news + past)
+    got = attn.chunk_attention(q, cache, batch, dim ** -0.5, window)
+    cache.check()
+    ref.within(got, *ref.attention(q, k, v, past, dim ** -0.5, window))
+
+
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 256), (512, 32)])
 def test_chunk_reports_pages_outside_the_cache(attn, cuda_device, dim, page):
     """One that a row sees reads as zeros and is reported; those in front of a window and behind the last key are nobody's."""
