@@ -347,6 +347,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > in_head)) - 1;
         const long long in_front = __shfl_sync(0xffffffffu, upto, (owner + 31) & 31);
         long long offset = in_head - before - (owner > 0 ? in_front : 0);
+        const long long of_first = __shfl_sync(0xffffffffu, upto, owner) - (owner > 0 ? in_front : 0);  // key tiles of the run's first sequence
         s += owner;
         while (ok && at < run_end) {
           load_sequences(s & ~31);
@@ -354,21 +355,28 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const int length = __shfl_sync(0xffffffffu, lane_length, s & 31);
           if (news > 0) {
             const AttnSequence q = attn_sequence(news, length, step);
-            int tile = attn_find_query_tile(q, offset, step, p.window);
             // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as when a
             // chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of each
-            // one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 535 us).
-            int last = -1;
+            // one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 533 us).
+            int tile = 0, last = -1;
             long long end = run_end;
-            const long long ends_at = offset + run_end - at;
-            if (offset > 0 && tile + 1 < q.query_tiles && ends_at <= attn_tiles_before(q, q.query_tiles, step, p.window)) {
-              const int ends_in = attn_find_query_tile(q, ends_at - 1, step, p.window);
-              if (ends_in > tile) {
-                last = ends_in;
-                end = run_end - (ends_at - attn_tiles_before(q, last, step, p.window));
+#pragma unroll 1  // (a short reply's time is that of code fetched for the first time: this only once)
+            for (int i = q.query_tiles > 1 && offset > 0 && offset + (run_end - at) <= of_first ? 1 : 0; i >= 0; --i) {
+              const long long target = i > 0 ? offset + (run_end - at) - 1 : offset;
+              const int found = attn_find_query_tile(q, target, step, p.window);
+              const long long begin = attn_tiles_before(q, found, step, p.window);
+              if (i > 0) {
+                last = found;
+                end = run_end - (target + 1 - begin);
+              } else {
+                tile = found;
+                offset -= begin;
               }
             }
-            offset -= attn_tiles_before(q, tile, step, p.window);
+            if (last == tile) {
+              last = -1;
+              end = run_end;
+            }
             const int first = tile;
             const long long first_offset = offset, first_at = at;
             bool ahead = last >= 0;
