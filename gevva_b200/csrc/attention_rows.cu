@@ -129,7 +129,7 @@ struct AppendParams {
   AttnRows q, k, v;
   AttnPages pages;
   const int* token_offsets;
-  int sequences, heads, kv_heads;
+  int sequences, tokens, heads, kv_heads;
   const double* frequencies;
   int half;        // frequencies: the pairs (j, half + j) turn
   int page_shift;
@@ -140,15 +140,16 @@ struct AppendParams {
   int* status;
 };
 
-// A CTA takes one token, so that an angle is worked out once for all heads.  A thread holds eight pairs of a head: the two halves of a
+// A CTA takes a token, or one after the other where there are many, so that an angle is worked out once for all heads.  A thread holds eight pairs of a head: the two halves of a
 // pair come from two 16-byte vectors, (u, half / 8 + u) where pairs turn and two neighbours behind them, so nothing is exchanged.  Its first
-// vectors are asked for before the token's place is looked up.
-// 4608 tokens of 32 heads of 256, packed: 28.8 us of bytes; through shared memory, a vector of eight a thread: 106 us.
+// vectors are asked for before the token's place is looked up, behind the last ones of the token before.
+// 4608 tokens of 32 heads of 256, packed: 39.0 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
+constexpr int kAppendThreads = 512, kAppendManyThreads = 128, kAppendManyCtas = 5;  // (six of an SM: 80 registers, which do not hold it all)
 template <int kDim, int kThreads>
-__global__ void __launch_bounds__(kThreads, 768 / kThreads) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAppendManyCtas : 1) kv_append_kernel(const AppendParams p) {
   constexpr int kLanes = kDim / 16;  // threads of a head
+  constexpr bool kMany = kThreads == kAppendManyThreads;
   __shared__ alignas(16) float cosines[kMaxDim / 2], sines[kMaxDim / 2];
-  const int token = blockIdx.x;
   const int u = threadIdx.x % kLanes, in_block = threadIdx.x / kLanes, heads_at_once = blockDim.x / kLanes;
   const int eighth = p.half / 8;
   const bool turns = u < eighth;
@@ -157,32 +158,38 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) kv_append_kernel(con
   grid_launch_dependents();
   grid_dependency_wait();
 
-  const auto source = [&](int h) {
+  const auto source = [&](int token, int h) {
     const AttnRows& from = h < p.heads ? p.q : h < p.heads + p.kv_heads ? p.k : p.v;
     const int head = h < p.heads ? h : h < p.heads + p.kv_heads ? h - p.heads : h - p.heads - p.kv_heads;
     return reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(from.data) + token * from.token_stride + head * from.head_stride);
   };
   uint4 a[2], b[2];  // of two heads, asked for together
-  const auto ask = [&](int first) {
+  const auto ask = [&](int token, int first) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int h = first + k * heads_at_once;
       a[k] = b[k] = make_uint4(0, 0, 0, 0);
       if (h < total) {
-        a[k] = source(h)[low];
-        b[k] = source(h)[high];
+        a[k] = source(token, h)[low];
+        b[k] = source(token, h)[high];
       }
     }
   };
-  ask(in_block);
+  ask(blockIdx.x, in_block);
 
+#pragma unroll 1
+  for (int token = blockIdx.x; token < p.tokens; token += gridDim.x) {
+  const int next_token = kMany ? token + static_cast<int>(gridDim.x) : p.tokens;
   // the sequence: offsets up to the token's
   int upto = 0;
   for (int base = 0; base <= p.sequences; base += blockDim.x) {
     const int s = base + static_cast<int>(threadIdx.x);
     upto += __syncthreads_count(s <= p.sequences && p.token_offsets[s] <= token);
   }
-  if (upto == 0 || upto > p.sequences) return;  // a row in front of the first or behind the last sequence: left as it was
+  if (upto == 0 || upto > p.sequences) {  // a row in front of the first or behind the last sequence: left as it was
+    if (next_token < p.tokens) ask(next_token, in_block);
+    continue;
+  }
   const int sequence = upto - 1;
   const int position = p.pages.lengths[sequence] - p.token_offsets[upto] + token;
   const int page_index = position >> p.page_shift;
@@ -209,7 +216,8 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) kv_append_kernel(con
 #pragma unroll 1
   for (int first_head = in_block; first_head < total; first_head += 2 * heads_at_once) {
   const uint4 low_now[2] = {a[0], a[1]}, high_now[2] = {b[0], b[1]};
-  if (first_head + 2 * heads_at_once < total) ask(first_head + 2 * heads_at_once);
+  const bool more = first_head + 2 * heads_at_once < total;
+  if (more || next_token < p.tokens) ask(more ? token : next_token, more ? first_head + 2 * heads_at_once : in_block);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int h = first_head + k * heads_at_once;
@@ -272,6 +280,8 @@ __global__ void __launch_bounds__(kThreads, 768 / kThreads) kv_append_kernel(con
     }
   }
   }
+  if constexpr (kMany) __syncthreads();  // (the angles are another token's next)
+  }
 }
 
 }  // namespace
@@ -313,6 +323,7 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
   p.pages = call.pages;
   p.token_offsets = call.token_offsets;
   p.sequences = call.sequences;
+  p.tokens = call.tokens;
   p.heads = call.heads;
   p.kv_heads = call.kv_heads;
   p.frequencies = call.frequencies;
@@ -327,17 +338,20 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
   p.status = call.status;
   while ((1 << p.page_shift) < call.pages.page_size) ++p.page_shift;
   // Threads for all heads of a token at once; with tokens for all SMs several times over four warps a token, so that more
-  // tokens' chains of look-ups run side by side (64 tokens 4.3 and 5.6 us, 4608 tokens 47 and 40 us with up to eight warps and four).
+  // tokens' chains of look-ups run side by side (64 tokens 4.3 and 5.6 us, 4608 tokens 47 and 41 us with up to eight warps and four).
   const int wanted = ((call.heads + 2 * call.kv_heads) * (call.dim / 16) + 31) / 32 * 32;
   const bool many = call.tokens >= 4 * sm_count;
-  const int most = many ? 128 : 512;
-  const dim3 grid(call.tokens), block(wanted < most ? wanted : most);
+  const int most = many ? kAppendManyThreads : kAppendThreads;
+  const dim3 grid(many && call.tokens > kAppendManyCtas * sm_count ? kAppendManyCtas * sm_count : call.tokens), block(wanted < most ? wanted : most);
+#define GV_APPEND(dim) \
+  launch_chained(many ? kv_append_kernel<dim, kAppendManyThreads> : kv_append_kernel<dim, kAppendThreads>, grid, block, 0, stream, p)
   switch (call.dim) {
-    case 64: return launch_chained(many ? kv_append_kernel<64, 128> : kv_append_kernel<64, 512>, grid, block, 0, stream, p);
-    case 128: return launch_chained(many ? kv_append_kernel<128, 128> : kv_append_kernel<128, 512>, grid, block, 0, stream, p);
-    case 256: return launch_chained(many ? kv_append_kernel<256, 128> : kv_append_kernel<256, 512>, grid, block, 0, stream, p);
-    default: return launch_chained(many ? kv_append_kernel<512, 128> : kv_append_kernel<512, 512>, grid, block, 0, stream, p);
+    case 64: return GV_APPEND(64);
+    case 128: return GV_APPEND(128);
+    case 256: return GV_APPEND(256);
+    default: return GV_APPEND(512);
   }
+#undef GV_APPEND
 }
 
 }  // namespace gv

@@ -286,6 +286,33 @@ def test_append(attn, cuda_device, dim, news, lengths, heads, kv_heads, page, ro
         assert torch.equal(now, old)  # nothing else has been written
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 1), (16, 8)])
+def test_append_of_many_tokens(attn, cuda_device, dim, heads, kv_heads):
+    """More tokens than are in work at a time, with rows in front of the first and behind the last sequence and a sequence without pages:
+    the same bits as a few tokens at a time."""
+    news, page, tokens = [700, 0, 1, 900, 600], 32, 2300
+    batch, pages = make_batch(attn, news, [n + 40 for n in news], page, cuda_device, 2)
+    batch.token_offsets += 30
+    batch.table[2] = -1
+    q, k, v = (randn((tokens, h, dim), cuda_device, 3 + i) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    weight = randn((dim,), cuda_device, 6)
+    freq = torch.rand(dim // 4, dtype=torch.float64, device=cuda_device)
+
+    norms = (weight, weight, True, 1e-6)
+    cache, want_cache = (attn.KvCache.empty(pages, page, kv_heads, dim, cuda_device) for _ in range(2))
+    got = attn.kv_append(q, k, v, cache, batch, freq, *norms, packed=True)
+    offsets = batch.token_offsets.tolist()
+    for s, (begin, end) in enumerate(zip(offsets, offsets[1:])):
+        for at in range(begin, end, 300):
+            to = min(at + 300, end)
+            part = attn.PagedBatch(offsets_of([to - at], cuda_device), batch.lengths[s:s + 1] - (end - to), batch.table[s:s + 1])
+            for x, y in zip(got, attn.kv_append(q[at:to], k[at:to], v[at:to], want_cache, part, freq, *norms, packed=True)):
+                assert torch.equal(x[at:to], y), (s, at)
+    assert cache.last_status() == want_cache.last_status() == -7
+    assert torch.equal(cache.k, want_cache.k) and torch.equal(cache.v, want_cache.v) and cache.k.any()
+
+
 def test_append_without_pages_and_behind_the_last_sequence(attn, cuda_device):
     page, dim = 16, 64
     cache = attn.KvCache.empty(3, page, 1, dim, cuda_device)
