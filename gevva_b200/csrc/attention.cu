@@ -5,30 +5,34 @@
 //
 // in one pass over the keys: a row keeps a reference m_i, the sum of its p and the sum of p * v.  The sums may be taken against any
 // reference, so m_i follows the row's maximum only when that has grown by more than 8 binary orders (p stays below 256); only then is what
-// has been summed scaled down.  p is rounded to bf16 for its product with v (2^-9 of each term, as v itself is); its sum is of the unrounded values.
+// has been summed scaled down.  p is rounded to bf16 for its product with v (2^-8 of each term at most, as v itself was); its sum is of the
+// unrounded values.
 //
 // A query tile is 128 rows: floor(128 / group) tokens times the query heads of one key head, so that a key tile of 128 keys is read
-// once for all of them, with one token as with many.  Scores and outputs are products of the tensor pipe (tcgen05.mma, M = 128): S = Q K^T with both operands
-// in shared memory, O += P V with P in tensor memory, where the softmax threads leave it over the scores it came from.
+// once for all of them, with one token as with many.  Scores and outputs are products of the tensor pipe (tcgen05.mma, M = 128): S = Q K^T
+// with both operands in shared memory, O += P V with P in tensor memory, where the softmax threads leave it over the scores it came from.
 //   warp 0    fetches Q, K and V by TMA, a page's slots at a time where the keys are paged
-//   warp 1    issues the products, by one thread: the tensor pipe holds few of them ahead, so an issuer's votes and branches are time that it
-//             stands still (heads of 512: 1190 -> 1068 us; with a second issuer for the outputs 1295, since the two kinds of product then alternate)
+//   warp 1    issues the products, by one thread: the tensor pipe holds few of them ahead, so an issuer's votes and branches are time
+//             that it stands still (heads of 512: 1190 -> 1068 us; with a second issuer for the outputs 1295, since the two kinds of
+//             product then alternate)
 //   warp 2    works out the pieces of work, a step ahead of the others
 //   warps 4+  softmax and epilogue, a row per thread, by two warpgroups
-// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile. Its key tiles are
-// taken by the warpgroups in turn, and the scores of the next are worked out while the softmax of this one runs, over the end of a piece too; a key
-// tile takes the tensor pipe 2048 cycles, and half as much again for 512, whose scores both items work out.
+// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile. Its
+// key tiles are taken by the warpgroups in turn, and the scores of the next are worked out while the softmax of this one runs, over the
+// end of a piece too; a key tile takes the tensor pipe 2048 cycles, and half as much again for 512, whose scores both items work out.
 // Heads of 64 and 128: two query tiles, a warpgroup each, since there a tile's exponentials take as long as its products or longer.
 //
-// Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the items, a sequence's
-// last and longest first, further ones by cancelling launches that have not started (clusterlaunchcontrol).  Chunks: a CTA takes an equal
-// run of key tiles, whatever the sequences' lengths, which only the device knows; an item that a run's end cuts leaves sums in the
-// workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
+// Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the
+// items, a sequence's last and longest first, further ones by cancelling launches that have not started (clusterlaunchcontrol).  Chunks:
+// a CTA takes an equal run of key tiles, whatever the sequences' lengths, which only the device knows; an item that a run's end cuts
+// leaves sums in the workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
 //
-// What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: the pace at which products are issued beside the softmax warps, some 80 to 95 cycles
-// one instead of the tensor pipe's 64: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128 1216, 32 of 64 718 (exponentials), 16 of 512 1050 (1575 with the
-// scores that are worked out twice).  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
-// latencies, 15 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
+// What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128
+// 1216, 32 of 64 718, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
+// bytes a cycle a key tile's products and TMA writes take 2560 and 4096 cycles, more than the tensor pipe (4608 tokens, heads of 512:
+// 371 us, without the writes 286).  Heads of 128: products issued at 80 to 95 cycles instead of 64 beside the softmax warps.  Heads
+// of 64: exponentials.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
+// latencies, 14 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -43,15 +47,15 @@ namespace {
 
 constexpr int kRows = 128;         // rows of a query tile
 constexpr int kKeys = kAttnKeys;   // keys of a key tile
-constexpr int kPieceSlots = 3;     // pieces in work at most: one whose outputs are read, one whose scores are, and one whose operands are fetched
-// Items that CTAs take from one another are better not taken far ahead (1500, 1, 2049 and 1058 tokens through a window of 1024: 67.7 -> 65.7 us), but with heads of
-// 64 the time to the next counts more (8192 tokens: 383 and 391 us).
+constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, one whose operands are fetched
+// Items that CTAs take from one another are better not taken far ahead (1500, 1, 2049 and 1058 tokens through a window of 1024: 67.7 ->
+// 65.7 us), but with heads of 64 the time to the next counts more (8192 tokens: 383 and 391 us).
 template <int kTiles, bool kPaged>
 constexpr uint32_t kSlotsOf = kPaged || kTiles == 2 ? kPieceSlots : 2;
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
 constexpr float kGrowth = 8.0f;    // binary orders by which a row's maximum may exceed its reference
-constexpr int kLeastRun = 1;       // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256: 16.0 us,
-                                   // with 2 16.4, with 4 20.8)
+constexpr int kLeastRun = 1;       // key tiles of the shortest run that a CTA is given (one reply of 700 tokens, 8 key heads of 256:
+                                   // 16.0 us, with 2 16.4, with 4 20.8)
 
 // One run of key tiles of one item.
 struct Piece {
@@ -110,7 +114,8 @@ struct AttnSmem {
   uint64_t o_free[kTiles];    // the outputs of the last piece have been read
   uint64_t piece_full[kPieceSlots], piece_empty[kPieceSlots];
   uint64_t v_landed[2];       // values of a tile that has rows to be cleared, by softmax warpgroup
-  // One query tile: the warpgroups take the key tiles in turn, and hand each row's reference and sum on (a barrier for each quarter's warps).
+  // One query tile: the warpgroups take the key tiles in turn, and hand each row's reference and sum on (a barrier for each quarter's
+  // warps).
   uint64_t reference_ready[2][4], sum_ready[2][4];
   uint64_t next_full;
   alignas(16) uint4 next_item;  // answer to a request for another item
@@ -144,9 +149,9 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// The same for two exponents on the multiply-add units: 2^n of the nearest whole n into the exponent, and for what is left, in [-1/2, 1/2], the polynomial
-// of degree four with the smallest largest relative error (2.7e-6, by iterated reweighted least squares), far below the rounding of p to
-// bf16.  Zero below 2^-126, as from the other.
+// The same for two exponents on the multiply-add units: 2^n of the nearest whole n into the exponent, and for what is left, in [-1/2,
+// 1/2], the polynomial of degree four with the smallest largest relative error (2.7e-6, by iterated reweighted least squares), far below
+// the rounding of p to bf16.  Zero below 2^-126, as from the other.
 __device__ __forceinline__ void exp2_by_polynomial(unsigned long long x, float& a, float& b) {
   constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which then stands in the low bits
   const unsigned long long t = add2(x, two(kShift, kShift));
@@ -184,8 +189,8 @@ __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::
 
 // 32 bytes, to an address that is a multiple of that.
 __device__ __forceinline__ void store_32(void* to, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
-               "r"(v[6]), "r"(v[7])
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
 // D (+)= A B^T, bf16 operands, fp32 sums, K = 16; A from shared memory or from tensor memory.
@@ -200,8 +205,8 @@ __device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, u
                : "memory");
 }
 
-// Instruction descriptors: fp32 sums (bit 4), bf16 operands (1 at [7,10) and [10,13)), B with its rows (keys) along K instead of N for the values
-// (bit 16), N at [17,23) in units of 8, M at [24,29) in units of 16.
+// Instruction descriptors: fp32 sums (bit 4), bf16 operands (1 at [7,10) and [10,13)), B with its rows (keys) along K instead of N for
+// the values (bit 16), N at [17,23) in units of 8, M at [24,29) in units of 16.
 constexpr uint32_t kIdescScores = (1u << 4) | (1u << 7) | (1u << 10) | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
 template <int kColumns>
 constexpr uint32_t kIdescValues = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((kColumns >> 3) << 17) | ((kRows >> 4) << 24);
@@ -347,7 +352,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > in_head)) - 1;
         const long long in_front = __shfl_sync(0xffffffffu, upto, (owner + 31) & 31);
         long long offset = in_head - before - (owner > 0 ? in_front : 0);
-        const long long of_first = __shfl_sync(0xffffffffu, upto, owner) - (owner > 0 ? in_front : 0);  // key tiles of the run's first sequence
+        const long long of_first = __shfl_sync(0xffffffffu, upto, owner) - (owner > 0 ? in_front : 0);  // of the run's first sequence
         s += owner;
         while (ok && at < run_end) {
           load_sequences(s & ~31);
@@ -355,9 +360,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const int length = __shfl_sync(0xffffffffu, lane_length, s & 31);
           if (news > 0) {
             const AttnSequence q = attn_sequence(news, length, step);
-            // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as when a
-            // chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of each
-            // one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 533 us).
+            // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as
+            // when a chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of
+            // each one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 533 us).
             int tile = 0, last = -1;
             long long end = run_end;
 #pragma unroll 1  // (a short reply's time is that of code fetched for the first time: this only once)
@@ -589,7 +594,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
         for (int i = 0; i < kBoxes; ++i) {
           const int t = i / (kDim / 64), c = i % (kDim / 64);
-          tma_load_3d(smem->queries[t] + c * kColumnBytes, &map_q, &smem->q_full, 64 * c, piece.kv_head * p.group, piece.query0 + t * p.step);
+          tma_load_3d(smem->queries[t] + c * kColumnBytes, &map_q, &smem->q_full, 64 * c, piece.kv_head * p.group,
+                      piece.query0 + t * p.step);
         }
       }
       __syncwarp();
@@ -628,8 +634,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
     if (elect_one()) {
-    // The tensor pipe holds few instructions ahead, so what lies between two batches of products is time that it stands still: one wait for all that a
-    // batch needs (a lane for each barrier), and few, wide products.
+    // The tensor pipe holds few instructions ahead, so what lies between two batches of products is time that it stands still: one wait
+    // for all that a batch needs (a lane for each barrier), and few, wide products.
     const uint64_t q_desc = make_smem_desc(smem_u32(smem->queries[0]), 1024, 2);
     const uint64_t k_desc = make_smem_desc(smem_u32(smem->stage[0]), 1024, 2);
     // values: 64 columns a swizzle row, the next 64 a column block further (leading offset), keys eight rows a group (stride offset)
@@ -644,24 +650,28 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         phase ^= 1u;
       }
     };
-    // Waits until the next `count` stages are there, and `other`'s phase is over (null: nothing else); all are looked at before any is waited for.
+    // Waits until the next `count` stages are there, and `other`'s phase is over (null: nothing else); all are looked at before any is
+    // waited for.
     const auto ready = [&](uint32_t count, uint64_t* other, uint32_t other_parity) {
       const uint32_t behind = stage + 1 == S::kStages ? 0 : stage + 1, behind_phase = stage + 1 == S::kStages ? phase ^ 1u : phase;
       const bool first = mbar_try_wait(&smem->full[stage], phase);
       const bool second = count < 2 || mbar_try_wait(&smem->full[behind], behind_phase);
       const bool third = !other || mbar_try_wait(other, other_parity);
       if (first && second && third) return true;
-      return wait_or_abort(&smem->full[stage], phase, smem, p.status) && (count < 2 || wait_or_abort(&smem->full[behind], behind_phase, smem, p.status)) &&
+      return wait_or_abort(&smem->full[stage], phase, smem, p.status) &&
+             (count < 2 || wait_or_abort(&smem->full[behind], behind_phase, smem, p.status)) &&
              (!other || wait_or_abort(other, other_parity, smem, p.status));
     };
     const auto wait_for = [&](uint64_t* bar, uint32_t parity) { return wait_or_abort(bar, parity, smem, p.status); };
-    // The products of one stage: 128 (64) of the columns that scores sum over; or of the outputs' columns, of one stage or of two that lie side by side.
+    // The products of one stage: 128 (64) of the columns that scores sum over; or of the outputs' columns, of one stage or of two that
+    // lie side by side.
     const auto scores_of_stage = [&](uint32_t d, int tile, int part) {
       const uint64_t b = k_desc + stage * (S::kStageBytes >> 4);
 #pragma unroll
       for (int i = 0; i < S::kStageDim / 16; ++i) {
         const uint32_t at = (i / 4) * kColumnBytes + (i % 4) * 32;
-        mma_shared(d, q_desc + ((tile * S::kQueryTileBytes + part * 2 * kColumnBytes + at) >> 4), b + (at >> 4), kIdescScores, part > 0 || i > 0 ? 1u : 0u);
+        mma_shared(d, q_desc + ((tile * S::kQueryTileBytes + part * 2 * kColumnBytes + at) >> 4), b + (at >> 4), kIdescScores,
+                   part > 0 || i > 0 ? 1u : 0u);
       }
     };
     const auto values_of_stage = [&](uint32_t d, uint32_t at_stage, uint32_t a, uint32_t accumulate, uint32_t descriptor) {
@@ -835,8 +845,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   } else {
     // ---------------- softmax and epilogue ----------------
     more_registers();
-    // This warpgroup's query tile; or, of the one query tile there is, the key tiles that are its turn: those whose scores stand in its half
-    // of the score columns.
+    // This warpgroup's query tile; or, of the one query tile there is, the key tiles that are its turn: those whose scores stand in its
+    // half of the score columns.
     const int own = (warp - 4) / 4;
     const int tile_of_rows = kTiles == 2 ? own : 0;
     const int quarter = warp & 3;              // the tensor-memory lanes this warp may read
@@ -928,8 +938,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (lane == 0) mbar_arrive(&smem->reference_ready[own][quarter]);
           }
           if (any_grow && j > 0) {
-            // (A wait can tell a phase from the one before it, not from the one after the next: each of these barriers is one phase behind at most, since
-            // the scores at hand were asked for behind the outputs of two tiles before, and one ahead at most.)
+            // (A wait can tell a phase from the one before it, not from the one after the next: each of these barriers is one phase
+            // behind at most, since the scores at hand were asked for behind the outputs of two tiles before, and one ahead at most.)
             const uint32_t before = kTiles == 2 ? n - 1 : (n - 1) >> 1;
             ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[kTiles == 2 ? own : own ^ 1], before & 1u, smem, p.status));
             if (!ok) break;
@@ -953,8 +963,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             for (int i = 0; i < 16; ++i) {
               const unsigned long long v = fma2(two(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, shift2);
               float a, b;
-              // Heads of 64: the exponentials of two query tiles take twice as long as their products; three of eight by the other units (8192 tokens, 32
-              // heads: 425 -> 382 us; heads of 128, a quarter: 451 and 452).
+              // Heads of 64: the exponentials of two query tiles take twice as long as their products; three of eight by the other units
+              // (8192 tokens, 32 heads: 425 -> 382 us; heads of 128, a quarter: 451 and 452).
               if (kTiles == 2 && kDim == 64 && (i % 8 == 2 || i % 8 == 5 || i % 8 == 7)) {
                 exp2_by_polynomial(v, a, b);
               } else {
@@ -1023,10 +1033,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         __nv_bfloat16* out = p.out + static_cast<long long>(piece.query0 + token) * p.out_token_stride +
                              static_cast<long long>(piece.kv_head * p.group + row_head) * p.out_head_stride + column0;
         const size_t partial_row = (static_cast<size_t>(piece.slot < 0 ? 0 : piece.slot) * kTiles + tile_of_rows) * kRows + row;
-        // A store of a row per lane keeps the store unit busy for 32 lines whatever it stores.  So lanes work in pairs: each has 64 bytes of a row, and they
-        // store first the one's, then the other's, 32 bytes each.
+        // A store of a row per lane keeps the store unit busy for 32 lines whatever it stores.  So lanes work in pairs: each has 64 bytes
+        // of a row, and they store first the one's, then the other's, 32 bytes each.
         const bool odd = lane & 1;
-        __nv_bfloat16* other_out = reinterpret_cast<__nv_bfloat16*>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 1));
+        __nv_bfloat16* other_out =
+            reinterpret_cast<__nv_bfloat16*>(__shfl_xor_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), 1));
         const bool other_valid = __shfl_xor_sync(0xffffffffu, valid ? 1 : 0, 1) != 0;
         __nv_bfloat16* const first_out = odd ? other_out + 16 : out;
         __nv_bfloat16* const second_out = odd ? out + 16 : other_out;
@@ -1035,7 +1046,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (piece.slot < 0) {
             uint32_t mine[16], theirs[8];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) mine[k] = pack_bf16x2(__uint_as_float(o[2 * k]) * inverse, __uint_as_float(o[2 * k + 1]) * inverse);
+            for (int k = 0; k < 16; ++k)
+              mine[k] = pack_bf16x2(__uint_as_float(o[2 * k]) * inverse, __uint_as_float(o[2 * k + 1]) * inverse);
 #pragma unroll
             for (int k = 0; k < 8; ++k) theirs[k] = __shfl_xor_sync(0xffffffffu, odd ? mine[k] : mine[8 + k], 1);
             uint32_t first[8], second[8];
@@ -1050,7 +1062,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             float* to = p.partial + partial_row * S::kValueDim + i;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t v[8] = {o[8 * k], o[8 * k + 1], o[8 * k + 2], o[8 * k + 3], o[8 * k + 4], o[8 * k + 5], o[8 * k + 6], o[8 * k + 7]};
+              const uint32_t v[8] = {o[8 * k],     o[8 * k + 1], o[8 * k + 2], o[8 * k + 3],
+                                     o[8 * k + 4], o[8 * k + 5], o[8 * k + 6], o[8 * k + 7]};
               store_32(to + 8 * k, v);
             }
           }
@@ -1089,8 +1102,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // Adds up the sums of the items that the ends of runs have cut: CTA x takes the item that begins in run x and does not end there, its
-// rows dealt out over the warps of gridDim.y CTAs.  Bound by latency: the record says where the parts are, and what of them is asked for, four
-// at a time, waits for nothing else.
+// rows dealt out over the warps of gridDim.y CTAs.  Bound by latency: the record says where the parts are, and what of them is asked for,
+// four at a time, waits for nothing else.
 template <int kValueDim>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p, int tiles) {
   grid_dependency_wait();
@@ -1217,7 +1230,8 @@ cudaError_t launch_shape(const AttnCall& call, cudaStream_t stream) {
     p.table_stride = c.table_stride;
     p.page_count = c.page_count;
     while ((1 << p.page_shift) < c.page_size) ++p.page_shift;
-    const uint64_t dims[4] = {kDim, static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(call.kv_heads), static_cast<uint64_t>(c.page_count)};
+    const uint64_t dims[4] = {kDim, static_cast<uint64_t>(c.page_size), static_cast<uint64_t>(call.kv_heads),
+                              static_cast<uint64_t>(c.page_count)};
     const uint32_t box[4] = {64, static_cast<uint32_t>(c.page_size < kKeys ? c.page_size : kKeys), 1, 1};
     const long long key_strides[3] = {c.key_slot_stride, c.key_head_stride, c.key_page_stride};
     const long long value_strides[3] = {c.value_slot_stride, c.value_head_stride, c.value_page_stride};
@@ -1243,7 +1257,8 @@ cudaError_t launch_shape(const AttnCall& call, cudaStream_t stream) {
   e = launch_chained(kernel, dim3(static_cast<unsigned>(items)), dim3(S::kThreads), kSmemBytes, stream, map_q, map_k, map_v, p);
   if (e != cudaSuccess) return e;
   if constexpr (kPaged)
-    e = launch_chained(attention_join_kernel<S::kValueDim>, dim3(static_cast<unsigned>(items), kJoinColumns), dim3(256), 0, stream, p, kTiles);
+    e = launch_chained(attention_join_kernel<S::kValueDim>, dim3(static_cast<unsigned>(items), kJoinColumns), dim3(256), 0, stream, p,
+                       kTiles);
   return e;
 }
 

@@ -84,7 +84,8 @@ void fill_attention(gv::AttnCall* call, const Args& a) {
 extern "C" {
 
 int gevva_attn_norm(const void* x, const void* weight, void* out, int rows, int width, float eps, gevva_stream_t stream) {
-  if (rows < 0 || !aligned_for(x, rows) || !aligned(weight) || !aligned_for(out, rows) || width < 8 || width > 32768 || width % 8 || !(eps >= 0.0f))
+  if (rows < 0 || !aligned_for(x, rows) || !aligned(weight) || !aligned_for(out, rows) || width < 8 || width > 32768 || width % 8 ||
+      !(eps >= 0.0f))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (rows == 0) return GEVVA_MOE_OK;
   gv::BlockNormCall call{};
@@ -99,9 +100,9 @@ int gevva_attn_norm(const void* x, const void* weight, void* out, int rows, int 
 
 int gevva_attn_norm_add(const void* x, const void* weight, const void* residual, const void* gate, const void* scale,
                         const void* next_weight, void* out, void* next, int rows, int width, float eps, gevva_stream_t stream) {
-  if (rows < 0 || !aligned_for(x, rows) || !aligned(weight) || !aligned_for(residual, rows) || !aligned_or_null(gate) || (reinterpret_cast<uintptr_t>(scale) & 1) ||
-      !aligned_or_null(next_weight) || !aligned_for(out, rows) || !aligned_or_null(next) || (rows > 0 && !next_weight != !next) || width < 8 ||
-      width > 32768 || width % 8 || !(eps >= 0.0f))
+  if (rows < 0 || !aligned_for(x, rows) || !aligned(weight) || !aligned_for(residual, rows) || !aligned_or_null(gate) ||
+      (reinterpret_cast<uintptr_t>(scale) & 1) || !aligned_or_null(next_weight) || !aligned_for(out, rows) || !aligned_or_null(next) ||
+      (rows > 0 && !next_weight != !next) || width < 8 || width > 32768 || width % 8 || !(eps >= 0.0f))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (rows == 0) return GEVVA_MOE_OK;
   gv::BlockNormCall call{};
@@ -155,7 +156,8 @@ int gevva_attn_prompt(const gevva_attn_prompt_args* a, gevva_stream_t stream) {
   if (!a || !heads_ok(a->tokens, a->heads, a->kv_heads, a->dim) ||
       !rows_ok(&call.q, a->q, a->q_token_stride, a->q_head_stride, a->tokens, a->heads, a->dim) ||
       !rows_ok(&call.k, a->k, a->k_token_stride, a->k_head_stride, a->tokens, a->kv_heads, a->dim) ||
-      !rows_ok(&call.v, a->v, a->v_token_stride, a->v_head_stride, a->tokens, a->kv_heads, a->dim) || !a->token_offsets || a->sequences < 1 ||
+      !rows_ok(&call.v, a->v, a->v_token_stride, a->v_head_stride, a->tokens, a->kv_heads, a->dim) || !a->token_offsets ||
+      a->sequences < 1 ||
       !attention_ok(a->tokens, a->scale, a->window) || !aligned_32(a->out, a->tokens) || a->reserved)
     return GEVVA_MOE_BAD_ARGUMENT;
   if (a->tokens == 0) return GEVVA_MOE_OK;

@@ -1,6 +1,6 @@
-// The row kernels around attention (declared in include/gevva_moe.h): RMS norms in front of and behind a block, and what happens to queries, keys and
-// values between their projection and attention.  All are bound by HBM, or by latency for a few tokens: a value is read once, held in registers in
-// 32 bits and written once.
+// The row kernels around attention (declared in include/gevva_moe.h): RMS norms in front of and behind a block, and what happens to
+// queries, keys and values between their projection and attention.  All are bound by HBM, or by latency for a few tokens: a value is read
+// once, held in registers in 32 bits and written once.
 #include "gv_attention.h"
 #include "gv_common.cuh"
 #include "gv_gemm_parts.cuh"
@@ -27,8 +27,8 @@ __device__ __forceinline__ float squares(const float (&x)[8]) {
 }
 
 // ---- RMS norms in front of and behind a block ------------------------------------------------------------
-// A row is held by a warp or by a block; each thread has kEach times eight values of it, as they came, in registers: the second norm works its
-// row out again instead of keeping it in 32 bits.
+// A row is held by a warp or by a block; each thread has kEach times eight values of it, as they came, in registers: the second norm
+// works its row out again instead of keeping it in 32 bits.
 struct NormParams {
   const uint4 *x, *weight, *residual, *gate, *next_weight;
   const __nv_bfloat16* scale;
@@ -140,11 +140,13 @@ struct AppendParams {
   int* status;
 };
 
-// A CTA takes a token, or one after the other where there are many, so that an angle is worked out once for all heads.  A thread holds eight pairs of a head: the two halves of a
-// pair come from two 16-byte vectors, (u, half / 8 + u) where pairs turn and two neighbours behind them, so nothing is exchanged.  Its first
-// vectors are asked for before the token's place is looked up, behind the last ones of the token before.
-// 4608 tokens of 32 heads of 256, packed: 39.0 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
-constexpr int kAppendThreads = 512, kAppendManyThreads = 128, kAppendManyCtas = 5;  // (six of an SM: 80 registers, which do not hold it all)
+// A CTA takes a token, or one after the other where there are many, so that an angle is worked out once for all heads.  A thread holds
+// eight pairs of a head: the two halves of a pair come from two 16-byte vectors, (u, half / 8 + u) where pairs turn and two neighbours
+// behind them, so nothing is exchanged.  Its first vectors are asked for before the token's place is looked up, behind the last ones of
+// the token before.
+// 4608 tokens of 32 heads of 256, packed: 38.6 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
+constexpr int kAppendThreads = 512, kAppendManyThreads = 128;
+constexpr int kAppendManyCtas = 5;  // of an SM (with six: 80 registers, which do not hold it all)
 template <int kDim, int kThreads>
 __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAppendManyCtas : 1) kv_append_kernel(const AppendParams p) {
   constexpr int kLanes = kDim / 16;  // threads of a head
@@ -161,7 +163,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   const auto source = [&](int token, int h) {
     const AttnRows& from = h < p.heads ? p.q : h < p.heads + p.kv_heads ? p.k : p.v;
     const int head = h < p.heads ? h : h < p.heads + p.kv_heads ? h - p.heads : h - p.heads - p.kv_heads;
-    return reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(from.data) + token * from.token_stride + head * from.head_stride);
+    return reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(from.data) + token * from.token_stride +
+                                          head * from.head_stride);
   };
   uint4 a[2], b[2];  // of two heads, asked for together
   const auto ask = [&](int token, int first) {
@@ -271,10 +274,11 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
       reinterpret_cast<uint4*>(out + row * kDim)[high] = second;
     }
     if (kind != 0 && stored) {
-      __nv_bfloat16* cache = kind == 1 ? static_cast<__nv_bfloat16*>(p.pages.keys) + page * p.pages.key_page_stride + slot * p.pages.key_slot_stride +
-                                             head * p.pages.key_head_stride
-                                       : static_cast<__nv_bfloat16*>(p.pages.values) + page * p.pages.value_page_stride +
-                                             slot * p.pages.value_slot_stride + head * p.pages.value_head_stride;
+      const AttnPages& c = p.pages;
+      __nv_bfloat16* cache = kind == 1 ? static_cast<__nv_bfloat16*>(c.keys) + page * c.key_page_stride + slot * c.key_slot_stride +
+                                             head * c.key_head_stride
+                                       : static_cast<__nv_bfloat16*>(c.values) + page * c.value_page_stride + slot * c.value_slot_stride +
+                                             head * c.value_head_stride;
       reinterpret_cast<uint4*>(cache)[low] = first;
       reinterpret_cast<uint4*>(cache)[high] = second;
     }
@@ -302,8 +306,8 @@ cudaError_t launch_block_norm(const BlockNormCall& call, int sm_count, cudaStrea
   p.eps = call.eps;
   if (p.vectors <= 32) return launch_chained(block_norm_kernel<false, 1, 128>, dim3((call.rows + 3) / 4), dim3(128), 0, stream, p);
   const dim3 grid(call.rows);
-  // Four warps a row where there are rows for all SMs several times over: sixteen rows of an SM at a time have more bytes on their way than five of
-  // eleven warps.
+  // Four warps a row where there are rows for all SMs several times over: sixteen rows of an SM at a time have more bytes on their way
+  // than five of eleven warps.
   if (p.vectors <= 512 && call.rows >= 4 * sm_count) {
     if (p.vectors <= 128) return launch_chained(block_norm_kernel<true, 1, 128>, grid, dim3(128), 0, stream, p);
     if (p.vectors <= 256) return launch_chained(block_norm_kernel<true, 2, 128>, grid, dim3(128), 0, stream, p);
@@ -342,7 +346,8 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
   const int wanted = ((call.heads + 2 * call.kv_heads) * (call.dim / 16) + 31) / 32 * 32;
   const bool many = call.tokens >= 4 * sm_count;
   const int most = many ? kAppendManyThreads : kAppendThreads;
-  const dim3 grid(many && call.tokens > kAppendManyCtas * sm_count ? kAppendManyCtas * sm_count : call.tokens), block(wanted < most ? wanted : most);
+  const int ctas = kAppendManyCtas * sm_count;
+  const dim3 grid(many && call.tokens > ctas ? ctas : call.tokens), block(wanted < most ? wanted : most);
 #define GV_APPEND(dim) \
   launch_chained(many ? kv_append_kernel<dim, kAppendManyThreads> : kv_append_kernel<dim, kAppendThreads>, grid, block, 0, stream, p)
   switch (call.dim) {

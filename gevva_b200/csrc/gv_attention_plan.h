@@ -3,8 +3,9 @@
 //
 // A sequence of `news` new tokens over `length` keys (the new ones included) has its token i at position length - news + i, which sees
 // the keys up to that position, the last `window` of them only where a window is set.  Tokens are taken `step` at a time (a query
-// tile) and keys 128 at a time (a key tile, counted from the sequence's first key).  An item is one query tile of one key head (and of one half
-// of the value columns, for heads of 512); its work is its number of key tiles, at least one, so that rows that see nothing are written too.
+// tile) and keys 128 at a time (a key tile, counted from the sequence's first key).  An item is one query tile of one key head (and of
+// one half of the value columns, for heads of 512); its work is its number of key tiles, at least one, so that rows that see nothing are
+// written too.
 #pragma once
 
 #ifdef __CUDACC__
@@ -83,14 +84,16 @@ GV_HD long long attn_tiles_before(const AttnSequence& s, int count, int step, in
   long long sum = blind;
   const int full = count < s.query_tiles - 1 ? count : s.query_tiles - 1;  // tiles of whole `step` tokens
   if (full > blind)
-    sum += attn_floor_sum(full - blind, kAttnKeys, step, static_cast<long long>(s.past) + static_cast<long long>(blind + 1) * step + kAttnKeys - 1);
+    sum += attn_floor_sum(full - blind, kAttnKeys, step,
+                          static_cast<long long>(s.past) + static_cast<long long>(blind + 1) * step + kAttnKeys - 1);
   if (count == s.query_tiles) sum += (s.past + s.news + kAttnKeys - 1) / kAttnKeys;
   if (window > 0) {
     const int lead = window - 1 - s.past;
     int from = lead > 0 ? (lead + step - 1) / step : 0;
     if (from < blind) from = blind;
     if (count > from)
-      sum -= attn_floor_sum(count - from, kAttnKeys, step, static_cast<long long>(s.past) + static_cast<long long>(from) * step - window + 1);
+      sum -= attn_floor_sum(count - from, kAttnKeys, step,
+                            static_cast<long long>(s.past) + static_cast<long long>(from) * step - window + 1);
   }
   return sum;
 }
@@ -106,8 +109,8 @@ GV_HD int attn_find_query_tile(const AttnSequence& s, long long at, int step, in
   return low;
 }
 
-// Work, `heads` times the same, is dealt out to at most `parts` CTAs in runs of equal length: to as many for each head where that leaves no more than a
-// sixteenth of them without, to fewer where a run would be shorter than `least` key tiles.
+// Work, `heads` times the same, is dealt out to at most `parts` CTAs in runs of equal length: to as many for each head where that leaves
+// no more than a sixteenth of them without, to fewer where a run would be shorter than `least` key tiles.
 GV_HD int attn_parts(long long work, int parts, int heads, int least) {
   const int even = heads <= parts ? parts / heads * heads : parts;
   if (16 * even >= 15 * parts) parts = even;
