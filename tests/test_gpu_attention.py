@@ -1,8 +1,14 @@
 """The attention operators on a GPU against plain forms in 64 bits."""
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 from tests import attention_ref as ref
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 pytestmark = pytest.mark.gpu
 
@@ -485,6 +491,37 @@ def test_what_a_call_makes_belongs_to_its_stream(attn, cuda_device):
                 held = [torch.empty_like(x) for _ in range(8)]
                 assert all(h.data_ptr() != at for h in held), i
     cache.check()
+
+
+def test_a_process_may_begin_with_a_captured_call(attn, cuda_device):
+    """Nothing has to be called once before it is captured."""
+    code = """
+import torch
+import gevva_b200 as g
+d = torch.device("cuda:0")
+bf16, i32 = torch.bfloat16, torch.int32
+qkv = torch.randn(40, 6, 256, device=d).to(bf16)
+weight, freq = torch.ones(256, dtype=bf16, device=d), torch.ones(128, dtype=torch.float64, device=d)
+cache = g.KvCache.empty(4, 32, 1, 256, d)
+batch = g.PagedBatch(torch.tensor([0, 40], dtype=i32, device=d), torch.tensor([40], dtype=i32, device=d), torch.arange(4, dtype=i32, device=d)[None])
+rows = qkv.view(40, 1536)
+row_weight = torch.ones(1536, dtype=bf16, device=d)
+
+def calls():
+    q, k, v = g.kv_append(*qkv.split((4, 1, 1), 1), cache, batch, freq, weight, weight, packed=True)
+    a, b = g.prompt_attention(q, k, v, batch.token_offsets, 0.06), g.chunk_attention(q, cache, batch, 0.06)
+    return a, b, g.block_norm(rows, row_weight), g.block_norm_add(rows, row_weight, rows)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = calls()
+graph.replay()
+torch.cuda.synchronize()
+for x, y in zip(captured, calls()):
+    assert torch.equal(x, y) and x.any()
+cache.check()
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=ROOT)
 
 
 def test_nothing_to_do(attn, cuda_device):
