@@ -97,6 +97,11 @@ struct Shape {
   static constexpr int kThreads = 128 + 32 * kSoftmaxWarps;
   // Whether a tile's values and the next one's keys fit side by side: scores of the next piece may then be asked for before this one's end.
   static constexpr bool kAhead = kTiles == 1 && kStages >= kKeyStages + kValueStages;
+  // Two query tiles of heads of 64 leave tensor memory for a third score tile: scores are then asked for half a round earlier, and the chain of a
+  // query tile is its softmax alone.  Score tile 2 * (key tile) + (query tile), modulo three.
+  static constexpr bool kSpare = kTiles == 2 && kDim == 64;
+  static constexpr uint32_t kOutputs = kSpare ? 384 : 256;  // first tensor-memory column of the outputs
+  static_assert(!kSpare || (kStages & (kStages - 1)) == 0, "stages are found by position");
   static_assert(kStages > kValueStages, "the values of a tile are in shared memory at the same time");
   static_assert(kTiles == 1 || kDim <= 128, "two query tiles need 2 * (128 + dim) columns of tensor memory");
 };
@@ -108,7 +113,7 @@ struct AttnSmem {
   uint8_t stage[S::kStages][S::kStageBytes];
   uint64_t full[S::kStages], empty[S::kStages];
   uint64_t q_full, q_empty;
-  uint64_t acc_full[2];       // scores: by key tile in turn (one query tile) or by query tile (two)
+  uint64_t acc_full[4];       // scores: by key tile in turn (one query tile), by query tile (two), or by both (2 * query tile + turn)
   uint64_t p_ready[2];
   uint64_t pv_done[2];        // outputs of a key tile are summed up; by key tile in turn or by query tile, like the scores
   uint64_t o_free[kTiles];    // the outputs of the last piece have been read
@@ -239,8 +244,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     mbar_init(&smem->q_full, 1);
     mbar_init(&smem->q_empty, 1);
+    for (int s = 0; s < 4; ++s) mbar_init(&smem->acc_full[s], 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&smem->acc_full[s], 1);
       mbar_init(&smem->p_ready[s], 4);
       mbar_init(&smem->pv_done[s], 1);
     }
@@ -600,11 +605,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       __syncwarp();
       ++q_issued;
-      if constexpr (kTiles == 1) fetch_keys(piece.first_tile, page);
+      constexpr bool kKeysFirst = kTiles == 1 || S::kSpare;  // K0 K1 V0 K2 V1 .., otherwise K0 V0 K1 V1 ..
+      if constexpr (kKeysFirst) fetch_keys(piece.first_tile, page);
       for (int j = 0; ok && j < piece.tiles; ++j) {
         const int tile = piece.first_tile + j;
         const int page_after = page_of(tile + 2);
-        if constexpr (kTiles == 1) {
+        if constexpr (kKeysFirst) {
           if (j + 1 < piece.tiles) fetch_keys(tile + 1, next_page);
         } else {
           fetch_keys(tile, page);
@@ -782,6 +788,61 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
           if (scored) skip_stages(S::kKeyStages);  // the next piece's keys stand behind these values, and have been used
         }
+      } else if constexpr (S::kSpare) {
+        // Score tiles are free again behind the products that read their P: the second query tile's next scores follow the first one's outputs, the
+        // first one's next but one the second one's.
+        const uint32_t ring = 2 * done;  // stages of the pieces before
+        const auto stage_at = [&](uint32_t at) {
+          stage = (ring + at) % S::kStages;
+          phase = ((ring + at) / S::kStages) & 1u;
+        };
+        const auto keys_at = [&](uint32_t j) { stage_at(j > 0 ? 2 * j - 1 : 0); };
+        const auto scores = [&](uint32_t j, int t) {  // (the keys are there)
+          const uint32_t n = done + j;
+          scores_of_stage(tmem_base + (2 * n + t) % 3 * kKeys, t, 0);
+          tc_commit(&smem->acc_full[2 * t + (n & 1u)]);
+          if (t == 1) tc_commit(&smem->empty[stage]);
+        };
+        keys_at(0);
+        ok = ready(1, nullptr, 0);
+        if (!ok) break;
+        scores(0, 0);
+        scores(0, 1);
+        if (tiles > 1) {
+          keys_at(1);
+          ok = ready(1, nullptr, 0);
+          if (!ok) break;
+          scores(1, 0);
+        }
+        for (int j = 0; ok && j < tiles; ++j) {
+          const uint32_t n = done + j;
+          const uint32_t accumulate = j > 0 ? 1u : 0u;
+          if (j == 0) ok = wait_for(&smem->o_free[0], (count & 1u) ^ 1u) && wait_for(&smem->o_free[1], (count & 1u) ^ 1u);
+          stage_at(min(j + 2, tiles) + j);
+          const uint32_t value_stage = stage;
+          if (ok && !seen_keys(piece, j, p.window).all()) {
+            ok = ready(1, nullptr, 0);
+            if (ok) mbar_arrive(&smem->v_landed[0]);
+          }
+          ok = ok && ready(1, &smem->p_ready[0], n & 1u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          values_of_stage(tmem_base + S::kOutputs, value_stage, tmem_base + 2 * n % 3 * kKeys, accumulate, kIdescValues<S::kStageDim>);
+          tc_commit(&smem->pv_done[0]);
+          if (j + 1 < tiles) {
+            keys_at(j + 1);
+            scores(j + 1, 1);
+          }
+          if (j + 2 < tiles) keys_at(j + 2);
+          ok = j + 2 < tiles ? ready(1, &smem->p_ready[1], n & 1u) : wait_for(&smem->p_ready[1], n & 1u);
+          if (!ok) break;
+          tc_fence_after_sync();
+          values_of_stage(tmem_base + S::kOutputs + kDim, value_stage, tmem_base + (2 * n + 1) % 3 * kKeys, accumulate, kIdescValues<S::kStageDim>);
+          tc_commit(&smem->pv_done[1]);
+          tc_commit(&smem->empty[value_stage]);
+          if (j + 2 < tiles) scores(j + 2, 0);
+          if (j + 2 == tiles || tiles == 1) tc_commit(&smem->q_empty);
+        }
       } else {
         // one stage holds a tile's keys, another its values
         ok = ready(1, nullptr, 0);
@@ -853,8 +914,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int row = quarter * 32 + lane;
     const int row_token = row / p.group, row_head = row - row_token * p.group;
     const uint32_t lanes = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-    const uint32_t scores = lanes + own * kKeys;
-    const uint32_t outputs = lanes + 256 + tile_of_rows * kDim;
+    const uint32_t outputs = lanes + S::kOutputs + tile_of_rows * kDim;
     const float c = p.scale_log2;
     uint32_t done = 0, ring = 0;  // key tiles and operand stages of the pieces before
     uint32_t cleared = 0;         // tiles with values that this warpgroup has cleared
@@ -879,8 +939,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll 1
       for (int j = first; j < piece.tiles; j += kTiles == 2 ? 1 : 2) {
         const uint32_t n = done + j;
-        const uint32_t turn = kTiles == 2 ? n : n >> 1;  // of this warpgroup
-        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->acc_full[own], turn & 1u, smem, p.status));
+        const uint32_t scores = lanes + (S::kSpare ? (2 * n + own) % 3 : own) * kKeys;
+        const uint32_t barrier = S::kSpare ? 2 * own + (n & 1u) : own;
+        const uint32_t turn = kTiles == 2 && !S::kSpare ? n : n >> 1;  // of that barrier
+        ok = __all_sync(0xffffffffu, wait_or_abort(&smem->acc_full[barrier], turn & 1u, smem, p.status));
         if (!ok) break;
         tc_fence_after_sync();
         const int key0 = (piece.first_tile + j) * kKeys;
@@ -991,8 +1053,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           ok = __all_sync(0xffffffffu, wait_or_abort(&smem->v_landed[own], cleared & 1u, smem, p.status));
           if (!ok) break;
           ++cleared;
-          // K0 K1 V0 K2 V1 .. with one query tile, K0 V0 K1 V1 .. with two
-          const uint32_t at = ring + (kTiles == 2 ? j * (S::kKeyStages + S::kValueStages) + S::kKeyStages
+          const uint32_t at = ring + (kTiles == 2 && !S::kSpare ? j * (S::kKeyStages + S::kValueStages) + S::kKeyStages
                                                   : min(j + 2, piece.tiles) * S::kKeyStages + j * S::kValueStages);
           if (row < seen.from || row >= seen.to)
             for (int i = 0; i < S::kValueStages; ++i)
