@@ -17,9 +17,10 @@
 //             product then alternate)
 //   warp 2    works out the pieces of work, a step ahead of the others
 //   warps 4+  softmax and epilogue, a row per thread, by two warpgroups
-// Tensor memory holds two score tiles and the outputs.  Heads of 256 and 512 (the value columns of 512 in two items): one query tile. Its
-// key tiles are taken by the warpgroups in turn, and the scores of the next are worked out while the softmax of this one runs, over the
-// end of a piece too; a key tile takes the tensor pipe 2048 cycles, and half as much again for 512, whose scores both items work out.
+// Tensor memory holds two score tiles (three with heads of 64) and the outputs.  Heads of 256 and 512 (the value columns of 512 in two
+// items): one query tile. Its key tiles are taken by the warpgroups in turn, and the scores of the next are worked out while the softmax
+// of this one runs, over the end of a piece too; a key tile takes the tensor pipe 2048 cycles, and half as much again for 512, whose
+// scores both items work out.
 // Heads of 64 and 128: two query tiles, a warpgroup each, since there a tile's exponentials take as long as its products or longer.
 //
 // Work is dealt out in key tiles (gv_attention_plan.h).  Prompts: an item, one query tile of one head, is never cut; CTAs take the
@@ -28,10 +29,10 @@
 // leaves sums in the workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
 //
 // What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128
-// 1216, 32 of 64 718, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
+// 1210, 32 of 64 844, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
 // bytes a cycle a key tile's products and TMA writes take 2560 and 4096 cycles, more than the tensor pipe (4608 tokens, heads of 512:
 // 371 us, without the writes 286).  Heads of 128: products issued at 80 to 95 cycles instead of 64 beside the softmax warps.  Heads
-// of 64: exponentials.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
+// of 64: the softmax warps' instructions.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
 // latencies, 14 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
 #include <cuda.h>
 #include <math_constants.h>
@@ -49,7 +50,7 @@ constexpr int kRows = 128;         // rows of a query tile
 constexpr int kKeys = kAttnKeys;   // keys of a key tile
 constexpr int kPieceSlots = 3;     // pieces in work: one whose outputs are read, one whose scores are, one whose operands are fetched
 // Items that CTAs take from one another are better not taken far ahead (1500, 1, 2049 and 1058 tokens through a window of 1024: 67.7 ->
-// 65.7 us), but with heads of 64 the time to the next counts more (8192 tokens: 383 and 391 us).
+// 65.7 us), but with two query tiles the time to the next counts more (8192 tokens, heads of 64: 383 and 391 us).
 template <int kTiles, bool kPaged>
 constexpr uint32_t kSlotsOf = kPaged || kTiles == 2 ? kPieceSlots : 2;
 constexpr int kColumnBytes = kKeys * 128;  // 64 columns of a tile: 128 rows of 128 bytes, one swizzle row each
@@ -97,8 +98,9 @@ struct Shape {
   static constexpr int kThreads = 128 + 32 * kSoftmaxWarps;
   // Whether a tile's values and the next one's keys fit side by side: scores of the next piece may then be asked for before this one's end.
   static constexpr bool kAhead = kTiles == 1 && kStages >= kKeyStages + kValueStages;
-  // Two query tiles of heads of 64 leave tensor memory for a third score tile: scores are then asked for half a round earlier, and the chain of a
-  // query tile is its softmax alone.  Score tile 2 * (key tile) + (query tile), modulo three.
+  // Two query tiles of heads of 64 leave tensor memory for a third score tile: scores are then asked for half a round earlier, and the
+  // chain of a query tile is its softmax alone (8192 tokens, 32 heads: 389 -> 347 us).  Score tile 2 * (key tile) + (query tile), modulo
+  // three.
   static constexpr bool kSpare = kTiles == 2 && kDim == 64;
   static constexpr uint32_t kOutputs = kSpare ? 384 : 256;  // first tensor-memory column of the outputs
   static_assert(!kSpare || (kStages & (kStages - 1)) == 0, "stages are found by position");
@@ -789,8 +791,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (scored) skip_stages(S::kKeyStages);  // the next piece's keys stand behind these values, and have been used
         }
       } else if constexpr (S::kSpare) {
-        // Score tiles are free again behind the products that read their P: the second query tile's next scores follow the first one's outputs, the
-        // first one's next but one the second one's.
+        // Score tiles are free again behind the products that read their P: the second query tile's next scores follow the first one's
+        // outputs, the first one's next but one the second one's.
         const uint32_t ring = 2 * done;  // stages of the pieces before
         const auto stage_at = [&](uint32_t at) {
           stage = (ring + at) % S::kStages;
@@ -837,7 +839,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           ok = j + 2 < tiles ? ready(1, &smem->p_ready[1], n & 1u) : wait_for(&smem->p_ready[1], n & 1u);
           if (!ok) break;
           tc_fence_after_sync();
-          values_of_stage(tmem_base + S::kOutputs + kDim, value_stage, tmem_base + (2 * n + 1) % 3 * kKeys, accumulate, kIdescValues<S::kStageDim>);
+          values_of_stage(tmem_base + S::kOutputs + kDim, value_stage, tmem_base + (2 * n + 1) % 3 * kKeys, accumulate,
+                          kIdescValues<S::kStageDim>);
           tc_commit(&smem->pv_done[1]);
           tc_commit(&smem->empty[value_stage]);
           if (j + 2 < tiles) scores(j + 2, 0);
@@ -1025,9 +1028,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             for (int i = 0; i < 16; ++i) {
               const unsigned long long v = fma2(two(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, shift2);
               float a, b;
-              // Heads of 64: the exponentials of two query tiles take twice as long as their products; three of eight by the other units
-              // (8192 tokens, 32 heads: 425 -> 382 us; heads of 128, a quarter: 451 and 452).
-              if (kTiles == 2 && kDim == 64 && (i % 8 == 2 || i % 8 == 5 || i % 8 == 7)) {
+              // Heads of 64: the exponentials of two query tiles take twice as long as their products; one of eight by the other units, of
+              // more the instructions cost more than they spare (8192 tokens, 32 heads: none 335 us, one 326, two 338, four 392; heads of
+              // 128, a quarter: 451 and 452).
+              if (kTiles == 2 && kDim == 64 && (i % 8 == 3)) {
                 exp2_by_polynomial(v, a, b);
               } else {
                 a = exp2_approx(low_of(v));
