@@ -31,7 +31,7 @@
 // What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128
 // 1210, 32 of 64 844, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
 // bytes a cycle a key tile's products and TMA writes take 2560 and 4096 cycles, more than the tensor pipe (4608 tokens, heads of 512:
-// 371 us, without the writes 286).  Heads of 128: products issued at 80 to 95 cycles instead of 64 beside the softmax warps.  Heads
+// 371 us, without the writes 286; 3990 cycles a key tile).  Heads of 128: a query tile's chain of softmax, outputs and next scores.  Heads
 // of 64: the softmax warps' instructions.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
 // latencies, 14 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
 #include <cuda.h>
