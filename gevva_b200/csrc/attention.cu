@@ -29,7 +29,7 @@
 // leaves sums in the workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
 //
 // What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128
-// 1210, 32 of 64 844, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
+// 1210, 32 of 64 827, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
 // bytes a cycle a key tile's products and TMA writes take 2560 and 4096 cycles, more than the tensor pipe (4608 tokens, heads of 512:
 // 371 us, without the writes 286; 3990 cycles a key tile).  Heads of 128: a query tile's chain of softmax, outputs and next scores.  Heads
 // of 64: the softmax warps' instructions.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
@@ -99,8 +99,8 @@ struct Shape {
   // Whether a tile's values and the next one's keys fit side by side: scores of the next piece may then be asked for before this one's end.
   static constexpr bool kAhead = kTiles == 1 && kStages >= kKeyStages + kValueStages;
   // Two query tiles of heads of 64 leave tensor memory for a third score tile: scores are then asked for half a round earlier, and the
-  // chain of a query tile is its softmax alone (8192 tokens, 32 heads: 389 -> 347 us).  Score tile 2 * (key tile) + (query tile), modulo
-  // three.
+  // chain of a query tile is its softmax alone (8192 tokens, 32 heads: 389 -> 347 us; with one exponential of eight instead of three on the
+  // multiply-add units 332).  Score tile 2 * (key tile) + (query tile), modulo three.
   static constexpr bool kSpare = kTiles == 2 && kDim == 64;
   static constexpr uint32_t kOutputs = kSpare ? 384 : 256;  // first tensor-memory column of the outputs
   static_assert(!kSpare || (kStages & (kStages - 1)) == 0, "stages are found by position");
@@ -115,9 +115,10 @@ struct AttnSmem {
   uint8_t stage[S::kStages][S::kStageBytes];
   uint64_t full[S::kStages], empty[S::kStages];
   uint64_t q_full, q_empty;
-  uint64_t acc_full[4];       // scores: by key tile in turn (one query tile), by query tile (two), or by both (2 * query tile + turn)
-  uint64_t p_ready[2];
-  uint64_t pv_done[2];        // outputs of a key tile are summed up; by key tile in turn or by query tile, like the scores
+  // Scores are there, P is, outputs of a key tile are summed up: by key tile in turn (one query tile), by query tile (two), or by both
+  // (three score tiles, 2 * query tile + turn: the next scores do not wait for all warps' P there, so that a warp whose rows do not exist
+  // may be a key tile ahead).
+  uint64_t acc_full[4], p_ready[4], pv_done[4];
   uint64_t o_free[kTiles];    // the outputs of the last piece have been read
   uint64_t piece_full[kPieceSlots], piece_empty[kPieceSlots];
   uint64_t v_landed[2];       // values of a tile that has rows to be cleared, by softmax warpgroup
@@ -246,8 +247,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     mbar_init(&smem->q_full, 1);
     mbar_init(&smem->q_empty, 1);
-    for (int s = 0; s < 4; ++s) mbar_init(&smem->acc_full[s], 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&smem->acc_full[s], 1);
       mbar_init(&smem->p_ready[s], 4);
       mbar_init(&smem->pv_done[s], 1);
     }
@@ -826,22 +827,23 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             ok = ready(1, nullptr, 0);
             if (ok) mbar_arrive(&smem->v_landed[0]);
           }
-          ok = ok && ready(1, &smem->p_ready[0], n & 1u);
+          ok = ok && ready(1, &smem->p_ready[n & 1u], (n >> 1) & 1u);
           if (!ok) break;
           tc_fence_after_sync();
           values_of_stage(tmem_base + S::kOutputs, value_stage, tmem_base + 2 * n % 3 * kKeys, accumulate, kIdescValues<S::kStageDim>);
-          tc_commit(&smem->pv_done[0]);
+          tc_commit(&smem->pv_done[n & 1u]);
           if (j + 1 < tiles) {
             keys_at(j + 1);
             scores(j + 1, 1);
           }
           if (j + 2 < tiles) keys_at(j + 2);
-          ok = j + 2 < tiles ? ready(1, &smem->p_ready[1], n & 1u) : wait_for(&smem->p_ready[1], n & 1u);
+          ok = j + 2 < tiles ? ready(1, &smem->p_ready[2 + (n & 1u)], (n >> 1) & 1u)
+                             : wait_for(&smem->p_ready[2 + (n & 1u)], (n >> 1) & 1u);
           if (!ok) break;
           tc_fence_after_sync();
           values_of_stage(tmem_base + S::kOutputs + kDim, value_stage, tmem_base + (2 * n + 1) % 3 * kKeys, accumulate,
                           kIdescValues<S::kStageDim>);
-          tc_commit(&smem->pv_done[1]);
+          tc_commit(&smem->pv_done[2 + (n & 1u)]);
           tc_commit(&smem->empty[value_stage]);
           if (j + 2 < tiles) scores(j + 2, 0);
           if (j + 2 == tiles || tiles == 1) tc_commit(&smem->q_empty);
@@ -1005,8 +1007,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (any_grow && j > 0) {
             // (A wait can tell a phase from the one before it, not from the one after the next: each of these barriers is one phase
             // behind at most, since the scores at hand were asked for behind the outputs of two tiles before, and one ahead at most.)
-            const uint32_t before = kTiles == 2 ? n - 1 : (n - 1) >> 1;
-            ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[kTiles == 2 ? own : own ^ 1], before & 1u, smem, p.status));
+            const uint32_t before = kTiles == 2 && !S::kSpare ? n - 1 : (n - 1) >> 1;
+            const uint32_t summed = S::kSpare ? 2 * own + ((n - 1) & 1u) : kTiles == 2 ? own : own ^ 1;
+            ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[summed], before & 1u, smem, p.status));
             if (!ok) break;
             tc_fence_after_sync();
 #pragma unroll 1
@@ -1069,7 +1072,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           fence_proxy_async_smem();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&smem->p_ready[own]);
+        if (lane == 0) mbar_arrive(&smem->p_ready[barrier]);
         if constexpr (kTiles == 1) {
           if (n > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&smem->sum_ready[own ^ 1][quarter], turn_before, smem, p.status));
           if (!ok) break;
@@ -1089,7 +1092,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (lane == 0) mbar_arrive(&smem->piece_empty[slot]);
         continue;
       }
-      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[own], (kTiles == 2 ? done - 1 : (done - 1) >> 1) & 1u, smem, p.status));
+      const uint32_t summed = S::kSpare ? 2 * own + ((done - 1) & 1u) : own;
+      const uint32_t sums_before = kTiles == 2 && !S::kSpare ? done - 1 : (done - 1) >> 1;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&smem->pv_done[summed], sums_before & 1u, smem, p.status));
       if (!ok) break;
       tc_fence_after_sync();
       if (active) {

@@ -176,6 +176,26 @@ def test_chunk_reports_lengths_beyond_the_table(attn, cuda_device):
     assert torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [1, 3, 8, 16])
+def test_query_tiles_with_few_rows_behind_many_keys(attn, cuda_device, dim, heads):
+    """The last query tile has rows for some of the warps only, and keys enough that the others could be far ahead of them."""
+    step = 128 // heads * 2
+    for n in [7 * 128 // step * step + rest for rest in (1, 31 // heads + 1, 64 // heads + 1, step // 2, step // 2 + 1, step - 1)]:
+        q, k, v = (randn((n, h, dim), cuda_device, n + i) for i, h in enumerate((heads, 1, 1)))
+        want, bound = ref.attention(q, k, v, 0, dim ** -0.5, 0)
+        for _ in range(3):
+            ref.within(attn.prompt_attention(q, k, v, offsets_of([n], cuda_device), dim ** -0.5), want, bound, f"{n} tokens")
+        batch, pages = make_batch(attn, [n], [n], 64, cuda_device, 2)
+        cache = attn.KvCache.empty(pages, 64, 1, dim, cuda_device)
+        at = batch.table[0, :-(-n // 64)].long()
+        for x, to in ((k, cache.k), (v, cache.v)):
+            whole = torch.zeros((len(at) * 64, 1, dim), dtype=torch.bfloat16, device=cuda_device)
+            whole[:n] = x
+            to[at] = whole.view(len(at), 64, 1, dim)
+        ref.within(attn.chunk_attention(q, cache, batch, dim ** -0.5), want, bound, f"{n} tokens over pages")
+
+
 @pytest.mark.parametrize("dim,news,past,window", [(64, 4096, 0, 100), (256, 4096, 37, 300), (256, 1000, 9000, 0), (512, 700, 5000, 0)])
 def test_chunk_of_many_query_tiles(attn, cuda_device, dim, news, past, window):
     """Runs of key tiles inside one sequence, longer and shorter than a query tile's, that begin and end inside them."""
