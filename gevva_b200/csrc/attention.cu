@@ -91,7 +91,7 @@ struct Shape {
   static constexpr int kKeyStages = kDim / kStageDim;
   static constexpr int kValueStages = kValueDim / kStageDim;
   static constexpr int kQueryTileBytes = kRows * kDim * 2;
-  static constexpr int kControlBytes = 3072;
+  static constexpr int kControlBytes = 3 << 10;
   static constexpr int kRoom = (232448 - kControlBytes - kTiles * kQueryTileBytes) / kStageBytes;
   static constexpr int kStages = kRoom < 8 ? kRoom : 8;
   static constexpr int kSoftmaxWarps = 8;
