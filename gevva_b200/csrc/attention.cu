@@ -157,9 +157,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// The same for two exponents on the multiply-add units: 2^n of the nearest whole n into the exponent, and for what is left, in [-1/2,
-// 1/2], the polynomial of degree four with the smallest largest relative error (2.7e-6, by iterated reweighted least squares), far below
-// the rounding of p to bf16.  Zero below 2^-126, as from the other.
+// The same for two exponents on the multiply-add units: 2^n of the nearest whole n, times the polynomial of degree four with the
+// smallest largest relative error for what is left, in [-1/2, 1/2] (2.7e-6, by iterated reweighted least squares), far below
+// the rounding of p to bf16.  Zero below 2^-126, as from the other; what is no number stays none (2^n put into the exponent by adding
+// whole numbers would make it the largest finite one).
 __device__ __forceinline__ void exp2_by_polynomial(unsigned long long x, float& a, float& b) {
   constexpr float kShift = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, which then stands in the low bits
   const unsigned long long t = add2(x, two(kShift, kShift));
@@ -168,10 +169,10 @@ __device__ __forceinline__ void exp2_by_polynomial(unsigned long long x, float& 
   p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
   p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
   p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
-  a = __uint_as_float(static_cast<uint32_t>(p) + (static_cast<uint32_t>(t) << 23));
-  b = __uint_as_float(static_cast<uint32_t>(p >> 32) + (static_cast<uint32_t>(t >> 32) << 23));
-  a = low_of(x) < -126.0f ? 0.0f : a;
-  b = high_of(x) < -126.0f ? 0.0f : b;
+  p = mul2(p, two(__uint_as_float((static_cast<uint32_t>(t) << 23) + 0x3f800000u),
+                  __uint_as_float((static_cast<uint32_t>(t >> 32) << 23) + 0x3f800000u)));
+  a = low_of(x) < -126.0f ? 0.0f : low_of(p);
+  b = high_of(x) < -126.0f ? 0.0f : high_of(p);
 }
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tensor_map, uint64_t* bar, int x, int y, int z, int w) {
