@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from tests import attention_ref as ref
 from tests.test_gpu_attention import attn, make_batch, randn  # noqa: F401  (attn: a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -27,3 +28,33 @@ def test_scores_that_are_no_numbers_give_none(attn, cuda_device, dim):
     for got in (attn.prompt_attention(q, k, v, batch.token_offsets, 0.125, window=1), attn.chunk_attention(q, cache, batch, 0.125, window=1)):
         assert torch.isnan(got[broken]).all()
         assert torch.equal(got[~broken], v[~broken])
+
+
+# ---- sharp rows -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+def test_a_row_of_few_keys_is_as_exact_as_its_output(attn, cuda_device, dim):
+    """Where a few keys have all the weight, what is rounded of p cancels: the sum that divides is of the rounded values, so that a result is a mean
+    of v whose weights are off, and errs by 2^-8 of what v differs from it."""
+    n, heads = 512, 4
+    q, k, v = (randn((n, heads, dim), cuda_device, 30 + i) for i in range(3))
+    q = (q.float() * 6).to(torch.bfloat16)
+    scale = dim ** -0.5
+    batch, pages = make_batch(attn, [n], [n], 64, cuda_device, 2)
+    cache = attn.KvCache.empty(pages, 64, heads, dim, cuda_device)
+    attn.kv_append(q, k, v, cache, batch, None)
+    q64, k64, v64 = q.double(), k.double(), v.double()
+    hidden = torch.ones(n, n, dtype=torch.bool, device=cuda_device).triu(1)
+    bound = torch.empty_like(q64)
+    want = torch.empty_like(q64)
+    for h in range(heads):
+        score = (q64[:, h] @ k64[:, h].T * scale).masked_fill(hidden, -torch.inf)
+        size = (q64[:, h].abs() @ k64[:, h].abs().T * scale).masked_fill(hidden, 0.0)
+        share = torch.softmax(score, -1)
+        want[:, h] = share @ v64[:, h]
+        # each weight is off by 2^-8 from its rounding, by what its score is off ((dim + 4) 2^-24 of its products' sizes) and its exponential (2^-18
+        # and the rounding of an exponent of 60 at most); the sum of the weights by as much, which is the 1.01
+        off = 1.01 * share * (ref.BF16 + (dim + 4) * ref.FP32 * size + 128 * ref.FP32)
+        bound[:, h] = torch.stack([(off * (v64[None, :, h, x] - want[:, h, x, None]).abs()).sum(1) for x in range(dim)], 1)
+        bound[:, h] += want[:, h].abs() * (ref.BF16 + 16 * ref.FP32) + (share @ v64[:, h].abs()) * 2.0 ** -23 * (n // 16)
+    for got, what in ((attn.prompt_attention(q, k, v, batch.token_offsets, scale), "prompt"), (attn.chunk_attention(q, cache, batch, scale), "chunk")):
+        ref.within(got, want, bound + 1e-30, what)
