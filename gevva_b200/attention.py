@@ -219,8 +219,9 @@ def kv_append(q, k, v, cache, batch, frequencies, q_weight=None, k_weight=None, 
     """Norms q and k over their heads (weights bf16 [dim], None: no norm) and, with normalize_v, v without a weight; turns the pairs
     (j, len(frequencies) + j) of q and k by position * frequencies[j] (a multiple of 8 float64 on the GPU, None: no rotation); stores k
     and v at their positions in the cache.  q, k, v are [tokens, heads, dim], views of one projection's rows for instance.  Returns the queries, with
-    `packed` also keys and values as [tokens, kv_heads, dim] for prompt_attention.  `out` takes the queries.  A token
-    without a page is not stored; cache.check() reports it."""
+    `packed` also keys and values as [tokens, kv_heads, dim] for prompt_attention.  `out` takes the queries; it
+    may be q itself where that is contiguous, and otherwise shares no memory with q, k or v.  A token without a page is not stored;
+    cache.check() reports it."""
     device, shape, q_rows = _queries(q)
     if stream is not None:
         with _on(stream, device):
@@ -247,7 +248,7 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
     """Causal attention of packed prompts: rows token_offsets[s] .. token_offsets[s + 1] - 1 (int32 on the GPU) are sequence s, and
     each sees its sequence's rows up to itself, the last `window` of them where that is not zero.  q [tokens, heads, dim], k and v
     [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`, and may hold anything in k
-    and v; a sequence's own keys and values have to be finite.  `status` is an optional int32 [1] device word."""
+    and v; a sequence's own keys and values have to be finite.  `out` shares no memory with q, k or v.  `status` is an optional int32 [1] device word."""
     device, shape, q_rows = _queries(q)
     if stream is not None:
         with _on(stream, device):
@@ -268,7 +269,8 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
 def chunk_attention(q, cache, batch, scale, window=0, out=None, stream=None):
     """Causal attention of new tokens over the pages of their sequences, which hold their keys and values already (kv_append):
     one token a sequence when decoding, several for verification and chunked prefill.  A row that sees no key is zero; rows outside the
-    offsets are left as they were in `out`.  Slots that no row of a sequence sees may hold anything, others have to be finite.  cache.check() reports lengths beyond the table and pages outside the cache."""
+    offsets are left as they were in `out`, which shares no memory with q or the cache.  Slots that no row of a sequence sees may hold
+    anything, others have to be finite.  cache.check() reports lengths beyond the table and pages outside the cache."""
     device, shape, q_rows = _queries(q)
     if stream is not None:
         with _on(stream, device):

@@ -39,6 +39,29 @@ bool rows_ok(gv::AttnRows* out, const void* data, long long token_stride, long l
   return stride_ok(out->head_stride, heads, dim) && stride_ok(out->token_stride, tokens, static_cast<long long>(heads) * dim);
 }
 
+// Whether `count` values at `out` share memory with these rows; what lies between the rows and between their heads is not theirs.
+bool meets(const void* out, long long count, const gv::AttnRows& rows, int tokens, int heads, int dim) {
+  long long at = static_cast<long long>(reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(rows.data)) / 2;  // (both are aligned)
+  const bool token_outer = rows.token_stride >= rows.head_stride;
+  const long long strides[2] = {token_outer ? rows.token_stride : rows.head_stride, token_outer ? rows.head_stride : rows.token_stride};
+  const long long extents[2] = {token_outer ? tokens : heads, token_outer ? heads : tokens};
+  for (int i = 0; i < 2; ++i) {
+    const long long piece = i == 0 ? (extents[1] - 1) * strides[1] + dim : dim;  // from the first value to behind the last of what one step holds
+    if (at + count <= 0) return false;
+    if (at <= 0) return true;
+    if (piece >= strides[i]) return at < (extents[i] - 1) * strides[i] + piece;
+    const long long step = at / strides[i];
+    if (step >= extents[i]) return false;
+    if (step + 1 < extents[i] && at + count > (step + 1) * strides[i]) return true;
+    at -= step * strides[i];
+  }
+  return at < dim;
+}
+
+bool packed(const gv::AttnRows& rows, int heads, int dim) {
+  return rows.head_stride == dim && rows.token_stride == static_cast<long long>(heads) * dim;
+}
+
 bool pages_ok(gv::AttnPages* out, const gevva_attn_cache* c, const gevva_attn_batch* b, int kv_heads, int dim) {
   if (!c || !b || !aligned(c->keys) || !aligned(c->values) || c->pages < 1 || c->page_size < 16 || (c->page_size & (c->page_size - 1)) ||
       !b->token_offsets || !b->lengths || !b->table || b->sequences < 1 || b->table_width < 1 || b->table_stride < b->table_width ||
@@ -132,6 +155,18 @@ int gevva_attn_append(const gevva_attn_append_args* a, gevva_stream_t stream) {
       !aligned_or_null(a->v_out) || (a->tokens > 0 && !a->k_out != !a->v_out) || a->reserved)
     return GEVVA_MOE_BAD_ARGUMENT;
   if (a->tokens == 0) return GEVVA_MOE_OK;
+  // A token's rows are written when that token's have been read, not when others' have: an output may stand where its own input does,
+  // row for row, and nowhere else among the inputs.
+  const gv::AttnRows* const inputs[3] = {&call.q, &call.k, &call.v};
+  void* const outputs[3] = {a->q_out, a->k_out, a->v_out};
+  for (int o = 0; o < 3; ++o) {
+    const auto heads = [&](int i) { return i == 0 ? a->heads : a->kv_heads; };
+    for (int i = 0; i < 3 && outputs[o]; ++i) {
+      if (o == i && outputs[o] == inputs[i]->data && packed(*inputs[i], heads(i), a->dim)) continue;
+      if (meets(outputs[o], static_cast<long long>(a->tokens) * heads(o) * a->dim, *inputs[i], a->tokens, heads(i), a->dim))
+        return GEVVA_MOE_BAD_ARGUMENT;
+    }
+  }
   call.token_offsets = a->batch->token_offsets;
   call.sequences = a->batch->sequences;
   call.tokens = a->tokens;
@@ -161,6 +196,10 @@ int gevva_attn_prompt(const gevva_attn_prompt_args* a, gevva_stream_t stream) {
       !attention_ok(a->tokens, a->scale, a->window) || !aligned_32(a->out, a->tokens) || a->reserved)
     return GEVVA_MOE_BAD_ARGUMENT;
   if (a->tokens == 0) return GEVVA_MOE_OK;
+  const long long values = static_cast<long long>(a->tokens) * a->heads * a->dim;
+  if (meets(a->out, values, call.q, a->tokens, a->heads, a->dim) || meets(a->out, values, call.k, a->tokens, a->kv_heads, a->dim) ||
+      meets(a->out, values, call.v, a->tokens, a->kv_heads, a->dim))
+    return GEVVA_MOE_BAD_ARGUMENT;
   call.token_offsets = a->token_offsets;
   call.sequences = a->sequences;
   fill_attention(&call, *a);
@@ -179,6 +218,7 @@ int gevva_attn_chunk(const gevva_attn_chunk_args* a, gevva_stream_t stream) {
       !aligned_32(a->out, a->tokens) || !aligned_32(a->workspace, 1))
     return GEVVA_MOE_BAD_ARGUMENT;
   if (a->tokens == 0) return GEVVA_MOE_OK;
+  if (meets(a->out, static_cast<long long>(a->tokens) * a->heads * a->dim, call.q, a->tokens, a->heads, a->dim)) return GEVVA_MOE_BAD_ARGUMENT;
   call.paged = true;
   call.token_offsets = a->batch->token_offsets;
   call.sequences = a->batch->sequences;

@@ -409,7 +409,8 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
  * a multiple of 16 up to dim, zero for none; values from `rotated` on stay).  Queries go to q_out [tokens, heads, dim], keys and
  * values to the cache and, where k_out and v_out are given (both or none), to [tokens, kv_heads, dim], which gevva_attn_prompt
  * reads.  A token without a page (position outside the table, page outside the cache) is not stored and reported as
- * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot.  q_out may be q. */
+ * GEVVA_MOE_BAD_PAGE.  No two tokens of a call may name one slot.  An output may be its own input where that has the output's layout
+ * (head stride dim, token stride heads * dim); outputs that share memory with q, k or v in any other way are refused. */
 typedef struct {
   const void* q;
   long long q_token_stride, q_head_stride;
@@ -435,7 +436,7 @@ int gevva_attn_append(const gevva_attn_append_args* args, gevva_stream_t stream)
 /* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
  * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  0 < scale <= 1e30.  No row sees another sequence's
  * keys, whatever their values are; within a sequence, keys and values that a row does not see have to be finite.  out may not
- * overlap what the call reads. */
+ * overlap what the call reads; one that shares memory with q, k or v is refused. */
 typedef struct {
   const void* q;
   long long q_token_stride, q_head_stride;
@@ -456,7 +457,7 @@ int gevva_attn_prompt(const gevva_attn_prompt_args* args, gevva_stream_t stream)
  * decoding, several in verification and chunked prefill.  Lengths are read on the device, so a captured call can be replayed with
  * others.  Row i of n sees the keys up to lengths[s] - n + i; a row that sees none is zero.  Slots that no row of a sequence sees
  * may hold anything, others have to be finite.  A length beyond the table is cut to it, a page outside the cache is read as zeros,
- * and both are reported as GEVVA_MOE_BAD_PAGE.  out may not overlap what the call reads.  `workspace` is device memory of
+ * and both are reported as GEVVA_MOE_BAD_PAGE.  out may not overlap what the call reads; one that shares memory with q is refused.  `workspace` is device memory of
  * gevva_attn_chunk_workspace_bytes(dim) bytes, in use until `stream` has passed the call; calls that may run at the same time need
  * one each. */
 size_t gevva_attn_chunk_workspace_bytes(int dim);

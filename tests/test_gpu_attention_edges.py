@@ -58,3 +58,37 @@ def test_a_row_of_few_keys_is_as_exact_as_its_output(attn, cuda_device, dim):
         bound[:, h] += want[:, h].abs() * (ref.BF16 + 16 * ref.FP32) + (share @ v64[:, h].abs()) * 2.0 ** -23 * (n // 16)
     for got, what in ((attn.prompt_attention(q, k, v, batch.token_offsets, scale), "prompt"), (attn.chunk_attention(q, cache, batch, scale), "chunk")):
         ref.within(got, want, bound + 1e-30, what)
+
+
+# ---- outputs in place of inputs -----------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [1, 5, 900])
+def test_append_in_place_of_packed_queries(attn, cuda_device, tokens):
+    heads, kv_heads, dim, page = 6, 2, 128, 16
+    batch, pages = make_batch(attn, [tokens], [tokens + 9], page, cuda_device, 3)
+    caches = [attn.KvCache.empty(pages, page, kv_heads, dim, cuda_device) for _ in range(2)]
+    q, k, v = (randn((tokens, h, dim), cuda_device, i) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    weight, freq = randn((dim,), cuda_device, 6), torch.rand(dim // 2, dtype=torch.float64, device=cuda_device)
+    want = attn.kv_append(q, k, v, caches[0], batch, freq, weight, weight)
+    assert attn.kv_append(q, k, v, caches[1], batch, freq, weight, weight, out=q) is q
+    assert torch.equal(q, want) and torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+
+
+def test_outputs_over_what_a_call_reads_are_refused(attn, cuda_device):
+    from gevva_b200 import GevvaMoeError
+    tokens, heads, kv_heads, dim = 40, 4, 2, 64
+    batch, pages = make_batch(attn, [tokens], [tokens], 16, cuda_device, 3)
+    cache = attn.KvCache.empty(pages, 16, kv_heads, dim, cuda_device)
+    rows = randn((tokens, heads + 2 * kv_heads, dim), cuda_device, 1)
+    q, k, v = rows.split((heads, kv_heads, kv_heads), 1)
+    before = rows.clone()
+    over = rows.view(-1)[:tokens * heads * dim].view(tokens, heads, dim)
+    packed = q.contiguous()
+    for call in (lambda: attn.kv_append(q, k, v, cache, batch, None, out=over),
+                 lambda: attn.kv_append(packed, packed[:, :2], v, cache, batch, None, out=packed),
+                 lambda: attn.prompt_attention(q, k, v, batch.token_offsets, 0.125, out=over),
+                 lambda: attn.prompt_attention(packed, k, v, batch.token_offsets, 0.125, out=packed),
+                 lambda: attn.chunk_attention(q, cache, batch, 0.125, out=over),
+                 lambda: attn.chunk_attention(packed, cache, batch, 0.125, out=packed)):
+        with pytest.raises(GevvaMoeError, match="argument"):
+            call()
+    assert torch.equal(rows, before) and torch.equal(packed, q)
