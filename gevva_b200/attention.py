@@ -146,9 +146,16 @@ def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None,
 
 class KvCache:
     """Keys and values in pages: two bf16 tensors [pages, page_size, kv_heads, dim] (any strides, the last dimension contiguous).
-    page_size is a power of two, at least 16.  `status` is the int32 word that calls on this cache report into."""
+    page_size is a power of two, at least 16.  `status` is the int32 word that calls on this cache report into.  `k` and `v` may be
+    replaced by tensors of the same shape; a captured call keeps those that it was captured with."""
 
     def __init__(self, k, v):
+        self._packed = _Cache()
+        self._address = ctypes.addressof(self._packed)
+        self._take(k, v)
+        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
+
+    def _take(self, k, v):
         if (k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16 or k.dim() != 4 or v.shape != k.shape or not k.is_cuda or
                 v.device != k.device or k.stride(3) != 1 or v.stride(3) != 1 or k.shape[3] not in HEAD_DIMS):
             raise ValueError(f"cache: expected two CUDA bfloat16 tensors (pages, page_size, kv_heads, 64|128|256|512), got {k.dtype} "
@@ -156,13 +163,14 @@ class KvCache:
         pages, page_size = k.shape[:2]
         if pages < 1 or page_size < 16 or page_size & (page_size - 1):
             raise ValueError(f"cache: page_size has to be a power of two, at least 16, and there has to be a page; got {tuple(k.shape)}")
-        self.k, self.v = k, v
+        self._k, self._v = k, v
         self.page_size, self.kv_heads, self.head_dim = page_size, k.shape[2], k.shape[3]
         self.device = k.device
-        self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
-        self._packed = _Cache(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
+        self._packed.__init__(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
                               pages, page_size)
-        self._address = ctypes.addressof(self._packed)
+
+    k = property(lambda self: self._k, lambda self, k: self._take(k, self._v))
+    v = property(lambda self: self._v, lambda self, v: self._take(self._k, v))
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, device="cuda:0"):
@@ -184,23 +192,33 @@ class KvCache:
 class PagedBatch:
     """The sequences of a call, int32 on the GPU: new tokens token_offsets[s] .. token_offsets[s + 1] - 1 (rows of the call's
     tensors), lengths[s] keys with the new ones counted, and table [sequences, pages a sequence], whose entry x / page_size is the page of
-    position x.  The tensors are read when the calls run, so a captured call can be replayed with other contents; rows outside the offsets
-    are left as they were."""
+    position x.  The tensors are read when the calls run, so a captured call can be replayed with other contents (written in place:
+    copy_, +=); rows outside the offsets are left as they were.  Each may be replaced by another for as many sequences, which later calls
+    read; a captured call keeps those that it was captured with."""
 
     def __init__(self, token_offsets, lengths, table):
+        self._packed = _Batch()
+        self._address = ctypes.addressof(self._packed)
+        self._take(token_offsets, lengths, table)
+
+    def _take(self, token_offsets, lengths, table):
         sequences = lengths.shape[0] if lengths.dim() == 1 else -1
         for tensor, shape, name in ((token_offsets, (sequences + 1,), "token_offsets"), (lengths, (sequences,), "lengths")):
             if not tensor.is_cuda:
                 raise ValueError(f"{name}: expected a CUDA tensor, got {tensor.device}")
             _at(tensor, torch.int32, shape, table.device, name)
         if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != sequences or table.shape[1] < 1 or sequences < 1 or (
-                table.stride(1) != 1 and table.shape[1] > 1):
-            raise ValueError(f"table: expected int32 ({sequences}, pages a sequence), got {table.dtype} {tuple(table.shape)}")
-        self.token_offsets, self.lengths, self.table = token_offsets, lengths, table
+                table.stride(1) != 1 and table.shape[1] > 1) or (sequences > 1 and table.stride(0) >= 1 << 31):
+            raise ValueError(f"table: expected int32 ({sequences}, pages a sequence), got {table.dtype} {tuple(table.shape)} strides "
+                             f"{table.stride()}")
+        self._token_offsets, self._lengths, self._table = token_offsets, lengths, table
         self.device = table.device
         stride = table.stride(0) if sequences > 1 else table.shape[1]
-        self._packed = _Batch(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
-        self._address = ctypes.addressof(self._packed)
+        self._packed.__init__(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
+
+    token_offsets = property(lambda self: self._token_offsets, lambda self, x: self._take(x, self._lengths, self._table))
+    lengths = property(lambda self: self._lengths, lambda self, x: self._take(self._token_offsets, x, self._table))
+    table = property(lambda self: self._table, lambda self, x: self._take(self._token_offsets, self._lengths, x))
 
 
 @dataclass

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests import attention_ref as ref
-from tests.test_gpu_attention import attn, make_batch, randn  # noqa: F401  (attn: a fixture)
+from tests.test_gpu_attention import attn, gathered, make_batch, randn  # noqa: F401  (attn: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,21 @@ def test_outputs_over_what_a_call_reads_are_refused(attn, cuda_device):
         with pytest.raises(GevvaMoeError, match="argument"):
             call()
     assert torch.equal(rows, before) and torch.equal(packed, q)
+
+
+def test_a_batch_follows_its_tensors(attn, cuda_device):
+    """Tensors of a batch and of a cache that are replaced are the ones that the next call reads."""
+    page, dim, length = 16, 64, 100
+    batch, pages = make_batch(attn, [1], [length], page, cuda_device, 3, width=20)
+    cache = attn.KvCache(*(randn((pages, page, 1, dim), cuda_device, i) for i in range(2)))
+    q = randn((1, 2, dim), cuda_device, 3)
+    for step in range(10):
+        batch.lengths = batch.lengths - 5
+        batch.table = batch.table.clone()
+        cache.v = cache.v.clone() + 1
+        junk = [torch.full((64,), 1 << 20, dtype=torch.int32, device=cuda_device) for _ in range(4)]  # (over what has been given back)
+        got = attn.chunk_attention(q, cache, batch, 0.125)
+        cache.check()
+        length -= 5
+        ref.within(got, *ref.attention(q, *gathered(cache, batch, 0, length), length - 1, 0.125, 0), f"step {step}")
+        del junk
