@@ -108,6 +108,8 @@ def _out(out, like, device, name="out"):
 def _rows(x, name="input"):
     if x.dtype is not torch.bfloat16 or x.dim() != 2 or not x.is_contiguous() or not x.is_cuda:
         raise ValueError(f"{name}: expected contiguous CUDA bfloat16 (rows, width), got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if max(x.shape) >= 1 << 31:
+        raise ValueError(f"{name}: at most 2^31 - 1 rows and values in one, got {tuple(x.shape)}")
     return x.device, x.shape
 
 

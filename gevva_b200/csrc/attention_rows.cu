@@ -304,7 +304,7 @@ cudaError_t launch_block_norm(const BlockNormCall& call, int sm_count, cudaStrea
   p.vectors = call.width / 8;
   p.inverse_width = 1.0f / static_cast<float>(call.width);
   p.eps = call.eps;
-  if (p.vectors <= 32) return launch_chained(block_norm_kernel<false, 1, 128>, dim3((call.rows + 3) / 4), dim3(128), 0, stream, p);
+  if (p.vectors <= 32) return launch_chained(block_norm_kernel<false, 1, 128>, dim3((static_cast<unsigned>(call.rows) + 3) / 4), dim3(128), 0, stream, p);
   const dim3 grid(call.rows);
   // Four warps a row where there are rows for all SMs several times over: sixteen rows of an SM at a time have more bytes on their way
   // than five of eleven warps.

@@ -1,0 +1,44 @@
+"""What the attention calls launch, and what they refuse as too large, on the CUDA runtime that records launches (see test_launch_sequence.py)."""
+import ctypes
+
+import pytest
+import torch
+
+from gevva_b200 import attention as attn
+from tests.test_launch_sequence import ADDRESS, recorder  # noqa: F401  (a fixture)
+
+
+@pytest.fixture(scope="module")
+def lib(recorder):  # noqa: F811
+    f32, vp, i32 = ctypes.c_float, ctypes.c_void_p, ctypes.c_int
+    recorder.lib.gevva_attn_norm.argtypes = [vp, vp, vp, i32, i32, f32, vp]
+    recorder.lib.gevva_attn_norm_add.argtypes = [vp] * 8 + [i32, i32, f32, vp]
+    return recorder
+
+
+@pytest.mark.parametrize("rows", [1, 4, 5, 2 ** 31 - 5, 2 ** 31 - 4, 2 ** 31 - 3, 2 ** 31 - 1])
+def test_norms_of_any_number_of_rows(lib, rows):
+    assert lib.lib.gevva_attn_norm(ADDRESS, ADDRESS, ADDRESS, rows, 64, 1e-6, None) == 0
+    assert lib.lib.gevva_attn_norm_add(ADDRESS, ADDRESS, ADDRESS, None, None, None, ADDRESS, None, rows, 64, 1e-6, None) == 0
+    assert [(x["kernel"], x["grid"]) for x in lib.launches()] == [("block_norm_kernel<0>", -(-rows // 4))] * 2
+    assert lib.lib.gevva_attn_norm(ADDRESS, ADDRESS, ADDRESS, rows, 2816, 1e-6, None) == 0
+    assert [x["grid"] for x in lib.launches()] == [rows]
+
+
+@pytest.mark.parametrize("shape", [(1 << 31, 8), ((1 << 32) + 5, 8), (8, (1 << 32) + 8)])
+def test_rows_that_an_argument_cannot_hold(shape):
+    """ctypes would cut them to 32 bits, and the call would leave the rest of the rows out."""
+    class Stand:
+        dtype, device, is_cuda = torch.bfloat16, torch.device("cuda:0"), True
+        shape = None
+
+        def dim(self):
+            return 2
+
+        def is_contiguous(self):
+            return True
+
+    Stand.shape = torch.Size(shape)
+    for call in (lambda: attn.block_norm(Stand(), None), lambda: attn.block_norm_add(Stand(), None, None)):
+        with pytest.raises(ValueError, match="at most"):
+            call()
