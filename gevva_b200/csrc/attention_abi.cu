@@ -79,6 +79,7 @@ bool pages_ok(gv::AttnPages* out, const gevva_attn_cache* c, const gevva_attn_ba
 int launched(cudaError_t e) {
   if (e == cudaSuccess) return GEVVA_MOE_OK;
   cudaGetLastError();  // reported here; not again by the next call
+  if (e == cudaErrorInvalidConfiguration) return GEVVA_MOE_TOO_LARGE;  // (more items than a grid has)
   return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
 }
 

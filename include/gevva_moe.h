@@ -436,7 +436,8 @@ int gevva_attn_append(const gevva_attn_append_args* args, gevva_stream_t stream)
 /* Causal attention of whole prompts over their own packed keys: row i of a sequence sees its rows j <= i, with a window (> 0)
  * those with j > i - window; out [tokens, heads, dim] = softmax(scale * q.k) v.  0 < scale <= 1e30.  No row sees another sequence's
  * keys, whatever their values are; within a sequence, keys and values that a row does not see have to be finite.  out may not
- * overlap what the call reads; one that shares memory with q, k or v is refused. */
+ * overlap what the call reads; one that shares memory with q, k or v is refused.  GEVVA_MOE_TOO_LARGE: the prompts have more than
+ * 2^31 - 1 query tiles times key heads. */
 typedef struct {
   const void* q;
   long long q_token_stride, q_head_stride;

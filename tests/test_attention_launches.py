@@ -42,3 +42,14 @@ def test_rows_that_an_argument_cannot_hold(shape):
     for call in (lambda: attn.block_norm(Stand(), None), lambda: attn.block_norm_add(Stand(), None, None)):
         with pytest.raises(ValueError, match="at most"):
             call()
+
+
+def test_a_prompt_of_more_items_than_a_grid_has(lib):
+    heads = 1024
+
+    def call(tokens):
+        rows = (ADDRESS, heads * 64, 64)
+        return lib.lib.gevva_attn_prompt(attn._PROMPT.pack(*rows, *rows, *rows, ADDRESS, 1 << 60, 0, 1, tokens, heads, heads, 64, 0, 0.1, 0), None)
+
+    assert call(1 << 28) == 0 and [x["grid"] for x in lib.launches()] == [heads * (((1 << 28) + 255) // 256)]
+    assert call(1 << 30) == -6 and lib.launches() == []
