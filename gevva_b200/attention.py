@@ -76,7 +76,7 @@ def _on(stream, device):
 def _pack(layout, *values):
     try:
         return layout.pack(*values)
-    except (struct.error, OverflowError) as error:
+    except struct.error as error:
         raise ValueError(f"argument out of range: {error}") from None
 
 

@@ -53,9 +53,3 @@ def test_a_prompt_of_more_items_than_a_grid_has(lib):
 
     assert call(1 << 28) == 0 and [x["grid"] for x in lib.launches()] == [heads * (((1 << 28) + 255) // 256)]
     assert call(1 << 30) == -6 and lib.launches() == []
-
-
-@pytest.mark.parametrize("scale", [1e39, -1e39, float(2 ** 128)])
-def test_a_scale_that_32_bits_do_not_hold(scale):
-    with pytest.raises(ValueError, match="out of range"):
-        attn._pack(attn._CHUNK, ADDRESS, 8, 8, ADDRESS, ADDRESS, ADDRESS, ADDRESS, 0, 1, 1, 1, 64, 0, scale)
