@@ -44,6 +44,7 @@ def _lib():
     lib.gevva_attn_norm_add.argtypes = [vp] * 8 + [i32, i32, f32, vp]
     for function in (lib.gevva_attn_append, lib.gevva_attn_prompt, lib.gevva_attn_chunk):
         function.argtypes = [ctypes.c_char_p, vp]  # the packed arguments, the stream
+    lib.gevva_attention_last_status.argtypes = []
     lib.gevva_attn_chunk_workspace_bytes.argtypes = [i32]
     lib.gevva_attn_chunk_workspace_bytes.restype = ctypes.c_size_t
     lib._gv_attn_ready = True
@@ -53,6 +54,17 @@ def _lib():
 def _status(status, where):
     if status != 0:
         raise GevvaMoeError(status, where)
+
+
+def last_status(device=None):
+    """Waits for the device (None: the current one), then returns and clears the status of the prompt_attention calls on it that were given no
+    status word (0 = ok)."""
+    with torch.cuda.device(device):
+        return _lib().gevva_attention_last_status()
+
+
+def check(device=None):
+    _status(last_status(device), "device status")
 
 
 def _at(tensor, dtype, shape, device, name):
@@ -268,7 +280,8 @@ def prompt_attention(q, k, v, token_offsets, scale, window=0, out=None, status=N
     """Causal attention of packed prompts: rows token_offsets[s] .. token_offsets[s + 1] - 1 (int32 on the GPU) are sequence s, and
     each sees its sequence's rows up to itself, the last `window` of them where that is not zero.  q [tokens, heads, dim], k and v
     [tokens, kv_heads, dim], kv_heads dividing heads.  Rows outside the offsets are left as they were in `out`, and may hold anything in k
-    and v; a sequence's own keys and values have to be finite.  `out` shares no memory with q, k or v.  `status` is an optional int32 [1] device word."""
+    and v; a sequence's own keys and values have to be finite.  `out` shares no memory with q, k or v.  `status` is an int32 [1] device
+    word that a wait which runs out is reported into (the output is then not whole); without one, check() of this module reports it."""
     device, shape, q_rows = _queries(q)
     if stream is not None:
         with _on(stream, device):

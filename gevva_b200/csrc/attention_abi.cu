@@ -2,6 +2,8 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "../../include/gevva_moe.h"
 #include "gv_attention.h"
 #include "gv_launchers.h"
@@ -83,6 +85,26 @@ int launched(cudaError_t e) {
   return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
 }
 
+// What calls without a status word of their own report into, one of each device.  (In host code the name is only a handle.)
+static __device__ int g_attention_status;
+constexpr int kMaxDevices = 64;
+std::atomic<int*> g_status_address[kMaxDevices];
+
+// The call's word, or else the current device's.
+cudaError_t status_word(int* own, int** out) {
+  *out = own;
+  if (own) return cudaSuccess;
+  int device = -1;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  *out = g_status_address[device].load(std::memory_order_relaxed);
+  if (*out) return cudaSuccess;
+  e = cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_attention_status);
+  if (e == cudaSuccess) g_status_address[device].store(*out, std::memory_order_relaxed);
+  return e;
+}
+
 bool attention_ok(int tokens, float scale, int window) {
   return tokens <= kMaxPositions && scale > 0.0f && scale <= 1e30f && window >= 0;
 }
@@ -99,7 +121,6 @@ void fill_attention(gv::AttnCall* call, const Args& a) {
   call->out = a.out;
   call->out_token_stride = static_cast<long long>(a.heads) * a.dim;
   call->out_head_stride = a.dim;
-  call->status = a.device_status;
   call->sm_count = gv::current_sm_count();
 }
 
@@ -183,7 +204,8 @@ int gevva_attn_append(const gevva_attn_append_args* a, gevva_stream_t stream) {
   call.q_out = a->q_out;
   call.k_out = a->k_out;
   call.v_out = a->v_out;
-  call.status = a->device_status;
+  const cudaError_t e = status_word(a->device_status, &call.status);
+  if (e != cudaSuccess) return launched(e);
   return launched(gv::launch_kv_append(call, gv::current_sm_count(), stream));
 }
 
@@ -204,6 +226,8 @@ int gevva_attn_prompt(const gevva_attn_prompt_args* a, gevva_stream_t stream) {
   call.token_offsets = a->token_offsets;
   call.sequences = a->sequences;
   fill_attention(&call, *a);
+  const cudaError_t e = status_word(a->device_status, &call.status);
+  if (e != cudaSuccess) return launched(e);
   return launched(gv::launch_attention(call, stream));
 }
 
@@ -226,7 +250,19 @@ int gevva_attn_chunk(const gevva_attn_chunk_args* a, gevva_stream_t stream) {
   call.workspace = a->workspace;
   fill_attention(&call, *a);
   if (call.sm_count < 1) return GEVVA_MOE_NO_DEVICE;
+  const cudaError_t e = status_word(a->device_status, &call.status);
+  if (e != cudaSuccess) return launched(e);
   return launched(gv::launch_attention(call, stream));
+}
+
+int gevva_attention_last_status(void) {
+  int* word = nullptr;
+  int status = 0;
+  cudaError_t e = status_word(nullptr, &word);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(&status, word, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && status != 0) e = cudaMemset(word, 0, sizeof(int));
+  return e == cudaSuccess ? -status : launched(e);
 }
 
 }  // extern "C"

@@ -369,8 +369,12 @@ int gevva_ff_layer_launch(const gevva_ff_layer* layer, const void* hidden, void*
  * are held in 32 bits, rotation angles in 64.  All pointers are 16-byte aligned (32-byte: `out` and `workspace` of the two
  * attention calls), strides are in elements, positive and multiples of 8.
  * Queries, keys and values are [tokens, heads, dim] with the last dimension contiguous, given as an address and two strides (of a token and
- * of a head): views of a fused projection's rows, for instance.  The calls keep no state; `device_status` is an optional device
- * status word that receives GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do. */
+ * of a head): views of a fused projection's rows, for instance.  The calls keep no state; `device_status` is a device
+ * status word that receives GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do; NULL: one that the library
+ * has for each device, which gevva_attention_last_status reads. */
+
+/* Reads and clears the status of the attention calls on the current device that were given no word (synchronises the device). */
+int gevva_attention_last_status(void);
 
 /* A paged cache: keys and values are bf16 [pages, page_size, kv_heads, dim] with strides of their own; page_size is a power of two,
  * at least 16. */

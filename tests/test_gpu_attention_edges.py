@@ -110,3 +110,28 @@ def test_a_batch_follows_its_tensors(attn, cuda_device):
         length -= 5
         ref.within(got, *ref.attention(q, *gathered(cache, batch, 0, length), length - 1, 0.125, 0), f"step {step}")
         del junk
+
+
+# ---- reports ------------------------------------------------------------------------------------------
+def test_calls_without_a_status_word_report_too(attn, cuda_device):
+    import ctypes
+    from gevva_b200 import GevvaMoeError
+    attn.check(cuda_device)
+    lib = attn._lib()
+    cache = attn.KvCache(randn((2, 16, 1, 64), cuda_device, 1), randn((2, 16, 1, 64), cuda_device, 2))
+    batch = attn.PagedBatch(torch.tensor([0, 1], dtype=torch.int32, device=cuda_device), torch.tensor([20], dtype=torch.int32, device=cuda_device),
+                            torch.tensor([[1, 2]], dtype=torch.int32, device=cuda_device))  # (there is no page 2)
+    q, out = randn((1, 1, 64), cuda_device, 3), torch.empty((1, 1, 64), dtype=torch.bfloat16, device=cuda_device)
+    workspace = torch.empty(lib.gevva_attn_chunk_workspace_bytes(64), dtype=torch.uint8, device=cuda_device)
+    stream = torch.cuda.current_stream().cuda_stream
+    chunk = attn._CHUNK.pack(q.data_ptr(), 64, 64, cache._address, batch._address, out.data_ptr(), workspace.data_ptr(), 0, 1, 1, 1, 64, 0, 0.125)
+    append = attn._APPEND.pack(q.data_ptr(), 64, 64, q.data_ptr(), 64, 64, q.data_ptr(), 64, 64, cache._address, batch._address, 0, 0, 0, out.data_ptr(), 0, 0,
+                               0, 1, 1, 1, 64, 0, 0, 1e-6, 0)
+    for call in (lambda: lib.gevva_attn_chunk(chunk, stream), lambda: lib.gevva_attn_append(append, stream)):
+        assert call() == 0
+        with pytest.raises(GevvaMoeError, match="page"):
+            attn.check()
+        assert attn.last_status(cuda_device) == 0
+    attn.prompt_attention(q, q, q, batch.token_offsets, 0.125)
+    attn.check()
+    assert cache.last_status() == 0
