@@ -353,9 +353,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int parts = attn_parts(work, static_cast<int>(gridDim.x), heads, kLeastRun);
       if (static_cast<int>(blockIdx.x) < parts) {
         const long long run_begin = attn_part_begin(work, parts, blockIdx.x), run_end = attn_part_begin(work, parts, blockIdx.x + 1);
-        int head = attn_quotient(run_begin, of_head);
+        const int head = attn_quotient(run_begin, of_head);
         const long long in_head = run_begin - head * of_head;
-        long long at = run_begin, before = 0;
+        long long before = 0;
         int s = 0;
         for (;; s += 32) {
           if (loaded != s) {
@@ -368,89 +368,42 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > in_head)) - 1;
         const long long in_front = __shfl_sync(0xffffffffu, upto, (owner + 31) & 31);
-        long long offset = in_head - before - (owner > 0 ? in_front : 0);
+        const long long offset = in_head - before - (owner > 0 ? in_front : 0);
         const long long of_first = __shfl_sync(0xffffffffu, upto, owner) - (owner > 0 ? in_front : 0);  // of the run's first sequence
         s += owner;
-        while (ok && at < run_end) {
-          load_sequences(s & ~31);
-          const int from = __shfl_sync(0xffffffffu, lane_from, s & 31), news = __shfl_sync(0xffffffffu, lane_news, s & 31);
-          const int length = __shfl_sync(0xffffffffu, lane_length, s & 31);
-          if (news > 0) {
-            const AttnSequence q = attn_sequence(news, length, step);
-            // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as
-            // when a chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of
-            // each one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 533 us).
-            int tile = 0, last = -1;
-            long long end = run_end;
-#pragma unroll 1  // (a short reply's time is that of code fetched for the first time: this only once)
-            for (int i = q.query_tiles > 1 && offset > 0 && offset + (run_end - at) <= of_first ? 1 : 0; i >= 0; --i) {
-              const long long target = i > 0 ? offset + (run_end - at) - 1 : offset;
-              const int found = attn_find_query_tile(q, target, step, p.window);
-              const long long begin = attn_tiles_before(q, found, step, p.window);
-              if (i > 0) {
-                last = found;
-                end = run_end - (target + 1 - begin);
-              } else {
-                tile = found;
-                offset -= begin;
-              }
-            }
-            if (last == tile) {
-              last = -1;
-              end = run_end;
-            }
-            const int first = tile;
-            const long long first_offset = offset, first_at = at;
-            bool ahead = last >= 0;
-            if (ahead) {
-              tile = last;
-              offset = 0;
-              at = end;
-            }
-            for (; ok && tile < q.query_tiles && (ahead || at < end); ++tile) {
-              const int tiles = attn_tiles(q, tile, step, p.window);
-              const int skip = static_cast<int>(offset);
-              const int take = static_cast<int>(min(static_cast<long long>(tiles - skip), (ahead ? run_end : end) - at));
-              Piece piece;
-              piece.tiles = take;
-              piece.first_tile = attn_first_tile(q, tile, step, p.window) + skip;
-              piece.query0 = from + tile * step;
-              piece.tokens = min(step, news - tile * step);
-              piece.position0 = q.past + tile * step;
-              piece.key_origin = 0;
-              piece.sequence = s;
-              piece.kv_head = head / S::kHalves;
-              piece.half = head % S::kHalves;
-              piece.slot = take == tiles ? -1 : 2 * static_cast<int>(blockIdx.x) + (skip == 0 ? 1 : 0);
-              if (skip == 0 && take < tiles) {
-                // the item goes on in the next CTAs' runs: what attention_join_kernel has to add up
-                int upto_part = blockIdx.x + 1;
-                while (attn_part_begin(work, parts, upto_part + 1) < at + tiles) ++upto_part;
-                record[0] = upto_part - static_cast<int>(blockIdx.x);
-                record[1] = piece.query0;
-                record[2] = piece.tokens;
-                record[3] = piece.kv_head;
-                record[4] = piece.half;
-              }
-              at += take;
-              offset = 0;
-              ok = room();
-              if (ok) hand_out(piece);
-              if (ahead) {
-                ahead = false;
-                tile = first - 1;
-                offset = first_offset;
-                at = first_at;
-              }
-            }
-            if (last >= 0) at = run_end;
+        int from = 0, past = 0, news = 0;
+        const auto load = [&](int sequence, int* of_news, int* length) {
+          load_sequences(sequence & ~31);
+          from = __shfl_sync(0xffffffffu, lane_from, sequence & 31);
+          news = *of_news = __shfl_sync(0xffffffffu, lane_news, sequence & 31);
+          *length = __shfl_sync(0xffffffffu, lane_length, sequence & 31);
+          past = *length - news;
+        };
+        const auto share_out = [&](const AttnShare& share) {
+          const AttnSequence q = {news, past, 0};
+          Piece piece;
+          piece.tiles = share.take;
+          piece.first_tile = attn_first_tile(q, share.tile, step, p.window) + share.skip;
+          piece.query0 = from + share.tile * step;
+          piece.tokens = min(step, news - share.tile * step);
+          piece.position0 = past + share.tile * step;
+          piece.key_origin = 0;
+          piece.sequence = share.sequence;
+          piece.kv_head = share.head / S::kHalves;
+          piece.half = share.head % S::kHalves;
+          piece.slot = share.slot;
+          if (share.behind > 0) {  // what attention_join_kernel has to add up
+            record[0] = share.behind;
+            record[1] = piece.query0;
+            record[2] = piece.tokens;
+            record[3] = piece.kv_head;
+            record[4] = piece.half;
           }
-          offset = 0;
-          if (++s == p.sequences) {
-            s = 0;
-            ++head;
-          }
-        }
+          if (!room()) return false;
+          hand_out(piece);
+          return true;
+        };
+        ok = attn_walk(work, parts, blockIdx.x, run_begin, run_end, head, s, offset, of_first, p.sequences, step, p.window, load, share_out);
       }
       if (lane == 0) {
         int4* slot = reinterpret_cast<int4*>(p.records + 8 * static_cast<size_t>(blockIdx.x));

@@ -126,4 +126,96 @@ GV_HD int attn_quotient(long long a, long long b) {
   return static_cast<int>(a / b);
 }
 
+// What a run has of one item: key tiles [skip, skip + take) of the `tiles` that query tile `tile` has.
+struct AttnShare {
+  int head, sequence, tile;
+  int skip, take, tiles;
+  int slot;    // of its sums among 2 * parts: 2 * part for a share that another run begins, the one behind for a share that this run's end
+               // cuts off; -1: the whole item
+  int behind;  // of a share that is cut off: in how many of the next runs the item goes on
+};
+
+// The shares of run `part`, key tiles [begin, end) of all work, in the order in which they are worked on: hand_out(share), false to end there.
+// The run begins in `sequence`, `offset` key tiles behind that sequence's first in `head` (of `of_first`); load(sequence, &news,
+// &length) tells a sequence's.  Behind the last of `sequences` comes the next head's first.
+template <class Load, class HandOut>
+GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long long end, int head, int sequence, long long offset,
+                     long long of_first, int sequences, int step, int window, Load&& load, HandOut&& hand_out) {
+  long long at = begin;
+  bool ok = true;
+  while (ok && at < end) {
+    int news, length;
+    load(sequence, &news, &length);
+    if (news > 0) {
+      const AttnSequence q = attn_sequence(news, length, step);
+      // A run inside one sequence that begins and ends inside items takes the last one first: runs of about an item's length, as
+      // when a chunk has about as many query tiles as there are CTAs, then read the same keys at about the same time instead of
+      // each one others (512 tokens behind 31488, heads of 512, 128 MB of keys and values: 690 -> 533 us).
+      int tile = 0, last = -1;
+      long long stop = end;
+#ifdef __CUDACC__
+#pragma unroll 1  // (a short reply's time is that of code fetched for the first time: this only once)
+#endif
+      for (int i = q.query_tiles > 1 && offset > 0 && offset + (end - at) <= of_first ? 1 : 0; i >= 0; --i) {
+        const long long target = i > 0 ? offset + (end - at) - 1 : offset;
+        const int found = attn_find_query_tile(q, target, step, window);
+        const long long before = attn_tiles_before(q, found, step, window);
+        if (i > 0) {
+          last = found;
+          stop = end - (target + 1 - before);
+        } else {
+          tile = found;
+          offset -= before;
+        }
+      }
+      if (last == tile) {
+        last = -1;
+        stop = end;
+      }
+      const int first = tile;
+      const long long first_offset = offset, first_at = at;
+      bool ahead = last >= 0;
+      if (ahead) {
+        tile = last;
+        offset = 0;
+        at = stop;
+      }
+      for (; ok && tile < q.query_tiles && (ahead || at < stop); ++tile) {
+        const int tiles = attn_tiles(q, tile, step, window);
+        const long long left = (ahead ? end : stop) - at;
+        AttnShare share;
+        share.head = head;
+        share.sequence = sequence;
+        share.tile = tile;
+        share.tiles = tiles;
+        share.skip = static_cast<int>(offset);
+        share.take = tiles - share.skip < left ? tiles - share.skip : static_cast<int>(left);
+        share.slot = share.take == tiles ? -1 : 2 * part + (share.skip == 0 ? 1 : 0);
+        share.behind = 0;
+        if (share.skip == 0 && share.take < tiles) {
+          int upto = part + 1;
+          while (attn_part_begin(work, parts, upto + 1) < at + tiles) ++upto;
+          share.behind = upto - part;
+        }
+        at += share.take;
+        offset = 0;
+        ok = hand_out(share);
+        if (ahead) {
+          ahead = false;
+          tile = first - 1;
+          offset = first_offset;
+          at = first_at;
+        }
+      }
+      if (last >= 0) at = end;
+    }
+    offset = 0;
+    if (++sequence == sequences) {
+      sequence = 0;
+      ++head;
+    }
+  }
+  return ok;
+}
+
 }  // namespace gv
