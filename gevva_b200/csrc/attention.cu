@@ -357,7 +357,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const long long in_head = run_begin - head * of_head;
         long long before = 0;
         int s = 0;
-        for (;; s += 32) {
+        for (; s < p.sequences; s += 32) {
           if (loaded != s) {
             load_sequences(s);
             upto = upto_lane();
@@ -403,7 +403,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           hand_out(piece);
           return true;
         };
-        ok = attn_walk(work, parts, blockIdx.x, run_begin, run_end, head, s, offset, of_first, p.sequences, step, p.window, load, share_out);
+        ok = attn_walk(work, parts, blockIdx.x, run_begin, run_end, heads, head, s, offset, of_first, p.sequences, step, p.window, load, share_out);
       }
       if (lane == 0) {
         int4* slot = reinterpret_cast<int4*>(p.records + 8 * static_cast<size_t>(blockIdx.x));

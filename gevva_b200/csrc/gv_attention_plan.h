@@ -138,12 +138,14 @@ struct AttnShare {
 // The shares of run `part`, key tiles [begin, end) of all work, in the order in which they are worked on: hand_out(share), false to end there.
 // The run begins in `sequence`, `offset` key tiles behind that sequence's first in `head` (of `of_first`); load(sequence, &news,
 // &length) tells a sequence's.  Behind the last of `sequences` comes the next head's first.
+// Ends by itself, and names no slot or run that there is not, whatever load() tells: lengths that change while a call runs give wrong results
+// and nothing worse.
 template <class Load, class HandOut>
-GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long long end, int head, int sequence, long long offset,
+GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long long end, int heads, int head, int sequence, long long offset,
                      long long of_first, int sequences, int step, int window, Load&& load, HandOut&& hand_out) {
   long long at = begin;
   bool ok = true;
-  while (ok && at < end) {
+  while (ok && at < end && head < heads) {
     int news, length;
     load(sequence, &news, &length);
     if (news > 0) {
@@ -183,6 +185,7 @@ GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long 
       for (; ok && tile < q.query_tiles && (ahead || at < stop); ++tile) {
         const int tiles = attn_tiles(q, tile, step, window);
         const long long left = (ahead ? end : stop) - at;
+        if (offset < 0 || offset >= tiles || left < 1) return ok;  // (the work is not what it was)
         AttnShare share;
         share.head = head;
         share.sequence = sequence;
@@ -193,8 +196,8 @@ GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long 
         share.slot = share.take == tiles ? -1 : 2 * part + (share.skip == 0 ? 1 : 0);
         share.behind = 0;
         if (share.skip == 0 && share.take < tiles) {
-          int upto = part + 1;
-          while (attn_part_begin(work, parts, upto + 1) < at + tiles) ++upto;
+          int upto = part;
+          while (upto + 1 < parts && attn_part_begin(work, parts, upto + 1) < at + tiles) ++upto;
           share.behind = upto - part;
         }
         at += share.take;
@@ -210,7 +213,7 @@ GV_HD bool attn_walk(long long work, int parts, int part, long long begin, long 
       if (last >= 0) at = end;
     }
     offset = 0;
-    if (++sequence == sequences) {
+    if (++sequence >= sequences) {
       sequence = 0;
       ++head;
     }

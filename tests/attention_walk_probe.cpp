@@ -1,9 +1,10 @@
-// Plays every CTA's run of attention work through on the host, by the code that the kernel walks it with (attn_walk, gv_attention_plan.h):
+// Without an argument: plays every CTA's run of attention work through on the host, by the code that the kernel walks it with (attn_walk, gv_attention_plan.h):
 // reads cases "window step heads parts least sequences (news length)..." and prints "ok <cases>" where
 //   - the shares hold every item's key tiles once (an item: head, sequence, query tile), none of them empty,
 //   - sums go to slots that no other share has,
 //   - an item that is whole goes to none; one that is cut is told of by the run it begins in and by no other, once a run, and the slots
 //     that attention_join_kernel then reads (the second of that run, the first of the next `behind`) hold its key tiles in their order.
+// With one: lengths that change while the work is walked.
 #include <cstdio>
 #include <map>
 #include <tuple>
@@ -23,6 +24,38 @@ struct Sums {
   Item item;
   int skip, take;
 };
+
+// Lengths that change with every look at them: the walk ends, and its shares name key tiles, slots and runs that there are.
+static bool change(int seed) {
+  unsigned long long state = 0x9e3779b97f4a7c15ull * (seed + 1);
+  const auto draw = [&](int low, int high) {
+    state = state * 6364136223846793005ull + 1442695040888963407ull;
+    return low + static_cast<int>((state >> 33) % (high - low + 1));
+  };
+  const int step = draw(1, 256), window = draw(0, 2) ? 0 : draw(1, 2000), heads = draw(1, 6), parts = draw(1, 160), sequences = draw(1, 90);
+  const long long work = draw(1, 100000), part = draw(0, parts - 1);
+  const long long begin = attn_part_begin(work, parts, part), end = attn_part_begin(work, parts, part + 1);
+  AttnSequence now{};
+  bool good = true;
+  long long loads = 0;
+  const int kind = draw(0, 3);  // all empty; all alike; any
+  const auto load = [&](int, int* news, int* length) {
+    *news = kind == 0 ? 0 : kind == 1 ? 1 : draw(0, 600);
+    *length = kind == 1 ? 1 : draw(0, 40000);
+    now = attn_sequence(*news, *length, step);
+    if (++loads > 2ll * heads * sequences + 1000) good = fail("loads", loads, sequences);
+  };
+  const auto hand_out = [&](const AttnShare& share) {
+    const int tiles = attn_tiles(now, share.tile, step, window);
+    if (share.tile < 0 || share.tile >= now.query_tiles || share.tiles != tiles || share.skip < 0 || share.take < 1 || share.skip + share.take > tiles)
+      return good = fail("share", share.skip, share.take);
+    if (share.slot < -1 || share.slot >= 2 * parts || share.behind < 0 || part + share.behind >= parts) return good = fail("slot", share.slot, share.behind);
+    return good;
+  };
+  attn_walk(work, parts, static_cast<int>(part), begin, end, heads, draw(0, heads), draw(0, sequences + 31), draw(-5, 3) * 1000000007ll, draw(0, 5000),
+            sequences, step, window, load, hand_out);
+  return good;
+}
 
 static bool play(int window, int step, int heads, int parts_most, int least, const std::vector<int>& news, const std::vector<int>& lengths) {
   const int sequences = static_cast<int>(news.size());
@@ -72,7 +105,7 @@ static bool play(int window, int step, int heads, int parts_most, int least, con
       }
       return true;
     };
-    if (!attn_walk(work, parts, part, begin, end, head, s, offset, of_sequence[s], sequences, step, window, load, hand_out) || !good) return false;
+    if (!attn_walk(work, parts, part, begin, end, heads, head, s, offset, of_sequence[s], sequences, step, window, load, hand_out) || !good) return false;
     if (taken != end - begin) return fail("run", taken, end - begin);
   }
   // every item's key tiles once
@@ -106,7 +139,13 @@ static bool play(int window, int step, int heads, int parts_most, int least, con
   return true;
 }
 
-int main() {
+int main(int argc, char**) {
+  if (argc > 1) {  // any argument: lengths that change
+    for (int seed = 0; seed < 200000; ++seed)
+      if (!change(seed)) return 1;
+    std::printf("ok\n");
+    return 0;
+  }
   int window, step, heads, parts, least, sequences, cases = 0;
   while (std::scanf("%d %d %d %d %d %d", &window, &step, &heads, &parts, &least, &sequences) == 6) {
     std::vector<int> news(sequences), lengths(sequences);

@@ -81,6 +81,12 @@ def test_work_past_the_divisions_in_32_bits(probe):
                   (5000, 64, 8, 148, 1, [(100000, 101234)] * 5)])
 
 
+def test_lengths_that_change_while_a_call_runs(probe):
+    """As when another stream writes them: the results are then wrong, but every CTA ends and stays within its workspace."""
+    done = subprocess.run([probe, "change"], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "ok", done.stdout
+
+
 @pytest.mark.parametrize("line,wrong", [
     ("share.slot = share.take == tiles ? -1 : 2 * part + (share.skip == 0 ? 1 : 0);", "share.slot = share.take == tiles ? -1 : 2 * part;"),
     ("share.behind = upto - part;", "share.behind = upto - part - 1;"),
