@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests import attention_ref as ref
-from tests.test_gpu_attention import attn, gathered, make_batch, randn  # noqa: F401  (attn: a fixture)
+from tests.test_gpu_attention import attn, gathered, make_batch, offsets_of, randn  # noqa: F401  (attn: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -28,6 +28,142 @@ def test_scores_that_are_no_numbers_give_none(attn, cuda_device, dim):
     for got in (attn.prompt_attention(q, k, v, batch.token_offsets, 0.125, window=1), attn.chunk_attention(q, cache, batch, 0.125, window=1)):
         assert torch.isnan(got[broken]).all()
         assert torch.equal(got[~broken], v[~broken])
+
+
+# ---- every key counts -----------------------------------------------------------------------------
+def counted(tokens, length, heads, kv_heads, dim, device, seed):
+    """Operands for which p is zero or one: every key has a class of its key head and a score of 128 for the queries of that class, zero for
+    the others, so that a row's result is the mean of v over the keys of its class (exp(-128) is nothing), or over all that it sees where
+    none is of its class.  v is whole numbers, so sums are exact; a key lost, seen twice or taken from elsewhere changes the mean by more than its
+    rounding."""
+    gen = torch.Generator(device=device)
+    gen.manual_seed(seed)
+    group = heads // kv_heads
+    kind = torch.randint(0, group, (length, kv_heads), generator=gen, device=device)
+    k = 128.0 * torch.nn.functional.one_hot(kind, dim)
+    q = torch.nn.functional.one_hot(torch.arange(heads, device=device) % group, dim).float().expand(tokens, heads, dim)
+    v = torch.randint(-2, 3, (length, kv_heads, dim), generator=gen, device=device)
+    return [x.to(torch.bfloat16).contiguous() for x in (q, k, v)]
+
+
+def whole_mean(got, q, k, v, past, window, what=""):
+    """The mean is rounded once; the sum that divides it and its inverse are off by a few 2^-24, an exponential of zero by 2^-18 at most."""
+    want, _ = ref.attention(q, k, v, past, 1.0, window)
+    ref.within(got, want, want.abs() * (ref.BF16 + 2.0 ** -17) + 1e-30, what)
+    # the test itself: one key less would have been noticed
+    h, group, row = q.shape[1] - 1, q.shape[1] // k.shape[1], q.shape[0] - 1
+    if past + row > 0 and window != 1:
+        low = max(0, past + row - window + 1) if window else 0
+        score = q[row, h].double() @ k[low:past + row + 1, h // group].double().T
+        mine = (score == score.amax()).nonzero()[:, 0] + low
+        lost = mine[len(mine) // 2]
+        less = (v[mine, h // group].double().sum(0) - v[lost, h // group].double()) / max(len(mine) - 1, 1)
+        assert ((less - want[row, h]).abs() > want[row, h].abs() * (ref.BF16 + 2.0 ** -17)).any(), (what, "a lost key would not be noticed")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("news,lengths,heads,kv_heads,page,window", [
+    ([1], [20000], 7, 1, 16, 0), ([1], [20000], 8, 8, 16, 0), ([1, 1, 1], [5000, 3, 12345], 12, 3, 32, 0), ([1, 1], [30000, 9000], 4, 2, 64, 7000),
+    ([5, 3], [6001, 129], 6, 1, 16, 1024), ([300], [2300], 8, 2, 128, 0), ([200, 7], [900, 4000], 3, 1, 1024, 333)])
+def test_chunk_counts_every_key(attn, cuda_device, dim, news, lengths, heads, kv_heads, page, window):
+    batch, pages = make_batch(attn, news, lengths, page, cuda_device, 3)
+    cache = attn.KvCache(*(torch.full((pages, page, kv_heads, dim), 96.0, dtype=torch.bfloat16, device=cuda_device) for _ in range(2)))
+    parts = [counted(n, length, heads, kv_heads, dim, cuda_device, s) for s, (n, length) in enumerate(zip(news, lengths))]
+    for s, ((_, k, v), length) in enumerate(zip(parts, lengths)):
+        at = torch.arange(length, device=cuda_device)
+        rows = batch.table[s].long()[at // page]
+        cache.k[rows, at % page] = k
+        cache.v[rows, at % page] = v
+    got = attn.chunk_attention(torch.cat([q for q, _, _ in parts]), cache, batch, 1.0, window)
+    cache.check()
+    at = 0
+    for s, ((q, k, v), n, length) in enumerate(zip(parts, news, lengths)):
+        whole_mean(got[at:at + n], q, k, v, length - n, window, f"sequence {s}")
+        at += n
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("news,heads,kv_heads,window", [([1500], 4, 2, 0), ([700, 0, 33, 260], 7, 1, 129), ([400, 650], 2, 2, 0)])
+def test_prompt_counts_every_key(attn, cuda_device, dim, news, heads, kv_heads, window):
+    parts = [counted(n, n, heads, kv_heads, dim, cuda_device, s) for s, n in enumerate(news)]
+    q, k, v = (torch.cat(x) for x in zip(*parts))
+    got = attn.prompt_attention(q, k, v, offsets_of(news, cuda_device), 1.0, window=window)
+    at = 0
+    for s, (n, part) in enumerate(zip(news, parts)):
+        if n:
+            whole_mean(got[at:at + n], *part, 0, window, f"sequence {s}")
+        at += n
+
+
+# ---- many heads to a key head, many sequences, long contexts ----------------------------------------
+@pytest.mark.parametrize("dim", [64, 128, 256, 512])
+@pytest.mark.parametrize("heads,kv_heads", [(17, 1), (34, 2), (32, 1), (65, 1), (100, 1), (128, 1), (256, 2)])
+def test_many_query_heads_to_a_key_head(attn, cuda_device, dim, heads, kv_heads):
+    news, lengths, page, window = [40, 1, 3], [40, 300, 200], 16, 37
+    q = randn((sum(news), heads, dim), cuda_device, 1)
+    k, v = (randn((sum(news), kv_heads, dim), cuda_device, 2 + i) for i in range(2))
+    got = attn.prompt_attention(q, k, v, offsets_of(news, cuda_device), dim ** -0.5, window=window)
+    batch, pages = make_batch(attn, news, lengths, page, cuda_device, 3)
+    cache = attn.KvCache(randn((pages, page, kv_heads, dim), cuda_device, 5), randn((pages, page, kv_heads, dim), cuda_device, 6))
+    paged = attn.chunk_attention(q, cache, batch, dim ** -0.5)
+    cache.check()
+    at = 0
+    for s, (n, length) in enumerate(zip(news, lengths)):
+        rows = slice(at, at + n)
+        ref.within(got[rows], *ref.attention(q[rows], k[rows], v[rows], 0, dim ** -0.5, window), f"prompt {s}")
+        ref.within(paged[rows], *ref.attention(q[rows], *gathered(cache, batch, s, length), length - n, dim ** -0.5, 0), f"sequence {s}")
+        at += n
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 2), (256, 2, 1)])
+def test_many_sequences(attn, cuda_device, dim, heads, kv_heads):
+    """More than a warp looks at together, some of them empty, as prompts, appended and over pages."""
+    news = [(0, 1, 3, 8, 0, 17, 2, 131)[i * 5 % 8] if i % 67 else 0 for i in range(500)]
+    q, k, v = (randn((sum(news), h, dim), cuda_device, i) for i, h in enumerate((heads, kv_heads, kv_heads)))
+    batch, pages = make_batch(attn, news, news, 16, cuda_device, 1)
+    cache = attn.KvCache.empty(pages, 16, kv_heads, dim, cuda_device)
+    packed = attn.kv_append(q, k, v, cache, batch, None, packed=True)
+    cache.check()
+    assert all(torch.equal(x, y) for x, y in zip(packed, (q, k, v)))
+    prompt = attn.prompt_attention(q, k, v, batch.token_offsets, 0.125)
+    chunk = attn.chunk_attention(q, cache, batch, 0.125)
+    at = 0
+    for s, n in enumerate(news):
+        if n:
+            want, bound = ref.attention(q[at:at + n], k[at:at + n], v[at:at + n], 0, 0.125, 0)
+            ref.within(prompt[at:at + n], want, bound, f"prompt {s}")
+            ref.within(chunk[at:at + n], want, bound, f"sequence {s}")
+        at += n
+
+
+def test_work_past_the_divisions_in_32_bits(attn, cuda_device):
+    """2^22 key tiles: 64 sequences of a million keys in 8 heads.  A sequence's table names one page again and again, and another at its end."""
+    sequences, heads, dim, page, width = 64, 8, 64, 256, 4096
+    pages = 24
+    batch = attn.PagedBatch(offsets_of([1] * sequences, cuda_device), torch.full((sequences,), width * page, dtype=torch.int32, device=cuda_device),
+                            (torch.arange(sequences, dtype=torch.int32, device=cuda_device) % 8)[:, None].repeat(1, width))
+    batch.table[:, -1] = 8 + torch.arange(sequences, dtype=torch.int32, device=cuda_device) % 16
+    cache = attn.KvCache(randn((pages, page, heads, dim), cuda_device, 1), randn((pages, page, heads, dim), cuda_device, 2))
+    # the last page's keys weigh about as much as all others together
+    cache.k[8:] *= 0
+    cache.k[8:, :, :, 0] = 10.5
+    q = randn((sequences, heads, dim), cuda_device, 3)
+    q[:, :, 0] = 7.0
+    got = attn.chunk_attention(q, cache, batch, 0.125)
+    cache.check()
+    q64, k64, v64 = q.double(), cache.k.double(), cache.v.double()
+    for s in range(sequences):
+        first, last = s % 8, 8 + s % 16
+        score = torch.cat([torch.einsum("hd,phd->hp", q64[s], k64[x]) for x in (first, last)], 1) * 0.125
+        times = torch.cat([torch.full((page,), width - 1.0), torch.ones(page)]).to(cuda_device).double()
+        p = torch.exp(score - score.amax(1, keepdim=True)) * times
+        total = p.sum(1, keepdim=True)
+        v = torch.cat([v64[first], v64[last]])
+        want, terms = torch.einsum("hp,phd->hd", p, v) / total, torch.einsum("hp,phd->hd", p, v.abs()) / total
+        # as in the 64-bit form of the tests, and the sums: 2^16 products of 16 keys and 2^13 key tiles, each added with an error of 2^-23 of the sum at most
+        size = torch.cat([torch.einsum("hd,phd->hp", q64[s].abs(), k64[x].abs()) for x in (first, last)], 1).amax(1, keepdim=True) * 0.125
+        off = ref.BF16 + 2 * (dim + 4) * ref.FP32 * size + 64 * ref.FP32 + 2.0 ** -23 * (2 ** 16 + 2 ** 13)
+        ref.within(got[s], want, ref.BF16 * want.abs() + terms * off, f"sequence {s}")
 
 
 # ---- sharp rows -------------------------------------------------------------------------------------
