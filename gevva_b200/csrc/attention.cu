@@ -159,7 +159,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 // The same for two exponents on the multiply-add units: 2^n of the nearest whole n, times the polynomial of degree four with the
-// smallest largest relative error for what is left, in [-1/2, 1/2] (2.7e-6, by iterated reweighted least squares), far below
+// smallest largest relative error for what is left, in [-1/2, 1/2] (2.7e-6; exp2_minimax in fit_transcendentals.py), far below
 // the rounding of p to bf16.  Zero below 2^-126, as from the other; what is no number stays none (2^n put into the exponent by adding
 // whole numbers would make it the largest finite one).
 __device__ __forceinline__ void exp2_by_polynomial(unsigned long long x, float& a, float& b) {

@@ -1,8 +1,9 @@
-"""Derives the polynomial coefficients hard-coded in gv_transcendentals.h.
+"""Derives the polynomial coefficients hard-coded in gv_transcendentals.h and in attention.cu.
 
 erf and exp are approximated by Chebyshev interpolants (converted to monomials in
 a centred, scaled variable) so that the CPU oracle and the CUDA kernels evaluate
-the very same fp32 fmaf chain and therefore agree bit for bit.  Run:
+the very same fp32 fmaf chain and therefore agree bit for bit.  2^f of attention is the polynomial with the smallest largest
+relative error, which no oracle repeats.  Run:
 
     python fit_transcendentals.py        # prints C initialisers + max errors
 """
@@ -32,6 +33,23 @@ def fmt(mono, width):
     return "{" + ", ".join(f"{np.float32(v):.9e}f" for v in m) + "}"
 
 
+def exp2_minimax(degree=4, rounds=2000):
+    """Coefficients (of f^0 first) for 2^f on [-1/2, 1/2] with the smallest largest relative error, by iterated reweighted least squares
+    (Lawson): each point's weight grows with its error.  The last place of a coefficient goes by the rounding of the least squares."""
+    f = 0.5 * np.cos(np.pi * (np.arange(4001) + 0.5) / 4001)
+    powers = np.vander(f, degree + 1, increasing=True) / np.exp2(f)[:, None]
+    weight, best, least = np.ones_like(f), None, np.inf
+    for _ in range(rounds):
+        root = np.sqrt(weight)
+        c = np.linalg.lstsq(powers * root[:, None], root, rcond=None)[0]
+        off = np.abs(powers @ c - 1)
+        if off.max() < least:
+            best, least = c, off.max()
+        weight = weight * off
+        weight /= weight.sum()
+    return best, least
+
+
 def main():
     # erf on [0,4): eight intervals of width 0.5, degree 6 in u = a - centre
     worst = 0.0
@@ -56,6 +74,10 @@ def main():
     e = np.abs(horner32(m2, r).astype(np.float64) / np.exp(r.astype(np.float64)) - 1).max()
     print(f"// exp core max rel err {e:.3e}")
     print("GV_EXP_POLY =", fmt(m2, 7))
+    # 2^f on [-1/2, 1/2], exp2_by_polynomial
+    c, worst = exp2_minimax()
+    print(f"// exp2 max rel err {worst:.3e}")
+    print("exp2_by_polynomial =", fmt(c, 5))
 
 
 if __name__ == "__main__":
