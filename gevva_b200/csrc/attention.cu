@@ -521,7 +521,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const auto page_of = [&](int tile) {  // of this lane's box
         if constexpr (!kPaged) return 0;
         const int index = (tile * kKeys + box * box_rows) >> p.page_shift;
-        return __ldg(table + min(index, p.table_width - 1));
+        return table[min(index, p.table_width - 1)];
       };
       const auto fetch = [&](const CUtensorMap* map, int x, int tile, int page) {
         ok = __all_sync(0xffffffffu, wait_or_abort(&smem->empty[stage], phase ^ 1u, smem, p.status));
