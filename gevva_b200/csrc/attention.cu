@@ -29,12 +29,15 @@
 // a CTA takes an equal run of key tiles, whatever the sequences' lengths, which only the device knows; an item that a run's end cuts
 // leaves sums in the workspace, and attention_join_kernel adds them up in the order of the keys: no atomics, and the same bits every time.
 //
-// What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured).  Prompts: 8192 tokens causal, 16 heads of 256 1350 TFLOP/s, 32 of 128
-// 1210, 32 of 64 827, 16 of 512 1050 (1575 with the scores that are worked out twice).  Heads of 256 and 512: shared memory, of whose 128
-// bytes a cycle a key tile's products and TMA writes take 2560 and 4096 cycles, more than the tensor pipe (4608 tokens, heads of 512:
-// 371 us, without the writes 286; 3990 cycles a key tile).  Heads of 128: a query tile's chain of softmax, outputs and next scores.  Heads
-// of 64: the softmax warps' instructions.  Decoding: HBM, 6.2 TB/s at 64 sequences of 8 key heads of 256; a single short one is a chain of
-// latencies, 14 us (launch and plan 3, first keys 2.5, softmax of cold code 1.3, outputs 2, second launch 4).
+// What bounds it (B200, of 1658 TFLOP/s and 6.56 TB/s measured; in a graph, on a cool GPU and, behind it, under its power limit, where the clock is
+// 1.6 GHz).  Prompts: 8192 tokens causal, 16 heads of 256 405 and 425 us (1360 and 1290 TFLOP/s), 32 of 64 339 and 405 (810 and 680), 8191
+// tokens, 32 of 128 454 and 534 (1210 and 1030), 4608 tokens, 16 of 512 361 to 373 (960 to 930, half as much again with the scores that are worked
+// out twice).  Neither L2 nor shared memory bounds them: with boxes outside the tensors, which TMA fills with zeros and reads nothing for, 674 k
+// cycles become 656 k (256), 860 k 839 k (128) and 602 k 568 k (512), without the writes too 680 k, 860 k and 538 k.  Heads of 256 and 512: the
+// tensor pipe, at work for 71 and 76 % of the cycles, and what lies between its batches.  Heads of 128: a query tile's chain of softmax, outputs
+// and next scores.  Heads of 64: the softmax warps' instructions.  Decoding: HBM, 5.7 to 6.2 TB/s in a graph at 64 sequences of 8 key heads of 256
+// (by where a process's caches lie; 5.1 over 6 GB of them in turn); a single short one is a chain of latencies, 14.6 us (launch and plan
+// 3, first keys 2.5, softmax of cold code 1.5, outputs 2, second launch 4).
 #include <cuda.h>
 #include <math_constants.h>
 
@@ -100,8 +103,8 @@ struct Shape {
   // Whether a tile's values and the next one's keys fit side by side: scores of the next piece may then be asked for before this one's end.
   static constexpr bool kAhead = kTiles == 1 && kStages >= kKeyStages + kValueStages;
   // Two query tiles of heads of 64 leave tensor memory for a third score tile: scores are then asked for half a round earlier, and the
-  // chain of a query tile is its softmax alone (8192 tokens, 32 heads: 389 -> 347 us; with one exponential of eight instead of three on the
-  // multiply-add units 332).  Score tile 2 * (key tile) + (query tile), modulo three.
+  // chain of a query tile is its softmax alone (8192 tokens, 32 heads: 389 -> 347 us; 339 now, with one exponential of eight instead of three on
+  // the multiply-add units).  Score tile 2 * (key tile) + (query tile), modulo three.
   static constexpr bool kSpare = kTiles == 2 && kDim == 64;
   static constexpr uint32_t kOutputs = kSpare ? 384 : 256;  // first tensor-memory column of the outputs
   static_assert(!kSpare || (kStages & (kStages - 1)) == 0, "stages are found by position");

@@ -141,10 +141,11 @@ bool make_operand_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, 
 // w13 codes [experts, 2 halves, 704 rows, 1408 bytes] through a box of both halves x 64 rows x 128 bytes.
 bool make_w13_unit_tensor_map(CUtensorMap* map, const void* base, uint64_t experts);
 
-// w2 codes [experts * 2816 rows, 352 bytes] as [64-row groups][8][4][2] rows with strides of 64, 2, 16 and 1
-// rows, through a box of 192 rows x 128 bytes: the column order of grouped_gemm_down.cu.
 // bf16 tensor of up to four dimensions, the first (innermost) one contiguous, strides of the others in bytes, through a box with the 128-byte swizzle.
 bool make_bf16_tensor_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* stride_bytes, const uint32_t* box);
+
+// w2 codes [experts * 2816 rows, 352 bytes] as [64-row groups][8][4][2] rows with strides of 64, 2, 16 and 1
+// rows, through a box of 192 rows x 128 bytes: the column order of grouped_gemm_down.cu.
 bool make_piece_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t row_bytes);  // 32 rows in that order
 bool make_w2_down_tensor_map(CUtensorMap* map, const void* base, uint64_t experts);
 
