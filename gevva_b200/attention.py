@@ -164,8 +164,6 @@ class KvCache:
     replaced by tensors of the same shape; a captured call keeps those that it was captured with."""
 
     def __init__(self, k, v):
-        self._packed = _Cache()
-        self._address = ctypes.addressof(self._packed)
         self._take(k, v)
         self.status = torch.zeros(1, dtype=torch.int32, device=k.device)
 
@@ -180,8 +178,10 @@ class KvCache:
         self._k, self._v = k, v
         self.page_size, self.kv_heads, self.head_dim = page_size, k.shape[2], k.shape[3]
         self.device = k.device
-        self._packed.__init__(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
+        # (a new one, so that a copy of this handle keeps its own)
+        self._packed = _Cache(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2),
                               pages, page_size)
+        self._address = ctypes.addressof(self._packed)
 
     k = property(lambda self: self._k, lambda self, k: self._take(k, self._v))
     v = property(lambda self: self._v, lambda self, v: self._take(self._k, v))
@@ -211,8 +211,6 @@ class PagedBatch:
     read; a captured call keeps those that it was captured with."""
 
     def __init__(self, token_offsets, lengths, table):
-        self._packed = _Batch()
-        self._address = ctypes.addressof(self._packed)
         self._take(token_offsets, lengths, table)
 
     def _take(self, token_offsets, lengths, table):
@@ -228,7 +226,8 @@ class PagedBatch:
         self._token_offsets, self._lengths, self._table = token_offsets, lengths, table
         self.device = table.device
         stride = table.stride(0) if sequences > 1 else table.shape[1]
-        self._packed.__init__(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
+        self._packed = _Batch(token_offsets.data_ptr(), lengths.data_ptr(), table.data_ptr(), sequences, table.shape[1], stride)
+        self._address = ctypes.addressof(self._packed)
 
     token_offsets = property(lambda self: self._token_offsets, lambda self, x: self._take(x, self._lengths, self._table))
     lengths = property(lambda self: self._lengths, lambda self, x: self._take(self._token_offsets, x, self._table))

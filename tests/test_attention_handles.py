@@ -1,4 +1,7 @@
 """KvCache and PagedBatch pass addresses on: they are those of the tensors that the handles hold now.  Stand-ins for tensors on a GPU."""
+import copy
+import ctypes
+
 import pytest
 import torch
 
@@ -40,14 +43,13 @@ def cache(monkeypatch):
 
 def test_a_batch_passes_the_tensors_that_it_holds():
     b = batch()
-    address = b._address
     b.lengths = Stand(1 << 16, (2,))
     b.token_offsets = Stand(1 << 17, (3,))
     b.table = Stand(1 << 18, (2, 5), strides=(7, 1))
     assert (b.lengths.address, b.token_offsets.address, b.table.address) == (1 << 16, 1 << 17, 1 << 18)
     p = b._packed
     assert (p.lengths, p.token_offsets, p.table, p.sequences, p.table_width, p.table_stride) == (1 << 16, 1 << 17, 1 << 18, 2, 5, 7)
-    assert b._address == address
+    assert b._address == ctypes.addressof(p)
 
 
 def test_a_batch_refuses_tensors_that_do_not_fit():
@@ -73,3 +75,13 @@ def test_a_cache_passes_the_tensors_that_it_holds(cache):
         with pytest.raises(ValueError, match="cache"):
             cache.v = wrong
     assert p.values == 1 << 22 and cache.v.address == 1 << 22
+
+
+def test_a_copy_of_a_handle_keeps_its_own(cache):
+    b = batch()
+    other, other_cache = copy.copy(b), copy.copy(cache)
+    other.lengths = Stand(1 << 16, (2,))
+    other_cache.v = Stand(1 << 22, (4, 16, 2, 64), torch.bfloat16)
+    for handle, copied, field in ((b, other, "lengths"), (cache, other_cache, "values")):
+        at = [type(h._packed).from_address(h._address) for h in (handle, copied)]
+        assert getattr(at[0], field) == (8192 if field == "lengths" else 1 << 20) and getattr(at[1], field) == (1 << 16 if field == "lengths" else 1 << 22)
