@@ -126,7 +126,8 @@ def _rows(x, name="input"):
 
 
 def block_norm(x, weight, eps=1e-6, out=None, stream=None):
-    """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768."""
+    """x / sqrt(mean(x^2) + eps) * weight over rows [rows, width] of bf16; width is a multiple of 8 up to 32768.  `out` may be x,
+    and otherwise shares no memory with the inputs."""
     device, shape = _rows(x)
     if stream is not None:
         with _on(stream, device):
@@ -140,7 +141,8 @@ def block_norm(x, weight, eps=1e-6, out=None, stream=None):
 
 def block_norm_add(x, weight, residual, gate=None, scale=None, next_weight=None, eps=1e-6, out=None, stream=None):
     """(residual + gate * norm(x) * weight) * scale, the norm behind a block; with `next_weight` also the next block's norm of
-    the result, returned as (out, next).  gate bf16 [width] and scale bf16 [1] are optional; out may be residual."""
+    the result, returned as (out, next).  gate bf16 [width] and scale bf16 [1] are optional; `out` may be residual or x, and otherwise shares no memory with
+    the inputs."""
     device, shape = _rows(x)
     if stream is not None:
         with _on(stream, device):

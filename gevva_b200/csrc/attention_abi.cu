@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/gevva_moe.h"
 #include "gv_attention.h"
@@ -58,6 +59,21 @@ bool meets(const void* out, long long count, const gv::AttnRows& rows, int token
     at -= step * strides[i];
   }
   return at < dim;
+}
+
+// Of the norms, whose rows and vectors are whole ranges: whether two of them share memory; none shares any with a null pointer.
+bool touch(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+  const intptr_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
+  return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+// A row is written when it has been read, not when others have: an output is an input, row for row, or lies apart from it, and apart from the vectors.
+bool norm_apart(const void* out, const gv::BlockNormCall& call) {
+  const long long vector = 2ll * call.width, rows = call.rows * vector;
+  for (const void* in : {call.x, call.residual})
+    if (in != out && touch(out, rows, in, rows)) return false;
+  for (const void* in : {call.weight, call.gate, call.next_weight})
+    if (touch(out, rows, in, vector)) return false;
+  return !touch(out, rows, call.scale, 2);
 }
 
 bool packed(const gv::AttnRows& rows, int heads, int dim) {
@@ -140,6 +156,7 @@ int gevva_attn_norm(const void* x, const void* weight, void* out, int rows, int 
   call.rows = rows;
   call.width = width;
   call.eps = eps;
+  if (!norm_apart(out, call)) return GEVVA_MOE_BAD_ARGUMENT;
   return launched(gv::launch_block_norm(call, gv::current_sm_count(), stream));
 }
 
@@ -162,6 +179,7 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
   call.rows = rows;
   call.width = width;
   call.eps = eps;
+  if (!norm_apart(out, call) || !norm_apart(next, call) || touch(out, 2ll * rows * width, next, 2ll * rows * width)) return GEVVA_MOE_BAD_ARGUMENT;
   return launched(gv::launch_block_norm(call, gv::current_sm_count(), stream));
 }
 

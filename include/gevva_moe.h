@@ -403,7 +403,8 @@ int gevva_attn_norm(const void* x, const void* weight, void* out, int rows, int 
 
 /* out = (residual + gate * norm(x) * weight) * scale: the norm behind a block with its residual (rmsnorm_add_2816_kernel,
  * src/cuda/runtime/prefill.cuh:1197-1199).  gate [width] and scale [1] are optional (NULL: one).  With next_weight (and next; both or none)
- * next = norm(out) * next_weight as well, of the values of `out` before they are rounded.  `out` may be `residual` or `x`. */
+ * next = norm(out) * next_weight as well, of the values of `out` before they are rounded.  `out` and `next` may be `residual` or `x` (and the `out` of
+ * gevva_attn_norm `x`), row for row; outputs that share memory with an input in another way, or with one another, are refused. */
 int gevva_attn_norm_add(const void* x, const void* weight, const void* residual, const void* gate, const void* scale,
                         const void* next_weight, void* out, void* next, int rows, int width, float eps,
                         gevva_stream_t stream);

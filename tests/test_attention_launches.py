@@ -18,10 +18,11 @@ def lib(recorder):  # noqa: F811
 
 @pytest.mark.parametrize("rows", [1, 4, 5, 2 ** 31 - 5, 2 ** 31 - 4, 2 ** 31 - 3, 2 ** 31 - 1])
 def test_norms_of_any_number_of_rows(lib, rows):
-    assert lib.lib.gevva_attn_norm(ADDRESS, ADDRESS, ADDRESS, rows, 64, 1e-6, None) == 0
-    assert lib.lib.gevva_attn_norm_add(ADDRESS, ADDRESS, ADDRESS, None, None, None, ADDRESS, None, rows, 64, 1e-6, None) == 0
+    x = 1 << 20  # (the weights lie in front of the rows)
+    assert lib.lib.gevva_attn_norm(x, ADDRESS, x, rows, 64, 1e-6, None) == 0
+    assert lib.lib.gevva_attn_norm_add(x, ADDRESS, x, None, None, None, x, None, rows, 64, 1e-6, None) == 0
     assert [(x["kernel"], x["grid"]) for x in lib.launches()] == [("block_norm_kernel<0>", -(-rows // 4))] * 2
-    assert lib.lib.gevva_attn_norm(ADDRESS, ADDRESS, ADDRESS, rows, 2816, 1e-6, None) == 0
+    assert lib.lib.gevva_attn_norm(x, ADDRESS, x, rows, 2816, 1e-6, None) == 0
     assert [x["grid"] for x in lib.launches()] == [rows]
 
 

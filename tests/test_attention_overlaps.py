@@ -101,3 +101,29 @@ def test_append_refuses_with_its_outputs_apart(lib, change):
 
 def test_an_append_without_rows_does_nothing(lib):
     assert refusals.append(lib, q=refusals.rows(None), tokens=0, q_out=None) == 0
+
+
+def test_norms_over_what_they_read(lib):
+    """Rows are read before they are written, other rows and the vectors are not: an output is an input, row for row, or shares nothing with any."""
+    rows, width = 7, 64
+    size, x, w, r, g, s, nw, out, nxt = 2 * rows * width, *(n << 30 for n in range(1, 9))
+
+    def norm(to=out, x=x, w=w):
+        return lib.gevva_attn_norm(x, w, to, rows, width, 1e-6, None)
+
+    def add(to=out, nxt=nxt, x=x, r=r):
+        return lib.gevva_attn_norm_add(x, w, r, g, s, nw, to, nxt, rows, width, 1e-6, None)
+
+    for to in (out, x, x - size, x + size, w - size, w + 2 * width):
+        assert norm(to) != BAD, to
+    for to in (out, x, r, x - size, r + size, g - size, s - size, s + 16, nw + 2 * width, nxt - size, nxt + size):
+        assert add(to) != BAD, to
+    for to in (nxt, x, r, out - size):
+        assert add(nxt=to) != BAD, to
+    for to in (x + 16, x - size + 16, x + size - 16, w, w - 16, w + 2 * width - 16):
+        assert norm(to) == BAD, to
+    for to in (x + 16, r - 16, w, g, g + 2 * width - 16, s - 16, s, nw, nxt, nxt + 16, nxt - size + 16):
+        assert add(to) == BAD, to
+    for to in (out, out + 16, x + 16, r - 16, w, g, s - size + 16, nw - 16):
+        assert add(nxt=to) == BAD, to
+    assert add(r=x) != BAD and add(r=x, to=x) != BAD
