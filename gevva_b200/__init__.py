@@ -1,4 +1,5 @@
-"""B200-native NVFP4 mixture-of-experts path of Gemma-4 26B-A4B, and the attention in front of it.
+"""B200-native NVFP4 mixture-of-experts path of Gemma-4 26B-A4B, the attention in front of it, and what a
+serving step has around its layers.
 
 Python mirror of the reference's operator interface for this path
 (``gevva::Nvfp4ExpertRunner``, include/gevva/gpu.hpp:217-247, and the inline
@@ -26,6 +27,14 @@ from .runtime import (  # noqa: F401
     route_128_top8,
     route_project,
 )
+from .step import (  # noqa: F401
+    PagePool,
+    StepPlan,
+    kv_append_at,
+    plan_step,
+    sample_tokens,
+    trim_step,
+)
 
 __all__ = [
     "AttentionLayer",
@@ -36,6 +45,12 @@ __all__ = [
     "chunk_attention",
     "kv_append",
     "prompt_attention",
+    "PagePool",
+    "StepPlan",
+    "kv_append_at",
+    "plan_step",
+    "sample_tokens",
+    "trim_step",
     "ExpertWeights",
     "GevvaMoeError",
     "Nvfp4ExpertRunner",

@@ -8,6 +8,38 @@
 #include "../../include/gevva_moe.h"
 #include "gv_attention.h"
 #include "gv_launchers.h"
+#include "gv_step.h"
+
+namespace gv {
+
+int launched(cudaError_t e) {
+  if (e == cudaSuccess) return GEVVA_MOE_OK;
+  cudaGetLastError();  // reported here; not again by the next call
+  if (e == cudaErrorInvalidConfiguration) return GEVVA_MOE_TOO_LARGE;  // (more items than a grid has)
+  return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
+}
+
+// What calls without a status word of their own report into, one of each device.  (In host code the name is only a handle.)
+static __device__ int g_attention_status;
+constexpr int kMaxDevices = 64;
+static std::atomic<int*> g_status_address[kMaxDevices];
+
+// The call's word, or else the current device's.
+cudaError_t status_word(int* own, int** out) {
+  *out = own;
+  if (own) return cudaSuccess;
+  int device = -1;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  *out = g_status_address[device].load(std::memory_order_relaxed);
+  if (*out) return cudaSuccess;
+  e = cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_attention_status);
+  if (e == cudaSuccess) g_status_address[device].store(*out, std::memory_order_relaxed);
+  return e;
+}
+
+}  // namespace gv
 
 namespace {
 
@@ -80,45 +112,69 @@ bool packed(const gv::AttnRows& rows, int heads, int dim) {
   return rows.head_stride == dim && rows.token_stride == static_cast<long long>(heads) * dim;
 }
 
-bool pages_ok(gv::AttnPages* out, const gevva_attn_cache* c, const gevva_attn_batch* b, int kv_heads, int dim) {
-  if (!c || !b || !aligned(c->keys) || !aligned(c->values) || c->pages < 1 || c->page_size < 16 || (c->page_size & (c->page_size - 1)) ||
-      !b->token_offsets || !b->lengths || !b->table || b->sequences < 1 || b->table_width < 1 || b->table_stride < b->table_width ||
-      static_cast<long long>(b->table_width) * c->page_size > kMaxPositions)
-    return false;
+bool ints(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
+bool cache_ok(gv::AttnPages* out, const gevva_attn_cache* c, int kv_heads, int dim) {
+  if (!c || !aligned(c->keys) || !aligned(c->values) || c->pages < 1 || c->page_size < 16 || (c->page_size & (c->page_size - 1))) return false;
   *out = gv::AttnPages{c->keys,           c->values,            c->key_page_stride,   c->key_slot_stride, c->key_head_stride,
                        c->value_page_stride, c->value_slot_stride, c->value_head_stride, c->pages,           c->page_size,
-                       b->lengths,        b->table,             b->table_width,       b->table_stride};
+                       nullptr,           nullptr,              0,                    0};
   const long long whole = static_cast<long long>(c->page_size) * kv_heads * dim;
   return stride_ok(out->key_head_stride, kv_heads, dim) && stride_ok(out->value_head_stride, kv_heads, dim) &&
          stride_ok(out->key_slot_stride, c->page_size, dim) && stride_ok(out->value_slot_stride, c->page_size, dim) &&
          stride_ok(out->key_page_stride, c->pages, whole) && stride_ok(out->value_page_stride, c->pages, whole);
 }
 
-int launched(cudaError_t e) {
-  if (e == cudaSuccess) return GEVVA_MOE_OK;
-  cudaGetLastError();  // reported here; not again by the next call
-  if (e == cudaErrorInvalidConfiguration) return GEVVA_MOE_TOO_LARGE;  // (more items than a grid has)
-  return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
+bool pages_ok(gv::AttnPages* out, const gevva_attn_cache* c, const gevva_attn_batch* b, int kv_heads, int dim) {
+  if (!cache_ok(out, c, kv_heads, dim) || !b || !b->token_offsets || !b->lengths || !b->table || b->sequences < 1 || b->table_width < 1 ||
+      b->table_stride < b->table_width || static_cast<long long>(b->table_width) * c->page_size > kMaxPositions)
+    return false;
+  out->lengths = b->lengths;
+  out->table = b->table;
+  out->table_width = b->table_width;
+  out->table_stride = b->table_stride;
+  return true;
 }
 
-// What calls without a status word of their own report into, one of each device.  (In host code the name is only a handle.)
-static __device__ int g_attention_status;
-constexpr int kMaxDevices = 64;
-std::atomic<int*> g_status_address[kMaxDevices];
+using gv::launched;
+using gv::status_word;
 
-// The call's word, or else the current device's.
-cudaError_t status_word(int* own, int** out) {
-  *out = own;
-  if (own) return cudaSuccess;
-  int device = -1;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return e;
-  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
-  *out = g_status_address[device].load(std::memory_order_relaxed);
-  if (*out) return cudaSuccess;
-  e = cudaGetSymbolAddress(reinterpret_cast<void**>(out), g_attention_status);
-  if (e == cudaSuccess) g_status_address[device].store(*out, std::memory_order_relaxed);
-  return e;
+// What both forms of the append have; the places of the tokens are the caller's to fill.
+template <class Args>
+bool fill_append(gv::AppendCall* call, const Args& a) {
+  if (!heads_ok(a.tokens, a.heads, a.kv_heads, a.dim) ||
+      !rows_ok(&call->q, a.q, a.q_token_stride, a.q_head_stride, a.tokens, a.heads, a.dim) ||
+      !rows_ok(&call->k, a.k, a.k_token_stride, a.k_head_stride, a.tokens, a.kv_heads, a.dim) ||
+      !rows_ok(&call->v, a.v, a.v_token_stride, a.v_head_stride, a.tokens, a.kv_heads, a.dim) || a.rotated < 0 || a.rotated > a.dim ||
+      a.rotated % 16 || (a.rotated > 0 && (!a.frequencies || (reinterpret_cast<uintptr_t>(a.frequencies) & 7))) ||
+      !aligned_or_null(a.q_weight) || !aligned_or_null(a.k_weight) || !(a.eps >= 0.0f) || !aligned_for(a.q_out, a.tokens) ||
+      !aligned_or_null(a.k_out) || !aligned_or_null(a.v_out) || (a.tokens > 0 && !a.k_out != !a.v_out))
+    return false;
+  // A token's rows are written when that token's have been read, not when others' have: an output may stand where its own input does,
+  // row for row, and nowhere else among the inputs.
+  const gv::AttnRows* const inputs[3] = {&call->q, &call->k, &call->v};
+  void* const outputs[3] = {a.q_out, a.k_out, a.v_out};
+  for (int o = 0; o < 3 && a.tokens > 0; ++o) {
+    const auto heads = [&](int i) { return i == 0 ? a.heads : a.kv_heads; };
+    for (int i = 0; i < 3 && outputs[o]; ++i) {
+      if (o == i && outputs[o] == inputs[i]->data && packed(*inputs[i], heads(i), a.dim)) continue;
+      if (meets(outputs[o], static_cast<long long>(a.tokens) * heads(o) * a.dim, *inputs[i], a.tokens, heads(i), a.dim)) return false;
+    }
+  }
+  call->tokens = a.tokens;
+  call->heads = a.heads;
+  call->kv_heads = a.kv_heads;
+  call->dim = a.dim;
+  call->frequencies = a.frequencies;
+  call->rotated = a.rotated;
+  call->q_weight = a.q_weight;
+  call->k_weight = a.k_weight;
+  call->normalize_v = a.normalize_v != 0;
+  call->eps = a.eps;
+  call->q_out = a.q_out;
+  call->k_out = a.k_out;
+  call->v_out = a.v_out;
+  return true;
 }
 
 bool attention_ok(int tokens, float scale, int window) {
@@ -185,46 +241,40 @@ int gevva_attn_norm_add(const void* x, const void* weight, const void* residual,
 
 int gevva_attn_append(const gevva_attn_append_args* a, gevva_stream_t stream) {
   gv::AppendCall call{};
-  if (!a || !heads_ok(a->tokens, a->heads, a->kv_heads, a->dim) ||
-      !rows_ok(&call.q, a->q, a->q_token_stride, a->q_head_stride, a->tokens, a->heads, a->dim) ||
-      !rows_ok(&call.k, a->k, a->k_token_stride, a->k_head_stride, a->tokens, a->kv_heads, a->dim) ||
-      !rows_ok(&call.v, a->v, a->v_token_stride, a->v_head_stride, a->tokens, a->kv_heads, a->dim) ||
-      !pages_ok(&call.pages, a->cache, a->batch, a->kv_heads, a->dim) || a->rotated < 0 || a->rotated > a->dim || a->rotated % 16 ||
-      (a->rotated > 0 && (!a->frequencies || (reinterpret_cast<uintptr_t>(a->frequencies) & 7))) || !aligned_or_null(a->q_weight) ||
-      !aligned_or_null(a->k_weight) || !(a->eps >= 0.0f) || !aligned_for(a->q_out, a->tokens) || !aligned_or_null(a->k_out) ||
-      !aligned_or_null(a->v_out) || (a->tokens > 0 && !a->k_out != !a->v_out) || a->reserved)
-    return GEVVA_MOE_BAD_ARGUMENT;
+  if (!a || !fill_append(&call, *a) || !pages_ok(&call.pages, a->cache, a->batch, a->kv_heads, a->dim) || a->reserved) return GEVVA_MOE_BAD_ARGUMENT;
   if (a->tokens == 0) return GEVVA_MOE_OK;
-  // A token's rows are written when that token's have been read, not when others' have: an output may stand where its own input does,
-  // row for row, and nowhere else among the inputs.
-  const gv::AttnRows* const inputs[3] = {&call.q, &call.k, &call.v};
-  void* const outputs[3] = {a->q_out, a->k_out, a->v_out};
-  for (int o = 0; o < 3; ++o) {
-    const auto heads = [&](int i) { return i == 0 ? a->heads : a->kv_heads; };
-    for (int i = 0; i < 3 && outputs[o]; ++i) {
-      if (o == i && outputs[o] == inputs[i]->data && packed(*inputs[i], heads(i), a->dim)) continue;
-      if (meets(outputs[o], static_cast<long long>(a->tokens) * heads(o) * a->dim, *inputs[i], a->tokens, heads(i), a->dim))
-        return GEVVA_MOE_BAD_ARGUMENT;
-    }
-  }
   call.token_offsets = a->batch->token_offsets;
   call.sequences = a->batch->sequences;
-  call.tokens = a->tokens;
-  call.heads = a->heads;
-  call.kv_heads = a->kv_heads;
-  call.dim = a->dim;
-  call.frequencies = a->frequencies;
-  call.rotated = a->rotated;
-  call.q_weight = a->q_weight;
-  call.k_weight = a->k_weight;
-  call.normalize_v = a->normalize_v != 0;
-  call.eps = a->eps;
-  call.q_out = a->q_out;
-  call.k_out = a->k_out;
-  call.v_out = a->v_out;
   const cudaError_t e = status_word(a->device_status, &call.status);
   if (e != cudaSuccess) return launched(e);
   return launched(gv::launch_kv_append(call, gv::current_sm_count(), stream));
+}
+
+int gevva_step_append(const gevva_step_append_args* a, gevva_stream_t stream) {
+  gv::PlacedCall call{};
+  if (!a || !fill_append(&call.rows, *a) || !cache_ok(&call.rows.pages, a->cache, a->kv_heads, a->dim) || a->axes < 1 || a->axes > 16 ||
+      (a->tokens > 0 && (!ints(a->slots) || !ints(a->positions))) || (a->axes > 1 && (a->position_stride < 0 || a->position_stride >= 1ll << 38)))
+    return GEVVA_MOE_BAD_ARGUMENT;
+  // (a slot is a whole number of 32 bits)
+  if (static_cast<long long>(a->cache->pages) * a->cache->page_size > 1ll << 31) return GEVVA_MOE_TOO_LARGE;
+  if (a->tokens == 0) return GEVVA_MOE_OK;
+  // A token's place is read when others' rows have been written.
+  const long long tokens = a->tokens, stride = a->axes > 1 ? a->position_stride : 0;
+  for (int o = 0; o < 3; ++o) {
+    void* const out = o == 0 ? a->q_out : o == 1 ? a->k_out : a->v_out;
+    const long long bytes = 2 * tokens * (o == 0 ? a->heads : a->kv_heads) * a->dim;
+    if (touch(out, bytes, a->slots, 4 * tokens) || touch(out, bytes, a->positions, 4 * ((a->axes - 1) * stride + tokens)) ||
+        (a->rotated > 0 && touch(out, bytes, a->frequencies, 4ll * a->axes * a->rotated)) || touch(out, bytes, a->q_weight, 2ll * a->dim) ||
+        touch(out, bytes, a->k_weight, 2ll * a->dim))
+      return GEVVA_MOE_BAD_ARGUMENT;
+  }
+  call.slots = a->slots;
+  call.positions = a->positions;
+  call.position_stride = stride;
+  call.axes = a->axes;
+  const cudaError_t e = status_word(a->device_status, &call.rows.status);
+  if (e != cudaSuccess) return launched(e);
+  return launched(gv::launch_kv_append_placed(call, gv::current_sm_count(), stream));
 }
 
 int gevva_attn_prompt(const gevva_attn_prompt_args* a, gevva_stream_t stream) {

@@ -4,6 +4,7 @@
 #include "gv_attention.h"
 #include "gv_common.cuh"
 #include "gv_gemm_parts.cuh"
+#include "gv_step.h"
 
 namespace gv {
 namespace {
@@ -138,6 +139,10 @@ struct AppendParams {
   float eps;
   __nv_bfloat16 *q_out, *k_out, *v_out;
   int* status;
+  // at given places
+  const int *slots, *positions;
+  long long position_stride;
+  int axes;
 };
 
 // A CTA takes a token, or one after the other where there are many, so that an angle is worked out once for all heads.  A thread holds
@@ -145,9 +150,11 @@ struct AppendParams {
 // behind them, so nothing is exchanged.  Its first vectors are asked for before the token's place is looked up, behind the last ones of
 // the token before.
 // 4608 tokens of 32 heads of 256, packed: 38.6 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
+// kPlaced: slots and positions are given, one read instead of the look-ups of sequence, length and page; a position for each axis, and
+// frequencies for each, most of them zero: a pair's angle is their sum of products, exactly its axis's product where the others are zero.
 constexpr int kAppendThreads = 512, kAppendManyThreads = 128;
 constexpr int kAppendManyCtas = 5;  // of an SM (with six: 80 registers, which do not hold it all)
-template <int kDim, int kThreads>
+template <int kDim, int kThreads, bool kPlaced>
 __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAppendManyCtas : 1) kv_append_kernel(const AppendParams p) {
   constexpr int kLanes = kDim / 16;  // threads of a head
   constexpr bool kMany = kThreads == kAppendManyThreads;
@@ -183,6 +190,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
 #pragma unroll 1
   for (int token = blockIdx.x; token < p.tokens; token += gridDim.x) {
   const int next_token = kMany ? token + static_cast<int>(gridDim.x) : p.tokens;
+  int position, page = -1, in_page;
+  if constexpr (kPlaced) {
+    const int at = p.slots[token];
+    if (__syncthreads_or(at < 0)) {  // a row that is no token: left as it was
+      if (next_token < p.tokens) ask(next_token, in_block);
+      continue;
+    }
+    page = at >> p.page_shift;
+    in_page = at & (p.pages.page_size - 1);
+    position = 0;
+  } else {
   // the sequence: offsets up to the token's
   int upto = 0;
   for (int base = 0; base <= p.sequences; base += blockDim.x) {
@@ -194,20 +212,29 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
     continue;
   }
   const int sequence = upto - 1;
-  const int position = p.pages.lengths[sequence] - p.token_offsets[upto] + token;
+  position = p.pages.lengths[sequence] - p.token_offsets[upto] + token;
   const int page_index = position >> p.page_shift;
-  int page = -1;
   if (position >= 0 && page_index < p.pages.table_width)
     page = p.pages.table[static_cast<size_t>(sequence) * p.pages.table_stride + page_index];
+  in_page = position & (p.pages.page_size - 1);
+  }
   const bool stored = page >= 0 && page < p.pages.page_count;
   if (!stored && threadIdx.x == 0 && p.status) atomicExch(p.status, static_cast<int>(kBadPage));
-  const long long slot = position & (p.pages.page_size - 1);
+  const long long slot = in_page;
 
   // position * frequency in 64 bits, whole turns taken off there: far positions keep the accuracy of near ones.  Groups of four of a
   // thread's eight stand in the two halves of the arrays, so that a warp's 16-byte reads follow one another.
   const int quarters = p.half / 8;
   for (int j = threadIdx.x; j < p.half; j += blockDim.x) {
-    const double angle = static_cast<double>(position) * p.frequencies[j] * 0.31830988618379067154;  // in half turns
+    double turned;
+    if constexpr (kPlaced) {
+      turned = static_cast<double>(p.positions[token]) * p.frequencies[j];
+      for (int axis = 1; axis < p.axes; ++axis)
+        turned += static_cast<double>(p.positions[axis * p.position_stride + token]) * p.frequencies[axis * p.half + j];
+    } else {
+      turned = static_cast<double>(position) * p.frequencies[j];
+    }
+    const double angle = turned * 0.31830988618379067154;  // in half turns
     float sine, cosine;
     sincospif(static_cast<float>(angle - 2.0 * rint(0.5 * angle)), &sine, &cosine);
     const int at = ((j >> 2) & 1) * 4 * quarters + (j >> 3) * 4 + (j & 3);
@@ -319,7 +346,9 @@ cudaError_t launch_block_norm(const BlockNormCall& call, int sm_count, cudaStrea
   return launch_chained(block_norm_kernel<true, 4, 1024>, grid, dim3((p.vectors + 127) / 128 * 32), 0, stream, p);
 }
 
-cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t stream) {
+namespace {
+
+AppendParams append_params(const AppendCall& call) {
   AppendParams p{};
   p.q = call.q;
   p.k = call.k;
@@ -341,6 +370,11 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
   p.v_out = static_cast<__nv_bfloat16*>(call.v_out);
   p.status = call.status;
   while ((1 << p.page_shift) < call.pages.page_size) ++p.page_shift;
+  return p;
+}
+
+template <bool kPlaced>
+cudaError_t launch_append(const AppendCall& call, const AppendParams& p, int sm_count, cudaStream_t stream) {
   // Threads for all heads of a token at once; with tokens for all SMs several times over four warps a token, so that more
   // tokens' chains of look-ups run side by side (64 tokens 4.3 and 5.6 us, 4608 tokens 47 and 41 us with up to eight warps and four).
   const int wanted = ((call.heads + 2 * call.kv_heads) * (call.dim / 16) + 31) / 32 * 32;
@@ -349,7 +383,7 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
   const int ctas = kAppendManyCtas * sm_count;
   const dim3 grid(many && call.tokens > ctas ? ctas : call.tokens), block(wanted < most ? wanted : most);
 #define GV_APPEND(dim) \
-  launch_chained(many ? kv_append_kernel<dim, kAppendManyThreads> : kv_append_kernel<dim, kAppendThreads>, grid, block, 0, stream, p)
+  launch_chained(many ? kv_append_kernel<dim, kAppendManyThreads, kPlaced> : kv_append_kernel<dim, kAppendThreads, kPlaced>, grid, block, 0, stream, p)
   switch (call.dim) {
     case 64: return GV_APPEND(64);
     case 128: return GV_APPEND(128);
@@ -357,6 +391,21 @@ cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t 
     default: return GV_APPEND(512);
   }
 #undef GV_APPEND
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const AppendCall& call, int sm_count, cudaStream_t stream) {
+  return launch_append<false>(call, append_params(call), sm_count, stream);
+}
+
+cudaError_t launch_kv_append_placed(const PlacedCall& call, int sm_count, cudaStream_t stream) {
+  AppendParams p = append_params(call.rows);
+  p.slots = call.slots;
+  p.positions = call.positions;
+  p.position_stride = call.position_stride;
+  p.axes = call.axes;
+  return launch_append<true>(call.rows, p, sm_count, stream);
 }
 
 }  // namespace gv

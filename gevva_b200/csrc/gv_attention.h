@@ -79,4 +79,9 @@ struct BlockNormCall {
 };
 cudaError_t launch_block_norm(const BlockNormCall& call, int sm_count, cudaStream_t stream);
 
+// What an entry point returns for a launch's result.
+int launched(cudaError_t e);
+// A call's status word, or else the current device's.
+cudaError_t status_word(int* own, int** out);
+
 }  // namespace gv

@@ -28,6 +28,7 @@ enum Status : int {
   kNoDevice = 5,
   kTooLarge = 6,
   kBadPage = 7,         // a new token's position has no page of the cache
+  kNoPages = 8,         // a page pool has too few pages left, or would get back more than it handed out
 };
 
 // Tile geometry of the grouped GEMM (tokens on MMA-M, weight rows on MMA-N).
@@ -184,6 +185,34 @@ inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 blo
   attribute[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+}
+
+// The same in clusters of `ctas` CTAs that follow one another in the grid; more than eight are allowed to the kernel first.
+template <class... Params, class... Args>
+inline cudaError_t launch_chained_clusters(void (*kernel)(Params...), unsigned ctas, dim3 grid, dim3 block, size_t smem_bytes,
+                                           cudaStream_t stream, Args&&... args) {
+  if (smem_bytes > 4096) {  // (with what the kernel declares by itself it may be more than the 48 KB that need no leave)
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes));
+    if (e != cudaSuccess) return e;
+  }
+  if (ctas > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = block;
+  config.dynamicSmemBytes = smem_bytes;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = ctas;
+  attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+  config.attrs = attributes;
+  config.numAttrs = 2;
   return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
 }
 

@@ -459,6 +459,7 @@ const char* gevva_moe_strerror(int status) {
     case GEVVA_MOE_BAD_EXPERT_ID: return "expert id outside [0,128)";
     case GEVVA_MOE_WAIT_TIMEOUT: return "bounded device wait expired";
     case GEVVA_MOE_BAD_PAGE: return "position without a page of the cache";
+    case GEVVA_MOE_NO_PAGES: return "too few pages in the pool, or more given back than handed out";
     case GEVVA_MOE_BAD_ARGUMENT: return "bad argument";
     case GEVVA_MOE_CUDA_ERROR: return g_error_text[0] ? g_error_text : "CUDA error";
     case GEVVA_MOE_NO_DEVICE: return "no sm_100 device or driver entry point";

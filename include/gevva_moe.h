@@ -38,7 +38,8 @@ enum gevva_moe_status {
   GEVVA_MOE_CUDA_ERROR = -4,
   GEVVA_MOE_NO_DEVICE = -5,     /* no sm_100 device / driver entry point missing */
   GEVVA_MOE_TOO_LARGE = -6,
-  GEVVA_MOE_BAD_PAGE = -7 /* device: a position has no page of the cache (gevva_attn_append, gevva_attn_chunk) */
+  GEVVA_MOE_BAD_PAGE = -7, /* device: a position has no page of the cache (gevva_attn_append, gevva_attn_chunk, gevva_step_*) */
+  GEVVA_MOE_NO_PAGES = -8 /* device: a pool has too few pages left, or would get back more than it handed out (gevva_step_plan, _trim) */
 };
 
 /* The eight sidecar tensors of one layer that the reference's constructor resolves
@@ -479,6 +480,114 @@ typedef struct {
   float scale;
 } gevva_attn_chunk_args;
 int gevva_attn_chunk(const gevva_attn_chunk_args* args, gevva_stream_t stream);
+
+/* ---- what a serving step has around its layers -------------------------------------------------
+ * The pages and places of its tokens, the append at those places, and the tokens that its logits give.  Nothing is kept between
+ * calls and nothing is read back: a captured step replays with the lengths, tables and settings that its tensors hold then.
+ * Statuses as above: `device_status`, or the device's word. */
+
+/* The rows, pages and places of a step's new tokens.  Request s has lengths[s] tokens in the cache and news[s] new ones; it holds the pages
+ * table[s * table_stride + 0 .. ceil(lengths[s] / page_size) - 1].  A pool is a list of pages, of which the first *taken are handed out.
+ *   token_offsets [sequences + 1]  first row of each request, and behind the last one's
+ *   lengths_out [sequences]        lengths + news: what gevva_attn_batch takes
+ *   table                          gets the pages that the new tokens need, pool[*taken ..], request after request
+ *   slots [tokens]                 page * page_size + slot in the page of every row's token; -1 for rows behind the last request's
+ *   positions [tokens]             position of every row's token, with shift[s] added where shift is given; 0 behind the last
+ *   taken_out [1]                  pages handed out after the call
+ * lengths_out may be lengths and taken_out taken, so that a captured step goes on by itself.  All or nothing: lengths below zero or
+ * beyond the table (GEVVA_MOE_BAD_PAGE), too few pages (GEVVA_MOE_NO_PAGES) or more new tokens than `tokens` rows
+ * (GEVVA_MOE_TOO_LARGE) leave lengths, table and pool as they are, and no row is a token.  A page of the table or the pool whose
+ * slots are no whole numbers of 32 bits gives slot -1 and GEVVA_MOE_BAD_PAGE.  At most 16384 requests; page_size a power of
+ * two, at least 16; table_width * page_size at most 2^30. */
+typedef struct {
+  const int* lengths;
+  const int* news;
+  const int* shift; /* NULL: zeros */
+  int* table;
+  const int* pool;  /* [pool_pages] */
+  const int* taken; /* [1] */
+  int* token_offsets;
+  int* lengths_out;
+  int* slots;
+  int* positions;
+  int* taken_out;
+  int* device_status;
+  int sequences, table_width, table_stride, pool_pages, page_size, tokens;
+} gevva_step_plan_args;
+int gevva_step_plan(const gevva_step_plan_args* args, gevva_stream_t stream);
+
+/* Requests that get shorter (rejected drafts) or end (keep 0): lengths_out[s] = min(lengths[s], max(keep[s], 0)), and the pages that are
+ * then not needed go back to the pool, in the places where gevva_step_plan would hand them out again in the same order.  The table
+ * is left as it is.  All or nothing as above; GEVVA_MOE_NO_PAGES: more pages than were handed out. */
+typedef struct {
+  const int* lengths;
+  const int* keep;
+  const int* table;
+  int* pool;
+  const int* taken;
+  int* lengths_out; /* may be lengths */
+  int* taken_out;   /* may be taken */
+  int* device_status;
+  int sequences, table_width, table_stride, pool_pages, page_size;
+  int reserved; /* 0 */
+} gevva_step_trim_args;
+int gevva_step_trim(const gevva_step_trim_args* args, gevva_stream_t stream);
+
+/* gevva_attn_append at given places and with positions of several axes (time, height, width).  Row t goes to slot slots[t] % page_size of
+ * page slots[t] / page_size; one below zero is no token, and its rows of the outputs are left as they were; one outside the cache is not stored
+ * and reported as GEVVA_MOE_BAD_PAGE.  Pair (j, rotated / 2 + j) turns by the sum over the axes a of
+ * positions[a * position_stride + t] * frequencies[a * rotated / 2 + j]: with a frequency for one axis and zeros for the others, by its
+ * axis's position.  1 to 16 axes; position_stride may be zero.  No two tokens of a call may name one slot.  Outputs share no memory with what the
+ * call reads but as in gevva_attn_append.  GEVVA_MOE_TOO_LARGE: a cache of more than 2^31 slots. */
+typedef struct {
+  const void* q;
+  long long q_token_stride, q_head_stride;
+  const void* k;
+  long long k_token_stride, k_head_stride;
+  const void* v;
+  long long v_token_stride, v_head_stride;
+  const gevva_attn_cache* cache;
+  const int* slots;          /* [tokens] */
+  const int* positions;      /* [axes, tokens] */
+  long long position_stride; /* of an axis */
+  const double* frequencies; /* [axes, rotated / 2] */
+  const void* q_weight;
+  const void* k_weight;
+  void* q_out;
+  void* k_out;
+  void* v_out;
+  int* device_status;
+  int tokens, heads, kv_heads, dim, rotated, axes, normalize_v;
+  float eps;
+} gevva_step_append_args;
+int gevva_step_append(const gevva_step_append_args* args, gevva_stream_t stream);
+
+/* Tokens from logits, one a row, by a random number of the caller's.  A token's share is exp((y - y_max) / temperature) with y the logit, or
+ * softcap * tanh(logit / softcap) where softcap is not zero.  Tokens are ranked by logit, the lower index first among equals.  Kept are
+ *   top_k   the first top_k by rank (0 or less: all)
+ *   top_p   of those, each one in front of which less than top_p of their shares' sum has been (1 or more: all; always the first)
+ *   min_p   of those, the ones with a share of at least min_p, that is min_p times the largest share (0 or less: all; more than 1 is 1)
+ * and the row's token is the first of the vocabulary up to which the sum of kept shares exceeds uniforms[row] (0 <= u < 1) times the sum of
+ * all kept ones.  A temperature that is not above zero takes the first by rank.  Minus infinity and NaN are never taken, a row of
+ * nothing else gives token -1 and probability 0; of infinite logits each has the same share and the others none.  Shares and
+ * sums are in 64 bits.  probabilities: the token's share of the kept ones' sum.  Settings are NULL or [rows]; row_stride may be
+ * zero (many tokens from one row).  logits are aligned to their type; up to 15 bytes in front of and behind a row are read, within the
+ * 16-byte lines that its ends lie in.  vocabulary up to 524288; at most 2^27 - 1 rows. */
+typedef struct {
+  const void* logits;
+  long long row_stride;
+  const float* uniforms;
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  int* tokens;
+  float* probabilities; /* NULL: not wanted */
+  int rows, vocabulary;
+  int f32; /* 1: f32 logits, 0: bf16 */
+  float softcap;
+} gevva_step_sample_args;
+int gevva_step_sample(const gevva_step_sample_args* args, gevva_stream_t stream);
 
 /* Per-tensor FP8 quantiser (tools/pack_fp8_dense.py:64-70): scale = amax/448, q = e4m3(w/scale). */
 int gevva_pack_fp8(const float* weights, size_t count, void* out, float* scale, gevva_stream_t stream);
