@@ -40,6 +40,16 @@ GV_SHARES_HD double exp2_rest(double f) {
   p = p * f + 0x1.62e42fef6d01bp-6;
   return p * f + 1.0;
 }
+// The same with a term more (the sixth's taken over in the same way, x^6 / 720 ~ (3/2 a^2 x^4 - 9/16 a^4 x^2 + a^6 / 32) / 720, its last part
+// left out): off by a^6 / 11520 = 2^-52.7.
+GV_SHARES_HD double exp2_rest_finely(double f) {
+  double p = 0x1.5d87fe78a6731p-35;
+  p = p * f + 0x1.3b2b301f0c04ap-27;
+  p = p * f + 0x1.c6b08d704a0c0p-20;
+  p = p * f + 0x1.ebfbdff7feebap-13;
+  p = p * f + 0x1.62e42fefa39efp-6;
+  return p * f + 1.0;
+}
 // value * 2^floor(n / 32), for n by its low bits (any multiple of 2^17 more is the same), where that is a normal number.
 GV_SHARES_HD double scaled_by(double value, uint32_t n) {
   const uint32_t exponent = n << 15 & 0xfff00000u;
@@ -71,6 +81,7 @@ GV_SHARES_HD uint32_t share_whole(float distance, float scale) {
 }
 // 2^(distance * scale / 32) with its whole part as given; `table` has entry j at [j * stride].  The whole part may be off by a little (it comes from
 // 32 bits): the rest is what it leaves.
+template <bool kFinely = false>
 GV_SHARES_HD double share_with(double distance, double scale, uint32_t n, const double* table, int stride) {
   // 2^52 and the bits, as a number of 64 bits, without a conversion
 #ifdef __CUDA_ARCH__
@@ -80,7 +91,7 @@ GV_SHARES_HD double share_with(double distance, double scale, uint32_t n, const 
   const double whole = static_cast<double>(n) - static_cast<double>(kShareWhole);
   const double rest = __builtin_fma(distance, scale, -whole);
 #endif
-  return scaled_by(exp2_rest(rest) * table[(n & (kExp2Entries - 1)) * stride], n);
+  return scaled_by((kFinely ? exp2_rest_finely(rest) : exp2_rest(rest)) * table[(n & (kExp2Entries - 1)) * stride], n);
 }
 
 // The same for any finite scale, zero below 2^-1020.

@@ -4,18 +4,18 @@
 // top_k, those whose better ranks have less than top_p of what top_k leaves, and those with w >= min_p.  The token is the first of the
 // vocabulary at which the sum of kept shares passes u times the sum of all kept ones.
 //
-// Floor: a row is read once.  A cluster of up to 16 CTAs holds a row in shared memory (two CTAs an SM: one row's reads run under another's work), and
-// every further pass goes over shared memory:
+// A row is gone through a few times, by a CTA or a cluster of up to 16, from HBM first and from L2 afterwards:
 //   1. the largest value, and for groups of threads of every size the smallest of their largest values: with at least k groups, at least k
-//      values are not below that, and with about k groups only some k ln k are.
-//   2. where a border by top_p, or by a large top_k, has to be found: all shares' sum, and how many values lie in each 32nd of an octave of
-//      share.  From these counts the border is known to a few of them.
-//   3. what may be kept goes to the first CTA's list, which sorts it, cuts it and walks over it; where more may be kept than a list holds, what lies
-//      about the border goes there, with the sum of the shares above it.
-//   4. then the kept shares are summed by CTAs, warps and steps in the order of the vocabulary, and the step that holds the token is walked over.
-// The counts only say where to look: the border itself is taken from sums of shares in 64 bits, and where it does not lie in the list (values too
-// many, too equal or too far apart for the counts) it is looked for by halving the range, a pass over shared memory a step.
+//      values are not below that, and with about k groups only some k ln k are.  Those go to a list.
+//   2. where top_p has to cut a whole row, or a large top_k: how many values lie in each of 1024 bins, and the shares' sum in 32 bits.  From these
+//      the border is known to a few bins.
+//   3. all shares in 64 bits, their sum and that of those above the border's bins; what lies in the bins goes to the list.  Sorted, it tells the border
+//      exactly; a border that is not there (the counts told wrong, or too many values in the bins) is looked for closer, at last by halving.
+//   4. the kept shares are summed by CTAs, warps and pieces of a warp in the order of the vocabulary, down to the piece that holds the token.
+// A list that has all that may be kept (most rows that are not flat) is cut by rank and walked over by index in the first CTA instead.
 // All sums are taken in an order that sizes alone give: the same inputs give the same token.
+//
+// The parts are functions of their own that find what they share in shared memory: inlined where they are called they were 360 KB of code.
 #include "gv_common.cuh"
 #include "gv_shares.h"
 #include "gv_step.h"
@@ -24,41 +24,87 @@ namespace gv {
 namespace {
 
 constexpr int kMostCtas = 16;
-constexpr int kLevels = 10;     // groups of 2^level threads
+constexpr int kLevels = 10;       // groups of 2^level threads
 constexpr int kSums = 3;
-constexpr int kBins = 1024;     // of a 32nd of an octave of share; the last one has all that is smaller
+constexpr int kBins = 1024;       // of equal width over a range of values
 constexpr int kTableCopies = 16;  // of the table of 2^(j/32), one for each lane of half a warp: no two lanes of a read meet in a bank
 
 struct SampleParams {
   SampleCall call;
   int ctas;         // of a row's cluster
-  int cta_vectors;  // 16-byte vectors of a row that a CTA holds
+  int cta_vectors;  // 16-byte vectors of a row that a CTA goes through
 };
 
-// Where the counts say that a border lies: bins first .. last hold it, and what is in front of them measures `above`.
+// What the counts say of a border: it lies in bins first .. last.
+enum BinsSay : int { kNotHere, kLookCloser, kInList, kListHasAll };  // (all: the list has everything from the largest value on, first is 0)
 struct BinWindow {
   int first, last;
-  int count;     // in the window
-  int whole;     // 1: the window has all from the largest value on (first is 0)
+  BinsSay says;
+  int sure_first, sure_last;  // what holds it in any case
+};
+// Bins of equal width from `high` (bin 0's middle) down to `low`; a bin's values are the nearest to its middle.
+struct Bins {
+  float low, high, per;  // bins for one
+};
+
+// How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values, or of any.
+enum ShareForm : int { kPlain, kCapped, kAny };
+// cap * tanh(x / cap), with e = exp(-2 |x| / cap): cap * (1 - e) / (1 + e).
+struct Cap {
+  double cap, scale;      // scale: of |x| in 32nds of an octave of e
+  float scale32, most32;  // beyond `most32` e is not noticed
+};
+
+// What all threads of a CTA know of its row.
+struct RowState {
+  const uint4* source;  // the row from the 16-byte boundary at or in front of its first value
+  int lead;             // values in front of it there
+  int vocabulary;
+  int vectors;          // that have values of the row
+  int cta_begin, cta_end, warp_vectors;  // the CTA's part of them, and how many a warp has of it
+  int ctas, rank;
+  ShareForm form;
+  int bounded;          // whether top_k or top_p have a border: order above border_key, or equal to it and index up to border_index
+  uint32_t border_key, border_index;
+  float border;         // border_key's
+  float scale32, top32, cut;  // kPlain: values below `cut` have no share
+  double scale, top;    // of y
+  Cap cap;
 };
 
 template <int kThreads>
 struct SampleShared {
-  static constexpr int kCap = 4 * kThreads;
+  static constexpr int kEach = kThreads >= 512 ? 2 : 4;  // a thread's entries of the list
+  static constexpr int kCap = kEach * kThreads;
   static constexpr int kWarps = kThreads / 32;
+  static constexpr int kFew = 128;
+  RowState row;
+  double few[kFew];
   double table[kExp2Entries * kTableCopies];
-  unsigned long long mine[kCap];   // candidates of this CTA
-  unsigned long long list[kCap];   // the cluster's, in its first CTA
-  uint4 first[kMostCtas][4];       // largest key, its index, levels, settings
+  union {
+    unsigned long long mine[kCap];   // candidates of this CTA
+    int4 bins4[kBins / 4];
+    int bins[kBins + 32];            // (behind them one for each lane that has nothing to count: no branch, no conflict)
+  };
+  union {
+    unsigned long long list[kCap];   // the cluster's, in its first CTA
+    int4 totals4[kBins / 4];         // the cluster's bins there
+    int totals[kBins];               // (elsewhere what the CTA adds up of them)
+  };
+  uint4 first[kMostCtas][4];       // largest key, levels, settings
   double slots[2][kMostCtas][kSums];
   double warp_sums[kWarps][kSums];
-  uint4 window;                    // a BinWindow, from the first CTA
+  uint4 window[2];                 // a BinWindow, from the first CTA, by turns
   unsigned long long border;       // from the first CTA
-  int bins[kBins];
   uint32_t warp_key[kWarps], warp_index[kWarps], warp_levels[kWarps][5];
   int mine_count, list_count, base, found;
   int edges[4];
 };
+extern __shared__ uint4 sample_memory[];
+template <int kThreads>
+__device__ __forceinline__ SampleShared<kThreads>& shared() {
+  return *reinterpret_cast<SampleShared<kThreads>*>(sample_memory);
+}
 
 __device__ __forceinline__ void cluster_store_double(uint32_t address, double v) {
   asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(address), "l"(__double_as_longlong(v)) : "memory");
@@ -66,9 +112,9 @@ __device__ __forceinline__ void cluster_store_double(uint32_t address, double v)
 __device__ __forceinline__ void cluster_store_u64(uint32_t address, unsigned long long v) {
   asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(address), "l"(v) : "memory");
 }
-__device__ __forceinline__ int cluster_load(uint32_t address) {
-  int v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+__device__ __forceinline__ int4 cluster_load4(uint32_t address) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
   return v;
 }
 __device__ __forceinline__ int cluster_add(uint32_t address, int v) {
@@ -97,32 +143,7 @@ __device__ __forceinline__ uint32_t order_above(uint32_t order) { return order =
 
 static __constant__ double g_exp2_table[kExp2Entries] = GV_EXP2_TABLE_INIT;
 
-template <typename T>
-struct Vector;
-template <>
-struct Vector<float> {
-  static constexpr int kValues = 4;
-  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
-    x[0] = __uint_as_float(v.x);
-    x[1] = __uint_as_float(v.y);
-    x[2] = __uint_as_float(v.z);
-    x[3] = __uint_as_float(v.w);
-  }
-};
-template <>
-struct Vector<__nv_bfloat16> {
-  static constexpr int kValues = 8;
-  static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-};
-
-  // One step of a bitonic sort between lanes, or between a lane's two values.
+// One step of a bitonic sort between lanes, or between a lane's two values.
   __device__ __forceinline__ void order_lanes(unsigned long long& x, int stride, bool up) {
     const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, stride);
     const bool lower = (threadIdx.x & stride) == 0;
@@ -135,7 +156,7 @@ __device__ __noinline__ void sort_list(unsigned long long* list, int count) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int whole = 64;
-    while (whole < count) whole *= 2;
+    while (whole < count && whole < SampleShared<kThreads>::kCap) whole *= 2;
     for (int i = count + threadIdx.x; i < whole; i += kThreads) list[i] = ~0ull;
     __syncthreads();
     for (int size = 64; size <= whole; size *= 2) {
@@ -181,567 +202,1071 @@ __device__ __noinline__ void sort_list(unsigned long long* list, int count) {
     }
   }
 
-// How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values, or of any.
-enum ShareForm : int { kPlain, kCapped, kAny };
-
-__device__ __noinline__ double softened(float x, double cap) {
-  // tanh(z) = 1 - 2 / (1 + exp(2 z)), of |z|
-  const double z = fabs(static_cast<double>(x)) / cap;
-  const double y = cap * (1.0 - 2.0 / (1.0 + exp(2.0 * z)));
-  return x < 0.0f ? -y : y;
-}
-
-// The share of any value that may be taken, and its bin.
-struct BinnedShare {
-  double share;
-  int bin;
+__device__ __forceinline__ float ranked_value(unsigned long long entry) { return value_of(~static_cast<uint32_t>(entry >> 32)); }
+// What top_k and top_p leave: values above `value`, and those equal to it up to `index`.
+struct Border {
+  float value;
+  uint32_t index;
+  __device__ __forceinline__ bool inside(float x, uint32_t i) const { return (x > value) | ((x == value) & (i <= index)); }
 };
-__device__ __noinline__ BinnedShare other_share(float x, ShareForm form, double scale, double top, double cap, const double* table) {
-  double distance = form == kCapped ? softened(x, cap) - top : static_cast<double>(x) - top;
-  if (form == kAny) {
-    if (isinf(x)) distance = 0.0;  // (the largest value is infinite then, and so is this one)
-    else if (isinf(top)) return {0.0, kBins - 1};
-  }
-  const double at = -distance * scale;
-  return {share_of(distance, scale, table, kTableCopies), at < kBins - 1 ? static_cast<int>(at + 0.5) : kBins - 1};
+__device__ __forceinline__ Border border_of(const RowState& row) { return {row.border, row.border_index}; }
+
+// ---- shares
+
+__device__ __forceinline__ double softened(float x, const Cap& c, const double* table) {
+  const float size = fminf(fabsf(x), c.most32);
+  const double e = share_with<true>(-static_cast<double>(size), c.scale, share_whole(-size, c.scale32), table, kTableCopies);
+  // 1 / (1 + e) by two steps of Newton's from 32 bits
+  const double d = 1.0 + e;
+  float guess;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(guess) : "f"(static_cast<float>(d)));
+  double r = static_cast<double>(guess);
+  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
+  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
+  return copysign(c.cap * ((1.0 - e) * r), static_cast<double>(x));
+}
+// By its distance from the largest in y, in two precisions: none beyond kShareOctaves.
+__device__ __forceinline__ double capped_share(float x, double scale, float scale32, double top, const Cap& cap, const double* table) {
+  const double distance = softened(x, cap, table) - top;
+  const float distance32 = static_cast<float>(distance);
+  const double share = share_with(distance, scale, share_whole(distance32, scale32), table, kTableCopies);
+  return distance32 * scale32 > -kShareOctaves * kExp2Entries ? share : 0.0;
+}
+__device__ __forceinline__ double plain_share(float x, double scale, float scale32, double top, float top32, const double* table) {
+  return share_with(static_cast<double>(x) - top, scale, share_whole(x - top32, scale32), table, kTableCopies);
+}
+template <int kThreads>
+__device__ __forceinline__ const double* lane_table() {
+  return shared<kThreads>().table + (threadIdx.x & (kTableCopies - 1));
 }
 
+// The share of any value that may be taken.
+template <int kThreads>
+__device__ __noinline__ double share(float x) {
+  const RowState& row = shared<kThreads>().row;
+  const double* table = lane_table<kThreads>();
+  if (row.form == kPlain) return x >= row.cut ? plain_share(x, row.scale, row.scale32, row.top, row.top32, table) : 0.0;
+  if (row.form == kCapped) return capped_share(x, row.scale, row.scale32, row.top, row.cap, table);
+  if (isinf(x)) return 1.0;  // (the largest value is infinite then, and so is this one)
+  return isinf(row.top) ? 0.0 : share_of(static_cast<double>(x) - row.top, row.scale, table, kTableCopies);
+}
+
+struct Eight {
+  double w[8];
+};
+// Of eight values, side by side (a share is a chain of a dozen operations that wait for one another), where the form is not the plain one.
+template <int kThreads>
+__device__ __noinline__ Eight other_shares(float a, float b, float c, float d, float e, float f, float g, float h) {
+  const RowState& row = shared<kThreads>().row;
+  const float x[8] = {a, b, c, d, e, f, g, h};
+  Eight out;
+  if (row.form == kCapped) {
+    const Cap cap = row.cap;
+    const double scale = row.scale, top = row.top;
+    const float scale32 = row.scale32;
+    const double* table = lane_table<kThreads>();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.w[i] = capped_share(x[i], scale, scale32, top, cap, table);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.w[i] = x[i] > -INFINITY ? share<kThreads>(x[i]) : 0.0;
+  }
+  return out;
+}
+
+// ---- going through a row
+
+template <typename T>
+struct Vector;
+template <>
+struct Vector<float> {
+  static constexpr int kValues = 4;
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
+  }
+};
+template <>
+struct Vector<__nv_bfloat16> {
+  static constexpr int kValues = 8;
+  static __device__ __forceinline__ void unpack(const uint4& v, float* x) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+
+// A thread's way through its warp's part of a row, vectors that follow one another in steps of 32, eight values at a time.
 template <typename T, int kThreads>
-struct Row {
+struct Walk {
   static constexpr int kE = Vector<T>::kValues;
-  using Shared = SampleShared<kThreads>;
-  static constexpr int kWarps = Shared::kWarps, kCap = Shared::kCap;
+  static constexpr int kGroup = 8 / kE;
+  const uint4* source;
+  int begin, end;  // vectors
+  int last;        // the row's last one
+  int lead;
+  unsigned limit;  // indexes that are the row's, and of vectors up to the end
 
-  Shared& sh;
-  const uint4* slice;  // this CTA's part of the row
-  int vectors;         // of it
-  int begin_index;     // vocabulary index of its first value
-  int ctas, rank;
-  int lane, warp;
-  int parity = 0;
-
-  // shares
-  ShareForm form;
-  double scale, top, cap;  // of y
-  float scale32, top32, cut;  // smaller values have no share (kPlain)
-  // what top_k and top_p keep: order above border_key, or equal to it and index up to border_index
-  bool bounded = false;
-  uint32_t border_key = kNothing + 1, border_index = 0xffffffffu;
-
-  __device__ __forceinline__ const double* table() const { return sh.table + (lane & (kTableCopies - 1)); }
-  __device__ __forceinline__ uint32_t plain_whole(float x) const { return share_whole(x - top32, scale32); }
-  __device__ __forceinline__ double plain_share(float x, uint32_t whole) const {
-    return share_with(static_cast<double>(x) - top, scale, whole, table(), kTableCopies);
+  __device__ __forceinline__ Walk(int begin, int end) : begin(begin), end(end) {
+    const RowState& row = shared<kThreads>().row;
+    source = row.source;
+    last = row.vectors - 1;
+    lead = row.lead;
+    limit = static_cast<unsigned>(max(0, min(row.vocabulary, end * kE - lead)));
   }
-  __device__ __forceinline__ BinnedShare other(float x) const { return other_share(x, form, scale, top, cap, table()); }
-  __device__ __forceinline__ double share(float x) const {
-    if (form == kPlain) return x >= cut ? plain_share(x, plain_whole(x)) : 0.0;
-    return other(x).share;
+  // This warp's part.
+  static __device__ __forceinline__ Walk mine() {
+    const RowState& row = shared<kThreads>().row;
+    const int begin = min(row.cta_end, row.cta_begin + static_cast<int>(threadIdx.x >> 5) * row.warp_vectors);
+    return Walk(begin, min(row.cta_end, begin + row.warp_vectors));
   }
-  static __device__ __forceinline__ int plain_bin(uint32_t whole) { return min(max(static_cast<int>(kShareWhole - whole), 0), kBins - 1); }
-  __device__ __forceinline__ int bin_of(float x) const {
-    if (form == kPlain) return x >= cut ? plain_bin(plain_whole(x)) : kBins - 1;
-    return other(x).bin;
+  __device__ __forceinline__ int index_of(int v) const { return v * kE - lead; }
+  // Values that are not of these vectors, or none of the row's, are minus infinity.
+  __device__ __forceinline__ void mask(int v, float* x) const {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) x[i] = static_cast<unsigned>(index_of(v) + i) < limit ? x[i] : -INFINITY;
   }
-  __device__ __forceinline__ bool inside(float x, uint32_t index) const {
-    const float border = value_of(border_key);
-    return x > border || (x == border && index <= border_index);
-  }
-
-  // A warp has vectors that follow one another, in steps of 32.
-  __device__ __forceinline__ int warp_vectors() const { return (vectors + kWarps * 32 - 1) / (kWarps * 32) * 32; }
-
+  // f(value, index) of vector v's.
   template <class F>
   __device__ __forceinline__ void one_vector(int v, F&& f) const {
     float x[kE];
-    Vector<T>::unpack(slice[v], x);
+    Vector<T>::unpack(source[v], x);
+    mask(v, x);
 #pragma unroll
-    for (int i = 0; i < kE; ++i) f(x[i], begin_index + v * kE + i);
+    for (int i = 0; i < kE; ++i) f(x[i], index_of(v) + i);
   }
+  // f(values, the first vector's number): value i is of vector + 32 * (i / kE).  The next values are on their way meanwhile.
   template <class F>
-  __device__ __forceinline__ void each_value(F&& f) const {
-    const int each = warp_vectors(), end = min(vectors, (warp + 1) * each);
+  __device__ __forceinline__ void each_eight(F&& f) const {
+    const int lane = threadIdx.x & 31;
+    uint4 next[2][kGroup];
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) next[d][g] = source[min(begin + lane + 32 * (kGroup * d + g), last)];
 #pragma unroll 1
-    for (int v = warp * each + lane; v < end; v += 32) one_vector(v, f);
-  }
-
-  __device__ __forceinline__ void cluster_barrier() {
-    __syncwarp();
-    if (ctas > 1) cluster_sync_all();
-    else __syncthreads();
-  }
-
-  // Sums over the cluster, in every thread the same; sh.slots[which][rank] has the CTAs' own, sh.warp_sums the warps' of this one.
-  template <int kCount>
-  __device__ __forceinline__ int cluster_sums(double (&v)[kCount]) {
+    for (int at = begin; at < end; at += 32 * kGroup) {
+      const int v = at + lane;
+      float x[8];
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) v[i] = warp_sum(v[i]);
-    if (lane == 0) {
-#pragma unroll
-      for (int i = 0; i < kCount; ++i) sh.warp_sums[warp][i] = v[i];
-    }
-    __syncthreads();
-    const int which = parity;
-    parity ^= 1;
-    if (warp == 0 && lane < ctas) {
-      const uint32_t peer = cluster_map_shared(smem_u32(&sh.slots[which][rank][0]), lane);
-#pragma unroll
-      for (int i = 0; i < kCount; ++i) {
-        double sum = 0.0;
-        for (int w = 0; w < kWarps; ++w) sum += sh.warp_sums[w][i];
-        cluster_store_double(peer + 8 * i, sum);
+      for (int g = 0; g < kGroup; ++g) {
+        Vector<T>::unpack(next[0][g], x + g * kE);
+        next[0][g] = next[1][g];
+        next[1][g] = source[min(v + 32 * (2 * kGroup + g), last)];
       }
-    }
-    cluster_barrier();
+      if (at == 0 || at + 32 * kGroup >= end) {  // (the ends; the same for the whole warp)
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      v[i] = 0.0;
-      for (int r = 0; r < ctas; ++r) v[i] += sh.slots[which][r][i];
+        for (int g = 0; g < kGroup; ++g) mask(v + 32 * g, x + g * kE);
+      }
+      f(x, v);
     }
-    return which;
   }
+  __device__ __forceinline__ int index_in(int v, int i) const { return index_of(v + 32 * (i / kE)) + i % kE; }
+};
 
-  // What lies from `low` to `high` in order and is inside goes to the first CTA's list; returns how many there are in all (more
-  // than kCap: the list is not whole).  above(x, index) is called for what is inside and higher.
-  template <class Above>
-  __device__ __forceinline__ int gather(uint32_t low, uint32_t high, Above&& above) {
-    const float from = value_of(low), upto = value_of(high);
-    if (threadIdx.x == 0) sh.mine_count = 0;
-    __syncthreads();
-    const bool all = !bounded;
-    each_value([&](float x, int index) {
-      if (x >= from && (all || inside(x, index))) {
-        if (x <= upto) {
-          const int at = atomicAdd(&sh.mine_count, 1);
-          if (at < kCap) sh.mine[at] = static_cast<unsigned long long>(~order_of(x)) << 32 | static_cast<uint32_t>(index);
-        } else {
-          above(x);
+template <int kThreads>
+__device__ __forceinline__ void cluster_barrier() {
+  __syncwarp();
+  if (shared<kThreads>().row.ctas > 1) cluster_sync_all();
+  else __syncthreads();
+}
+
+struct Three {
+  double a, b, c;
+};
+// Sums over the cluster, in every thread the same; slots[which][rank] has the CTAs' own, warp_sums the warps' of this one.
+template <int kThreads>
+__device__ __noinline__ Three cluster_sums(double a, double b, double c, int which) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas;
+  a = warp_sum(a);
+  b = warp_sum(b);
+  c = warp_sum(c);
+  if (lane == 0) {
+    sh.warp_sums[warp][0] = a;
+    sh.warp_sums[warp][1] = b;
+    sh.warp_sums[warp][2] = c;
+  }
+  __syncthreads();
+  if (warp == 0 && lane < ctas) {
+    const uint32_t peer = cluster_map_shared(smem_u32(&sh.slots[which][sh.row.rank][0]), lane);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      double sum = 0.0;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += sh.warp_sums[w][i];
+      cluster_store_double(peer + 8 * i, sum);
+    }
+  }
+  cluster_barrier<kThreads>();
+  const double* slot = sh.slots[which][lane & (kMostCtas - 1)];
+  const bool mine = lane < ctas;
+  return {warp_sum(mine ? slot[0] : 0.0), warp_sum(mine ? slot[1] : 0.0), warp_sum(mine ? slot[2] : 0.0)};
+}
+
+// ---- passes
+
+template <typename T, int kThreads>
+__device__ __noinline__ float largest_value() {
+  // (from HBM: eight vectors of a thread on their way)
+  using W = Walk<T, kThreads>;
+  const auto walk = W::mine();
+  constexpr int kAhead = 8;
+  float most[kAhead];
+#pragma unroll
+  for (int g = 0; g < kAhead; ++g) most[g] = -INFINITY;
+#pragma unroll 1
+  for (int at = walk.begin; at < walk.end; at += 32 * kAhead) {
+    uint4 vectors[kAhead];
+    const int v = at + (threadIdx.x & 31);
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) vectors[g] = walk.source[min(v + 32 * g, walk.last)];
+    const bool ends = at == 0 || at + 32 * kAhead >= walk.end;
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g) {
+      float x[W::kE];
+      Vector<T>::unpack(vectors[g], x);
+      if (ends) walk.mask(v + 32 * g, x);
+#pragma unroll
+      for (int i = 0; i < W::kE; ++i) most[g] = fmaxf(most[g], x[i]);  // (of a number and none, the number)
+    }
+  }
+#pragma unroll
+  for (int g = 1; g < kAhead; ++g) most[0] = fmaxf(most[0], most[g]);
+  return most[0];
+}
+
+template <typename T, int kThreads>
+__device__ __noinline__ uint32_t first_index_of(float value) {
+  const auto walk = Walk<T, kThreads>::mine();
+  uint32_t index = 0xffffffffu;
+  walk.each_eight([&](const float (&x)[8], int v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) index = x[i] == value ? min(index, static_cast<uint32_t>(walk.index_in(v, i))) : index;
+  });
+  return index;
+}
+
+// (the whole number stands in the low bits; of ranges without an extent it means nothing: sums tell whether the border is where counts say)
+__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return (share_whole(bins.high - x, bins.per) - kShareWhole) & (kBins - 1); }
+__device__ __forceinline__ Bins bins_between(float low, float high) { return {low, high, static_cast<float>(kBins - 1) / (high - low)}; }
+
+template <int kThreads>
+__device__ __forceinline__ void clear_bins() {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) shared<kThreads>().bins[i] = 0;
+  __syncthreads();
+}
+
+// Counts what is inside by bins; with `shares` also this lane's sum of shares, in 32 bits: where to look, no more.
+template <typename T, int kThreads>
+__device__ __noinline__ float look(Bins bins, bool shares) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  const auto walk = Walk<T, kThreads>::mine();
+  const Border border = border_of(sh.row);
+  const int nothing = kBins + (threadIdx.x & 31);
+  const bool all = !sh.row.bounded, plain = sh.row.form == kPlain;
+  const float top32 = sh.row.top32, rate = sh.row.scale32 * (1.0f / kExp2Entries);
+  float sum = 0.0f;
+  walk.each_eight([&](const float (&x)[8], int v) {
+    bool in[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) in[i] = true;
+    if (!all) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) in[i] = border.inside(x[i], walk.index_in(v, i));
+    }
+    if (shares) {
+      if (plain) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float t = (fmaxf(x[i], -3.402823466e38f) - top32) * rate;  // (no number: none)
+          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w[i]) : "f"(t));
+          w[i] = in[i] ? w[i] : 0.0f;
         }
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      } else {
+        const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += in[i] & (x[i] > -INFINITY) ? static_cast<float>(eight.w[i]) : 0.0f;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) atomicAdd(&sh.bins[in[i] & (x[i] >= bins.low) ? bin_of(bins, x[i]) : nothing], 1);
+  });
+  return sum;
+}
+
+// Of what is inside: what lies from `low` to `high` is put on this CTA's list or, with bins, counted in them.  Measured for this lane: what is above
+// `high` and not above `before`, by shares or by how many; and with `whole`, the shares of all.
+struct Sifted {
+  double above, all;
+};
+template <typename T, int kThreads, bool kGeneral>
+__device__ __noinline__ Sifted sift(bool binned, float low, float high, float before, bool measured, bool shares, bool whole, Bins bins) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kCap = SampleShared<kThreads>::kCap;
+  const auto walk = Walk<T, kThreads>::mine();
+  constexpr int kE = Walk<T, kThreads>::kE, kGroup = Walk<T, kThreads>::kGroup;
+  const Border border = border_of(sh.row);
+  const int nothing = kBins + (threadIdx.x & 31);
+  const double scale = sh.row.scale, top = sh.row.top;
+  const float scale32 = sh.row.scale32, top32 = sh.row.top32, cut = sh.row.cut;
+  const double* table = lane_table<kThreads>();
+  Sifted sifted{0.0, 0.0};
+  // Hits are a few of thousands: which values they are is noted in bits, and they are put on the list behind some rounds of the loop together.
+  unsigned long long noted = 0;
+  int noted_from = walk.begin + (threadIdx.x & 31), rounds = 0;
+  const auto put = [&]() {
+    if (noted == 0) return;
+    int to = atomicAdd(&sh.mine_count, __popcll(noted));
+    while (noted != 0) {
+      const int bit = __ffsll(noted) - 1, i = bit & 7;
+      noted &= noted - 1;
+      const int v = noted_from + (bit >> 3) * 32 * kGroup + i / kE * 32;
+      const float x = static_cast<float>(reinterpret_cast<const T*>(walk.source + v)[i % kE]);
+      if (to < kCap) sh.mine[to] = static_cast<unsigned long long>(~order_of(x)) << 32 | static_cast<uint32_t>(walk.index_of(v) + i % kE);
+      ++to;
+    }
+  };
+  walk.each_eight([&](const float (&x)[8], int v) {
+    uint32_t hits = 0, higher = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bool in = (x[i] >= low) & (x[i] <= before);  // (no branches: eight values side by side)
+      if (kGeneral) in &= border.inside(x[i], walk.index_in(v, i));
+      const bool up = x[i] > high;
+      hits |= in & !up ? 1u << i : 0u;
+      higher |= in & up ? 1u << i : 0u;
+    }
+    if (whole || (measured && shares && higher != 0)) {
+      double w[8];
+      if (!kGeneral) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
+      } else if (sh.row.form == kPlain) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = (x[i] >= cut) & border.inside(x[i], walk.index_in(v, i)) ? w[i] : 0.0;
+      } else {
+        const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) ? eight.w[i] : 0.0;
+      }
+      double up[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) up[i] = higher >> i & 1 ? w[i] : 0.0;
+      sifted.above += ((up[0] + up[1]) + (up[2] + up[3])) + ((up[4] + up[5]) + (up[6] + up[7]));
+      sifted.all += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    }
+    if (measured && !shares) sifted.above += __popc(higher);
+    if (binned) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) atomicAdd(&sh.bins[hits >> i & 1 ? bin_of(bins, x[i]) : nothing], 1);
+    } else {
+      noted |= static_cast<unsigned long long>(hits) << (8 * rounds);
+      if (++rounds == 8) {
+        put();
+        noted_from += 8 * 32 * kGroup;
+        rounds = 0;
+      }
+    }
+  });
+  if (!binned) put();
+  return sifted;
+}
+template <typename T, int kThreads>
+__device__ __forceinline__ Sifted sift_row(bool binned, float low, float high, float before, bool measured, bool shares, bool whole, const Bins& bins) {
+  const RowState& row = shared<kThreads>().row;
+  if (row.form == kPlain && !row.bounded) return sift<T, kThreads, false>(binned, low, high, before, measured, shares, whole, bins);
+  return sift<T, kThreads, true>(binned, low, high, before, measured, shares, whole, bins);
+}
+
+// This lane's sum of the shares, of vectors begin .. end - 1, that are inside and not below `least`.
+template <typename T, int kThreads>
+__device__ __noinline__ double sum_shares(int begin, int end, double least) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  const Walk<T, kThreads> walk(begin, end);
+  const double scale = sh.row.scale, top = sh.row.top;
+  const float scale32 = sh.row.scale32, top32 = sh.row.top32, cut = sh.row.cut;
+  const double* table = lane_table<kThreads>();
+  const Border border = border_of(sh.row);
+  double sum = 0.0;
+  if (sh.row.form == kPlain && !sh.row.bounded && !(least > 0.0)) {  // the ordinary case by itself: a dozen instructions a value fewer
+    walk.each_eight([&](const float (&x)[8], int) {
+      double w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
+      sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     });
-    __syncthreads();
-    const int count = sh.mine_count;
-    const int which = parity;
-    parity ^= 1;
-    if (warp == 0) {
-      if (lane < ctas) cluster_store_double(cluster_map_shared(smem_u32(&sh.slots[which][rank][0]), lane), static_cast<double>(count));
-      if (lane == 0) sh.base = count > 0 && count <= kCap ? cluster_add(cluster_map_shared(smem_u32(&sh.list_count), 0), count) : kCap;
-    }
-    __syncthreads();
-    if (count <= kCap) {
-      const uint32_t list = cluster_map_shared(smem_u32(sh.list), 0);
-      const int base = sh.base;
-      for (int i = threadIdx.x; i < count; i += kThreads)
-        if (base + i < kCap) cluster_store_u64(list + 8 * (base + i), sh.mine[i]);
-    }
-    cluster_barrier();
-    double sum = 0.0;
-    for (int r = 0; r < ctas; ++r) sum += sh.slots[which][r][0];
-    if (threadIdx.x == 0) sh.list_count = 0;  // (for the next gathering, which a barrier comes before)
-    return static_cast<int>(sum);
+    return sum;
   }
-
-  // Sums up to each of a thread's four entries of the list, over the whole CTA; returns the sum of all.
-  __device__ __forceinline__ double list_upto(const double (&w)[4], double (&upto)[4], double& in_front) {
-    const double inclusive = warp_upto(w[0] + w[1] + w[2] + w[3]);
-    if (lane == 31) sh.warp_sums[warp][0] = inclusive;
-    __syncthreads();
-    double before = 0.0, all = 0.0;
-    for (int v = 0; v < kWarps; ++v) {
-      if (v == warp) before = all;
-      all += sh.warp_sums[v][0];
+  const bool plain = sh.row.form == kPlain;
+  walk.each_eight([&](const float (&x)[8], int v) {
+    double w[8];
+    if (plain) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
+    } else {
+      const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = eight.w[i];
     }
-    const double previous = __shfl_up_sync(0xffffffffu, inclusive, 1);
-    in_front = before + (lane > 0 ? previous : 0.0);
-    double sum = in_front;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) upto[j] = sum += w[j];
-    __syncthreads();
-    return all;
-  }
-  static __device__ __forceinline__ float ranked_value(unsigned long long entry) { return value_of(~static_cast<uint32_t>(entry >> 32)); }
+    for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) & (w[i] >= least) ? w[i] : 0.0;
+    sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  });
+  return sum;
+}
 
-  // In the list, sorted by rank: the first at which `above` and the measure of the entries up to it come to `target`; count: none does.
-  __device__ __forceinline__ int list_border(int count, bool shares, double above, double target) {
-    double w[4], upto[4], in_front;
+// The same of a few: those that are inside, from `low` to `high`.  Or (ties) how many these are.
+template <typename T, int kThreads>
+__device__ __noinline__ double sum_few(int begin, int end, float low, float high, bool ties) {
+  const Border border = border_of(shared<kThreads>().row);
+  const Walk<T, kThreads> walk(begin, end);
+  double sum = 0.0;
+  walk.each_eight([&](const float (&x)[8], int v) {
+    uint32_t near = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * threadIdx.x + j;
-      w[j] = i >= count ? 0.0 : shares ? share(ranked_value(sh.list[i])) : 1.0;
+    for (int i = 0; i < 8; ++i) near |= (x[i] >= low) & (x[i] <= high) & border.inside(x[i], walk.index_in(v, i)) ? 1u << i : 0u;
+    if (ties) {
+      sum += __popc(near);
+      return;
+    }
+    if (near == 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (near >> i & 1) sum += share<kThreads>(x[i]);
+  });
+  return sum;
+}
+
+// The first CTA's list gets what lies from `low` to `high` in order and is inside; `count` of them (more than kCap: the list is not whole).
+struct Gathered {
+  int count;
+  Sifted sifted;  // this lane's
+};
+template <typename T, int kThreads>
+__device__ __noinline__ Gathered gather(uint32_t low, uint32_t high, float before, bool measured, bool shares, bool whole, int which) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kCap = SampleShared<kThreads>::kCap;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas;
+  if (threadIdx.x == 0) sh.mine_count = 0;
+  __syncthreads();
+  Gathered got;
+  got.sifted = sift_row<T, kThreads>(false, value_of(low), value_of(high), before, measured, shares, whole, Bins{});
+  __syncthreads();
+  const int count = sh.mine_count;
+  if (warp == 0) {
+    if (lane < ctas) cluster_store_double(cluster_map_shared(smem_u32(&sh.slots[which][sh.row.rank][0]), lane), static_cast<double>(count));
+    if (lane == 0) sh.base = count > 0 && count <= kCap ? cluster_add(cluster_map_shared(smem_u32(&sh.list_count), 0), count) : kCap;
+  }
+  __syncthreads();
+  if (count <= kCap) {
+    const uint32_t list = cluster_map_shared(smem_u32(sh.list), 0);
+    const int base = sh.base;
+    for (int i = threadIdx.x; i < count; i += kThreads)
+      if (base + i < kCap) cluster_store_u64(list + 8 * (base + i), sh.mine[i]);
+  }
+  cluster_barrier<kThreads>();
+  double sum = 0.0;
+  for (int r = 0; r < ctas; ++r) sum += sh.slots[which][r][0];
+  if (threadIdx.x == 0) sh.list_count = 0;  // (for the next gathering, which a barrier comes before)
+  got.count = static_cast<int>(sum);
+  return got;
+}
+
+// ---- the first CTA's list
+
+// The entries of the list, which has more than `ranks`, up to the bin of their value that the last of the first `ranks` is in: to
+// `mine`; returns how many.
+template <int kThreads>
+__device__ __noinline__ int prune(int count, int ranks, float highest) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kFewBins = kThreads, kEach = SampleShared<kThreads>::kEach, kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  sh.bins[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    sh.edges[0] = kFewBins - 1;
+    sh.edges[1] = 0;
+  }
+  float lowest = highest;
+  unsigned long long entries[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = threadIdx.x + j * kThreads;
+    entries[j] = i < count ? sh.list[i] : 0;
+    if (i < count) lowest = fminf(lowest, ranked_value(entries[j]));
+  }
+  const uint32_t low = __reduce_min_sync(0xffffffffu, order_of(lowest));
+  if (lane == 0) sh.warp_index[warp] = low;
+  __syncthreads();
+  uint32_t least = sh.warp_index[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) least = min(least, sh.warp_index[w]);
+  const float per = static_cast<float>(kFewBins - 1) / (highest - value_of(least));
+  const auto bin = [&](unsigned long long entry) { return static_cast<int>((share_whole(highest - ranked_value(entry), per) - kShareWhole) & (kFewBins - 1)); };
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (threadIdx.x + j * kThreads < count) atomicAdd(&sh.bins[bin(entries[j])], 1);
+  __syncthreads();
+  int upto = sh.bins[threadIdx.x];
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int more = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += more;
+  }
+  if (lane == 31) sh.warp_index[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) upto += w < warp ? sh.warp_index[w] : 0;
+  if (upto >= ranks) atomicMin(&sh.edges[0], static_cast<int>(threadIdx.x));
+  __syncthreads();
+  const int last = sh.edges[0];
+  uint32_t keep = 0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) keep |= threadIdx.x + j * kThreads < count && bin(entries[j]) <= last ? 1u << j : 0u;
+  int to = keep ? atomicAdd(&sh.edges[1], __popc(keep)) : 0;  // (sorted afterwards: any order will do)
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (keep >> j & 1) sh.mine[to++] = entries[j];
+  __syncthreads();
+  return sh.edges[1];
+}
+
+// Sums up to each of a thread's entries, over the whole CTA.
+template <int kThreads>
+struct Upto {
+  double upto[SampleShared<kThreads>::kEach], in_front, all;
+};
+template <int kThreads>
+__device__ __forceinline__ Upto<kThreads> list_upto(const double (&w)[SampleShared<kThreads>::kEach]) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kEach = SampleShared<kThreads>::kEach, kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Upto<kThreads> out;
+  double mine = 0.0;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) mine += w[j];
+  const double inclusive = warp_upto(mine);
+  if (lane == 31) sh.warp_sums[warp][0] = inclusive;
+  __syncthreads();
+  double before = 0.0;
+  out.all = 0.0;
+#pragma unroll
+  for (int v = 0; v < kWarps; ++v) {
+    if (v == warp) before = out.all;
+    out.all += sh.warp_sums[v][0];
+  }
+  const double previous = __shfl_up_sync(0xffffffffu, inclusive, 1);
+  out.in_front = before + (lane > 0 ? previous : 0.0);
+  double sum = out.in_front;
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) out.upto[j] = sum += w[j];
+  __syncthreads();
+  return out;
+}
+
+// The border out of the first CTA's list of `count`, in all CTAs: the first entry by rank at which `above` and the measure of the entries up to it come
+// to `target`.  False: it is not there.  (`surely`: the last entry where rounding leaves none.)
+template <int kThreads>
+__device__ __noinline__ bool border_from_list(int count, bool shares, double above, double target, bool surely) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kEach = SampleShared<kThreads>::kEach;
+  if (sh.row.rank == 0) {
+    sort_list<kThreads>(sh.list, count);
+    double w[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = kEach * threadIdx.x + j;
+      w[j] = i >= count ? 0.0 : shares ? share<kThreads>(ranked_value(sh.list[i])) : 1.0;
     }
     if (threadIdx.x == 0) sh.found = count;
-    list_upto(w, upto, in_front);
+    const Upto<kThreads> sums = list_upto<kThreads>(w);
+    if (above < target || surely) {
 #pragma unroll
-    for (int j = 3; j >= 0; --j) {
-      const int i = 4 * threadIdx.x + j;
-      if (i < count && above + upto[j] >= target) atomicMin(&sh.found, i);
+      for (int j = kEach - 1; j >= 0; --j) {
+        const int i = kEach * threadIdx.x + j;
+        if (i < count && above + sums.upto[j] >= target) atomicMin(&sh.found, i);
+      }
     }
     __syncthreads();
-    return sh.found;
+    int at = sh.found;
+    if (surely && count > 0) at = min(at, count - 1);
+    const unsigned long long entry = at < count ? sh.list[at] : 0;
+    if (threadIdx.x < sh.row.ctas) cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), threadIdx.x), entry);
   }
-
-  // The border out of the first CTA's list of `count`, in all CTAs; false: it is not there.  (`surely`: the last entry where rounding leaves none.)
-  __device__ __forceinline__ bool border_from_list(int count, bool shares, double above, double target, bool surely) {
-    if (rank == 0) {
-      sort_list<kThreads>(sh.list, count);
-      int at = above < target || surely ? list_border(count, shares, above, target) : count;
-      if (surely && count > 0) at = min(at, count - 1);
-      const unsigned long long entry = at < count ? sh.list[at] : 0;
-      if (warp == 0 && lane < ctas) cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), lane), entry);
-    }
-    cluster_barrier();
-    const unsigned long long entry = sh.border;
-    if (entry == 0) return false;  // (no value that may be taken has the complement of zero for its order)
-    border_key = ~static_cast<uint32_t>(entry >> 32);
-    border_index = static_cast<uint32_t>(entry);
-    bounded = true;
-    return true;
+  cluster_barrier<kThreads>();
+  const unsigned long long entry = sh.border;
+  if (entry == 0) return false;  // (no value that may be taken has the complement of zero for its order)
+  if (threadIdx.x == 0) {
+    sh.row.border_key = ~static_cast<uint32_t>(entry >> 32);
+    sh.row.border_index = static_cast<uint32_t>(entry);
+    sh.row.border = ranked_value(entry);
+    sh.row.bounded = 1;
   }
+  __syncthreads();
+  return true;
+}
 
-  // ---- by counts of values in 32nds of an octave of share
+// ---- where counts say that a border is
 
-  // The smallest order with a bin of at most `bin` (the largest value's is 0); searched by 32 lanes at a time.
-  __device__ __forceinline__ uint32_t order_with(int bin, uint32_t largest) const {
-    uint32_t low = kNothing + 1, high = largest;
-    while (low < high) {
-      const uint32_t step = (high - low) / 32 + 1, at = min(low + step * lane, high);
-      const uint32_t yes = __ballot_sync(0xffffffffu, bin_of(value_of(at)) <= bin);  // ascending: none, then all
-      if (yes & 1) return low;
-      const int first = yes ? __ffs(yes) - 1 : 32;
-      const uint32_t next = min(low + step * first, high);
-      low = min(low + step * (first - 1) + 1, next);
-      high = next;
-    }
-    return low;
+// The smallest order from `low` on (up to `high`, for which it holds) with a bin of at most `bin`; searched by 32 lanes at a time.
+__device__ __noinline__ uint32_t order_with(Bins bins, int bin, uint32_t low, uint32_t high) {
+  const int lane = threadIdx.x & 31;
+  if (low < high) {  // most often it is among the 32 numbers about the bin's edge
+    const uint32_t edge = order_of(bins.high - (static_cast<float>(bin) + 0.5f) / bins.per);
+    const uint32_t begin = edge > low + 16 && edge < high ? edge - 16 : low, at = min(begin + lane, high);
+    const uint32_t yes = __ballot_sync(0xffffffffu, at == high || bin_of(bins, value_of(at)) <= bin);
+    if (yes != 0 && (yes & 1) == 0) return min(begin + __ffs(yes) - 1, high);
+    if (yes & 1) high = begin;  // (begin is not below low)
+    else low = begin + 32;
   }
+  while (low < high) {
+    const uint32_t step = (high - low) / 32 + 1, at = min(low + step * lane, high);
+    const uint32_t yes = __ballot_sync(0xffffffffu, at == high || bin_of(bins, value_of(at)) <= bin);  // ascending: none, then all
+    if (yes & 1) return low;
+    const int first = yes ? __ffs(yes) - 1 : 32;
+    const uint32_t next = min(low + step * first, high);
+    low = min(low + step * (first - 1) + 1, next);
+    high = next;
+  }
+  return low;
+}
 
-  // Counts what is inside by bins and, with `shares`, sums its shares; `sum` is of the cluster.
-  __device__ __forceinline__ void count_bins(bool shares, double& sum) {
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.bins[i] = 0;
+// Where the counts say that `target` is reached, with `above` in front of the bins.  Counts times the shares of their bins' middles are off by up to
+// `off` of themselves: the border lies between where they reach the target with that much more and with that much less.  Where
+// that is more than the list holds, it is looked at with a fiftieth of it (errors of many bins cancel; sums will tell), or closer.
+template <int kThreads>
+__device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double above, double target, double off, int turn) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kCap = SampleShared<kThreads>::kCap, kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas, rank = sh.row.rank;
+  if (ctas > 1) {
+    // Each CTA adds up its part of the bins, a quarter of a thousand reads of 16 bytes, and puts it with the first one's.
+    const int part = kBins / 4 / ctas;  // (a power of two)
+    for (int i = threadIdx.x; i < 4 * part; i += kThreads) sh.totals[i] = 0;
     __syncthreads();
-    double v[1] = {0.0};
-    if (form == kPlain && !bounded) {
-      const float from = cut;
-      if (shares) {
-        each_value([&](float x, int) {
-          const uint32_t whole = plain_whole(x);
-          const double w = plain_share(x, whole);
-          if (x >= from) {
-            v[0] += w;
-            atomicAdd(&sh.bins[plain_bin(whole)], 1);
-          }
-        });
-      } else {
-        each_value([&](float x, int) {
-          if (x >= from) atomicAdd(&sh.bins[plain_bin(plain_whole(x))], 1);
-        });
-      }
-    } else {
-      each_value([&](float x, int index) {
-        if (inside(x, index)) {
-          const BinnedShare it = form == kPlain ? BinnedShare{share(x), bin_of(x)} : other(x);
-          v[0] += it.share;
-          atomicAdd(&sh.bins[it.bin], 1);
-        }
-      });
+    for (int i = threadIdx.x; i < kBins / 4; i += kThreads) {
+      const int quad = i & (part - 1);
+      const int4 four = cluster_load4(cluster_map_shared(smem_u32(&sh.bins4[rank * part + quad]), i / part));
+      if (four.x) atomicAdd(&sh.totals[4 * quad], four.x);
+      if (four.y) atomicAdd(&sh.totals[4 * quad + 1], four.y);
+      if (four.z) atomicAdd(&sh.totals[4 * quad + 2], four.z);
+      if (four.w) atomicAdd(&sh.totals[4 * quad + 3], four.w);
     }
-    cluster_sums(v);
-    sum = v[0];
+    __syncthreads();
+    if (rank > 0) {  // (the first one's own part stands where it belongs, the others' behind it)
+      const uint32_t to = cluster_map_shared(smem_u32(&sh.totals4[rank * part]), 0);
+      for (int i = threadIdx.x; i < part; i += kThreads) {
+        const int4 four = sh.totals4[i];
+        cluster_store_uint4(to + 16 * i, make_uint4(four.x, four.y, four.z, four.w));
+      }
+    }
+    cluster_barrier<kThreads>();
+  } else {
+    __syncthreads();
   }
-
-  // Where the counts say that the first `target` (shares, or values) end.  Counts times the shares of their bins' middles are off by up to 1.1 %:
-  // so far to both sides, or, where that is more than the list holds, a tenth of it.  No border among the bins: count is zero.
-  __device__ __forceinline__ BinWindow window_of_bins(bool shares, double target) {
-    if (rank == 0) {
-      constexpr int kEach = kBins / kThreads;
-      int count[kEach];
-      double mass[kEach], counted = 0.0, massed = 0.0;
+  if (rank == 0) {
+    constexpr int kOf = kBins / kThreads;
+    const float rate = sh.row.scale32 * (1.0f / kExp2Entries), top32 = sh.row.top32;
+    const bool plain = sh.row.form == kPlain;
+    int count[kOf], counted = 0;
+    float mass[kOf], massed = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int bin = threadIdx.x * kEach + i;
-        const uint32_t at = smem_u32(&sh.bins[bin]);
-        count[i] = 0;
-        for (int r = 0; r < ctas; ++r) count[i] += cluster_load(cluster_map_shared(at, r));
-        // (what the last bin has lies at any distance: it is no place for a border)
-        mass[i] = bin == kBins - 1 ? 0.0 : count[i] * scaled_by(table()[((0u - bin) & (kExp2Entries - 1)) * kTableCopies], 0u - bin);
-        if (bin == kBins - 1) count[i] = 0;
-        counted += count[i];
-        massed += mass[i];
-      }
-      const double counts = warp_upto(counted), masses = warp_upto(massed);
-      if (lane == 31) {
-        sh.warp_sums[warp][0] = counts;
-        sh.warp_sums[warp][1] = masses;
-      }
-      if (threadIdx.x < 4) sh.edges[threadIdx.x] = kBins;
-      __syncthreads();
-      double count_upto = counts - counted, mass_upto = masses - massed;
-      for (int w = 0; w < warp; ++w) {
-        count_upto += sh.warp_sums[w][0];
-        mass_upto += sh.warp_sums[w][1];
-      }
-      const double most = target * (1.0 + 0.011), least = target * (1.0 - 0.011), more = target * (1.0 + 0.0011), less = target * (1.0 - 0.0011);
+    for (int i = 0; i < kOf; ++i) {
+      const int bin = threadIdx.x * kOf + i;
+      count[i] = ctas > 1 ? sh.totals[bin] : sh.bins[bin];
+      const float middle = fmaxf(bins.high - static_cast<float>(bin) / bins.per, bins.low);
+      mass[i] = 0.0f;
+      if (shares && count[i] > 0) mass[i] = count[i] * (plain ? exp2f((middle - top32) * rate) : static_cast<float>(share<kThreads>(middle)));
+      counted += count[i];
+      massed += mass[i];
+    }
+    int counts = counted;
+    float masses = massed;
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) {
-        const int bin = threadIdx.x * kEach + i;
-        count_upto += count[i];
-        mass_upto += mass[i];
-        sh.bins[bin] = static_cast<int>(count_upto);
-        const double upto = shares ? mass_upto : count_upto;
-        if (count[i] > 0) {
-          if (upto >= (shares ? least : target)) atomicMin(&sh.edges[0], bin);
-          if (upto >= (shares ? most : target)) atomicMin(&sh.edges[1], bin);
-          if (upto >= (shares ? less : target)) atomicMin(&sh.edges[2], bin);
-          if (upto >= (shares ? more : target)) atomicMin(&sh.edges[3], bin);
-        }
-      }
-      __syncthreads();
-      if (warp == 0) {
-        BinWindow window{};
-        for (int wide = 0; wide < 4 && window.count == 0; wide += 2) {
-          const int first = sh.edges[wide];
-          if (first == kBins) break;
-          const int last = min(sh.edges[wide + 1], kBins - 2);
-          const int in_front = first > 0 ? sh.bins[first - 1] : 0, upto = sh.bins[last];
-          // (all of it only where it surely reaches the target)
-          if (upto <= kCap && sh.edges[wide + 1] < kBins - 1 && (wide == 0 || !shares)) window = BinWindow{0, last, upto, 1};
-          else if (upto - in_front <= kCap) window = BinWindow{first, last, upto - in_front, 0};
-        }
-        if (lane < ctas)
-          cluster_store_uint4(cluster_map_shared(smem_u32(&sh.window), lane), make_uint4(window.first, window.last, window.count, window.whole));
+    for (int d = 1; d < 32; d *= 2) {
+      const int c = __shfl_up_sync(0xffffffffu, counts, d);
+      const float m = __shfl_up_sync(0xffffffffu, masses, d);
+      if (lane >= d) {
+        counts += c;
+        masses += m;
       }
     }
-    cluster_barrier();
-    const uint4 w = sh.window;
-    return BinWindow{static_cast<int>(w.x), static_cast<int>(w.y), static_cast<int>(w.z), static_cast<int>(w.w)};
+    if (lane == 31) {
+      sh.warp_index[warp] = counts;
+      sh.warp_key[warp] = __float_as_uint(masses);
+    }
+    if (threadIdx.x < 4) sh.edges[threadIdx.x] = kBins;
+    __syncthreads();
+    int count_upto = counts - counted;
+    float mass_upto = masses - massed;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      count_upto += w < warp ? sh.warp_index[w] : 0;
+      mass_upto += w < warp ? __uint_as_float(sh.warp_key[w]) : 0.0f;
+    }
+    // the target for counts' sums, by each edge
+    const float rest = static_cast<float>(target - above), o = static_cast<float>(off), few = 0.02f * fminf(o, 1.0f);
+    const float edge[4] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY, rest / (1.0f + few), rest / (1.0f - few)};
+    const double missing = target - above;
+#pragma unroll
+    for (int i = 0; i < kOf; ++i) {
+      const int bin = threadIdx.x * kOf + i;
+      const float mass_before = mass_upto;
+      const int count_before = count_upto;
+      count_upto += count[i];
+      mass_upto += mass[i];
+      sh.bins[bin] = count_upto;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // (each edge is passed in one bin)
+        if (shares ? mass_upto >= edge[e] && (mass_before < edge[e] || bin == 0) : count_upto >= missing && (count_before < missing || bin == 0))
+          atomicMin(&sh.edges[e], bin);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const auto upto = [&](int bin) { return bin < 0 ? 0 : sh.bins[bin]; };
+      const int sure_first = sh.edges[0], sure_last = min(sh.edges[1], kBins - 1);
+      BinWindow window{sure_first, sure_last, kNotHere, sure_first, sure_last};
+      if (window.first < kBins) {
+        if (sh.edges[1] < kBins && above == 0.0 && upto(window.last) <= kCap) {
+          window.first = 0;
+          window.says = kListHasAll;
+        } else if (upto(window.last) - upto(window.first - 1) <= kCap) {
+          window.says = kInList;
+        } else if (sh.edges[3] < kBins && upto(sh.edges[3]) - upto(sh.edges[2] - 1) <= kCap) {
+          window.first = sh.edges[2];
+          window.last = sh.edges[3];
+          window.says = kInList;
+        } else if (window.first > 0 || window.last < kBins - 1) {  // (else a closer look would see the same)
+          window.says = kLookCloser;
+        }
+      }
+      if (lane < ctas)
+        cluster_store_uint4(cluster_map_shared(smem_u32(&sh.window[turn & 1]), lane), make_uint4(window.first, window.last, window.says, sure_first << 16 | sure_last));
+    }
   }
+  cluster_barrier<kThreads>();
+  const uint4 w = sh.window[turn & 1];
+  return BinWindow{static_cast<int>(w.x), static_cast<int>(w.y), static_cast<BinsSay>(w.z), static_cast<int>(w.w >> 16), static_cast<int>(w.w & 0xffffu)};
+}
 
-  // ---- by halving
+// ---- the token
 
-  // The value, and among its ties the index, at which the measure (shares, or how many) of what is inside and ranks up to there comes to
-  // `target`.  Sets the border; none where all that is inside does not come to it.
-  __device__ __forceinline__ void find_border(bool shares, double target, uint32_t low, uint32_t high) {
-    double above = 0.0, count = 2.0 * kCap;  // what is higher than `high` measures; how many lie from `low` to `high` (at first: many)
-    for (int step = 0; low < high && count > kCap; ++step) {  // (every other step halves the range of orders: it ends in 64)
-      const float middle = 0.5f * value_of(low) + 0.5f * value_of(high);
-      uint32_t mid = step & 1 ? low + (high - low) / 2 : order_of(middle);
-      mid = max(low, min(mid, order_below(high)));
-      if (mid == 0x7fffffffu) mid = high > 0x80000000u ? 0x80000000u : 0x7ffffffeu;
-      const float from = value_of(mid), bottom = value_of(low), upto = value_of(high);
-      double v[3] = {0.0, 0.0, 0.0};  // how many, how many above the middle, what those measure
-      each_value([&](float x, int index) {
-        if (x >= bottom && x <= upto && inside(x, index)) {
-          v[0] += 1.0;
-          if (x > from) {
-            v[1] += 1.0;
-            if (shares) v[2] += share(x);
-          }
-        }
-      });
-      cluster_sums(v);
-      const double measure = shares ? v[2] : v[1];
-      if (above + measure >= target) {
-        low = order_above(mid);
-        count = v[1];
-      } else {
-        high = mid;
-        above += measure;
-        count = v[0] - v[1];
-        if (count == 0.0) return;  // (there are not as many: all stay)
-      }
-    }
-    if (low < high || count <= kCap) {
-      const int gathered = gather(low, high, [](float) {});
-      if (gathered <= kCap) {
-        border_from_list(gathered, shares, above, target, true);
-        return;
-      }
-    }
-    // More ties than the list holds: so many of them, in the order of the vocabulary.
-    const float value = value_of(low);
-    double v[1] = {0.0};
-    each_value([&](float x, int index) { v[0] += x == value && inside(x, index) ? 1.0 : 0.0; });
-    cluster_sums(v);
-    double ties = target - above;
-    if (shares) ties /= share(value);
-    ties = fmin(fmax(ceil(ties), 1.0), v[0]);
-    const auto one = [&](float x, int i) { return x == value && inside(x, i) ? 1.0 : 0.0; };
-    locate(
-        0.0, one, one, [&](double) { return ties - 0.5; },
-        [&](float, int i, double, double) {
-          for (int r = 0; r < ctas; ++r) cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), r), static_cast<unsigned long long>(static_cast<uint32_t>(i)));
-        });
-    cluster_barrier();
-    border_key = low;
-    border_index = static_cast<uint32_t>(sh.border);
-    bounded = true;
-  }
-
-  // The first value of the vocabulary at which the sum of weights passes target_of(sum of all weights): found(value, index, weight, sum of all)
-  // in one thread.  A lane's weights are `begun` and what rest(value, index) gives of each value.
-  template <class Rest, class W, class Target, class Found>
-  __device__ __forceinline__ void locate(double begun, Rest&& rest, W&& weight, Target&& target_of, Found&& found) {
-    double v[1] = {begun};
-    each_value([&](float x, int index) { v[0] += rest(x, index); });
-    const int which = cluster_sums(v);
-    const double all = v[0], target = target_of(all);
-    // the CTA: the last with any weight where rounding leaves the target above all sums
-    int cta = -1, last = 0;
-    double front = 0.0, last_front = 0.0, sum = 0.0;
-    for (int r = 0; r < ctas; ++r) {
-      const double own = sh.slots[which][r][0];
+// The first value of the vocabulary at which the sum of weights passes `of` times the sum of all, in one thread; the others have index -1.
+// A value's weight is its share where it is kept and not below `least`; or (ties) one where it is `value`, and the sum comes to `of`.  `mine` is
+// the sum of the lane's weights.
+struct Located {
+  int index;
+  double weight, all;
+};
+template <typename T, int kThreads>
+__device__ __noinline__ Located locate(double mine, bool ties, float value, double least, double of, int which) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kWarps = kThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas;
+  const Border border = border_of(sh.row);
+  const auto weight = [&](float x, int index) {
+    if (!border.inside(x, index)) return 0.0;
+    if (ties) return x == value ? 1.0 : 0.0;
+    const double w = share<kThreads>(x);
+    return w < least ? 0.0 : w;
+  };
+  Located it{-1, 0.0, 0.0};
+  const double all = cluster_sums<kThreads>(mine, 0.0, 0.0, which).a;
+  const double target = ties ? fmin(fmax(ceil(of), 1.0), all) - 0.5 : of * all;
+  // In what order sums follow one another: the part that holds the target, the last one with any weight where rounding leaves the target above all.
+  struct Part {
+    int hit, last;
+    double front, last_front, sum;
+    __device__ __forceinline__ void add(int part, double own, double target) {
       if (own > 0.0) {
-        last = r;
+        last = part;
         last_front = sum;
       }
-      if (cta < 0 && sum + own > target) {
-        cta = r;
+      if (hit < 0 && sum + own > target) {
+        hit = part;
         front = sum;
       }
       sum += own;
     }
-    if (cta < 0) {
-      cta = last;
-      front = last_front;
+    __device__ __forceinline__ void end() {
+      if (hit < 0) {
+        hit = last;
+        front = last_front;
+      }
     }
-    if (rank != cta || !(all > 0.0)) return;
-    // its warp, in the same way
-    int in_warp = -1;
-    double warp_front = 0.0;
-    sum = front;
-    last = 0;
-    last_front = front;
-    for (int w = 0; w < kWarps; ++w) {
-      const double own = sh.warp_sums[w][0];
-      if (own > 0.0) {
-        last = w;
-        last_front = sum;
-      }
-      if (in_warp < 0 && sum + own > target) {
-        in_warp = w;
-        warp_front = sum;
-      }
-      sum += own;
-    }
-    if (in_warp < 0) {
-      in_warp = last;
-      warp_front = last_front;
-    }
-    // its steps are summed by as many warps at a time, and the step that holds the target is walked through by one
-    const int each = warp_vectors(), begin = in_warp * each, end = min(vectors, begin + each), steps = (end - begin + 31) / 32;
-    double reached = warp_front;
-    int last_step = 0;
-    double last_reached = warp_front;
-    for (int base = 0; base < steps; base += kWarps) {
-      const int at = begin + (base + warp) * 32 + lane;
-      double own = 0.0;
-      if (at < end) one_vector(at, [&](float x, int index) { own += weight(x, index); });
-      own = warp_sum(own);
-      if (lane == 0) sh.warp_sums[warp][1] = own;
-      __syncthreads();
-      int hit = -1;
-      double hit_front = 0.0;
-      for (int w = 0; w < kWarps && base + w < steps; ++w) {
-        const double one = sh.warp_sums[w][1];
-        if (one > 0.0) {
-          last_step = base + w;
-          last_reached = reached;
-        }
-        if (hit < 0 && reached + one > target) {
-          hit = base + w;
-          hit_front = reached;
-        }
-        reached += one;
-      }
-      __syncthreads();
-      if (hit >= 0 || base + kWarps >= steps) {
-        const int step = hit >= 0 ? hit : last_step;
-        const double step_front = hit >= 0 ? hit_front : last_reached;
-        if (warp == 0) {
-          const int v_at = begin + step * 32 + lane;
-          double mine = 0.0;
-          if (v_at < end) one_vector(v_at, [&](float x, int index) { mine += weight(x, index); });
-          const double upto = warp_upto(mine), previous = __shfl_up_sync(0xffffffffu, upto, 1);
-          const double lane_front = step_front + (lane > 0 ? previous : 0.0);
-          const uint32_t passing = __ballot_sync(0xffffffffu, mine > 0.0 && step_front + upto > target);
-          const uint32_t some = __ballot_sync(0xffffffffu, mine > 0.0);
-          const int chosen = passing ? __ffs(passing) - 1 : 31 - __clz(some);
-          if (lane == chosen) {
-            double running = lane_front;
-            float value = 0.0f;
-            int index = -1;
-            double taken = 0.0;
-            bool done = false;
-            one_vector(v_at, [&](float x, int i) {
-              const double w = weight(x, i);
-              if (!done && w > 0.0) {
-                value = x;
-                index = i;
-                taken = w;
-              }
-              running += w;
-              if (w > 0.0 && running > target) done = true;
-            });
-            found(value, index, taken, all);
-          }
-        }
-        break;
-      }
+  };
+  Part cta{-1, 0, 0.0, 0.0, 0.0};
+  for (int r = 0; r < ctas; ++r) cta.add(r, sh.slots[which][r][0], target);
+  cta.end();
+  if (sh.row.rank != cta.hit || !(all > 0.0)) return it;
+  Part in_warp{-1, 0, cta.front, cta.front, cta.front};
+  for (int w = 0; w < kWarps; ++w) in_warp.add(w, sh.warp_sums[w][0], target);
+  in_warp.end();
+  // The warp's part is cut into as many pieces as there are warps, the piece that holds the target again, down to the 32 vectors that one
+  // warp walks over.
+  int from = sh.row.cta_begin + in_warp.hit * sh.row.warp_vectors, upto = min(sh.row.cta_end, from + sh.row.warp_vectors);
+  double reached = in_warp.front;
+  while (upto - from > 32) {
+    const int piece = ((upto - from + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const int mine_from = from + warp * piece, mine_upto = min(upto, mine_from + piece);
+    const double own = warp_sum(ties ? sum_few<T, kThreads>(mine_from, mine_upto, value, value, true) : sum_shares<T, kThreads>(mine_from, mine_upto, least));
+    if (lane == 0) sh.warp_sums[warp][1] = own;
+    __syncthreads();
+    Part in_piece{-1, 0, reached, reached, reached};
+    for (int w = 0; w < kWarps; ++w) in_piece.add(w, sh.warp_sums[w][1], target);
+    in_piece.end();
+    __syncthreads();
+    from += in_piece.hit * piece;
+    upto = min(upto, from + piece);
+    reached = in_piece.front;
+  }
+  if (warp == 0) {
+    const Walk<T, kThreads> end(from, upto);
+    const int v = from + lane;
+    double own = 0.0;
+    if (v < upto) end.one_vector(v, [&](float x, int index) { own += weight(x, index); });
+    const double sums = warp_upto(own), previous = __shfl_up_sync(0xffffffffu, sums, 1);
+    const uint32_t passing = __ballot_sync(0xffffffffu, own > 0.0 && reached + sums > target);
+    const uint32_t some = __ballot_sync(0xffffffffu, own > 0.0);
+    const int chosen = passing ? __ffs(passing) - 1 : 31 - __clz(some);
+    if (lane == chosen) {
+      double running = reached + (lane > 0 ? previous : 0.0);
+      bool done = false;
+      end.one_vector(v, [&](float x, int index) {
+        const double w = weight(x, index);
+        if (!done && w > 0.0) it = Located{index, w, all};
+        running += w;
+        done |= w > 0.0 && running > target;
+      });
     }
   }
+  return it;
+}
+
+// ---- a border by halving
+
+// Where all else fails (too many values, too equal or too far apart for bins): the value, and among its ties the index, at which the measure (shares,
+// or how many) of what is inside and ranks up to there comes to `target`; from `low` to `high`, above which it measures `above`.  Sets the
+// border; none where all that is inside does not come to it.
+template <typename T, int kThreads>
+__device__ __noinline__ int find_border(bool shares, double target, uint32_t low, uint32_t high, double above, int which) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kCap = SampleShared<kThreads>::kCap;
+  double count = 2.0 * kCap;  // how many lie from `low` to `high` (at first: many)
+  for (int step = 0; low < high && count > kCap; ++step) {  // (every other step halves the range of orders: it ends in 64)
+    const float middle = 0.5f * value_of(low) + 0.5f * value_of(high);
+    uint32_t mid = step & 1 ? low + (high - low) / 2 : order_of(middle);
+    mid = max(low, min(mid, order_below(high)));
+    if (mid == 0x7fffffffu) mid = high > 0x80000000u ? 0x80000000u : 0x7ffffffeu;
+    const float from = value_of(mid), bottom = value_of(low), upto = value_of(high);
+    double within = 0.0, upper = 0.0, measure = 0.0;
+    const auto walk = Walk<T, kThreads>::mine();
+    const Border border = border_of(sh.row);
+    walk.each_eight([&](const float (&x)[8], int v) {
+      uint32_t in = 0, up = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool hit = (x[i] >= bottom) & (x[i] <= upto) & border.inside(x[i], walk.index_in(v, i));
+        in |= hit ? 1u << i : 0u;
+        up |= hit & (x[i] > from) ? 1u << i : 0u;
+      }
+      within += __popc(in);
+      upper += __popc(up);
+      if (shares && up != 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (up >> i & 1) measure += share<kThreads>(x[i]);
+      }
+    });
+    const Three sums = cluster_sums<kThreads>(within, upper, measure, which);
+    which ^= 1;
+    const double over = shares ? sums.c : sums.b;
+    if (above + over >= target) {
+      low = order_above(mid);
+      count = sums.b;
+    } else {
+      high = mid;
+      above += over;
+      count = sums.a - sums.b;
+      if (count == 0.0) return which;  // (there are not as many: all stay)
+    }
+  }
+  if (low < high || count <= kCap) {
+    const int gathered = gather<T, kThreads>(low, high, value_of(high), false, false, false, which).count;
+    which ^= 1;
+    if (gathered <= kCap) {
+      border_from_list<kThreads>(gathered, shares, above, target, true);
+      return which;
+    }
+  }
+  // More ties than the list holds: so many of them, in the order of the vocabulary.
+  const float value = value_of(low);
+  const auto part = Walk<T, kThreads>::mine();
+  const double mine = sum_few<T, kThreads>(part.begin, part.end, value, value, true);
+  double ties = target - above;
+  if (shares) ties /= share<kThreads>(value);
+  const Located it = locate<T, kThreads>(mine, true, value, 0.0, ties, which);
+  which ^= 1;
+  if (it.index >= 0)
+    for (int r = 0; r < sh.row.ctas; ++r)
+      cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), r), static_cast<unsigned long long>(static_cast<uint32_t>(it.index)));
+  cluster_barrier<kThreads>();
+  if (threadIdx.x == 0) {
+    sh.row.border_key = low;
+    sh.row.border_index = static_cast<uint32_t>(sh.border);
+    sh.row.border = value;
+    sh.row.bounded = 1;
+  }
+  __syncthreads();
+  return which;
+}
+
+// What a list that has all that may be kept gives.  counted: by rank the first top_k stay; by_sum: those in front of which less than top_p of the sum has
+// been (of `whole_sum`, or where that is negative of the list's own); by_floor: shares of at least min_p.
+struct Rules {
+  int top_k;
+  bool by_count, by_sum, by_floor;
+  double top_p, min_p, u;
 };
+struct Taken {
+  int index;  // -1: another thread has it
+  float probability;
+};
+template <int kThreads>
+__device__ __noinline__ Taken finish(int count, double whole_sum, const Rules& rules, float most) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kEach = SampleShared<kThreads>::kEach, kFew = SampleShared<kThreads>::kFew;
+  const int thread = threadIdx.x;
+  Taken taken{-1, 0.0f};
+  unsigned long long* list = sh.list;
+  if (rules.by_count && count > 64 && count > rules.top_k) {  // nothing behind the bin that holds the top_k-th
+    list = sh.mine;
+    count = prune<kThreads>(count, rules.top_k, most);
+  }
+  sort_list<kThreads>(list, count);
+  const int ranks = rules.by_count ? min(count, rules.top_k) : count;
+  double w[kEach];
+  unsigned long long entries[kEach];
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = kEach * thread + j;
+    entries[j] = i < ranks ? list[i] : ~0ull;
+    w[j] = i < ranks ? share<kThreads>(ranked_value(entries[j])) : 0.0;
+  }
+  const Upto<kThreads> sums = list_upto<kThreads>(w);
+  const double target = rules.top_p * (whole_sum >= 0.0 ? whole_sum : sums.all);
+  if (thread == 0) sh.found = ranks;
+  __syncthreads();
+#pragma unroll
+  for (int j = kEach - 1; j >= 0; --j) {
+    const int i = kEach * thread + j;
+    const bool stays = i == 0 || !((rules.by_sum && (j == 0 ? sums.in_front : sums.upto[j > 0 ? j - 1 : 0]) >= target) || (rules.by_floor && w[j] < rules.min_p));
+    if (i < ranks && !stays) atomicMin(&sh.found, i);
+    list[i] = entries[j] << 32 | entries[j] >> 32;  // by index now, with the order behind it
+  }
+  __syncthreads();
+  const int kept = sh.found;  // by rank; what is behind the first that goes, goes
+  __syncthreads();            // (all have read it)
+  if (kept <= kFew) {
+    // Each with the sum of all up to its index: of few, sooner than sorted.
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (kEach * thread + j < kept) sh.few[kEach * thread + j] = w[j];
+    if (thread == 0) sh.found = 0x7fffffff;
+    __syncthreads();
+    double mine = 0.0, all = 0.0;
+    const unsigned long long own = thread < kept ? list[thread] : 0;
+    if (thread < kFew) {
+#pragma unroll 4
+      for (int j = 0; j < kept; ++j) {
+        const double one = sh.few[j];
+        all += one;
+        mine += list[j] <= own ? one : 0.0;
+      }
+      // (the last by index has the whole sum, in the same order)
+      if (thread < kept && mine > rules.u * all) atomicMin(&sh.found, static_cast<int>(own >> 32));
+    }
+    __syncthreads();
+    if (thread < kept && static_cast<int>(own >> 32) == sh.found) taken = Taken{sh.found, static_cast<float>(sh.few[thread] / all)};
+    return taken;
+  }
+  sort_list<kThreads>(list, kept);
+#pragma unroll
+  for (int j = 0; j < kEach; ++j) {
+    const int i = kEach * thread + j;
+    entries[j] = i < kept ? list[i] : ~0ull;
+    w[j] = i < kept ? share<kThreads>(value_of(~static_cast<uint32_t>(entries[j]))) : 0.0;
+  }
+  if (thread == 0) sh.found = kept - 1;
+  const Upto<kThreads> again = list_upto<kThreads>(w);
+#pragma unroll
+  for (int j = kEach - 1; j >= 0; --j)
+    if (kEach * thread + j < kept && again.upto[j] > rules.u * again.all) atomicMin(&sh.found, kEach * thread + j);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kEach; ++j)
+    if (sh.found == kEach * thread + j) taken = Taken{static_cast<int>(entries[j] >> 32), static_cast<float>(w[j] / again.all)};
+  return taken;
+}
 
 template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const SampleParams params) {
-  using R = Row<T, kThreads>;
-  constexpr int kE = R::kE, kWarps = R::kWarps, kCap = R::kCap;
-  static __shared__ SampleShared<kThreads> sh;
-  extern __shared__ uint4 held[];
+__global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const SampleParams params) {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  constexpr int kE = Vector<T>::kValues, kWarps = kThreads / 32, kCap = SampleShared<kThreads>::kCap;
   const SampleCall& p = params.call;
-  const int ctas = params.ctas, row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas;  // (a cluster is CTAs that follow one another)
+  const int ctas = params.ctas, at_row = blockIdx.x / ctas, rank = static_cast<int>(ctas > 1 ? cluster_cta_rank() : 0);
   const int thread = threadIdx.x, lane = thread & 31, warp = thread >> 5;
-  for (int i = thread; i < kExp2Entries * kTableCopies; i += kThreads) sh.table[i] = g_exp2_table[i / kTableCopies];
-  if (thread == 0) sh.list_count = 0;
   if (ctas > 1) cluster_arrive();  // (a CTA writes to the others when all have begun)
+  for (int i = thread; i < kExp2Entries * kTableCopies; i += kThreads) sh.table[i] = g_exp2_table[i / kTableCopies];
+  if (thread == 0) {
+    sh.list_count = 0;
+    // The row from the 16-byte boundary at or in front of its first value: what a vector has of other rows, or of the bytes in front of
+    // and behind the tensor (of the same 16, and so of the same allocation), counts as nothing.
+    const T* const data = static_cast<const T*>(p.logits) + at_row * p.row_stride;
+    RowState& row = sh.row;
+    row.lead = static_cast<int>((reinterpret_cast<uintptr_t>(data) & 15) / sizeof(T));
+    row.source = reinterpret_cast<const uint4*>(data - row.lead);
+    row.vocabulary = p.vocabulary;
+    row.vectors = (row.lead + p.vocabulary + kE - 1) / kE;
+    row.cta_begin = min(row.vectors, rank * params.cta_vectors);
+    row.cta_end = min(row.vectors, row.cta_begin + params.cta_vectors);
+    row.warp_vectors = params.cta_vectors / kWarps;
+    row.ctas = ctas;
+    row.rank = rank;
+    row.bounded = 0;
+    row.border_key = kNothing + 1;
+    row.border_index = 0xffffffffu;
+    row.border = -3.402823466e38f;
+  }
+  __syncthreads();
   grid_launch_dependents();
   grid_dependency_wait();
+  float temperature = p.temperature ? p.temperature[at_row] : 1.0f;
+  int top_k = p.top_k ? p.top_k[at_row] : 0;
+  float top_p = p.top_p ? p.top_p[at_row] : 1.0f, floor = p.min_p ? p.min_p[at_row] : 0.0f;
+  const float uniform = p.uniforms[at_row];
 
-  // The row from the 16-byte boundary at or in front of its first value: what a vector has of other rows, or of the bytes in front of
-  // and behind the tensor (of the same 16, and so of the same allocation), counts as nothing.
-  const T* const data = static_cast<const T*>(p.logits) + row * p.row_stride;
-  const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(data) & 15) / sizeof(T));
-  const uint4* const source = reinterpret_cast<const uint4*>(data - lead);
-  const int whole = (lead + p.vocabulary + kE - 1) / kE;  // vectors of the row
-  const int first_vector = min(whole, rank * params.cta_vectors);
-  R me{sh, held, min(whole - first_vector, params.cta_vectors), first_vector * kE - lead, ctas, rank, lane, warp};
-
-  // settings of the row, read while its values are on their way
-  const int each = me.warp_vectors(), end = min(me.vectors, (warp + 1) * each);
-  for (int v = warp * each + lane; v < end; v += 32)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + v)), "l"(source + first_vector + v) : "memory");
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  float temperature = p.temperature ? p.temperature[row] : 1.0f;
-  int top_k = p.top_k ? p.top_k[row] : 0;
-  float top_p = p.top_p ? p.top_p[row] : 1.0f, floor = p.min_p ? p.min_p[row] : 0.0f;
-  const double u = fmin(fmax(static_cast<double>(p.uniforms[row]), 0.0), 1.0 - 0x1p-24);  // (not a number: zero)
-  asm volatile("cp.async.wait_all;" ::: "memory");
-
-  // ---- the largest value, the lowest index that has it, and the levels
-  float highest = -INFINITY;
-  for (int v = warp * each + lane; v < end; v += 32) {
-    const int at = me.begin_index + v * kE;
-    if (at < 0 || at + kE > p.vocabulary) {
-      T values[kE];
-      memcpy(values, held + v, 16);
-#pragma unroll
-      for (int i = 0; i < kE; ++i)
-        if (at + i < 0 || at + i >= p.vocabulary) values[i] = static_cast<T>(-INFINITY);
-      memcpy(held + v, values, 16);
-    }
-    me.one_vector(v, [&](float x, int) { highest = fmaxf(highest, x); });  // (of a number and none, the number)
-  }
-  const uint32_t key = order_of(highest);
+  // ---- the largest value, and the levels
   {
+    const uint32_t key = order_of(largest_value<T, kThreads>());
     uint32_t group = key, levels[5];
     levels[0] = __reduce_min_sync(0xffffffffu, group);
 #pragma unroll
@@ -757,13 +1282,12 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     }
   }
   __syncthreads();
-  if (warp != 0 && ctas > 1) cluster_wait();
+  if (ctas > 1) cluster_wait();
   if (warp == 0) {
     const bool mine = lane < kWarps;
     uint32_t out[16];
     uint32_t group = mine ? sh.warp_key[lane] : 0;
-    const uint32_t most = __reduce_max_sync(0xffffffffu, group);
-    out[0] = most;
+    out[0] = __reduce_max_sync(0xffffffffu, group);
     out[1] = 0;
 #pragma unroll
     for (int l = 0; l < 5; ++l) out[2 + l] = __reduce_min_sync(0xffffffffu, mine ? sh.warp_levels[lane][l] : 0xffffffffu);
@@ -776,14 +1300,13 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     out[13] = static_cast<uint32_t>(top_k);
     out[14] = __float_as_uint(top_p);
     out[15] = __float_as_uint(floor);
-    if (ctas > 1) cluster_wait();
     if (lane < ctas) {
       const uint32_t peer = cluster_map_shared(smem_u32(&sh.first[rank][0]), lane);
 #pragma unroll
       for (int i = 0; i < 4; ++i) cluster_store_uint4(peer + 16 * i, make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]));
     }
   }
-  me.cluster_barrier();
+  cluster_barrier<kThreads>();
 
   // The first CTA's settings are those of all: what CTAs meet at barriers by has to be the same in each, whatever another stream writes.
   const uint4 settings = sh.first[0][3];
@@ -792,14 +1315,20 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   top_p = __uint_as_float(settings.z);
   floor = __uint_as_float(settings.w);
   const bool sampled = temperature > 0.0f;
-  const double min_p = floor > 0.0f ? fmin(static_cast<double>(floor), 1.0) : 0.0;
-  const bool by_count = sampled && top_k > 0 && top_k < p.vocabulary, by_sum = sampled && top_p < 1.0f, by_floor = sampled && min_p > 0.0;
+  Rules rules;
+  rules.top_k = top_k;
+  rules.by_count = sampled && top_k > 0 && top_k < p.vocabulary;
+  rules.by_sum = sampled && top_p < 1.0f;
+  rules.by_floor = sampled && floor > 0.0f;
+  rules.top_p = static_cast<double>(top_p);
+  rules.min_p = rules.by_floor ? fmin(static_cast<double>(floor), 1.0) : 0.0;
+  rules.u = fmin(fmax(static_cast<double>(uniform), 0.0), 1.0 - 0x1p-24);  // (not a number: zero)
 
-  uint32_t largest = kNothing, lower = kNothing + 1;  // at least top_k values are not below `lower`
+  uint32_t largest, lower = kNothing + 1;  // at least top_k values are not below `lower`
   {
     const uint32_t* entry = reinterpret_cast<const uint32_t*>(&sh.first[lane < ctas ? lane : 0][0]);
     largest = __reduce_max_sync(0xffffffffu, entry[0]);
-    if (by_count) {
+    if (rules.by_count) {
       int level = -1;
       for (int l = 0; l < kLevels && (1 << l) <= kThreads; ++l)
         if ((ctas * kThreads >> l) >= top_k) level = l;
@@ -807,8 +1336,8 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
     }
   }
   const auto answer = [&](int token, float probability) {
-    p.tokens[row] = token;
-    if (p.probabilities) p.probabilities[row] = probability;
+    p.tokens[at_row] = token;
+    if (p.probabilities) p.probabilities[at_row] = probability;
   };
   if (largest <= kNothing) {  // nothing to take
     if (rank == 0 && thread == 0) answer(-1, 0.0f);
@@ -816,186 +1345,188 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) sample_kernel(const
   }
   const float most = value_of(largest);
   if (!sampled) {  // the best: the lowest index that has it, of the first CTA that has one
-    uint32_t index = 0xffffffffu;
-    me.each_value([&](float x, int i) {
-      if (x == most) index = min(index, static_cast<uint32_t>(i));
-    });
-    index = __reduce_min_sync(0xffffffffu, index);
+    bool before = false;
+    for (int r = 0; r < rank; ++r) before |= sh.first[r][0].x == largest;
+    if (before || sh.first[rank][0].x != largest) return;
+    uint32_t index = __reduce_min_sync(0xffffffffu, first_index_of<T, kThreads>(most));
     if (lane == 0) sh.warp_index[warp] = index;
     __syncthreads();
     if (thread < kWarps) index = sh.warp_index[thread];
     if (warp == 0) index = __reduce_min_sync(0xffffffffu, index);
-    bool before = false;
-    for (int r = 0; r < rank; ++r) before |= sh.first[r][0].x == largest;
-    if (!before && thread == 0 && index != 0xffffffffu) answer(static_cast<int>(index), 1.0f);
+    if (thread == 0) answer(static_cast<int>(index), 1.0f);
     return;
   }
-  const double degrees = static_cast<double>(temperature);
-  me.cap = p.softcap;
-  me.scale = 1.4426950408889634074 * kExp2Entries / degrees;
-  me.top = p.softcap > 0.0f ? softened(most, me.cap) : static_cast<double>(most);
-  me.scale32 = static_cast<float>(me.scale);
-  me.top32 = most;
-  me.cut = fmaxf(__double2float_rd(static_cast<double>(most) - kShareOctaves * 0.69314718055994530942 * degrees), -3.402823466e38f);
-  // (sizes at which 32 bits hold the whole part of every share that there is)
-  const bool ordinary = fabsf(most) < 1e30f && me.cut > -1e30f && temperature > 1e-30f && temperature < 1e30f;
-  me.form = p.softcap > 0.0f ? kCapped : ordinary ? kPlain : kAny;
+  const bool capped = p.softcap > 0.0f;
+  // (the scale of a capped row's shares is a number of 32 bits too: below this temperature there are no shares but the largest's)
+  const double degrees = capped ? fmax(static_cast<double>(temperature), 1e-30) : static_cast<double>(temperature);
+  if (thread == 0) {
+    RowState& row = sh.row;
+    constexpr double octave = 1.4426950408889634074 * kExp2Entries;
+    if (capped) {
+      const double rate = 2.0 * octave / p.softcap;
+      row.cap = Cap{p.softcap, rate, static_cast<float>(rate), 24.0f * p.softcap};  // (2^-69 of one)
+    }
+    row.scale = octave / degrees;
+    row.top = capped ? softened(most, row.cap, sh.table) : static_cast<double>(most);
+    row.scale32 = static_cast<float>(row.scale);
+    row.top32 = most;
+    row.cut = fmaxf(__double2float_rd(static_cast<double>(most) - kShareOctaves * 0.69314718055994530942 * degrees), -3.402823466e38f);
+    // (sizes at which 32 bits hold the whole part of every share that there is)
+    const bool ordinary = fabsf(most) < 1e30f && row.cut > -1e30f && temperature > 1e-30f && temperature < 1e30f;
+    row.form = capped ? kCapped : ordinary ? kPlain : kAny;
+  }
+  __syncthreads();
 
-  // The list has all that may be kept, inside the border: sorted by rank it is cut, sorted by index it is walked over.
-  const auto finish = [&](int count, bool summed, double whole_sum) {
-    sort_list<kThreads>(sh.list, count);
-    const int ranks = by_count ? min(count, top_k) : count;
-    double w[4], upto[4], in_front;
-    unsigned long long entries[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * thread + j;
-      entries[j] = i < ranks ? sh.list[i] : ~0ull;
-      w[j] = i < ranks ? me.share(R::ranked_value(entries[j])) : 0.0;
-    }
-    const double sum = me.list_upto(w, upto, in_front);
-    const double target = static_cast<double>(top_p) * (summed ? whole_sum : sum);
-    int kept = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * thread + j;
-      const bool stays = i < ranks && (i == 0 || !by_sum || (j == 0 ? in_front : upto[j - 1]) < target) && !(by_floor && w[j] < min_p);
-      kept += __syncthreads_count(stays);
-      // by index now, with the order behind it
-      sh.list[i] = stays ? entries[j] << 32 | entries[j] >> 32 : ~0ull;
-    }
-    __syncthreads();
-    sort_list<kThreads>(sh.list, count);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = 4 * thread + j;
-      entries[j] = i < kept ? sh.list[i] : ~0ull;
-      w[j] = i < kept ? me.share(value_of(~static_cast<uint32_t>(entries[j]))) : 0.0;
-    }
-    if (thread == 0) sh.found = kept - 1;
-    const double all = me.list_upto(w, upto, in_front);
-#pragma unroll
-    for (int j = 3; j >= 0; --j)
-      if (4 * thread + j < kept && upto[j] > u * all) atomicMin(&sh.found, 4 * thread + j);
-    __syncthreads();
-    const int found = sh.found;
-    if (found >> 2 == thread) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if ((found & 3) == j) answer(static_cast<int>(entries[j] >> 32), static_cast<float>(w[j] / all));
-    }
-  };
   // Where the list may have all that may be kept: from which order on.  Up to kCap / 8 groups give some kCap / 8 * ln(kCap / 8) candidates,
   // which a list holds; of more groups it would not.
   uint32_t from = 0;
-  if (p.vocabulary <= kCap && (by_count || by_sum)) {
+  if (p.vocabulary <= kCap && (rules.by_count || rules.by_sum)) {
     from = kNothing + 1;
-  } else if (by_count) {
+  } else if (rules.by_count) {
     if (top_k <= kCap / 8) from = lower;
-  } else if (by_floor && !by_sum) {
+  } else if (rules.by_floor && !rules.by_sum) {
     // Nothing further below the largest than this has a share of min_p; capped values: above where the cap's inverse is.
-    double y = me.top + degrees * log(min_p);
-    if (me.form == kCapped) {
-      const double z = y / me.cap - 1e-12;
-      y = z > -1.0 ? me.cap * 0.5 * log((1.0 + z) / fmax(1.0 - z, 1e-30)) : -INFINITY;
+    double y = sh.row.top + degrees * log(rules.min_p);
+    if (capped) {
+      const double z = y / p.softcap - 1e-12;
+      y = z > -1.0 ? p.softcap * 0.5 * log((1.0 + z) / fmax(1.0 - z, 1e-30)) : -INFINITY;
     }
     y -= 1e-6 * (fabs(y) + fabs(static_cast<double>(most)));
     const float bound = y > static_cast<double>(most) ? most : __double2float_rd(y);
     from = bound == bound ? max(order_of(bound), kNothing + 1) : kNothing + 1;
   }
+  int which = 0;  // of the slots that the next exchange takes
   int listed = -1;  // entries of a list that has all
-  bool summed = false;
-  double whole_sum = 0.0;
+  double whole_sum = -1.0;
   if (from != 0) {
-    const int count = me.gather(from, largest, [](float) {});
+    const int count = gather<T, kThreads>(from, largest, most, false, false, false, which).count;
+    which ^= 1;
     if (count <= kCap) listed = count;
   }
-  double above_mine = 0.0;  // this lane's part of the sum above the border's window
+  const auto part = Walk<T, kThreads>::mine();
+  double above_mine = 0.0;  // this lane's part of the sum above what `window_high` names
   uint32_t window_high = 0;
   bool begun = false;
 #pragma unroll 1
   for (int rule = 0; rule < 2 && listed < 0; ++rule) {  // top_k, then top_p
-    if (rule == 0 ? !by_count : !by_sum) continue;
+    if (rule == 0 ? !rules.by_count : !rules.by_sum) continue;
     const bool shares = rule == 1;
-    double sum = 0.0, target = top_k;
-    bool done = false;
-    if (me.form != kAny) {
-      me.count_bins(shares, sum);
-      if (shares) target = static_cast<double>(top_p) * sum;
-      const BinWindow window = me.window_of_bins(shares, target);
-      if (window.count > 0) {
-        const uint32_t low = max(me.order_with(window.last, largest), me.border_key);
-        const uint32_t high = window.first > 0 ? order_below(me.order_with(window.first - 1, largest)) : largest;
-        double v[1] = {0.0};
-        const int count = me.gather(low, high, [&](float x) { v[0] += shares ? me.share(x) : 1.0; });
-        if (window.whole && count <= kCap) {
-          listed = count;
-          summed = shares;
-          whole_sum = sum;
+    // Counts: from the bound that the groups gave.  Shares: those from 2^-35 of the largest on; where the border is further down, halving finds it.
+    const uint32_t border_key = sh.row.border_key;
+    const uint32_t near = max(order_of(__double2float_rd(static_cast<double>(most) - 24.0 * degrees)), border_key);
+    uint32_t low = min(shares || value_of(lower) < -1e30f ? near : lower, largest), high = largest;
+    uint32_t sure_low = border_key, sure_high = largest;  // the border lies between these
+    double target = top_k, above = 0.0, all = 0.0;
+    float seen = most;  // what is above has been measured
+    bool done = false, known = !shares;  // (whether the target is)
+    above_mine = 0.0;
+#pragma unroll 1
+    for (int turn = 0; turn < 5; ++turn) {
+      const Bins bins = bins_between(value_of(low), value_of(high));
+      if (turn == 0) {
+        clear_bins<kThreads>();
+        const float sum = look<T, kThreads>(bins, shares);
+        all = cluster_sums<kThreads>(sum, 0.0, 0.0, which).a;
+        which ^= 1;
+        if (shares) target = rules.top_p * all;
+      }
+      // (half a bin, and what 32 bits lose of it)
+      const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
+      const double off = shares ? (0.505 / (kBins - 1) * (static_cast<double>(bins.high) - bins.low) + 0x1p-22 * size) / degrees + 1e-4 : 0.0;
+      const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, turn);
+      if (window.says == kNotHere || low == high) break;
+      if (window.says == kInList || window.says == kListHasAll) {
+        const uint32_t next_low = order_with(bins, window.last, low, high);
+        const uint32_t next_high = window.first > 0 ? order_below(order_with(bins, window.first - 1, low, high)) : high;
+        const bool has_all = window.says == kListHasAll;
+        const Gathered got = gather<T, kThreads>(next_low, next_high, seen, !has_all, shares, !known, which);
+        which ^= 1;
+        const Three sums = cluster_sums<kThreads>(got.sifted.above, got.sifted.all, 0.0, which);
+        which ^= 1;
+        if (!known) {
+          all = sums.b;
+          target = rules.top_p * all;
+          known = true;
+        }
+        if (has_all && got.count <= kCap) {
+          listed = got.count;
+          whole_sum = shares ? all : -1.0;
           break;
         }
-        above_mine = v[0];
-        me.cluster_sums(v);
-        done = count > 0 && count <= kCap && me.border_from_list(count, shares, v[0], target, false);
-        if (done && shares) {
-          begun = !by_floor;
-          window_high = high;
+        done = got.count > 0 && got.count <= kCap && border_from_list<kThreads>(got.count, shares, above + sums.a, target, false);
+        if (done) {
+          if (shares) {
+            begun = !rules.by_floor;
+            above_mine += got.sifted.above;
+            window_high = next_high;
+          }
+          break;
         }
       }
-    } else if (shares) {
-      double v[1] = {0.0};
-      me.each_value([&](float x, int i) { v[0] += me.inside(x, i) ? me.share(x) : 0.0; });
-      me.cluster_sums(v);
-      target = static_cast<double>(top_p) * v[0];
+      // Closer.
+      const uint32_t next_low = order_with(bins, window.sure_last, low, high);
+      const uint32_t next_high = window.sure_first > 0 ? order_below(order_with(bins, window.sure_first - 1, low, high)) : high;
+      if (next_low == low && next_high == high) break;
+      const Bins closer = bins_between(value_of(next_low), value_of(next_high));
+      clear_bins<kThreads>();
+      const Sifted sifted = sift_row<T, kThreads>(true, closer.low, closer.high, seen, true, shares, !known, closer);
+      const Three sums = cluster_sums<kThreads>(sifted.above, sifted.all, 0.0, which);
+      which ^= 1;
+      above_mine += sifted.above;
+      above += sums.a;
+      if (!known) {
+        all = sums.b;
+        target = rules.top_p * all;
+        known = true;
+      }
+      seen = closer.high;
+      sure_low = low = next_low;
+      sure_high = high = next_high;
     }
-    if (!done) me.find_border(shares, target, me.border_key, largest);
+    if (!done && listed < 0) {
+      if (!known) {
+        const double mine = sum_shares<T, kThreads>(part.begin, part.end, 0.0);
+        target = rules.top_p * cluster_sums<kThreads>(mine, 0.0, 0.0, which).a;
+        which ^= 1;
+      }
+      which = find_border<T, kThreads>(shares, target, sure_low, sure_high, above, which);
+    }
   }
   if (listed >= 0) {
-    if (rank == 0) finish(listed, summed, whole_sum);
+    if (rank == 0) {
+      const Taken taken = finish<kThreads>(listed, whole_sum, rules, most);
+      if (taken.index >= 0) answer(taken.index, taken.probability);
+    }
     return;
   }
-  // The kept shares in the order of the vocabulary.
-  const auto kept_share = [&](float x, int i) {
-    if (!me.inside(x, i)) return 0.0;
-    const double w = me.share(x);
-    return by_floor && w < min_p ? 0.0 : w;
-  };
-  const auto target_of = [&](double all) { return u * all; };
-  const auto found = [&](float, int i, double w, double all) { answer(i, static_cast<float>(w / all)); };
-  if (begun) {  // what is above the window has been summed
-    const float upto = value_of(window_high), from = value_of(me.border_key);
-    me.locate(above_mine, [&](float x, int i) { return x >= from && x <= upto && me.inside(x, i) ? me.share(x) : 0.0; }, kept_share, target_of, found);
-  } else if (me.form == kPlain && !me.bounded && !by_floor) {
-    const float from = me.cut;
-    me.locate(
-        0.0,
-        [&](float x, int) {
-          const double w = me.plain_share(x, me.plain_whole(x));
-          return x >= from ? w : 0.0;
-        },
-        kept_share, target_of, found);
-  } else {
-    me.locate(0.0, kept_share, kept_share, target_of, found);
-  }
+  // The kept shares in the order of the vocabulary; what is above the border's window has been summed.
+  const double least = rules.by_floor ? rules.min_p : 0.0;
+  const double mine = begun ? above_mine + sum_few<T, kThreads>(part.begin, part.end, sh.row.border, value_of(window_high), false)
+                            : sum_shares<T, kThreads>(part.begin, part.end, least);
+  const Located it = locate<T, kThreads>(mine, false, 0.0f, least, rules.u, which);
+  if (it.index >= 0) answer(it.index, static_cast<float>(it.weight / it.all));
 }
 
 template <typename T, int kThreads>
 cudaError_t launch_threads(const SampleCall& call, int ctas, cudaStream_t stream) {
   constexpr int kE = Vector<T>::kValues;
   SampleParams p{call, ctas, 0};
-  p.cta_vectors = (call.vocabulary + 2 * (kE - 1) + kE * ctas - 1) / (kE * ctas);  // (with the lead at its largest)
+  // As many vectors for each warp (with the lead at its largest, where rows do not begin at a 16-byte boundary).
+  const bool whole = (reinterpret_cast<uintptr_t>(call.logits) & 15) == 0 && (call.row_stride * sizeof(T) & 15) == 0;
+  const int vectors = (call.vocabulary + (whole ? 0 : kE - 1) + kE - 1) / kE, warps = ctas * (kThreads / 32);
+  p.cta_vectors = (vectors + warps - 1) / warps * (kThreads / 32);
   return launch_chained_clusters(sample_kernel<T, kThreads>, ctas, dim3(static_cast<unsigned>(call.rows) * ctas), dim3(kThreads),
-                                 16 * static_cast<size_t>(p.cta_vectors), stream, p);
+                                 sizeof(SampleShared<kThreads>), stream, p);
 }
 
 template <typename T>
 cudaError_t launch_type(const SampleCall& call, int sm_count, cudaStream_t stream) {
   const long long bytes = static_cast<long long>(call.vocabulary) * sizeof(T);
   if (bytes <= 4096) return launch_threads<T, 128>(call, 1, stream);
-  // As many CTAs as a row needs for 64 KB each, two of which an SM holds with their lists; more where rows are few, down to 8 KB each.
+  // Two CTAs an SM hold as many rows as there are; where there are fewer, as many CTAs a row as that leaves, down to 8 KB each.
   int ctas = 1;
-  while (ctas < kMostCtas && (bytes > 65536ll * ctas || (bytes > 16384ll * ctas && 2ll * ctas * call.rows <= 2 * sm_count))) ctas *= 2;
-  return launch_threads<T, 512>(call, ctas, stream);
+  while (ctas < kMostCtas && 2ll * ctas * call.rows <= 2 * sm_count && bytes > 16384ll * ctas) ctas *= 2;
+  return launch_threads<T, 256>(call, ctas, stream);
 }
 
 }  // namespace
