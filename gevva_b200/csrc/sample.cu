@@ -27,6 +27,7 @@ constexpr int kMostCtas = 16;
 constexpr int kLevels = 10;       // groups of 2^level threads
 constexpr int kSums = 3;
 constexpr int kBins = 1024;       // of equal width over a range of values
+constexpr int kAhead = 8;         // vectors that a thread has on their way: an L2 read takes as long as a warp works on these
 constexpr int kTableCopies = 16;  // of the table of 2^(j/32), one for each lane of half a warp: no two lanes of a read meet in a bank
 
 struct SampleParams {
@@ -78,6 +79,7 @@ struct SampleShared {
   static constexpr int kCap = kEach * kThreads;
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kFew = 128;
+  uint4 ring[kWarps][kAhead][32];  // vectors on their way, of each lane its own
   RowState row;
   double few[kFew];
   double table[kExp2Entries * kTableCopies];
@@ -340,31 +342,41 @@ struct Walk {
 #pragma unroll
     for (int i = 0; i < kE; ++i) f(x[i], index_of(v) + i);
   }
-  // f(values, the first vector's number): value i is of vector + 32 * (i / kE).  The next values are on their way meanwhile.
+  // f(values, the first vector's number): value i is of vector + 32 * (i / kE).  The next values are on their way meanwhile, by asynchronous copies
+  // that a lane waits for and reads itself.
   template <class F>
   __device__ __forceinline__ void each_eight(F&& f) const {
+    constexpr int kDepth = kAhead / kGroup;
     const int lane = threadIdx.x & 31;
-    uint4 next[2][kGroup];
+    uint4* const ring = &shared<kThreads>().ring[threadIdx.x >> 5][0][lane];
+    const uint32_t to = smem_u32(ring);
+    const auto ask = [&](int at, int slot) {
+      if (at < end) {
 #pragma unroll
-    for (int d = 0; d < 2; ++d)
+        for (int g = 0; g < kGroup; ++g)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + 512 * (slot * kGroup + g)), "l"(source + min(at + lane + 32 * g, last)) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
 #pragma unroll
-      for (int g = 0; g < kGroup; ++g) next[d][g] = source[min(begin + lane + 32 * (kGroup * d + g), last)];
+    for (int d = 0; d < kDepth; ++d) ask(begin + 32 * kGroup * d, d);
+    int slot = 0;
 #pragma unroll 1
     for (int at = begin; at < end; at += 32 * kGroup) {
       const int v = at + lane;
       float x[8];
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
 #pragma unroll
-      for (int g = 0; g < kGroup; ++g) {
-        Vector<T>::unpack(next[0][g], x + g * kE);
-        next[0][g] = next[1][g];
-        next[1][g] = source[min(v + 32 * (2 * kGroup + g), last)];
-      }
+      for (int g = 0; g < kGroup; ++g) Vector<T>::unpack(ring[32 * (slot * kGroup + g)], x + g * kE);
       if (at == 0 || at + 32 * kGroup >= end) {  // (the ends; the same for the whole warp)
 #pragma unroll
         for (int g = 0; g < kGroup; ++g) mask(v + 32 * g, x + g * kE);
       }
       f(x, v);
+      ask(at + 32 * kGroup * kDepth, slot);  // (its values have been read: they have been worked on)
+      slot = (slot + 1) & (kDepth - 1);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __device__ __forceinline__ int index_in(int v, int i) const { return index_of(v + 32 * (i / kE)) + i % kE; }
 };
@@ -414,32 +426,13 @@ __device__ __noinline__ Three cluster_sums(double a, double b, double c, int whi
 
 template <typename T, int kThreads>
 __device__ __noinline__ float largest_value() {
-  // (from HBM: eight vectors of a thread on their way)
-  using W = Walk<T, kThreads>;
-  const auto walk = W::mine();
-  constexpr int kAhead = 8;
-  float most[kAhead];
-#pragma unroll
-  for (int g = 0; g < kAhead; ++g) most[g] = -INFINITY;
-#pragma unroll 1
-  for (int at = walk.begin; at < walk.end; at += 32 * kAhead) {
-    uint4 vectors[kAhead];
-    const int v = at + (threadIdx.x & 31);
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) vectors[g] = walk.source[min(v + 32 * g, walk.last)];
-    const bool ends = at == 0 || at + 32 * kAhead >= walk.end;
-#pragma unroll
-    for (int g = 0; g < kAhead; ++g) {
-      float x[W::kE];
-      Vector<T>::unpack(vectors[g], x);
-      if (ends) walk.mask(v + 32 * g, x);
-#pragma unroll
-      for (int i = 0; i < W::kE; ++i) most[g] = fmaxf(most[g], x[i]);  // (of a number and none, the number)
-    }
-  }
-#pragma unroll
-  for (int g = 1; g < kAhead; ++g) most[0] = fmaxf(most[0], most[g]);
-  return most[0];
+  const auto walk = Walk<T, kThreads>::mine();
+  float a = -INFINITY, b = -INFINITY;
+  walk.each_eight([&](const float (&x)[8], int) {  // (fmaxf of a number and none is the number)
+    a = fmaxf(fmaxf(a, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+    b = fmaxf(fmaxf(b, fmaxf(x[4], x[5])), fmaxf(x[6], x[7]));
+  });
+  return fmaxf(a, b);
 }
 
 template <typename T, int kThreads>
@@ -562,11 +555,16 @@ __device__ __noinline__ Sifted sift(bool binned, float low, float high, float be
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) ? eight.w[i] : 0.0;
       }
-      double up[8];
+      // (what is above, and what is not)
+      double up[2] = {0.0, 0.0}, rest[2] = {0.0, 0.0};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) up[i] = higher >> i & 1 ? w[i] : 0.0;
-      sifted.above += ((up[0] + up[1]) + (up[2] + up[3])) + ((up[4] + up[5]) + (up[6] + up[7]));
-      sifted.all += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      for (int i = 0; i < 8; ++i) {
+        if (higher >> i & 1) up[i & 1] += w[i];
+        else rest[i & 1] += w[i];
+      }
+      const double over = up[0] + up[1];
+      sifted.above += over;
+      sifted.all += over + (rest[0] + rest[1]);
     }
     if (measured && !shares) sifted.above += __popc(higher);
     if (binned) {
