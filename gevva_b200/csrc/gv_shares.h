@@ -52,7 +52,7 @@ GV_SHARES_HD double exp2_rest_finely(double f) {
 }
 // value * 2^floor(n / 32), for n by its low bits (any multiple of 2^17 more is the same), where that is a normal number.
 GV_SHARES_HD double scaled_by(double value, uint32_t n) {
-  const uint32_t exponent = n << 15 & 0xfff00000u;
+  const uint32_t exponent = (n >> 5) * (1u << 20);
 #ifdef __CUDA_ARCH__
   return __hiloint2double(__double2hiint(value) + static_cast<int>(exponent), __double2loint(value));
 #else

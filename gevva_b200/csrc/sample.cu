@@ -69,6 +69,7 @@ struct RowState {
   uint32_t border_key, border_index;
   float border;         // border_key's
   float scale32, top32, cut;  // kPlain: values below `cut` have no share
+  float largest;
   double scale, top;    // of y
   Cap cap;
 };
@@ -80,9 +81,9 @@ struct SampleShared {
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kFew = 128;
   uint4 ring[kWarps][kAhead][32];  // vectors on their way, of each lane its own
+  double table[kExp2Entries * kTableCopies];
   RowState row;
   double few[kFew];
-  double table[kExp2Entries * kTableCopies];
   union {
     unsigned long long mine[kCap];   // candidates of this CTA
     int4 bins4[kBins / 4];
@@ -97,10 +98,10 @@ struct SampleShared {
   double slots[2][kMostCtas][kSums];
   double warp_sums[kWarps][kSums];
   uint4 window[2];                 // a BinWindow, from the first CTA, by turns
-  unsigned long long border;       // from the first CTA
+  unsigned long long border, kept; // from the first CTA: the border's entry, and how many of the list are up to it
   uint32_t warp_key[kWarps], warp_index[kWarps], warp_levels[kWarps][5];
   int mine_count, list_count, base, found;
-  int edges[4];
+  int edges[6];
 };
 extern __shared__ uint4 sample_memory[];
 template <int kThreads>
@@ -117,6 +118,11 @@ __device__ __forceinline__ void cluster_store_u64(uint32_t address, unsigned lon
 __device__ __forceinline__ int4 cluster_load4(uint32_t address) {
   int4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ unsigned long long cluster_load_u64(uint32_t address) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(address) : "memory");
   return v;
 }
 __device__ __forceinline__ int cluster_add(uint32_t address, int v) {
@@ -234,20 +240,38 @@ __device__ __forceinline__ double capped_share(float x, double scale, float scal
   const double share = share_with(distance, scale, share_whole(distance32, scale32), table, kTableCopies);
   return distance32 * scale32 > -kShareOctaves * kExp2Entries ? share : 0.0;
 }
-__device__ __forceinline__ double plain_share(float x, double scale, float scale32, double top, float top32, const double* table) {
-  return share_with(static_cast<double>(x) - top, scale, share_whole(x - top32, scale32), table, kTableCopies);
-}
 template <int kThreads>
 __device__ __forceinline__ const double* lane_table() {
   return shared<kThreads>().table + (threadIdx.x & (kTableCopies - 1));
 }
+
+// Shares of the plain form.  Values below `cut`, and what is no number, have the share of `cut`, 2^-200: a sum does not notice it, and a comparison
+// and a choice for each value are saved (comparisons, choices and logic run at half the rate of the rest, and bound a pass).
+struct PlainShares {
+  double scale, top;
+  float scale32, top32, cut;
+  uint32_t table;  // address of this lane's copy
+  template <int kThreads>
+  static __device__ __forceinline__ PlainShares of() {
+    const RowState& row = shared<kThreads>().row;
+    return {row.scale, row.top, row.scale32, row.top32, row.cut, smem_u32(lane_table<kThreads>())};
+  }
+  __device__ __forceinline__ double operator()(float value) const {
+    const float x = fmaxf(value, cut);
+    const uint32_t n = share_whole(x - top32, scale32);
+    double entry;
+    asm("ld.shared.f64 %0, [%1];" : "=d"(entry) : "r"((n & (kExp2Entries - 1)) * (8 * kTableCopies) + table));
+    const double whole = __hiloint2double(0x43300000, static_cast<int>(n)) - (0x1p52 + kShareWhole);
+    return scaled_by(exp2_rest(__fma_rn(static_cast<double>(x) - top, scale, -whole)) * entry, n);
+  }
+};
 
 // The share of any value that may be taken.
 template <int kThreads>
 __device__ __noinline__ double share(float x) {
   const RowState& row = shared<kThreads>().row;
   const double* table = lane_table<kThreads>();
-  if (row.form == kPlain) return x >= row.cut ? plain_share(x, row.scale, row.scale32, row.top, row.top32, table) : 0.0;
+  if (row.form == kPlain) return x >= row.cut ? PlainShares::of<kThreads>()(x) : 0.0;
   if (row.form == kCapped) return capped_share(x, row.scale, row.scale32, row.top, row.cap, table);
   if (isinf(x)) return 1.0;  // (the largest value is infinite then, and so is this one)
   return isinf(row.top) ? 0.0 : share_of(static_cast<double>(x) - row.top, row.scale, table, kTableCopies);
@@ -447,7 +471,8 @@ __device__ __noinline__ uint32_t first_index_of(float value) {
 }
 
 // (the whole number stands in the low bits; of ranges without an extent it means nothing: sums tell whether the border is where counts say)
-__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return (share_whole(bins.high - x, bins.per) - kShareWhole) & (kBins - 1); }
+__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return share_whole(bins.high - x, bins.per) & (kBins - 1); }
+static_assert(kShareWhole % kBins == 0, "the bits behind a whole number");
 __device__ __forceinline__ Bins bins_between(float low, float high) { return {low, high, static_cast<float>(kBins - 1) / (high - low)}; }
 
 template <int kThreads>
@@ -509,9 +534,8 @@ __device__ __noinline__ Sifted sift(bool binned, float low, float high, float be
   constexpr int kE = Walk<T, kThreads>::kE, kGroup = Walk<T, kThreads>::kGroup;
   const Border border = border_of(sh.row);
   const int nothing = kBins + (threadIdx.x & 31);
-  const double scale = sh.row.scale, top = sh.row.top;
-  const float scale32 = sh.row.scale32, top32 = sh.row.top32, cut = sh.row.cut;
-  const double* table = lane_table<kThreads>();
+  const PlainShares plain_share = PlainShares::of<kThreads>();
+  const bool all_before = before >= sh.row.largest;
   Sifted sifted{0.0, 0.0};
   // Hits are a few of thousands: which values they are is noted in bits, and they are put on the list behind some rounds of the loop together.
   unsigned long long noted = 0;
@@ -529,44 +553,63 @@ __device__ __noinline__ Sifted sift(bool binned, float low, float high, float be
     }
   };
   walk.each_eight([&](const float (&x)[8], int v) {
-    uint32_t hits = 0, higher = 0;
+    // (most often nothing is between `low` and `high`: bits only where something is)
+    bool any = false, over[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      bool in = (x[i] >= low) & (x[i] <= before);  // (no branches: eight values side by side)
-      if (kGeneral) in &= border.inside(x[i], walk.index_in(v, i));
-      const bool up = x[i] > high;
-      hits |= in & !up ? 1u << i : 0u;
-      higher |= in & up ? 1u << i : 0u;
+      over[i] = x[i] > high;
+      any |= (x[i] >= low) & !over[i];
     }
-    if (whole || (measured && shares && higher != 0)) {
-      double w[8];
-      if (!kGeneral) {
+    if (!all_before) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
-      } else if (sh.row.form == kPlain) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = (x[i] >= cut) & border.inside(x[i], walk.index_in(v, i)) ? w[i] : 0.0;
-      } else {
-        const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) ? eight.w[i] : 0.0;
-      }
-      // (what is above, and what is not)
-      double up[2] = {0.0, 0.0}, rest[2] = {0.0, 0.0};
+      for (int i = 0; i < 8; ++i) over[i] &= x[i] <= before;
+    }
+    uint32_t hits = 0;
+    if (any || binned) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (higher >> i & 1) up[i & 1] += w[i];
-        else rest[i & 1] += w[i];
+        bool in = (x[i] >= low) & (x[i] <= high);
+        if (kGeneral) in &= border.inside(x[i], walk.index_in(v, i));
+        hits |= in ? 1u << i : 0u;
       }
-      const double over = up[0] + up[1];
-      sifted.above += over;
-      sifted.all += over + (rest[0] + rest[1]);
     }
-    if (measured && !shares) sifted.above += __popc(higher);
+    if (kGeneral) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) over[i] &= border.inside(x[i], walk.index_in(v, i));
+    }
+    if (whole || measured) {
+      bool higher = false;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) higher |= over[i];
+      if (!shares) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sifted.above += over[i] ? 1.0 : 0.0;
+      } else if (whole || higher) {
+        double w[8];
+        if (!kGeneral || sh.row.form == kPlain) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i]);
+        } else {
+          const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = eight.w[i];
+        }
+        if (kGeneral) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) ? w[i] : 0.0;
+        }
+        // (what is above, and what is not)
+        double up[2] = {0.0, 0.0}, rest[2] = {0.0, 0.0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (over[i]) up[i & 1] += w[i];
+          else rest[i & 1] += w[i];
+        }
+        const double above = up[0] + up[1];
+        sifted.above += above;
+        sifted.all += above + (rest[0] + rest[1]);
+      }
+    }
     if (binned) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) atomicAdd(&sh.bins[hits >> i & 1 ? bin_of(bins, x[i]) : nothing], 1);
@@ -594,18 +637,16 @@ template <typename T, int kThreads>
 __device__ __noinline__ double sum_shares(int begin, int end, double least) {
   SampleShared<kThreads>& sh = shared<kThreads>();
   const Walk<T, kThreads> walk(begin, end);
-  const double scale = sh.row.scale, top = sh.row.top;
-  const float scale32 = sh.row.scale32, top32 = sh.row.top32, cut = sh.row.cut;
-  const double* table = lane_table<kThreads>();
+  const PlainShares plain_share = PlainShares::of<kThreads>();
   const Border border = border_of(sh.row);
   double sum = 0.0;
   if (sh.row.form == kPlain && !sh.row.bounded && !(least > 0.0)) {  // the ordinary case by itself: a dozen instructions a value fewer
     walk.each_eight([&](const float (&x)[8], int) {
       double w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
+      for (int i = 0; i < 8; ++i) w[i] = x[i] >= plain_share.cut ? w[i] : 0.0;  // (none at all: a random number of zero finds the first that has some)
       sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     });
     return sum;
@@ -615,40 +656,54 @@ __device__ __noinline__ double sum_shares(int begin, int end, double least) {
     double w[8];
     if (plain) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i], scale, scale32, top, top32, table);
+      for (int i = 0; i < 8; ++i) w[i] = plain_share(x[i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = x[i] >= cut ? w[i] : 0.0;
+      for (int i = 0; i < 8; ++i) w[i] = x[i] >= plain_share.cut ? w[i] : 0.0;
     } else {
       const Eight eight = other_shares<kThreads>(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) w[i] = eight.w[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) & (w[i] >= least) ? w[i] : 0.0;
+    for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) & (w[i] >= least) & (x[i] > -INFINITY) ? w[i] : 0.0;
     sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   });
   return sum;
 }
 
-// The same of a few: those that are inside, from `low` to `high`.  Or (ties) how many these are.
+// How many of them are inside and equal to `value`.
 template <typename T, int kThreads>
-__device__ __noinline__ double sum_few(int begin, int end, float low, float high, bool ties) {
+__device__ __noinline__ double count_ties(int begin, int end, float value) {
   const Border border = border_of(shared<kThreads>().row);
   const Walk<T, kThreads> walk(begin, end);
-  double sum = 0.0;
+  int count = 0;
   walk.each_eight([&](const float (&x)[8], int v) {
-    uint32_t near = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) near |= (x[i] >= low) & (x[i] <= high) & border.inside(x[i], walk.index_in(v, i)) ? 1u << i : 0u;
-    if (ties) {
-      sum += __popc(near);
-      return;
-    }
-    if (near == 0) return;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (near >> i & 1) sum += share<kThreads>(x[i]);
+    for (int i = 0; i < 8; ++i) count += (x[i] == value) & border.inside(x[i], walk.index_in(v, i)) ? 1 : 0;
   });
+  return count;
+}
+
+// This lane's sum of the shares that the first CTA's list has up to the border, of values in this warp's part.
+template <typename T, int kThreads>
+__device__ __noinline__ double sum_listed() {
+  SampleShared<kThreads>& sh = shared<kThreads>();
+  const auto walk = Walk<T, kThreads>::mine();
+  const int kept = static_cast<int>(sh.kept), rank = sh.row.rank;
+  const unsigned long long* list = sh.list;
+  if (rank > 0) {  // (the first CTA waits for all at the next exchange)
+    list = sh.mine;
+    const uint32_t from = cluster_map_shared(smem_u32(sh.list), 0);
+    for (int i = threadIdx.x; i < kept; i += kThreads) sh.mine[i] = cluster_load_u64(from + 8 * i);
+    __syncthreads();
+  }
+  const int first = walk.index_of(walk.begin), behind = walk.index_of(walk.end);
+  double sum = 0.0;
+  for (int i = threadIdx.x & 31; i < kept; i += 32) {
+    const unsigned long long entry = list[i];
+    const int index = static_cast<int>(entry);
+    if (index >= first && index < behind) sum += share<kThreads>(ranked_value(entry));
+  }
   return sum;
 }
 
@@ -806,7 +861,10 @@ __device__ __noinline__ bool border_from_list(int count, bool shares, double abo
     int at = sh.found;
     if (surely && count > 0) at = min(at, count - 1);
     const unsigned long long entry = at < count ? sh.list[at] : 0;
-    if (threadIdx.x < sh.row.ctas) cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), threadIdx.x), entry);
+    if (threadIdx.x < sh.row.ctas) {
+      cluster_store_u64(cluster_map_shared(smem_u32(&sh.border), threadIdx.x), entry);
+      cluster_store_u64(cluster_map_shared(smem_u32(&sh.kept), threadIdx.x), at < count ? at + 1 : 0);
+    }
   }
   cluster_barrier<kThreads>();
   const unsigned long long entry = sh.border;
@@ -848,7 +906,7 @@ __device__ __noinline__ uint32_t order_with(Bins bins, int bin, uint32_t low, ui
 
 // Where the counts say that `target` is reached, with `above` in front of the bins.  Counts times the shares of their bins' middles are off by up to
 // `off` of themselves: the border lies between where they reach the target with that much more and with that much less.  Where
-// that is more than the list holds, it is looked at with a fiftieth of it (errors of many bins cancel; sums will tell), or closer.
+// that is more than the list holds, it is looked at with a quarter or a sixteenth of it (errors of many bins cancel; sums will tell), or closer.
 template <int kThreads>
 __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double above, double target, double off, int turn) {
   SampleShared<kThreads>& sh = shared<kThreads>();
@@ -910,7 +968,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       sh.warp_index[warp] = counts;
       sh.warp_key[warp] = __float_as_uint(masses);
     }
-    if (threadIdx.x < 4) sh.edges[threadIdx.x] = kBins;
+    if (threadIdx.x < 6) sh.edges[threadIdx.x] = kBins;
     __syncthreads();
     int count_upto = counts - counted;
     float mass_upto = masses - massed;
@@ -920,8 +978,8 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       mass_upto += w < warp ? __uint_as_float(sh.warp_key[w]) : 0.0f;
     }
     // the target for counts' sums, by each edge
-    const float rest = static_cast<float>(target - above), o = static_cast<float>(off), few = 0.02f * fminf(o, 1.0f);
-    const float edge[4] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY, rest / (1.0f + few), rest / (1.0f - few)};
+    const float rest = static_cast<float>(target - above), o = static_cast<float>(off), less = 0.25f * fminf(o, 1.0f), few = 0.06f * fminf(o, 1.0f);
+    const float edge[6] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY, rest / (1.0f + less), rest / (1.0f - less), rest / (1.0f + few), rest / (1.0f - few)};
     const double missing = target - above;
 #pragma unroll
     for (int i = 0; i < kOf; ++i) {
@@ -932,7 +990,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       mass_upto += mass[i];
       sh.bins[bin] = count_upto;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {  // (each edge is passed in one bin)
+      for (int e = 0; e < 6; ++e) {  // (each edge is passed in one bin)
         if (shares ? mass_upto >= edge[e] && (mass_before < edge[e] || bin == 0) : count_upto >= missing && (count_before < missing || bin == 0))
           atomicMin(&sh.edges[e], bin);
       }
@@ -951,6 +1009,10 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
         } else if (sh.edges[3] < kBins && upto(sh.edges[3]) - upto(sh.edges[2] - 1) <= kCap) {
           window.first = sh.edges[2];
           window.last = sh.edges[3];
+          window.says = kInList;
+        } else if (sh.edges[5] < kBins && upto(sh.edges[5]) - upto(sh.edges[4] - 1) <= kCap) {
+          window.first = sh.edges[4];
+          window.last = sh.edges[5];
           window.says = kInList;
         } else if (window.first > 0 || window.last < kBins - 1) {  // (else a closer look would see the same)
           window.says = kLookCloser;
@@ -1025,7 +1087,7 @@ __device__ __noinline__ Located locate(double mine, bool ties, float value, doub
   while (upto - from > 32) {
     const int piece = ((upto - from + kWarps - 1) / kWarps + 31) / 32 * 32;
     const int mine_from = from + warp * piece, mine_upto = min(upto, mine_from + piece);
-    const double own = warp_sum(ties ? sum_few<T, kThreads>(mine_from, mine_upto, value, value, true) : sum_shares<T, kThreads>(mine_from, mine_upto, least));
+    const double own = warp_sum(ties ? count_ties<T, kThreads>(mine_from, mine_upto, value) : sum_shares<T, kThreads>(mine_from, mine_upto, least));
     if (lane == 0) sh.warp_sums[warp][1] = own;
     __syncthreads();
     Part in_piece{-1, 0, reached, reached, reached};
@@ -1118,7 +1180,7 @@ __device__ __noinline__ int find_border(bool shares, double target, uint32_t low
   // More ties than the list holds: so many of them, in the order of the vocabulary.
   const float value = value_of(low);
   const auto part = Walk<T, kThreads>::mine();
-  const double mine = sum_few<T, kThreads>(part.begin, part.end, value, value, true);
+  const double mine = count_ties<T, kThreads>(part.begin, part.end, value);
   double ties = target - above;
   if (shares) ties /= share<kThreads>(value);
   const Located it = locate<T, kThreads>(mine, true, value, 0.0, ties, which);
@@ -1367,7 +1429,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     row.scale = octave / degrees;
     row.top = capped ? softened(most, row.cap, sh.table) : static_cast<double>(most);
     row.scale32 = static_cast<float>(row.scale);
-    row.top32 = most;
+    row.top32 = row.largest = most;
     row.cut = fmaxf(__double2float_rd(static_cast<double>(most) - kShareOctaves * 0.69314718055994530942 * degrees), -3.402823466e38f);
     // (sizes at which 32 bits hold the whole part of every share that there is)
     const bool ordinary = fabsf(most) < 1e30f && row.cut > -1e30f && temperature > 1e-30f && temperature < 1e30f;
@@ -1402,8 +1464,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     if (count <= kCap) listed = count;
   }
   const auto part = Walk<T, kThreads>::mine();
-  double above_mine = 0.0;  // this lane's part of the sum above what `window_high` names
-  uint32_t window_high = 0;
+  double above_mine = 0.0;  // this lane's part of the sum above what the list has
   bool begun = false;
 #pragma unroll 1
   for (int rule = 0; rule < 2 && listed < 0; ++rule) {  // top_k, then top_p
@@ -1456,7 +1517,6 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
           if (shares) {
             begun = !rules.by_floor;
             above_mine += got.sifted.above;
-            window_high = next_high;
           }
           break;
         }
@@ -1499,8 +1559,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   }
   // The kept shares in the order of the vocabulary; what is above the border's window has been summed.
   const double least = rules.by_floor ? rules.min_p : 0.0;
-  const double mine = begun ? above_mine + sum_few<T, kThreads>(part.begin, part.end, sh.row.border, value_of(window_high), false)
-                            : sum_shares<T, kThreads>(part.begin, part.end, least);
+  const double mine = begun ? above_mine + sum_listed<T, kThreads>() : sum_shares<T, kThreads>(part.begin, part.end, least);
   const Located it = locate<T, kThreads>(mine, false, 0.0f, least, rules.u, which);
   if (it.index >= 0) answer(it.index, static_cast<float>(it.weight / it.all));
 }
