@@ -481,6 +481,19 @@ __device__ __forceinline__ void clear_bins() {
   __syncthreads();
 }
 
+__device__ __forceinline__ float power_of_two(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// softened(), in 32 bits.
+__device__ __forceinline__ float capped_in_32_bits(float x, float cap, float rate) {
+  const float e = power_of_two(-fabsf(x) * rate);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return copysignf(cap * (1.0f - e) * r, x);
+}
+
 // Counts what is inside by bins; with `shares` also this lane's sum of shares, in 32 bits: where to look, no more.
 template <typename T, int kThreads>
 __device__ __noinline__ float look(Bins bins, bool shares) {
@@ -488,8 +501,10 @@ __device__ __noinline__ float look(Bins bins, bool shares) {
   const auto walk = Walk<T, kThreads>::mine();
   const Border border = border_of(sh.row);
   const int nothing = kBins + (threadIdx.x & 31);
-  const bool all = !sh.row.bounded, plain = sh.row.form == kPlain;
-  const float top32 = sh.row.top32, rate = sh.row.scale32 * (1.0f / kExp2Entries);
+  const bool all = !sh.row.bounded;
+  const ShareForm form = sh.row.form;
+  const float top32 = form == kCapped ? static_cast<float>(sh.row.top) : sh.row.top32, rate = sh.row.scale32 * (1.0f / kExp2Entries);
+  const float cap = static_cast<float>(sh.row.cap.cap), cap_rate = sh.row.cap.scale32 * (1.0f / kExp2Entries);
   float sum = 0.0f;
   walk.each_eight([&](const float (&x)[8], int v) {
     bool in[8];
@@ -500,13 +515,14 @@ __device__ __noinline__ float look(Bins bins, bool shares) {
       for (int i = 0; i < 8; ++i) in[i] = border.inside(x[i], walk.index_in(v, i));
     }
     if (shares) {
-      if (plain) {
+      if (form != kAny) {
         float w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float t = (fmaxf(x[i], -3.402823466e38f) - top32) * rate;  // (no number: none)
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w[i]) : "f"(t));
-          w[i] = in[i] ? w[i] : 0.0f;
+          w[i] = fmaxf(x[i], -3.402823466e38f);  // (no number: none)
+          if (form == kCapped) w[i] = capped_in_32_bits(w[i], cap, cap_rate);
+          w[i] = power_of_two((w[i] - top32) * rate);
+          w[i] = in[i] & (x[i] > -INFINITY) ? w[i] : 0.0f;
         }
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       } else {
@@ -1444,7 +1460,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     from = kNothing + 1;
   } else if (rules.by_count) {
     if (top_k <= kCap / 8) from = lower;
-  } else if (rules.by_floor && !rules.by_sum) {
+  } else if (rules.by_floor) {
     // Nothing further below the largest than this has a share of min_p; capped values: above where the cap's inverse is.
     double y = sh.row.top + degrees * log(rules.min_p);
     if (capped) {
@@ -1455,6 +1471,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     const float bound = y > static_cast<double>(most) ? most : __double2float_rd(y);
     from = bound == bound ? max(order_of(bound), kNothing + 1) : kNothing + 1;
   }
+  const auto part = Walk<T, kThreads>::mine();
   int which = 0;  // of the slots that the next exchange takes
   int listed = -1;  // entries of a list that has all
   double whole_sum = -1.0;
@@ -1462,8 +1479,11 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     const int count = gather<T, kThreads>(from, largest, most, false, false, false, which).count;
     which ^= 1;
     if (count <= kCap) listed = count;
+    if (listed >= 0 && rules.by_sum && !rules.by_count && p.vocabulary > kCap) {  // (the list is what the floor leaves: top_p is of all)
+      whole_sum = cluster_sums<kThreads>(sum_shares<T, kThreads>(part.begin, part.end, 0.0), 0.0, 0.0, which).a;
+      which ^= 1;
+    }
   }
-  const auto part = Walk<T, kThreads>::mine();
   double above_mine = 0.0;  // this lane's part of the sum above what the list has
   bool begun = false;
 #pragma unroll 1
@@ -1491,7 +1511,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
       }
       // (half a bin, and what 32 bits lose of it)
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
-      const double off = shares ? (0.505 / (kBins - 1) * (static_cast<double>(bins.high) - bins.low) + 0x1p-22 * size) / degrees + 1e-4 : 0.0;
+      const double off = shares ? (0.505 / (kBins - 1) * (static_cast<double>(bins.high) - bins.low) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
       const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, turn);
       if (window.says == kNotHere || low == high) break;
       if (window.says == kInList || window.says == kListHasAll) {
@@ -1515,7 +1535,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         done = got.count > 0 && got.count <= kCap && border_from_list<kThreads>(got.count, shares, above + sums.a, target, false);
         if (done) {
           if (shares) {
-            begun = !rules.by_floor;
+            begun = !rules.by_floor || share<kThreads>(sh.row.border) >= rules.min_p;  // (else some above the border go too)
             above_mine += got.sifted.above;
           }
           break;
