@@ -152,13 +152,15 @@ struct AppendParams {
 // 4608 tokens of 32 heads of 256, packed: 38.6 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
 // kPlaced: slots and positions are given, one read instead of the look-ups of sequence, length and page; a position for each axis, and
 // frequencies for each, most of them zero: a pair's angle is their sum of products, exactly its axis's product where the others are zero.
+// The next token's are asked for in front of a token's heads and worked out behind them, into the other half of the arrays: one barrier a token.
 constexpr int kAppendThreads = 512, kAppendManyThreads = 128;
 constexpr int kAppendManyCtas = 5;  // of an SM (with six: 80 registers, which do not hold it all)
 template <int kDim, int kThreads, bool kPlaced>
 __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAppendManyCtas : 1) kv_append_kernel(const AppendParams p) {
   constexpr int kLanes = kDim / 16;  // threads of a head
   constexpr bool kMany = kThreads == kAppendManyThreads;
-  __shared__ alignas(16) float cosines[kMaxDim / 2], sines[kMaxDim / 2];
+  constexpr int kBuffers = kPlaced ? 2 : 1;
+  __shared__ alignas(16) float all_cosines[kBuffers][kMaxDim / 2], all_sines[kBuffers][kMaxDim / 2];
   const int u = threadIdx.x % kLanes, in_block = threadIdx.x / kLanes, heads_at_once = blockDim.x / kLanes;
   const int eighth = p.half / 8;
   const bool turns = u < eighth;
@@ -187,14 +189,56 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   };
   ask(blockIdx.x, in_block);
 
+  // position * frequency in 64 bits, whole turns taken off there: far positions keep the accuracy of near ones.  Groups of four of a
+  // thread's eight stand in the two halves of the arrays, so that a warp's 16-byte reads follow one another.
+  const int quarters = p.half / 8;
+  const auto turn = [&](int j, double turned, int buffer) {
+    const double angle = turned * 0.31830988618379067154;  // in half turns
+    float sine, cosine;
+    sincospif(static_cast<float>(angle - 2.0 * rint(0.5 * angle)), &sine, &cosine);
+    const int at = ((j >> 2) & 1) * 4 * quarters + (j >> 3) * 4 + (j & 3);
+    all_cosines[buffer][at] = cosine;
+    all_sines[buffer][at] = sine;
+  };
+  // of a given place: its slot, and its positions along the first axes
+  constexpr int kAxes = 4;
+  int place = 0, places[kAxes] = {0, 0, 0, 0}, buffer = 0;
+  const auto look_up = [&](int token) {
+    place = p.slots[token];
+#pragma unroll
+    for (int axis = 0; axis < kAxes; ++axis) places[axis] = axis < p.axes ? p.positions[axis * p.position_stride + token] : 0;
+  };
+  const auto turn_placed = [&](int token, int into) {
+    for (int j = threadIdx.x; j < p.half; j += blockDim.x) {
+      double turned = static_cast<double>(places[0]) * p.frequencies[j];
+#pragma unroll
+      for (int axis = 1; axis < kAxes; ++axis)
+        if (axis < p.axes) turned += static_cast<double>(places[axis]) * p.frequencies[axis * p.half + j];
+      for (int axis = kAxes; axis < p.axes; ++axis)
+        turned += static_cast<double>(p.positions[axis * p.position_stride + token]) * p.frequencies[axis * p.half + j];
+      turn(j, turned, into);
+    }
+  };
+  if constexpr (kPlaced) {
+    look_up(blockIdx.x);
+    turn_placed(blockIdx.x, 0);
+  }
+
 #pragma unroll 1
   for (int token = blockIdx.x; token < p.tokens; token += gridDim.x) {
   const int next_token = kMany ? token + static_cast<int>(gridDim.x) : p.tokens;
   int position, page = -1, in_page;
   if constexpr (kPlaced) {
-    const int at = p.slots[token];
-    if (__syncthreads_or(at < 0)) {  // a row that is no token: left as it was
-      if (next_token < p.tokens) ask(next_token, in_block);
+    const int at = place;
+    const bool none = __syncthreads_or(at < 0);  // (and the token's angles are there)
+    const bool again = next_token < p.tokens;
+    if (again) look_up(next_token);
+    if (none) {  // a row that is no token: left as it was
+      if (again) {
+        ask(next_token, in_block);
+        buffer ^= 1;
+        turn_placed(next_token, buffer);
+      }
       continue;
     }
     page = at >> p.page_shift;
@@ -222,26 +266,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   if (!stored && threadIdx.x == 0 && p.status) atomicExch(p.status, static_cast<int>(kBadPage));
   const long long slot = in_page;
 
-  // position * frequency in 64 bits, whole turns taken off there: far positions keep the accuracy of near ones.  Groups of four of a
-  // thread's eight stand in the two halves of the arrays, so that a warp's 16-byte reads follow one another.
-  const int quarters = p.half / 8;
-  for (int j = threadIdx.x; j < p.half; j += blockDim.x) {
-    double turned;
-    if constexpr (kPlaced) {
-      turned = static_cast<double>(p.positions[token]) * p.frequencies[j];
-      for (int axis = 1; axis < p.axes; ++axis)
-        turned += static_cast<double>(p.positions[axis * p.position_stride + token]) * p.frequencies[axis * p.half + j];
-    } else {
-      turned = static_cast<double>(position) * p.frequencies[j];
-    }
-    const double angle = turned * 0.31830988618379067154;  // in half turns
-    float sine, cosine;
-    sincospif(static_cast<float>(angle - 2.0 * rint(0.5 * angle)), &sine, &cosine);
-    const int at = ((j >> 2) & 1) * 4 * quarters + (j >> 3) * 4 + (j & 3);
-    cosines[at] = cosine;
-    sines[at] = sine;
+  if constexpr (!kPlaced) {
+    for (int j = threadIdx.x; j < p.half; j += blockDim.x) turn(j, static_cast<double>(position) * p.frequencies[j], 0);
+    __syncthreads();
   }
-  __syncthreads();
+  const float* const cosines = all_cosines[kPlaced ? buffer : 0];
+  const float* const sines = all_sines[kPlaced ? buffer : 0];
 
 #pragma unroll 1
   for (int first_head = in_block; first_head < total; first_head += 2 * heads_at_once) {
@@ -311,7 +341,14 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
     }
   }
   }
-  if constexpr (kMany) __syncthreads();  // (the angles are another token's next)
+  if constexpr (kPlaced) {
+    if (next_token < p.tokens) {
+      buffer ^= 1;
+      turn_placed(next_token, buffer);
+    }
+  } else if constexpr (kMany) {
+    __syncthreads();  // (the angles are another token's next)
+  }
   }
 }
 
