@@ -30,6 +30,7 @@ from .runtime import (  # noqa: F401
 from .step import (  # noqa: F401
     PagePool,
     StepPlan,
+    TokenHead,
     kv_append_at,
     plan_step,
     sample_tokens,
@@ -47,6 +48,7 @@ __all__ = [
     "prompt_attention",
     "PagePool",
     "StepPlan",
+    "TokenHead",
     "kv_append_at",
     "plan_step",
     "sample_tokens",

@@ -336,7 +336,7 @@ class AttentionLayer:
     out_w: torch.Tensor          # bf16 [hidden, heads * dim]
     q_norm: torch.Tensor         # bf16 [dim], or None
     k_norm: torch.Tensor
-    frequencies: torch.Tensor    # f64 [pairs that turn]
+    frequencies: torch.Tensor    # f64 [pairs that turn], or with a step.StepPlan [axes, pairs]
     cache: KvCache
     heads: int
     scale: float
@@ -344,18 +344,41 @@ class AttentionLayer:
     normalize_v: bool = True
     eps: float = 1e-6
 
-    def forward(self, hidden, batch, prompt=False):
+    def forward(self, hidden, batch, prompt=False, positions=None):
         """The layer's output, a new tensor [tokens, hidden]; appends the tokens' keys and values to the cache.  With `prompt` every
         sequence is new, a whole prompt of its own, and attention reads the packed keys; otherwise it reads the pages.  Every row of `hidden`
-        is a token of a sequence."""
+        is a token of a sequence.  `batch` may be a step.StepPlan: tokens then go to the plan's slots, turned by `positions` (int32 [tokens] or
+        [axes, tokens]; None: the plan's, the same along all axes), and rows behind the last sequence's pass through with attention of zero."""
         tokens, kv_heads, dim = hidden.shape[0], self.cache.kv_heads, self.cache.head_dim
         x = block_norm(hidden, self.pre, self.eps)
         qkv = torch.mm(x, self.qkv_w.t()).view(tokens, self.heads + 2 * kv_heads, dim)
         q, k, v = qkv.split((self.heads, kv_heads, kv_heads), 1)
+        if hasattr(batch, "slots"):
+            return self._planned(hidden, q, k, v, batch, prompt, positions)
+        if positions is not None:
+            raise ValueError("positions: they go with a plan")
         got = kv_append(q, k, v, self.cache, batch, self.frequencies, self.q_norm, self.k_norm, self.normalize_v, self.eps, packed=prompt)
         if prompt:
             seen = prompt_attention(got.q, got.k, got.v, batch.token_offsets, self.scale, self.window, status=self.cache.status)
         else:
             seen = chunk_attention(got, self.cache, batch, self.scale, self.window)
-        y = torch.mm(seen.view(tokens, self.heads * dim), self.out_w.t())
+        return self._behind(hidden, seen)
+
+    def _planned(self, hidden, q, k, v, plan, prompt, positions):
+        from .step import kv_append_at
+        if positions is None:
+            positions = plan.positions
+            if self.frequencies is not None and self.frequencies.dim() == 2:
+                positions = positions.expand(self.frequencies.shape[0], -1)
+        got = kv_append_at(q, k, v, self.cache, plan.slots, positions, self.frequencies, self.q_norm, self.k_norm, self.normalize_v, self.eps,
+                           packed=prompt)
+        seen = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        if prompt:
+            prompt_attention(got.q, got.k, got.v, plan.token_offsets, self.scale, self.window, out=seen, status=self.cache.status)
+        else:
+            chunk_attention(got, self.cache, plan.batch, self.scale, self.window, out=seen)
+        return self._behind(hidden, seen)
+
+    def _behind(self, hidden, seen):
+        y = torch.mm(seen.view(hidden.shape[0], -1), self.out_w.t())
         return block_norm_add(y, self.post, hidden, eps=self.eps)

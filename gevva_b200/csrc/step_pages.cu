@@ -124,14 +124,35 @@ __global__ void __launch_bounds__(kPagesThreads, 1) step_pages_kernel(const Page
 
   const int whole = threads * ctas, me = rank * threads + thread;
   const int base = kTrim ? taken - static_cast<int>(all_pages) : taken;  // of the pages that move, in the pool's list
-  if (!bad) {
-    // Pages by themselves, whoever's they are: one long request among many takes no longer than its share.
-#pragma unroll 4
-    for (int g = me; g < all_pages; g += whole) {
-      const int s = find_request(page_begins, n, g);
-      int* entry = p.table + static_cast<size_t>(s) * p.table_stride + pages_for(tokens[s], shift) + (g - page_begins[s]);
-      if (kTrim) p.pool[base + g] = *entry;
-      else *entry = p.pool[base + g];
+  if (!bad && all_pages <= whole) {  // a thread for each page
+    if (me < all_pages) {
+      const int s = find_request(page_begins, n, me);
+      int* const entry = p.table + static_cast<size_t>(s) * p.table_stride + pages_for(tokens[s], shift) + (me - page_begins[s]);
+      if (kTrim) p.pool[base + me] = *entry;
+      else *entry = p.pool[base + me];
+    }
+  } else if (!bad) {
+    // Pages by themselves, whoever's they are: one long request among many takes no longer than its share.  A warp takes pages that follow
+    // one another, looks up whose the first is and goes on from there; four of a lane are on their way together.
+    const long long each_warp = (all_pages + (whole >> 5) - 1) / (whole >> 5);
+    const int from = static_cast<int>(min(all_pages, (me >> 5) * each_warp)), upto = static_cast<int>(min(all_pages, from + each_warp));
+    int s = from < upto ? find_request(page_begins, n, from) : 0;
+    for (long long first = from; first < upto; first += 4 * 32) {
+      const int g = static_cast<int>(min(first + lane, static_cast<long long>(upto)));
+      int* out[4];
+      int page[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (32 * k >= upto - g) break;
+        const int at = g + 32 * k;
+        while (page_begins[s + 1] <= at) ++s;  // (page_begins[n] is behind all)
+        int* const entry = p.table + static_cast<size_t>(s) * p.table_stride + pages_for(tokens[s], shift) + (at - page_begins[s]);
+        out[k] = kTrim ? p.pool + base + at : entry;
+        page[k] = kTrim ? *entry : p.pool[base + at];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (32 * k < upto - g) *out[k] = page[k];
     }
   }
   if constexpr (!kTrim) {

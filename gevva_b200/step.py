@@ -16,7 +16,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .attention import Appended, PagedBatch, _at, _heads, _on, _out, _pack, _queries, _status
+from .attention import Appended, PagedBatch, _at, _heads, _on, _out, _pack, _queries, _status, block_norm
 from .runtime import _address, _enqueue, library
 
 MAX_REQUESTS = 16384
@@ -238,3 +238,21 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
                  vocabulary, logits.dtype is f32, softcap)
     _status(_enqueue(_lib().gevva_step_sample, device, None, args), "sample_tokens")
     return (out, shares) if probability else out
+
+
+@dataclass
+class TokenHead:
+    """What stands behind the last layer: norm, the product with the vocabulary's rows (a library's, torch.mm) and the token of each row.  The
+    reference caps these logits at 30 (src/cuda/runtime/decision_logits.cuh)."""
+    norm: torch.Tensor           # bf16 [hidden]
+    rows: torch.Tensor           # bf16 [vocabulary, hidden]
+    softcap: float = 30.0
+    eps: float = 1e-6
+
+    def logits(self, hidden):
+        """bf16 [tokens, vocabulary], not capped yet."""
+        return torch.mm(block_norm(hidden, self.norm, self.eps), self.rows.t())
+
+    def forward(self, hidden, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, probability=False, out=None):
+        """A token for each row of `hidden` [tokens, hidden], by sample_tokens."""
+        return sample_tokens(self.logits(hidden), uniforms, temperature, top_k, top_p, min_p, self.softcap, probability, out)

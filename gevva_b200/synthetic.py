@@ -162,9 +162,10 @@ class SyntheticStack:
     identity: per layer the MoE above plus a dense FP8 GeGLU MLP of width 2112 (weights
     ~N(0, 0.02), per-tensor scale amax/448), norm weights 1, layer scalar 1.  With
     `distinct_experts=False` every layer shares one packed expert set (tests).  With `attention` (a SyntheticAttention)
-    every layer has an attention half in front, with weights and a cache of its own, and `forward` takes the batch."""
+    every layer has an attention half in front, with weights and a cache of its own, and `forward` takes the batch.  With `vocabulary`
+    as well it has rows of so many tokens, and `decode` goes from tokens to tokens."""
 
-    def __init__(self, layers, max_tokens, device="cuda:0", seed=0, distinct_experts=True, s1=None, s2=None, attention=None):
+    def __init__(self, layers, max_tokens, device="cuda:0", seed=0, distinct_experts=True, s1=None, s2=None, attention=None, vocabulary=0):
         from .feedforward import DENSE, DenseMlp, FeedForwardLayer, pack_fp8
         self.device = torch.device(device)
         gen = torch.Generator(device=self.device)
@@ -198,6 +199,11 @@ class SyntheticStack:
             self._keep = getattr(self, "_keep", []) + [base]
         self.attention = [self._attention_layer(index, attention, seed) for index in range(layers)] if attention else None
         self.aux = torch.cuda.Stream(device=self.device)
+        self.head = None
+        if vocabulary:
+            from .step import TokenHead
+            gen.manual_seed(seed + 777)
+            self.head = TokenHead(ones, _randn((vocabulary, HIDDEN), 0.05, gen, self.device).to(torch.bfloat16))
 
     def _attention_layer(self, index, shape, seed):
         from .attention import AttentionLayer, KvCache
@@ -214,7 +220,7 @@ class SyntheticStack:
             scale=shape.head_dim ** -0.5, window=0 if (index + 1) % shape.whole_every == 0 else shape.window)
 
     def forward(self, hidden, concurrent=True, batch=None, prompt=False):
-        """`batch` (an attention.PagedBatch) and `prompt` (every sequence is a whole prompt) go with a stack that has attention."""
+        """`batch` (an attention.PagedBatch or a step.StepPlan) and `prompt` (every sequence is a whole prompt) go with a stack that has attention."""
         if (batch is not None) != (self.attention is not None):
             raise ValueError("a stack with attention takes a batch, one without takes none")
         for index, layer in enumerate(self.layers):
@@ -222,3 +228,11 @@ class SyntheticStack:
                 hidden = self.attention[index].forward(hidden, batch, prompt)
             hidden = layer.forward(hidden, self.aux if concurrent else None)
         return hidden
+
+    def decode(self, tokens, plan, uniforms, concurrent=True, **settings):
+        """The next token of each row: int32 `tokens` of the step that `plan` (a step.StepPlan) places, through the layers and the head.  `settings` are
+        those of step.sample_tokens."""
+        if self.head is None or self.attention is None:
+            raise ValueError("a stack that decodes has attention and a vocabulary")
+        hidden = self.forward(self.head.rows[tokens.long()], concurrent, plan)
+        return self.head.forward(hidden, uniforms, **settings)

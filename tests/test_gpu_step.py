@@ -1,8 +1,9 @@
 """What a serving step has around its layers, through its Python mirror, against plain forms on the host.
 
 Whole numbers have to be equal.  A token is compared where no rule's border lies within 2^-40 of the whole of what decides it: shares are off by at
-most some 2^-46 of themselves (a table entry rounded by 2^-53, five terms by 2^-48.6, an exponent of at most 2^10 rounded by 2^-53 of itself), and so
-are their sums, whatever the order.  Probabilities are rounded once to 32 bits (2^-24)."""
+most 2^-42.8 of themselves (tests/test_step_shares.py), and so are their sums, whatever the order.  (Capped ones by 2^-53 of the cap over
+the temperature more: 2^-43 of themselves at a cap of 30 and a temperature of 0.03.)  Probabilities are rounded once to 32 bits
+(2^-24), of numbers that are off by much less."""
 import math
 
 import numpy as np
@@ -533,3 +534,114 @@ def test_calls_at_once_on_states_of_their_own():
         want = step_ref.plan(lengths, [1 + i] * (50 + i), table, free, taken, 16, (1 + i) * (50 + i))
         for one in plan:
             assert one.slots.tolist() == want[2] and one.lengths.tolist() == want[1]
+
+
+# ---- in a layer, and from tokens to tokens --------------------------------------------------------------------
+
+def attention_layer(gen, axes=1, hidden=256, heads=4, kv_heads=2, dim=64, window=0):
+    frequencies = 1e4 ** (-torch.arange(dim // 2, dtype=torch.float64, device=DEV) / (dim // 2))
+    if axes > 1:
+        mine = torch.arange(dim // 2, device=DEV)[None] % axes == torch.arange(axes, device=DEV)[:, None]
+        frequencies = torch.where(mine, frequencies, 0.0)
+    return attn.AttentionLayer(
+        pre=randn(gen, hidden), post=randn(gen, hidden), qkv_w=randn(gen, (heads + 2 * kv_heads) * dim, hidden, std=0.1),
+        out_w=randn(gen, hidden, heads * dim, std=0.1), q_norm=randn(gen, dim), k_norm=randn(gen, dim), frequencies=frequencies,
+        cache=attn.KvCache.empty(64, 16, kv_heads, dim), heads=heads, scale=dim ** -0.5, window=window)
+
+
+def test_a_layer_over_a_plan_is_the_layer_over_the_batch():
+    """Prompts, then steps of several tokens, with rows behind the last request's: bit for bit what the batch gives."""
+    gen = generator(61)
+    layer = attention_layer(gen)
+    pool, table, lengths = step.PagePool.whole(64, DEV), torch.full((5, 12), -1, dtype=torch.int32, device=DEV), ints([0] * 5)
+    caches = [layer.cache, attn.KvCache.empty(64, 16, 2, 64)]
+    for turn, news in enumerate(([20, 1, 0, 37, 5], [1, 2, 0, 1, 5], [1, 1, 30, 1, 0])):
+        tokens = sum(news)
+        hidden = randn(gen, tokens + 3, 256)
+        plan = step.plan_step(lengths, ints(news), table, pool, 16, tokens + 3)
+        layer.cache = caches[0]
+        prompt = turn == 0
+        got = layer.forward(hidden, plan, prompt)
+        layer.cache = caches[1]
+        want = layer.forward(hidden[:tokens].contiguous(), plan.batch, prompt)
+        assert torch.equal(got[:tokens], want) and torch.isfinite(got[tokens:].float()).all()
+        assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+        lengths, pool.taken = plan.lengths, plan.taken
+    pool.check()
+    with pytest.raises(ValueError, match="plan"):
+        layer.forward(hidden, plan.batch, positions=plan.positions)
+
+
+def test_a_layer_with_positions_of_three_axes():
+    """Positions that differ along the axes turn differently; the same along all axes they are the plan's own."""
+    gen = generator(62)
+    layer = attention_layer(gen, axes=3)
+    pool, table = step.PagePool.whole(64, DEV), torch.full((2, 12), -1, dtype=torch.int32, device=DEV)
+    plan = step.plan_step(ints([0, 0]), ints([30, 12]), table, pool, 16, 42)
+    hidden = randn(gen, 42, 256)
+    one = layer.forward(hidden, plan, True)
+    keys = layer.cache.k.clone()
+    two = layer.forward(hidden, plan, True, plan.positions.repeat(3, 1))
+    assert torch.equal(one, two) and torch.equal(keys, layer.cache.k)
+    layer.forward(hidden, plan, True, torch.stack([plan.positions, plan.positions // 5, plan.positions % 5]))
+    assert not torch.equal(keys, layer.cache.k)
+
+
+def test_a_stack_decodes_from_tokens_to_tokens():
+    """The layers, the head and the plans together, against the same calls over a batch and a token chosen by the plain form."""
+    from gevva_b200.synthetic import SyntheticAttention, SyntheticStack
+    gen = generator(63)
+    stack = SyntheticStack(2, 256, DEV, distinct_experts=False, attention=SyntheticAttention(window=24, whole_every=2, pages=32, page_size=16), vocabulary=1201)
+    pool, table, state = step.PagePool.whole(32, DEV), torch.full((3, 8), -1, dtype=torch.int32, device=DEV), ints([0, 0, 0])
+    news = [9, 1, 30]
+    plan = step.plan_step(state, ints(news), table, pool, 16, 40)
+    state, pool.taken = plan.lengths, plan.taken
+    tokens = torch.randint(0, 1201, (40,), generator=gen, device=DEV, dtype=torch.int32)
+    hidden = stack.forward(stack.head.rows[tokens.long()], batch=plan, prompt=True)
+    rows = hidden[(plan.token_offsets[1:] - 1).long()].contiguous()
+    given = dict(temperature=torch.tensor([1.0, 0.0, 0.8], device=DEV), top_k=ints([0, 0, 40]), top_p=torch.tensor([0.9, 1.0, 1.0], device=DEV))
+    u = torch.rand(3, generator=gen, device=DEV)
+    last = stack.head.forward(rows, u, **given)
+    compare(stack.head.logits(rows), u, given, 30.0)
+    places = step.StepPlan.in_place(state, table, pool, 3)
+    for _ in range(20):
+        u = torch.rand(3, generator=gen, device=DEV)
+        step.plan_step(state, ints([1, 1, 1]), table, pool, 16, 3, out=places)
+        chosen = stack.decode(last, places, u, **given)
+        # again over the batch: the same slots get the same keys and values
+        again = stack.forward(stack.head.rows[last.long()], batch=places.batch)
+        assert torch.equal(compare(stack.head.logits(again), u, given, 30.0), chosen)
+        last = chosen
+    pool.check()
+    with pytest.raises(ValueError, match="vocabulary"):
+        SyntheticStack(1, 16, DEV, distinct_experts=False).decode(last, places, u)
+
+
+def test_other_devices_and_types_are_refused():
+    logits, u = torch.zeros(2, 7, device=DEV), torch.zeros(2, device=DEV)
+    for name, value in (("uniforms", u.cpu()), ("uniforms", u.double()), ("uniforms", u[:1])):
+        with pytest.raises(ValueError, match=name):
+            step.sample_tokens(logits, value)
+    for name, value in (("temperature", u.int()), ("top_k", u), ("top_p", u[:1]), ("min_p", u.half()), ("out", u)):
+        with pytest.raises(ValueError, match=name):
+            step.sample_tokens(logits, u, **{name: value})
+    with pytest.raises(ValueError, match="contiguous values"):
+        step.sample_tokens(torch.zeros(7, 2, device=DEV).t(), u)
+    pool, table, two = step.PagePool.whole(4, DEV), torch.zeros(2, 3, dtype=torch.int32, device=DEV), ints([0, 0])
+    with pytest.raises(ValueError, match="news"):
+        step.plan_step(two, ints([1]), table, pool, 16, 2)
+    with pytest.raises(ValueError, match="table"):
+        step.plan_step(two, two, table[:1], pool, 16, 2)
+    with pytest.raises(ValueError, match="another table"):
+        step.plan_step(two, two, table, pool, 16, 2, out=step.StepPlan.empty(2, table[:, :2], 2))
+    with pytest.raises(ValueError, match="out.slots"):
+        step.plan_step(two, two, table, pool, 16, 3, out=step.StepPlan.empty(2, table, 2))
+    with pytest.raises(step.GevvaMoeError if hasattr(step, "GevvaMoeError") else RuntimeError):
+        step.plan_step(two, two, table, pool, 24, 2)
+    x = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device=DEV)
+    cache = attn.KvCache.empty(2, 16, 1, 64)
+    frequencies = torch.zeros(2, 8, dtype=torch.float64, device=DEV)
+    for bad in (dict(slots=two.long()), dict(positions=two.float()), dict(positions=ints([[0, 0]] * 17)), dict(positions=ints([0, 0, 0])),
+                dict(frequencies=frequencies), dict(frequencies=frequencies[0].float())):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            step.kv_append_at(x, x, x, cache, **dict(dict(slots=two, positions=two, frequencies=frequencies[0]), **bad))
