@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "gv_exact.h"
 #include "gv_transcendentals.h"
 
@@ -188,18 +190,25 @@ inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, dim3 blo
   return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
 }
 
-// The same in clusters of `ctas` CTAs that follow one another in the grid; more than eight are allowed to the kernel first.
+// Leave for a kernel of up to `smem_bytes` of dynamic shared memory in clusters of any size, asked for once on each device.
+template <class... Params>
+inline cudaError_t allow_clusters(void (*kernel)(Params...), int smem_bytes, std::atomic<unsigned long long>* devices) {
+  int device = -1;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = device >= 0 && device < 64 ? 1ull << device : 0;
+  if (devices->load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) devices->fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+// The same in clusters of `ctas` CTAs that follow one another in the grid.  What the kernel needs leave for, more than 48 KB of shared memory with what it
+// declares by itself, or more than eight CTAs, has been asked for (allow_clusters).
 template <class... Params, class... Args>
 inline cudaError_t launch_chained_clusters(void (*kernel)(Params...), unsigned ctas, dim3 grid, dim3 block, size_t smem_bytes,
                                            cudaStream_t stream, Args&&... args) {
-  if (smem_bytes > 4096) {  // (with what the kernel declares by itself it may be more than the 48 KB that need no leave)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_bytes));
-    if (e != cudaSuccess) return e;
-  }
-  if (ctas > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
   config.blockDim = block;

@@ -1592,6 +1592,9 @@ cudaError_t launch_threads(const SampleCall& call, int ctas, cudaStream_t stream
   const bool whole = (reinterpret_cast<uintptr_t>(call.logits) & 15) == 0 && (call.row_stride * sizeof(T) & 15) == 0;
   const int vectors = (call.vocabulary + (whole ? 0 : kE - 1) + kE - 1) / kE, warps = ctas * (kThreads / 32);
   p.cta_vectors = (vectors + warps - 1) / warps * (kThreads / 32);
+  static std::atomic<unsigned long long> allowed{0};
+  const cudaError_t e = allow_clusters(sample_kernel<T, kThreads>, sizeof(SampleShared<kThreads>), &allowed);
+  if (e != cudaSuccess) return e;
   return launch_chained_clusters(sample_kernel<T, kThreads>, ctas, dim3(static_cast<unsigned>(call.rows) * ctas), dim3(kThreads),
                                  sizeof(SampleShared<kThreads>), stream, p);
 }

@@ -200,7 +200,11 @@ cudaError_t launch_step_pages(const PagesCall& call, cudaStream_t stream) {
   const int threads = items >= kPagesThreads ? kPagesThreads : (items + 31) / 32 * 32;
   int ctas = 1;
   while (ctas < kPagesCtas && ctas * kPagesThreads < items) ctas *= 2;
-  return launch_chained_clusters(call.trim ? step_pages_kernel<true> : step_pages_kernel<false>, ctas, dim3(ctas), dim3(threads), bytes, stream, p);
+  static std::atomic<unsigned long long> allowed[2];
+  const auto kernel = call.trim ? step_pages_kernel<true> : step_pages_kernel<false>;
+  const cudaError_t e = allow_clusters(kernel, sizeof(int) * (3 * kMaxPlanSequences + 2), &allowed[call.trim]);
+  if (e != cudaSuccess) return e;
+  return launch_chained_clusters(kernel, ctas, dim3(ctas), dim3(threads), bytes, stream, p);
 }
 
 }  // namespace gv

@@ -16,7 +16,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .attention import Appended, PagedBatch, _at, _heads, _on, _out, _pack, _queries, _status, block_norm
+from .attention import Appended, PagedBatch, _at, _empty, _heads, _on, _out, _pack, _queries, _status, block_norm
 from .runtime import _address, _enqueue, library
 
 MAX_REQUESTS = 16384
@@ -42,17 +42,22 @@ def _lib():
 class PagePool:
     """Pages of a cache that requests get and give back: `free` int32 [pages] lists them, in any order, and the first `taken` (int32 [1], on
     the GPU as well) are handed out.  plan_step takes from it and trim_step gives back.  `status` is the int32 word that calls on this
-    pool report into."""
+    pool report into.  Each may be replaced, which later calls follow; a captured call keeps those that it was captured with."""
 
     def __init__(self, free, taken=None, status=None):
+        taken = torch.zeros(1, dtype=torch.int32, device=free.device) if taken is None else taken
+        self._take(free, taken, torch.zeros(1, dtype=torch.int32, device=free.device) if status is None else status)
+
+    def _take(self, free, taken, status):
         if not free.is_cuda or free.dtype is not torch.int32 or free.dim() != 1 or free.numel() < 1 or not free.is_contiguous():
             raise ValueError(f"free: expected contiguous CUDA int32 (pages,), got {free.dtype} {tuple(free.shape)} on {free.device}")
-        self.device = free.device
-        self.free = free
-        self.taken = torch.zeros(1, dtype=torch.int32, device=free.device) if taken is None else taken
-        self.status = torch.zeros(1, dtype=torch.int32, device=free.device) if status is None else status
-        for tensor, name in ((self.taken, "taken"), (self.status, "status")):
-            _at(tensor, torch.int32, (1,), self.device, name)
+        addresses = (free.data_ptr(), _at(taken, torch.int32, (1,), free.device, "taken"), _at(status, torch.int32, (1,), free.device, "status"))
+        self.device, self.pages = free.device, free.numel()
+        self._free, self._taken, self._status, self._addresses = free, taken, status, addresses
+
+    free = property(lambda self: self._free, lambda self, x: self._take(x, self._taken, self._status))
+    taken = property(lambda self: self._taken, lambda self, x: self._take(self._free, x, self._status))
+    status = property(lambda self: self._status, lambda self, x: self._take(self._free, self._taken, x))
 
     @classmethod
     def whole(cls, pages, device="cuda:0"):
@@ -81,8 +86,8 @@ class StepPlan:
 
     @classmethod
     def empty(cls, sequences, table, tokens, lengths=None, taken=None):
-        own = torch.empty(2 * sequences + 2 + 2 * tokens, dtype=torch.int32, device=table.device)
-        offsets, after, slots, positions, count = own.split((sequences + 1, sequences, tokens, tokens, 1))
+        own = _empty(2 * sequences + 2 + 2 * tokens, dtype=torch.int32, device=table.device)
+        offsets, after, slots, positions, count = own.split_with_sizes((sequences + 1, sequences, tokens, tokens, 1))
         return cls(offsets, after if lengths is None else lengths, slots, positions, count if taken is None else taken, table)
 
     @classmethod
@@ -105,22 +110,21 @@ class Trimmed:
 
 
 def _requests(lengths, counts, name, table, pool):
-    """(device, number of requests, address and stride of the table) of a call over a pool."""
-    device, sequences = lengths.device, lengths.shape[0] if lengths.dim() == 1 else -1
-    if device.type != "cuda" or sequences < 1:
-        raise ValueError(f"lengths: expected CUDA int32 (sequences,), got {lengths.dtype} {tuple(lengths.shape)} on {device}")
+    """(device, number of requests, stride of the table) of a call over a pool."""
+    device, i32 = pool.device, torch.int32
+    sequences = lengths.shape[0] if lengths.dim() == 1 else -1
+    if sequences < 1 or not lengths.is_cuda:
+        raise ValueError(f"lengths: expected CUDA int32 (sequences,), got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
     if sequences > MAX_REQUESTS:
         raise ValueError(f"lengths: at most {MAX_REQUESTS} requests, got {sequences}")
-    _at(lengths, torch.int32, (sequences,), device, "lengths")
-    _at(counts, torch.int32, (sequences,), device, name)
-    if pool.device != device:
-        raise ValueError(f"pool: expected one on {device}, got one on {pool.device}")
-    _at(pool.free, torch.int32, pool.free.shape, device, "free")
-    if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != sequences or table.shape[1] < 1 or table.device != device or
-            (table.stride(1) != 1 and table.shape[1] > 1)):
+    _at(lengths, i32, (sequences,), device, "lengths")
+    _at(counts, i32, (sequences,), device, name)
+    rows, width = table.shape if table.dim() == 2 else (-1, 0)
+    stride, one = table.stride() if rows > 0 else (0, 1)
+    if table.dtype is not i32 or rows != sequences or width < 1 or table.device != device or (one != 1 and width > 1):
         raise ValueError(f"table: expected int32 ({sequences}, pages a sequence) on {device}, got {table.dtype} {tuple(table.shape)} strides "
                          f"{table.stride()} on {table.device}")
-    return device, sequences, table.stride(0) if sequences > 1 else table.shape[1]
+    return device, sequences, stride if sequences > 1 else width
 
 
 def plan_step(lengths, news, table, pool, page_size, tokens, shift=None, out=None, stream=None):
@@ -137,16 +141,17 @@ def plan_step(lengths, news, table, pool, page_size, tokens, shift=None, out=Non
     i32 = torch.int32
     if out is None:
         out = StepPlan.empty(sequences, table, tokens)
-        addresses = [t.data_ptr() for t in (out.token_offsets, out.lengths, out.slots, out.positions, out.taken)]
+        at = out.token_offsets.data_ptr()
+        addresses = (at, at + 4 * (sequences + 1), at + 4 * (2 * sequences + 1), at + 4 * (2 * sequences + 1 + tokens), at + 4 * (2 * sequences + 1 + 2 * tokens))
     else:
         if out.table is not table and (out.table.data_ptr() != table.data_ptr() or out.table.shape != table.shape or out.table.stride() != table.stride()):
             raise ValueError("out: a plan for another table")
-        addresses = [_at(out.token_offsets, i32, (sequences + 1,), device, "out.token_offsets"), _at(out.lengths, i32, (sequences,), device, "out.lengths"),
+        addresses = (_at(out.token_offsets, i32, (sequences + 1,), device, "out.token_offsets"), _at(out.lengths, i32, (sequences,), device, "out.lengths"),
                      _at(out.slots, i32, (tokens,), device, "out.slots"), _at(out.positions, i32, (tokens,), device, "out.positions"),
-                     _at(out.taken, i32, (1,), device, "out.taken")]
-    args = _pack(_PLAN, lengths.data_ptr(), news.data_ptr(), _at(shift, i32, (sequences,), device, "shift"), table.data_ptr(), pool.free.data_ptr(),
-                 _at(pool.taken, i32, (1,), device, "taken"), *addresses, _at(pool.status, i32, (1,), device, "status"), sequences, table.shape[1], stride,
-                 pool.free.numel(), page_size, tokens)
+                     _at(out.taken, i32, (1,), device, "out.taken"))
+    free, taken, status = pool._addresses
+    args = _pack(_PLAN, lengths.data_ptr(), news.data_ptr(), _at(shift, i32, (sequences,), device, "shift"), table.data_ptr(), free, taken, *addresses, status,
+                 sequences, table.shape[1], stride, pool.pages, page_size, tokens)
     _status(_enqueue(_lib().gevva_step_plan, device, None, args), "plan_step")
     return out
 
@@ -162,10 +167,10 @@ def trim_step(lengths, keep, table, pool, page_size, out=None, stream=None):
             return trim_step(lengths, keep, table, pool, page_size, out)
     i32 = torch.int32
     if out is None:
-        out = Trimmed(*torch.empty(sequences + 1, dtype=i32, device=device).split((sequences, 1)))
-    args = _pack(_TRIM, lengths.data_ptr(), keep.data_ptr(), table.data_ptr(), pool.free.data_ptr(), _at(pool.taken, i32, (1,), device, "taken"),
-                 _at(out.lengths, i32, (sequences,), device, "out.lengths"), _at(out.taken, i32, (1,), device, "out.taken"),
-                 _at(pool.status, i32, (1,), device, "status"), sequences, table.shape[1], stride, pool.free.numel(), page_size, 0)
+        out = Trimmed(*_empty(sequences + 1, dtype=i32, device=device).split_with_sizes((sequences, 1)))
+    free, taken, status = pool._addresses
+    args = _pack(_TRIM, lengths.data_ptr(), keep.data_ptr(), table.data_ptr(), free, taken, _at(out.lengths, i32, (sequences,), device, "out.lengths"),
+                 _at(out.taken, i32, (1,), device, "out.taken"), status, sequences, table.shape[1], stride, pool.pages, page_size, 0)
     _status(_enqueue(_lib().gevva_step_trim, device, None, args), "trim_step")
     return out
 
@@ -230,8 +235,8 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
         raise ValueError(f"logits: expected 1 to {MAX_VOCABULARY} contiguous values a row, got {tuple(logits.shape)} strides {logits.stride()}")
     f32, i32, each = torch.float32, torch.int32, (rows,)
     if out is None:
-        out = torch.empty(rows, dtype=i32, device=device)
-    shares = torch.empty(rows, dtype=f32, device=device) if probability else None
+        out = _empty(rows, dtype=i32, device=device)
+    shares = _empty(rows, dtype=f32, device=device) if probability else None
     args = _pack(_SAMPLE, logits.data_ptr(), logits.stride(0) if rows > 1 else 0, _at(uniforms, f32, each, device, "uniforms"),
                  _at(temperature, f32, each, device, "temperature"), _at(top_k, i32, each, device, "top_k"), _at(top_p, f32, each, device, "top_p"),
                  _at(min_p, f32, each, device, "min_p"), _at(out, i32, each, device, "out"), shares.data_ptr() if probability else 0, rows,

@@ -139,14 +139,18 @@ def test_every_declared_call_is_exported():
         assert hasattr(lib, name)
 
 
+class Pool:
+    device = torch.device("cuda:0")
+
+
 def test_python_mirror_refuses():
     ints, rows = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="CUDA"):
         step.PagePool(ints)
     with pytest.raises(ValueError, match="lengths"):
-        step.plan_step(ints, ints, ints.view(3, 1), None, 16, 3)
+        step.plan_step(ints, ints, ints.view(3, 1), Pool, 16, 3)
     with pytest.raises(ValueError, match="lengths"):
-        step.trim_step(ints, ints, ints.view(3, 1), None, 16)
+        step.trim_step(ints, ints, ints.view(3, 1), Pool, 16)
     with pytest.raises(ValueError, match="CUDA"):
         step.kv_append_at(rows, rows, rows, None, ints, ints, None)
     for logits in (torch.zeros(2, 5), torch.zeros(2, 5, dtype=torch.float16), torch.zeros(5)):
