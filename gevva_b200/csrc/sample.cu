@@ -1603,9 +1603,12 @@ template <typename T>
 cudaError_t launch_type(const SampleCall& call, int sm_count, cudaStream_t stream) {
   const long long bytes = static_cast<long long>(call.vocabulary) * sizeof(T);
   if (bytes <= 4096) return launch_threads<T, 128>(call, 1, stream);
-  // Two CTAs an SM hold as many rows as there are; where there are fewer, as many CTAs a row as that leaves, down to 8 KB each.
+  // Two CTAs an SM take as many rows as there are; where there are fewer, as many CTAs a row as that leaves, down to 8 KB each.  With rules to find
+  // borders for, rows take up to five times as long as one another: twice as many CTAs then (64 rows of 262144, each with rules of its
+  // own, 243 -> 146 us; 256 rows of 128000 by nucleus 300 -> 265; without rules 256 rows of 50257 would go 38 -> 47).
+  const long long ctas_at_once = (call.top_k || call.top_p || call.min_p ? 4ll : 2ll) * sm_count;
   int ctas = 1;
-  while (ctas < kMostCtas && 2ll * ctas * call.rows <= 2 * sm_count && bytes > 16384ll * ctas) ctas *= 2;
+  while (ctas < kMostCtas && 2ll * ctas * call.rows <= ctas_at_once && bytes > 16384ll * ctas) ctas *= 2;
   return launch_threads<T, 256>(call, ctas, stream);
 }
 
