@@ -48,7 +48,8 @@ struct Bins {
   float low, high, per;  // bins for one
 };
 
-// How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values, or of any.
+// How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values where cap and
+// temperature are, or of any.
 enum ShareForm : int { kPlain, kCapped, kAny };
 // cap * tanh(x / cap), with e = exp(-2 |x| / cap): cap * (1 - e) / (1 + e).
 struct Cap {
@@ -221,24 +222,56 @@ __device__ __forceinline__ Border border_of(const RowState& row) { return {row.b
 
 // ---- shares
 
-__device__ __forceinline__ double softened(float x, const Cap& c, const double* table) {
-  const float size = fminf(fabsf(x), c.most32);
-  const double e = share_with<true>(-static_cast<double>(size), c.scale, share_whole(-size, c.scale32), table, kTableCopies);
-  // 1 / (1 + e) by two steps of Newton's from 32 bits
-  const double d = 1.0 + e;
-  float guess;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(guess) : "f"(static_cast<float>(d)));
-  double r = static_cast<double>(guess);
-  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
-  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
-  return copysign(c.cap * ((1.0 - e) * r), static_cast<double>(x));
+__device__ __forceinline__ float power_of_two(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-// By its distance from the largest in y, in two precisions: none beyond kShareOctaves.
-__device__ __forceinline__ double capped_share(float x, double scale, float scale32, double top, const Cap& cap, const double* table) {
-  const double distance = softened(x, cap, table) - top;
-  const float distance32 = static_cast<float>(distance);
-  const double share = share_with(distance, scale, share_whole(distance32, scale32), table, kTableCopies);
-  return distance32 * scale32 > -kShareOctaves * kExp2Entries ? share : 0.0;
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// cap * tanh(x / cap) in both precisions.
+struct Softened {
+  double y;
+  float y32;
+};
+__device__ __forceinline__ Softened softened(float x, const Cap& c, float cap32, const double* table) {
+  const float size = fminf(fabsf(x), c.most32);
+  const double e = share_with<true>(-wide_of(size), c.scale, share_whole(-size, c.scale32), table, kTableCopies);
+  const float e32 = power_of_two(-size * (c.scale32 * (1.0f / kExp2Entries))), r32 = reciprocal(1.0f + e32);
+  // 1 / (1 + e) by two steps of Newton's from 32 bits (2^-21: 2^-42, 2^-84)
+  const double d = 1.0 + e;
+  double r = wide_of(r32);
+  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
+  r = __fma_rn(r, __fma_rn(-d, r, 1.0), r);
+  const double y = c.cap * ((1.0 - e) * r);
+  return {x < 0.0f ? -y : y, copysignf(cap32 * ((1.0f - e32) * r32), x)};
+}
+// A cap of at most this many times the temperature is of ordinary size: y in 32 bits is off by cap * 2^-22, so that a distance's whole part is
+// by 2 * 128 * 46 * 2^-22 = 0.003 32nds, and y in 64 bits by cap * 2^-51.3, a share's exponent by 2^-43: no more than the series leaves.
+constexpr double kMostCap = 128.0;
+// By its distance from the largest in y, whose whole part needs 32 bits only: none beyond kShareOctaves.
+__device__ __forceinline__ double capped_share(float x, double scale, float scale32, double top, float top32, const Cap& cap, float cap32, const double* table) {
+  const Softened it = softened(x, cap, cap32, table);
+  const float octaves = (it.y32 - top32) * scale32;
+  const double share = share_with(it.y - top, scale, share_whole(fmaxf(it.y32 - top32, -1e30f), scale32), table, kTableCopies);
+  return octaves > -kShareOctaves * kExp2Entries ? share : 0.0;
+}
+// cap * tanh(x / cap) for any cap, to a few steps of 64 bits: 1 - e keeps too little of a value that is small next to its cap.  There the series
+// x (1 - z^2 / 3 + 2 z^4 / 15 - 17 z^6 / 315) is off by 62 z^8 / 2835, 2^-65 at z = ln 2 / 128, where e's exponent is half a 32nd.
+__device__ __noinline__ double softened_any(float x, const Cap& c, const double* table) {
+  const double size = fmin(fabs(static_cast<double>(x)), 24.0 * c.cap), octaves = size * c.scale;
+  double y;
+  if (octaves <= 0.5) {
+    const double z = size / c.cap, q = z * z;
+    y = size * (1.0 - q * (1.0 / 3.0 - q * (2.0 / 15.0 - q * (17.0 / 315.0))));
+  } else {
+    const double e = share_with<true>(-size, c.scale, share_whole(-static_cast<float>(octaves), 1.0f), table, kTableCopies);
+    y = c.cap * ((1.0 - e) / (1.0 + e));
+  }
+  return x < 0.0f ? -y : y;
 }
 template <int kThreads>
 __device__ __forceinline__ const double* lane_table() {
@@ -272,7 +305,8 @@ __device__ __noinline__ double share(float x) {
   const RowState& row = shared<kThreads>().row;
   const double* table = lane_table<kThreads>();
   if (row.form == kPlain) return x >= row.cut ? PlainShares::of<kThreads>()(x) : 0.0;
-  if (row.form == kCapped) return capped_share(x, row.scale, row.scale32, row.top, row.cap, table);
+  if (row.form == kCapped) return capped_share(x, row.scale, row.scale32, row.top, row.top32, row.cap, static_cast<float>(row.cap.cap), table);
+  if (row.cap.cap > 0.0) return share_of(softened_any(x, row.cap, table) - row.top, row.scale, table, kTableCopies);
   if (isinf(x)) return 1.0;  // (the largest value is infinite then, and so is this one)
   return isinf(row.top) ? 0.0 : share_of(static_cast<double>(x) - row.top, row.scale, table, kTableCopies);
 }
@@ -289,10 +323,10 @@ __device__ __noinline__ Eight other_shares(float a, float b, float c, float d, f
   if (row.form == kCapped) {
     const Cap cap = row.cap;
     const double scale = row.scale, top = row.top;
-    const float scale32 = row.scale32;
+    const float scale32 = row.scale32, top32 = row.top32, cap32 = static_cast<float>(cap.cap);
     const double* table = lane_table<kThreads>();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.w[i] = capped_share(x[i], scale, scale32, top, cap, table);
+    for (int i = 0; i < 8; ++i) out.w[i] = capped_share(x[i], scale, scale32, top, top32, cap, cap32, table);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) out.w[i] = x[i] > -INFINITY ? share<kThreads>(x[i]) : 0.0;
@@ -481,17 +515,10 @@ __device__ __forceinline__ void clear_bins() {
   __syncthreads();
 }
 
-__device__ __forceinline__ float power_of_two(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // softened(), in 32 bits.
 __device__ __forceinline__ float capped_in_32_bits(float x, float cap, float rate) {
   const float e = power_of_two(-fabsf(x) * rate);
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return copysignf(cap * (1.0f - e) * r, x);
+  return copysignf(cap * ((1.0f - e) * reciprocal(1.0f + e)), x);
 }
 
 // Counts what is inside by bins; with `shares` also this lane's sum of shares, in 32 bits: where to look, no more.
@@ -503,7 +530,7 @@ __device__ __noinline__ float look(Bins bins, bool shares) {
   const int nothing = kBins + (threadIdx.x & 31);
   const bool all = !sh.row.bounded;
   const ShareForm form = sh.row.form;
-  const float top32 = form == kCapped ? static_cast<float>(sh.row.top) : sh.row.top32, rate = sh.row.scale32 * (1.0f / kExp2Entries);
+  const float top32 = sh.row.top32, rate = sh.row.scale32 * (1.0f / kExp2Entries);
   const float cap = static_cast<float>(sh.row.cap.cap), cap_rate = sh.row.cap.scale32 * (1.0f / kExp2Entries);
   float sum = 0.0f;
   walk.each_eight([&](const float (&x)[8], int v) {
@@ -614,16 +641,10 @@ __device__ __noinline__ Sifted sift(bool binned, float low, float high, float be
 #pragma unroll
           for (int i = 0; i < 8; ++i) w[i] = border.inside(x[i], walk.index_in(v, i)) ? w[i] : 0.0;
         }
-        // (what is above, and what is not)
-        double up[2] = {0.0, 0.0}, rest[2] = {0.0, 0.0};
+        sifted.all += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (over[i]) up[i & 1] += w[i];
-          else rest[i & 1] += w[i];
-        }
-        const double above = up[0] + up[1];
-        sifted.above += above;
-        sifted.all += above + (rest[0] + rest[1]);
+        for (int i = 0; i < 8; ++i) w[i] = over[i] ? w[i] : 0.0;
+        sifted.above += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       }
     }
     if (binned) {
@@ -1438,18 +1459,27 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   if (thread == 0) {
     RowState& row = sh.row;
     constexpr double octave = 1.4426950408889634074 * kExp2Entries;
+    row.cap = Cap{};
     if (capped) {
       const double rate = 2.0 * octave / p.softcap;
       row.cap = Cap{p.softcap, rate, static_cast<float>(rate), 24.0f * p.softcap};  // (2^-69 of one)
     }
     row.scale = octave / degrees;
-    row.top = capped ? softened(most, row.cap, sh.table) : static_cast<double>(most);
     row.scale32 = static_cast<float>(row.scale);
-    row.top32 = row.largest = most;
+    row.largest = most;
+    const bool ordinary = (capped ? p.softcap > 1e-30f && p.softcap <= kMostCap * temperature : fabsf(most) < 1e30f) && temperature > 1e-30f && temperature < 1e30f;
+    row.top = static_cast<double>(most);
+    row.top32 = most;
+    if (capped && ordinary) {
+      const Softened it = softened(most, row.cap, p.softcap, sh.table);
+      row.top = it.y;
+      row.top32 = it.y32;
+    } else if (capped) {
+      row.top = softened_any(most, row.cap, sh.table);
+    }
     row.cut = fmaxf(__double2float_rd(static_cast<double>(most) - kShareOctaves * 0.69314718055994530942 * degrees), -3.402823466e38f);
     // (sizes at which 32 bits hold the whole part of every share that there is)
-    const bool ordinary = fabsf(most) < 1e30f && row.cut > -1e30f && temperature > 1e-30f && temperature < 1e30f;
-    row.form = capped ? kCapped : ordinary ? kPlain : kAny;
+    row.form = !ordinary ? kAny : capped ? kCapped : row.cut > -1e30f ? kPlain : kAny;
   }
   __syncthreads();
 
@@ -1461,8 +1491,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   } else if (rules.by_count) {
     if (top_k <= kCap / 8) from = lower;
   } else if (rules.by_floor) {
-    // Nothing further below the largest than this has a share of min_p; capped values: above where the cap's inverse is.
-    double y = sh.row.top + degrees * log(rules.min_p);
+    // Nothing further below the largest than this has a share of min_p (a share next to it may be rounded to it: at high temperatures many are
+    // one); capped values: above where the cap's inverse is.
+    double y = sh.row.top + degrees * (log(rules.min_p) - 1e-12);
     if (capped) {
       const double z = y / p.softcap - 1e-12;
       y = z > -1.0 ? p.softcap * 0.5 * log((1.0 + z) / fmax(1.0 - z, 1e-30)) : -INFINITY;

@@ -33,6 +33,15 @@ int main() {
     if (scale < 1e30) ends &= gv::share_with(0.0, scale, gv::share_whole(0.0f, static_cast<float>(scale)), table, 1) == 1.0;
   }
   ends &= gv::share_of(-1e6, 46.0, table, 1) == 0.0 && gv::share_of(-INFINITY, 46.0, table, 1) == 0.0;
+  // floats as doubles
+  bool wide = true;
+  for (uint32_t bits = 0x00800000u; bits < 0x7f800000u; bits += 9973u) {
+    float x;
+    memcpy(&x, &bits, 4);
+    wide &= gv::wide_of(x) == static_cast<double>(x) && gv::wide_of(-x) == -static_cast<double>(x);
+  }
+  wide &= fabs(gv::wide_of(0.0f)) < 1e-38 && fabs(gv::wide_of(-0.0f)) < 1e-38 && fabs(gv::wide_of(1e-45f)) < 2e-38;
+  wide &= gv::wide_of(3.402823466e38f) == static_cast<double>(3.402823466e38f);
   // the order of floats
   const float values[] = {-INFINITY, -3.402823466e38f, -1.0f, -1e-45f, 0.0f, 1e-45f, 1.0f, 3.402823466e38f, INFINITY};
   bool order = gv::order_of(-INFINITY) == gv::kNothing && gv::order_of(-0.0f) == gv::order_of(0.0f);
@@ -40,7 +49,7 @@ int main() {
     order &= gv::value_of(gv::order_of(values[i])) == values[i];
     if (i) order &= gv::order_of(values[i]) > gv::order_of(values[i - 1]);
   }
-  printf("%.2f %.2f %.2f %.2f %.2f %d %d\n", static_cast<double>(log2l(worst_table)), static_cast<double>(log2l(worst_rest)),
-         static_cast<double>(log2l(worst_finely)), static_cast<double>(log2l(worst_with)), static_cast<double>(log2l(worst_of)), ends, order);
+  printf("%.2f %.2f %.2f %.2f %.2f %d %d %d\n", static_cast<double>(log2l(worst_table)), static_cast<double>(log2l(worst_rest)),
+         static_cast<double>(log2l(worst_finely)), static_cast<double>(log2l(worst_with)), static_cast<double>(log2l(worst_of)), ends, wide, order);
   return 0;
 }

@@ -290,7 +290,8 @@ def settings(name, rows):
     return {n: torch.tensor([x[i % len(x)] for i in range(rows)], dtype=kinds[n], device=DEV) for n, x in SETTINGS[name].items()}
 
 
-def compare(logits, uniforms, given, softcap=0.0, most_near=0.2, **more):
+def compare(logits, uniforms, given, softcap=0.0, most_near=0.2, off=0.0, **more):
+    """`off`: by how much exponents may be off beyond the last bits of 64."""
     tokens, shares = step.sample_tokens(logits, uniforms, softcap=softcap, probability=True, **given, **more)
     rows = logits.float().cpu().numpy().astype(np.float64)
     host = {n: t.cpu().double().tolist() for n, t in given.items()}
@@ -301,11 +302,11 @@ def compare(logits, uniforms, given, softcap=0.0, most_near=0.2, **more):
         if "top_k" in one:
             one["top_k"] = int(one["top_k"])
         token, share, border = step_ref.sample(rows[r], u[r], softcap=softcap, **one)
-        if border < NEAR:
+        if border < NEAR + 2 * off:
             near += 1
             continue
         assert got[r] == token, (r, one, got[r], token, border)
-        assert abs(got_shares[r] - share) <= 2.0 ** -23 * share, (r, one, got_shares[r], share)
+        assert abs(got_shares[r] - share) <= (2.0 ** -23 + 2 * off) * share, (r, one, got_shares[r], share)
     assert near <= most_near * len(rows)
     return tokens
 
@@ -349,6 +350,45 @@ def test_capped(name, softcap, vocabulary):
     for dtype in (torch.float32, torch.bfloat16):
         for kind in ("ahead", "masked"):
             compare(logits_of(kind, gen, 5, vocabulary, dtype), torch.rand(5, generator=gen, device=DEV), settings(name, 5), softcap)
+
+
+@pytest.mark.parametrize("softcap", [1e-40, 1e-6, 0.02, 100.0, 1e3, 1e5, 1e8, 1e20, 1e38])
+@pytest.mark.parametrize("vocabulary", [100, 9000, 70001])
+def test_capped_by_any_size(softcap, vocabulary):
+    """Caps far above the logits change next to nothing, those far below them leave ranks alone; temperatures on both sides of the cap's size.
+    Two of five floors are one, to which
+    the shares 1 - 2 exp(-2 |x| / cap) cap / T of values beyond 13 caps come nearer than can be told.  (Where |x| is over cap / 185, softened values are off by cap * 2^-51, of |x| <= 15 at most 2775 * 2^-51 = 1.3e-12 over T = 0.3, twice.)"""
+    gen = generator(vocabulary + 3)
+    for temperature in (0.3, 1.0, max(softcap, 1e-30)):
+        for name in ("open", "count", "sum", "floor"):
+            given = settings(name, 5)
+            given["temperature"] = torch.full((5,), min(temperature, 1e37), device=DEV)
+            for kind in ("ahead", "masked"):
+                compare(logits_of(kind, gen, 5, vocabulary, torch.float32), torch.rand(5, generator=gen, device=DEV), given, softcap, off=1e-11, most_near=0.4)
+            assert given["temperature"].isfinite().all()
+
+
+@pytest.mark.parametrize("vocabulary", [100, 9000, 70001])
+def test_hot(vocabulary):
+    """Shares that are one, or next to it, at temperatures far above the logits.  (Two of seven floors are one, to which 1 - 10 / T comes nearer
+    than can be told at 10^12.)"""
+    gen = generator(vocabulary + 4)
+    for temperature in (1e3, 1e12, 1e20, 1e36):
+        for name in ("open", "count", "sum", "floor"):
+            given = dict(settings(name, 7), temperature=torch.full((7,), temperature, device=DEV))
+            compare(logits_of("masked", gen, 7, vocabulary, torch.bfloat16), torch.rand(7, generator=gen, device=DEV), given, most_near=0.3)
+
+
+@pytest.mark.parametrize("temperature", [1e-7, 1e-5, 1e-3, 0.05, 0.2, 0.24])
+def test_capped_and_cold(temperature):
+    """Values a few steps of 32 bits apart, whose shares are apart by ordinary factors at low temperatures.  (Softened values of up
+    to 30 are off by 30 * 2^-51.3 here and 12 * 3 * 2^-53 there, a distance by twice that: 3e-14, over T.)"""
+    gen = generator(5)
+    for vocabulary in (64, 5000, 70001):
+        logits = 12.0 + torch.rand(6, vocabulary, generator=gen, device=DEV) * temperature * 30
+        given = dict(temperature=torch.full((6,), temperature, device=DEV))
+        compare(logits, torch.rand(6, generator=gen, device=DEV), given, 30.0, off=3e-14 / temperature)
+        compare(logits, torch.rand(6, generator=gen, device=DEV), dict(given, top_p=torch.full((6,), 0.8, device=DEV)), 30.0, off=3e-14 / temperature)
 
 
 @pytest.mark.parametrize("name", list(SETTINGS))
