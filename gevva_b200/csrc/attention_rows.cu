@@ -126,18 +126,24 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) block_norm_kernel(c
 // ---- queries, keys and values: per-head norms, rotation, the cache -----------------------------------------
 constexpr int kMaxDim = 512;
 
+// Of queries, keys and values by number: what a head has is read by its kind, which costs an indexed read of the constants instead of a
+// choice for each word of each.
+struct AppendSide {
+  const uint4* weight;
+  __nv_bfloat16 *out, *cache;
+  long long page_stride, slot_stride, head_stride;  // of the cache
+  int first_head, heads, norm, turns;
+};
 struct AppendParams {
-  AttnRows q, k, v;
+  AttnRows rows[3];
+  AppendSide side[3];
   AttnPages pages;
   const int* token_offsets;
   int sequences, tokens, heads, kv_heads;
   const double* frequencies;
   int half;        // frequencies: the pairs (j, half + j) turn
   int page_shift;
-  const uint4 *q_weight, *k_weight;
-  bool normalize_v;
   float eps;
-  __nv_bfloat16 *q_out, *k_out, *v_out;
   int* status;
   // at given places
   const int *slots, *positions;
@@ -169,11 +175,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   grid_launch_dependents();
   grid_dependency_wait();
 
+  const auto kind_of = [&](int h) { return (h >= p.heads) + (h >= p.heads + p.kv_heads); };
   const auto source = [&](int token, int h) {
-    const AttnRows& from = h < p.heads ? p.q : h < p.heads + p.kv_heads ? p.k : p.v;
-    const int head = h < p.heads ? h : h < p.heads + p.kv_heads ? h - p.heads : h - p.heads - p.kv_heads;
+    const int kind = kind_of(h);
+    const AttnRows& from = p.rows[kind];
     return reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(from.data) + token * from.token_stride +
-                                          head * from.head_stride);
+                                          (h - p.side[kind].first_head) * from.head_stride);
   };
   uint4 a[2], b[2];  // of two heads, asked for together
   const auto ask = [&](int token, int first) {
@@ -182,8 +189,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
       const int h = first + k * heads_at_once;
       a[k] = b[k] = make_uint4(0, 0, 0, 0);
       if (h < total) {
-        a[k] = source(token, h)[low];
-        b[k] = source(token, h)[high];
+        const uint4* const from = source(token, h);
+        a[k] = from[low];
+        b[k] = from[high];
       }
     }
   };
@@ -282,13 +290,13 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   for (int k = 0; k < 2; ++k) {
     const int h = first_head + k * heads_at_once;
     if (h >= total) break;
-    const int kind = h < p.heads ? 0 : h < p.heads + p.kv_heads ? 1 : 2;  // query, key, value
-    const int head = kind == 0 ? h : kind == 1 ? h - p.heads : h - p.heads - p.kv_heads;
+    const AppendSide& side = p.side[kind_of(h)];
+    const int head = h - side.first_head;
     float x[8], y[8];
     unpack8(low_now[k], x);
     unpack8(high_now[k], y);
-    const uint4* weight = kind == 0 ? p.q_weight : kind == 1 ? p.k_weight : nullptr;
-    if (kind == 2 ? p.normalize_v : weight != nullptr) {  // (the same for all threads of a head, which are in one warp)
+    const uint4* weight = side.weight;
+    if (side.norm) {  // (the same for all threads of a head, which are in one warp)
       float s = squares(x) + squares(y);
       const uint32_t mates = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes);
 #pragma unroll
@@ -309,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
         }
       }
     }
-    if (kind != 2 && turns) {
+    if (side.turns && turns) {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
         const float4 c = *reinterpret_cast<const float4*>(cosines + g * 4 * quarters + 4 * u);
@@ -324,18 +332,15 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
       }
     }
     const uint4 first = pack8(x), second = pack8(y);
-    const size_t row = static_cast<size_t>(token) * (kind == 0 ? p.heads : p.kv_heads) + head;
-    __nv_bfloat16* out = kind == 0 ? p.q_out : kind == 1 ? p.k_out : p.v_out;
+    const size_t row = static_cast<size_t>(token) * side.heads + head;
+    __nv_bfloat16* out = side.out;
     if (out) {
       reinterpret_cast<uint4*>(out + row * kDim)[low] = first;
       reinterpret_cast<uint4*>(out + row * kDim)[high] = second;
     }
-    if (kind != 0 && stored) {
-      const AttnPages& c = p.pages;
-      __nv_bfloat16* cache = kind == 1 ? static_cast<__nv_bfloat16*>(c.keys) + page * c.key_page_stride + slot * c.key_slot_stride +
-                                             head * c.key_head_stride
-                                       : static_cast<__nv_bfloat16*>(c.values) + page * c.value_page_stride + slot * c.value_slot_stride +
-                                             head * c.value_head_stride;
+    __nv_bfloat16* cache = side.cache;
+    if (cache && stored) {
+      cache += page * side.page_stride + slot * side.slot_stride + head * side.head_stride;
       reinterpret_cast<uint4*>(cache)[low] = first;
       reinterpret_cast<uint4*>(cache)[high] = second;
     }
@@ -387,10 +392,16 @@ namespace {
 
 AppendParams append_params(const AppendCall& call) {
   AppendParams p{};
-  p.q = call.q;
-  p.k = call.k;
-  p.v = call.v;
-  p.pages = call.pages;
+  p.rows[0] = call.q;
+  p.rows[1] = call.k;
+  p.rows[2] = call.v;
+  const AttnPages& c = call.pages;
+  p.side[0] = {static_cast<const uint4*>(call.q_weight), static_cast<__nv_bfloat16*>(call.q_out), nullptr, 0, 0, 0, 0, call.heads, call.q_weight != nullptr, 1};
+  p.side[1] = {static_cast<const uint4*>(call.k_weight), static_cast<__nv_bfloat16*>(call.k_out), static_cast<__nv_bfloat16*>(c.keys),
+               c.key_page_stride, c.key_slot_stride, c.key_head_stride, call.heads, call.kv_heads, call.k_weight != nullptr, 1};
+  p.side[2] = {nullptr, static_cast<__nv_bfloat16*>(call.v_out), static_cast<__nv_bfloat16*>(c.values),
+               c.value_page_stride, c.value_slot_stride, c.value_head_stride, call.heads + call.kv_heads, call.kv_heads, call.normalize_v, 0};
+  p.pages = c;
   p.token_offsets = call.token_offsets;
   p.sequences = call.sequences;
   p.tokens = call.tokens;
@@ -398,13 +409,7 @@ AppendParams append_params(const AppendCall& call) {
   p.kv_heads = call.kv_heads;
   p.frequencies = call.frequencies;
   p.half = call.rotated / 2;
-  p.q_weight = static_cast<const uint4*>(call.q_weight);
-  p.k_weight = static_cast<const uint4*>(call.k_weight);
-  p.normalize_v = call.normalize_v;
   p.eps = call.eps;
-  p.q_out = static_cast<__nv_bfloat16*>(call.q_out);
-  p.k_out = static_cast<__nv_bfloat16*>(call.k_out);
-  p.v_out = static_cast<__nv_bfloat16*>(call.v_out);
   p.status = call.status;
   while ((1 << p.page_shift) < call.pages.page_size) ++p.page_shift;
   return p;
