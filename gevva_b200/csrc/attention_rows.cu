@@ -172,8 +172,24 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   const bool turns = u < eighth;
   const int low = turns ? u : 2 * u, high = turns ? u + eighth : 2 * u + 1;  // vectors
   const int total = p.heads + 2 * p.kv_heads;
+  // Many tokens: the weights of queries and of keys, of each lane its two vectors by halves, as numbers of 32 bits.
+  __shared__ float4 weights[kMany ? 2 : 1][4][kMany ? kLanes : 1];
   grid_launch_dependents();
   grid_dependency_wait();
+  if constexpr (kMany) {
+    if (threadIdx.x < 2 * kLanes) {
+      const int kind = threadIdx.x / kLanes;
+      if (p.side[kind].weight) {
+        float w[8], z[8];
+        unpack8(p.side[kind].weight[low], w);
+        unpack8(p.side[kind].weight[high], z);
+        weights[kind][0][u] = make_float4(w[0], w[1], w[2], w[3]);
+        weights[kind][1][u] = make_float4(w[4], w[5], w[6], w[7]);
+        weights[kind][2][u] = make_float4(z[0], z[1], z[2], z[3]);
+        weights[kind][3][u] = make_float4(z[4], z[5], z[6], z[7]);
+      }
+    }
+  }
 
   const auto kind_of = [&](int h) { return (h >= p.heads) + (h >= p.heads + p.kv_heads); };
   const auto source = [&](int token, int h) {
@@ -290,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
   for (int k = 0; k < 2; ++k) {
     const int h = first_head + k * heads_at_once;
     if (h >= total) break;
-    const AppendSide& side = p.side[kind_of(h)];
+    const int kind = kind_of(h);
+    const AppendSide& side = p.side[kind];
     const int head = h - side.first_head;
     float x[8], y[8];
     unpack8(low_now[k], x);
@@ -304,8 +321,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == kAppendManyThreads ? kAp
       const float inverse = rsqrtf(fmaf(s, 1.0f / kDim, p.eps));
       float w[8], z[8];
       if (weight) {
-        unpack8(weight[low], w);
-        unpack8(weight[high], z);
+        if constexpr (kMany) {
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const float4 first = weights[kind][g][u], second = weights[kind][2 + g][u];
+            w[4 * g] = first.x, w[4 * g + 1] = first.y, w[4 * g + 2] = first.z, w[4 * g + 3] = first.w;
+            z[4 * g] = second.x, z[4 * g + 1] = second.y, z[4 * g + 2] = second.z, z[4 * g + 3] = second.w;
+          }
+        } else {
+          unpack8(weight[low], w);
+          unpack8(weight[high], z);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
