@@ -155,10 +155,13 @@ struct AppendParams {
 // eight pairs of a head: the two halves of a pair come from two 16-byte vectors, (u, half / 8 + u) where pairs turn and two neighbours
 // behind them, so nothing is exchanged.  Its first vectors are asked for before the token's place is looked up, behind the last ones of
 // the token before.
-// 4608 tokens of 32 heads of 256, packed: 38.6 us, of which 28.8 are its bytes; with a CTA for each token 40.8.
+// 4608 tokens of 32 heads of 256, packed: 35.9 us, of which 28.8 are its bytes (38.7 with queries, keys and values told apart by choices
+// and weights read as they are; with a CTA for each token 2 more).
 // kPlaced: slots and positions are given, one read instead of the look-ups of sequence, length and page; a position for each axis, and
 // frequencies for each, most of them zero: a pair's angle is their sum of products, exactly its axis's product where the others are zero.
 // The next token's are asked for in front of a token's heads and worked out behind them, into the other half of the arrays: one barrier a token.
+// 64 tokens 2.8 us, 4608 (as above, three axes) 37.1, 16384 of 48 heads of 128 90 of 62 for its bytes: two thirds of the issue slots are taken, at 20 warps an SM.
+// (Multiplications two an instruction 94 us; six CTAs an SM with 80 registers 104.)
 constexpr int kAppendThreads = 512, kAppendManyThreads = 128;
 constexpr int kAppendManyCtas = 5;  // of an SM (with six: 80 registers, which do not hold it all)
 template <int kDim, int kThreads, bool kPlaced>

@@ -374,7 +374,7 @@ int gevva_ff_layer_launch(const gevva_ff_layer* layer, const void* hidden, void*
  * status word that receives GEVVA_MOE_WAIT_TIMEOUT or GEVVA_MOE_BAD_PAGE, negated, as the runners' words do; NULL: one that the library
  * has for each device, which gevva_attention_last_status reads. */
 
-/* Reads and clears the status of the attention calls on the current device that were given no word (synchronises the device). */
+/* Reads and clears the status of the attention and step calls on the current device that were given no word (synchronises the device). */
 int gevva_attention_last_status(void);
 
 /* A paged cache: keys and values are bf16 [pages, page_size, kv_heads, dim] with strides of their own; page_size is a power of two,

@@ -379,6 +379,26 @@ def test_hot(vocabulary):
             compare(logits_of("masked", gen, 7, vocabulary, torch.bfloat16), torch.rand(7, generator=gen, device=DEV), given, most_near=0.3)
 
 
+@pytest.mark.parametrize("vocabulary", [100, 9000, 70001])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_settings_at_the_ends_of_their_types(vocabulary, softcap):
+    gen = generator(vocabulary + 6)
+    for temperature in (1e-45, 1e-38, 1e-31, 3e38, math.inf):
+        for name in ("open", "count", "sum"):
+            given = dict(settings(name, 7), temperature=torch.full((7,), temperature, device=DEV))
+            compare(logits_of("masked", gen, 7, vocabulary, torch.bfloat16), torch.rand(7, generator=gen, device=DEV), given, softcap, off=1e-15)
+    # no number: none of that rule, and of a random number zero; others are taken to be in [0, 1)
+    logits = logits_of("bulk", gen, 5, vocabulary, torch.float32)
+    u = torch.rand(5, generator=gen, device=DEV)
+    nan = torch.full((5,), math.nan, device=DEV)
+    zeros, ones = torch.zeros(5, device=DEV), torch.full((5,), 1 - 2.0 ** -24, device=DEV)
+    assert torch.equal(step.sample_tokens(logits, u, top_p=nan, min_p=nan, softcap=softcap), step.sample_tokens(logits, u, softcap=softcap))
+    assert torch.equal(step.sample_tokens(logits, u, temperature=nan, softcap=softcap), logits.argmax(1).int())
+    for bad, same in ((nan, zeros), (zeros - 3, zeros), (zeros - math.inf, zeros), (zeros + 1, ones), (zeros + math.inf, ones)):
+        for more in ({}, dict(top_p=zeros + 0.9), dict(top_k=torch.full((5,), 70, dtype=torch.int32, device=DEV))):
+            assert torch.equal(step.sample_tokens(logits, bad, softcap=softcap, **more), step.sample_tokens(logits, same, softcap=softcap, **more))
+
+
 @pytest.mark.parametrize("temperature", [1e-7, 1e-5, 1e-3, 0.05, 0.2, 0.24])
 def test_capped_and_cold(temperature):
     """Values a few steps of 32 bits apart, whose shares are apart by ordinary factors at low temperatures.  (Softened values of up
