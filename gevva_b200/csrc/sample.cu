@@ -35,6 +35,7 @@ constexpr int kMostCtas = 16;
 constexpr int kLevels = 10;       // groups of 2^level threads
 constexpr int kSums = 3;
 constexpr int kBins = 1024;       // of equal width over a range of values
+constexpr int kEdges = 8;        // of four windows in the bins
 constexpr int kAhead = 8;         // vectors that a thread has on their way: an L2 read takes as long as a warp works on these
 constexpr int kTableCopies = 16;  // of the table of 2^(j/32), one for each lane of half a warp: no two lanes of a read meet in a bank
 
@@ -49,7 +50,7 @@ enum BinsSay : int { kNotHere, kLookCloser, kInList, kListHasAll };  // (all: th
 struct BinWindow {
   int first, last;
   BinsSay says;
-  int sure_first, sure_last;  // what holds it in any case
+  int sure_first, sure_last;  // what holds it in any case (kBins: that may be behind all bins)
 };
 // Bins of equal width from `high` (bin 0's middle) down to `low`; a bin's values are the nearest to its middle.
 struct Bins {
@@ -110,7 +111,7 @@ struct SampleShared {
   unsigned long long border, kept; // from the first CTA: the border's entry, and how many of the list are up to it
   uint32_t warp_key[kWarps], warp_index[kWarps], warp_levels[kWarps][5];
   int mine_count, list_count, base, found;
-  int edges[6];
+  int edges[kEdges];
 };
 extern __shared__ uint4 sample_memory[];
 template <int kThreads>
@@ -280,6 +281,15 @@ __device__ __noinline__ double softened_any(float x, const Cap& c, const double*
     y = c.cap * ((1.0 - e) / (1.0 + e));
   }
   return x < 0.0f ? -y : y;
+}
+// A little below the value with the largest one's y and so many temperatures less: where there is a cap, below where its inverse is.
+__device__ __noinline__ double value_below(const RowState& row, double degrees, double temperatures) {
+  double y = row.top - degrees * temperatures;
+  if (row.cap.cap > 0.0) {
+    const double z = y / row.cap.cap - 1e-12;
+    y = z > -1.0 ? row.cap.cap * 0.5 * log((1.0 + z) / fmax(1.0 - z, 1e-30)) : -INFINITY;
+  }
+  return y - 1e-6 * (fabs(y) + fabs(static_cast<double>(row.largest)));
 }
 template <int kThreads>
 __device__ __forceinline__ const double* lane_table() {
@@ -951,9 +961,10 @@ __device__ __noinline__ uint32_t order_with(Bins bins, int bin, uint32_t low, ui
 
 // Where the counts say that `target` is reached, with `above` in front of the bins.  Counts times the shares of their bins' middles are off by up to
 // `off` of themselves: the border lies between where they reach the target with that much more and with that much less.  Where
-// that is more than the list holds, it is looked at with a quarter or a sixteenth of it (errors of many bins cancel; sums will tell), or closer.
+// that is more than the list holds, it is looked at with a quarter, a sixteenth or a 64th of it (errors of many bins cancel; sums will tell), or
+// closer.  `surely`: it is in the bins, whatever the counts say.  (With a sixteenth as the least 48 of 256 rows of 128000 by top_p were looked at again.)
 template <int kThreads>
-__device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double above, double target, double off, int turn) {
+__device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double above, double target, double off, bool surely, int turn) {
   SampleShared<kThreads>& sh = shared<kThreads>();
   constexpr int kCap = SampleShared<kThreads>::kCap, kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas, rank = sh.row.rank;
@@ -1013,7 +1024,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       sh.warp_index[warp] = counts;
       sh.warp_key[warp] = __float_as_uint(masses);
     }
-    if (threadIdx.x < 6) sh.edges[threadIdx.x] = kBins;
+    if (threadIdx.x < kEdges) sh.edges[threadIdx.x] = kBins;
     __syncthreads();
     int count_upto = counts - counted;
     float mass_upto = masses - massed;
@@ -1023,8 +1034,14 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       mass_upto += w < warp ? __uint_as_float(sh.warp_key[w]) : 0.0f;
     }
     // the target for counts' sums, by each edge
-    const float rest = static_cast<float>(target - above), o = static_cast<float>(off), less = 0.25f * fminf(o, 1.0f), few = 0.06f * fminf(o, 1.0f);
-    const float edge[6] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY, rest / (1.0f + less), rest / (1.0f - less), rest / (1.0f + few), rest / (1.0f - few)};
+    const float rest = static_cast<float>(target - above), o = static_cast<float>(off);
+    float edge[kEdges] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY};
+#pragma unroll
+    for (int e = 2; e < kEdges; e += 2) {
+      const float less = fminf(o, 1.0f) / (e == 2 ? 4.0f : e == 4 ? 16.0f : 64.0f);
+      edge[e] = rest / (1.0f + less);
+      edge[e + 1] = rest / (1.0f - less);
+    }
     const double missing = target - above;
 #pragma unroll
     for (int i = 0; i < kOf; ++i) {
@@ -1035,7 +1052,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       mass_upto += mass[i];
       sh.bins[bin] = count_upto;
 #pragma unroll
-      for (int e = 0; e < 6; ++e) {  // (each edge is passed in one bin)
+      for (int e = 0; e < kEdges; ++e) {  // (each edge is passed in one bin)
         if (shares ? mass_upto >= edge[e] && (mass_before < edge[e] || bin == 0) : count_upto >= missing && (count_before < missing || bin == 0))
           atomicMin(&sh.edges[e], bin);
       }
@@ -1043,24 +1060,24 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
     __syncthreads();
     if (warp == 0) {
       const auto upto = [&](int bin) { return bin < 0 ? 0 : sh.bins[bin]; };
-      const int sure_first = sh.edges[0], sure_last = min(sh.edges[1], kBins - 1);
-      BinWindow window{sure_first, sure_last, kNotHere, sure_first, sure_last};
+      const int sure_first = sh.edges[0], sure_last = surely ? min(sh.edges[1], kBins - 1) : sh.edges[1];
+      BinWindow window{sure_first, min(sure_last, kBins - 1), kNotHere, sure_first, sure_last};
       if (window.first < kBins) {
         if (sh.edges[1] < kBins && above == 0.0 && upto(window.last) <= kCap) {
           window.first = 0;
           window.says = kListHasAll;
         } else if (upto(window.last) - upto(window.first - 1) <= kCap) {
           window.says = kInList;
-        } else if (sh.edges[3] < kBins && upto(sh.edges[3]) - upto(sh.edges[2] - 1) <= kCap) {
-          window.first = sh.edges[2];
-          window.last = sh.edges[3];
-          window.says = kInList;
-        } else if (sh.edges[5] < kBins && upto(sh.edges[5]) - upto(sh.edges[4] - 1) <= kCap) {
-          window.first = sh.edges[4];
-          window.last = sh.edges[5];
-          window.says = kInList;
-        } else if (window.first > 0 || window.last < kBins - 1) {  // (else a closer look would see the same)
-          window.says = kLookCloser;
+        } else {
+          if (window.first > 0 || window.last < kBins - 1) window.says = kLookCloser;  // (else it would see the same)
+          for (int e = 2; e < kEdges; e += 2) {
+            if (sh.edges[e + 1] < kBins && upto(sh.edges[e + 1]) - upto(sh.edges[e] - 1) <= kCap) {
+              window.first = sh.edges[e];
+              window.last = sh.edges[e + 1];
+              window.says = kInList;
+              break;
+            }
+          }
         }
       }
       if (lane < ctas)
@@ -1499,14 +1516,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   } else if (rules.by_count) {
     if (top_k <= kCap / 8) from = lower;
   } else if (rules.by_floor) {
-    // Nothing further below the largest than this has a share of min_p (a share next to it may be rounded to it: at high temperatures many are
-    // one); capped values: above where the cap's inverse is.
-    double y = sh.row.top + degrees * (log(rules.min_p) - 1e-12);
-    if (capped) {
-      const double z = y / p.softcap - 1e-12;
-      y = z > -1.0 ? p.softcap * 0.5 * log((1.0 + z) / fmax(1.0 - z, 1e-30)) : -INFINITY;
-    }
-    y -= 1e-6 * (fabs(y) + fabs(static_cast<double>(most)));
+    // Nothing further below the largest than this has a share of min_p (a share next to it may be rounded to it: at high temperatures many are one).
+    const double y = value_below(sh.row, degrees, 1e-12 - log(rules.min_p));
     const float bound = y > static_cast<double>(most) ? most : __double2float_rd(y);
     from = bound == bound ? max(order_of(bound), kNothing + 1) : kNothing + 1;
   }
@@ -1529,9 +1540,14 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   for (int rule = 0; rule < 2 && listed < 0; ++rule) {  // top_k, then top_p
     if (rule == 0 ? !rules.by_count : !rules.by_sum) continue;
     const bool shares = rule == 1;
-    // Counts: from the bound that the groups gave.  Shares: those from 2^-35 of the largest on; where the border is further down, halving finds it.
+    // Counts: from the bound that the groups gave.  Shares: n values below a share of (1 - top_p) / n have less than 1 - top_p together, which is less
+    // than what top_p leaves out (the largest alone has a share of one), so the border is above that; but no further than 24 temperatures (2^-35 of the
+    // largest), or bins would be wide: where the border is further down, halving finds it.
     const uint32_t border_key = sh.row.border_key;
-    const uint32_t near = max(order_of(__double2float_rd(static_cast<double>(most) - 24.0 * degrees)), border_key);
+    const double bottom = static_cast<double>(most) - 24.0 * degrees;
+    const double reach = shares ? value_below(sh.row, degrees, logf((rules.by_count ? top_k : p.vocabulary) / (1.0f - top_p)) + 0.01f) : bottom;
+    bool surely = reach >= bottom;
+    const uint32_t near = max(order_of(__double2float_rd(fmax(reach, bottom))), border_key);
     uint32_t low = min(shares || value_of(lower) < -1e30f ? near : lower, largest), high = largest;
     uint32_t sure_low = border_key, sure_high = largest;  // the border lies between these
     double target = top_k, above = 0.0, all = 0.0;
@@ -1551,7 +1567,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
       // (half a bin, and what 32 bits lose of it)
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
       const double off = shares ? (0.505 / (kBins - 1) * (static_cast<double>(bins.high) - bins.low) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
-      const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, turn);
+      const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, surely, turn);
       if (window.says == kNotHere || low == high) break;
       if (window.says == kInList || window.says == kListHasAll) {
         const uint32_t next_low = order_with(bins, window.last, low, high);
@@ -1581,6 +1597,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         }
       }
       // Closer.
+      if (window.sure_last >= kBins) break;
+      surely = true;
       const uint32_t next_low = order_with(bins, window.sure_last, low, high);
       const uint32_t next_high = window.sure_first > 0 ? order_below(order_with(bins, window.sure_first - 1, low, high)) : high;
       if (next_low == low && next_high == high) break;

@@ -379,6 +379,23 @@ def test_hot(vocabulary):
             compare(logits_of("masked", gen, 7, vocabulary, torch.bfloat16), torch.rand(7, generator=gen, device=DEV), given, most_near=0.3)
 
 
+@pytest.mark.parametrize("vocabulary", [9000, 70001, 262144])
+@pytest.mark.parametrize("softcap", [0.0, 1.0, 12.0, 40.0])
+def test_borders_far_below_the_largest(vocabulary, softcap):
+    """A border among many values whose shares are next to none, or whose cap leaves them as much as the largest.  (Shares of
+    exp(-25) = 1.4e-11 of the whole lie between borders: 2 * 2^-40 = 1.8e-12 of it is near one, in one of eight rows, by top_p and by the number.)"""
+    gen = generator(vocabulary + 7)
+    rows = 6
+    logits = torch.randn(rows, vocabulary, generator=gen, device=DEV) * torch.tensor([0.1, 1.0, 4.0, 0.5, 2.0, 8.0], device=DEV)[:, None] - 25.0
+    logits.scatter_(1, torch.randint(0, vocabulary, (rows, 1), generator=gen, device=DEV), 0.0)
+    for p in (1 - 2.0 ** -24, 1 - 2.0 ** -20, 0.9999, 0.99, 0.5):
+        for temperature in (1.0, 1.5, 6.0):
+            given = dict(temperature=torch.full((rows,), temperature, device=DEV), top_p=torch.full((rows,), p, device=DEV))
+            u = torch.rand(rows, generator=gen, device=DEV)
+            compare(logits, u, given, softcap, most_near=0.7)
+            compare(logits, 1 - u * 2.0 ** -18, given, softcap, most_near=0.7)
+
+
 @pytest.mark.parametrize("vocabulary", [100, 9000, 70001])
 @pytest.mark.parametrize("softcap", [0.0, 30.0])
 def test_settings_at_the_ends_of_their_types(vocabulary, softcap):
