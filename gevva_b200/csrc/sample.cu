@@ -99,11 +99,7 @@ struct SampleShared {
     int4 bins4[kBins / 4];
     int bins[kBins + 32];            // (behind them one for each lane that has nothing to count: no branch, no conflict)
   };
-  union {
-    unsigned long long list[kCap];   // the cluster's, in its first CTA
-    int4 totals4[kBins / 4];         // the cluster's bins there
-    int totals[kBins];               // (elsewhere what the CTA adds up of them)
-  };
+  unsigned long long list[kCap];     // the cluster's, in its first CTA
   uint4 first[kMostCtas][4];       // largest key, levels, settings
   double slots[2][kMostCtas][kSums];
   double warp_sums[kWarps][kSums];
@@ -766,6 +762,7 @@ __device__ __noinline__ double sum_listed() {
 struct Gathered {
   int count;
   Sifted sifted;  // this lane's
+  Sifted sums;    // the cluster's
 };
 template <typename T, int kThreads>
 __device__ __noinline__ Gathered gather(uint32_t low, uint32_t high, float before, bool measured, bool shares, bool whole, int which) {
@@ -776,10 +773,26 @@ __device__ __noinline__ Gathered gather(uint32_t low, uint32_t high, float befor
   __syncthreads();
   Gathered got;
   got.sifted = sift_row<T, kThreads>(false, value_of(low), value_of(high), before, measured, shares, whole, Bins{});
+  const double above = warp_sum(got.sifted.above), all = warp_sum(got.sifted.all);
+  if (lane == 0) {
+    sh.warp_sums[warp][0] = above;
+    sh.warp_sums[warp][1] = all;
+  }
   __syncthreads();
   const int count = sh.mine_count;
   if (warp == 0) {
-    if (lane < ctas) cluster_store_double(cluster_map_shared(smem_u32(&sh.slots[which][sh.row.rank][0]), lane), static_cast<double>(count));
+    if (lane < ctas) {  // (the sums go with the count: no exchange of their own)
+      double own[2] = {0.0, 0.0};
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) {
+        own[0] += sh.warp_sums[w][0];
+        own[1] += sh.warp_sums[w][1];
+      }
+      const uint32_t peer = cluster_map_shared(smem_u32(&sh.slots[which][sh.row.rank][0]), lane);
+      cluster_store_double(peer, static_cast<double>(count));
+      cluster_store_double(peer + 8, own[0]);
+      cluster_store_double(peer + 16, own[1]);
+    }
     if (lane == 0) sh.base = count > 0 && count <= kCap ? cluster_add(cluster_map_shared(smem_u32(&sh.list_count), 0), count) : kCap;
   }
   __syncthreads();
@@ -790,10 +803,11 @@ __device__ __noinline__ Gathered gather(uint32_t low, uint32_t high, float befor
       if (base + i < kCap) cluster_store_u64(list + 8 * (base + i), sh.mine[i]);
   }
   cluster_barrier<kThreads>();
-  double sum = 0.0;
-  for (int r = 0; r < ctas; ++r) sum += sh.slots[which][r][0];
+  const double* slot = sh.slots[which][lane & (kMostCtas - 1)];
+  const bool one = lane < ctas;
   if (threadIdx.x == 0) sh.list_count = 0;  // (for the next gathering, which a barrier comes before)
-  got.count = static_cast<int>(sum);
+  got.count = static_cast<int>(warp_sum(one ? slot[0] : 0.0));
+  got.sums = {warp_sum(one ? slot[1] : 0.0), warp_sum(one ? slot[2] : 0.0)};
   return got;
 }
 
@@ -968,41 +982,34 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
   SampleShared<kThreads>& sh = shared<kThreads>();
   constexpr int kCap = SampleShared<kThreads>::kCap, kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ctas = sh.row.ctas, rank = sh.row.rank;
-  if (ctas > 1) {
-    // Each CTA adds up its part of the bins, a quarter of a thousand reads of 16 bytes, and puts it with the first one's.
-    const int part = kBins / 4 / ctas;  // (a power of two)
-    for (int i = threadIdx.x; i < 4 * part; i += kThreads) sh.totals[i] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins / 4; i += kThreads) {
-      const int quad = i & (part - 1);
-      const int4 four = cluster_load4(cluster_map_shared(smem_u32(&sh.bins4[rank * part + quad]), i / part));
-      if (four.x) atomicAdd(&sh.totals[4 * quad], four.x);
-      if (four.y) atomicAdd(&sh.totals[4 * quad + 1], four.y);
-      if (four.z) atomicAdd(&sh.totals[4 * quad + 2], four.z);
-      if (four.w) atomicAdd(&sh.totals[4 * quad + 3], four.w);
-    }
-    __syncthreads();
-    if (rank > 0) {  // (the first one's own part stands where it belongs, the others' behind it)
-      const uint32_t to = cluster_map_shared(smem_u32(&sh.totals4[rank * part]), 0);
-      for (int i = threadIdx.x; i < part; i += kThreads) {
-        const int4 four = sh.totals4[i];
-        cluster_store_uint4(to + 16 * i, make_uint4(four.x, four.y, four.z, four.w));
-      }
-    }
-    cluster_barrier<kThreads>();
-  } else {
-    __syncthreads();
-  }
   if (rank == 0) {
     constexpr int kOf = kBins / kThreads;
     const float rate = sh.row.scale32 * (1.0f / kExp2Entries), top32 = sh.row.top32;
     const bool plain = sh.row.form == kPlain;
+    // A thread adds up its bins of all CTAs, which a barrier has been behind: 16 reads of 16 bytes from as many SMs on their way together.
     int count[kOf], counted = 0;
     float mass[kOf], massed = 0.0f;
 #pragma unroll
+    for (int i = 0; i < kOf; i += 4) {
+      const int4* const own = &sh.bins4[(threadIdx.x * kOf + i) / 4];
+      int4 sum = *own;
+      const uint32_t at = smem_u32(own);
+#pragma unroll 5
+      for (int r = 1; r < ctas; ++r) {
+        const int4 four = cluster_load4(cluster_map_shared(at, r));
+        sum.x += four.x;
+        sum.y += four.y;
+        sum.z += four.z;
+        sum.w += four.w;
+      }
+      count[i] = sum.x;
+      count[i + 1] = sum.y;
+      count[i + 2] = sum.z;
+      count[i + 3] = sum.w;
+    }
+#pragma unroll
     for (int i = 0; i < kOf; ++i) {
       const int bin = threadIdx.x * kOf + i;
-      count[i] = ctas > 1 ? sh.totals[bin] : sh.bins[bin];
       const float middle = fmaxf(bins.high - static_cast<float>(bin) / bins.per, bins.low);
       mass[i] = 0.0f;
       if (shares && count[i] > 0) mass[i] = count[i] * (plain ? exp2f((middle - top32) * rate) : static_cast<float>(share<kThreads>(middle)));
@@ -1033,30 +1040,35 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
       count_upto += w < warp ? sh.warp_index[w] : 0;
       mass_upto += w < warp ? __uint_as_float(sh.warp_key[w]) : 0.0f;
     }
-    // the target for counts' sums, by each edge
-    const float rest = static_cast<float>(target - above), o = static_cast<float>(off);
-    float edge[kEdges] = {rest / (1.0f + o), o < 1.0f ? rest / (1.0f - o) : INFINITY};
+    // the target for counts' sums, by each edge: in which bin it is reached first
+    const float rest = shares ? static_cast<float>(target - above) : static_cast<float>(ceil(target - above)), o = shares ? static_cast<float>(off) : 0.0f;
+    float edge[kEdges] = {__fdividef(rest, 1.0f + o), o < 1.0f ? __fdividef(rest, 1.0f - o) : INFINITY};
+    int hit[kEdges];
 #pragma unroll
     for (int e = 2; e < kEdges; e += 2) {
-      const float less = fminf(o, 1.0f) / (e == 2 ? 4.0f : e == 4 ? 16.0f : 64.0f);
-      edge[e] = rest / (1.0f + less);
-      edge[e + 1] = rest / (1.0f - less);
+      const float less = fminf(o, 1.0f) * (e == 2 ? 1.0f / 4 : e == 4 ? 1.0f / 16 : 1.0f / 64);
+      edge[e] = __fdividef(rest, 1.0f + less);
+      edge[e + 1] = __fdividef(rest, 1.0f - less);
     }
-    const double missing = target - above;
+#pragma unroll
+    for (int e = 0; e < kEdges; ++e) hit[e] = kBins;
 #pragma unroll
     for (int i = 0; i < kOf; ++i) {
       const int bin = threadIdx.x * kOf + i;
-      const float mass_before = mass_upto;
-      const int count_before = count_upto;
       count_upto += count[i];
       mass_upto += mass[i];
       sh.bins[bin] = count_upto;
+      const float upto = shares ? mass_upto : static_cast<float>(count_upto);
 #pragma unroll
-      for (int e = 0; e < kEdges; ++e) {  // (each edge is passed in one bin)
-        if (shares ? mass_upto >= edge[e] && (mass_before < edge[e] || bin == 0) : count_upto >= missing && (count_before < missing || bin == 0))
-          atomicMin(&sh.edges[e], bin);
-      }
+      for (int e = 0; e < kEdges; ++e) hit[e] = upto >= edge[e] ? min(hit[e], bin) : hit[e];
     }
+    int first = kBins;  // lane e's: of edge e in this warp
+#pragma unroll
+    for (int e = 0; e < kEdges; ++e) {
+      const int least = __reduce_min_sync(0xffffffffu, hit[e]);
+      first = lane == e ? least : first;
+    }
+    if (lane < kEdges && first < kBins) atomicMin(&sh.edges[lane], first);
     __syncthreads();
     if (warp == 0) {
       const auto upto = [&](int bin) { return bin < 0 ? 0 : sh.bins[bin]; };
@@ -1575,10 +1587,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         const bool has_all = window.says == kListHasAll;
         const Gathered got = gather<T, kThreads>(next_low, next_high, seen, !has_all, shares, !known, which);
         which ^= 1;
-        const Three sums = cluster_sums<kThreads>(got.sifted.above, got.sifted.all, 0.0, which);
-        which ^= 1;
         if (!known) {
-          all = sums.b;
+          all = got.sums.all;
           target = rules.top_p * all;
           known = true;
         }
@@ -1587,7 +1597,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
           whole_sum = shares ? all : -1.0;
           break;
         }
-        done = got.count > 0 && got.count <= kCap && border_from_list<kThreads>(got.count, shares, above + sums.a, target, false);
+        done = got.count > 0 && got.count <= kCap && border_from_list<kThreads>(got.count, shares, above + got.sums.above, target, false);
         if (done) {
           if (shares) {
             begun = !rules.by_floor || share<kThreads>(sh.row.border) >= rules.min_p;  // (else some above the border go too)
