@@ -160,7 +160,7 @@ struct AppendParams {
 // kPlaced: slots and positions are given, one read instead of the look-ups of sequence, length and page; a position for each axis, and
 // frequencies for each, most of them zero: a pair's angle is their sum of products, exactly its axis's product where the others are zero.
 // The next token's are asked for in front of a token's heads and worked out behind them, into the other half of the arrays: one barrier a token.
-// 64 tokens 2.8 us, 4608 (as above, three axes) 37.1, 16384 of 48 heads of 128 90 of 62 for its bytes: two thirds of the issue slots are taken, at 20 warps an SM.
+// 64 tokens 2.8 us, 4608 (as above, three axes) 37.1, 16384 of 48 heads of 128 90 of 62 for its bytes: 0.66 instructions a cycle and scheduler, at 20 warps an SM.
 // (Multiplications two an instruction 94 us; six CTAs an SM with 80 registers 104.)
 constexpr int kAppendThreads = 512, kAppendManyThreads = 128;
 constexpr int kAppendManyCtas = 5;  // of an SM (with six: 80 registers, which do not hold it all)
