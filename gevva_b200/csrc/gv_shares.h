@@ -6,6 +6,7 @@
 // are in 64 bits therefore.
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -106,6 +107,26 @@ GV_SHARES_HD double share_of(double distance, double scale, const double* table,
   const uint32_t n = static_cast<uint32_t>(static_cast<int>(whole));
 #endif
   return scaled_by(exp2_rest(rest) * table[(n & (kExp2Entries - 1)) * stride], n);
+}
+
+// From which value on the plain form works shares out of uncapped values: values below `cut` count as `cut`, kShareOctaves below the largest, rounded
+// down to 32 bits.  Where a step of 32 bits at the largest is many temperatures, that is thousands of octaves down, which an exponent's bits do not
+// hold, or the largest itself: the plain form fits between kShareOctaves (less one, for rounding) and twice as many.
+struct PlainRange {
+  float cut;
+  bool fits;
+};
+GV_SHARES_HD PlainRange plain_range(float largest, double degrees) {
+  const double bound = static_cast<double>(largest) - kShareOctaves * 0.69314718055994530942 * degrees;
+#ifdef __CUDA_ARCH__
+  const float down = __double2float_rd(bound);
+#else
+  float down = static_cast<float>(bound);
+  if (down > bound) down = nextafterf(down, -INFINITY);
+#endif
+  const float cut = fmaxf(down, -3.402823466e38f);
+  const double octaves = (static_cast<double>(largest) - cut) / degrees * 1.4426950408889634074;
+  return {cut, fabsf(largest) < 1e30f && cut > -1e30f && octaves >= kShareOctaves - 1.0f && octaves <= 2.0f * kShareOctaves};
 }
 
 // A float as a double by three whole-number operations, which leave the pipe of conversions free.  Exact for normal numbers; zero and what is next

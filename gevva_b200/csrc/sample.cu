@@ -1397,6 +1397,11 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
   int top_k = p.top_k ? p.top_k[at_row] : 0;
   float top_p = p.top_p ? p.top_p[at_row] : 1.0f, floor = p.min_p ? p.min_p[at_row] : 0.0f;
   const float uniform = p.uniforms[at_row];
+  const auto answer = [&](int token, float probability) {
+    p.tokens[at_row] = token;
+    if (p.probabilities) p.probabilities[at_row] = probability;
+  };
+  if (rank == 0 && thread == 0) answer(-1, 0.0f);  // until there is one, which barriers come before
 
   // ---- the largest value, and the levels
   {
@@ -1469,14 +1474,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
       if (level >= 0) lower = max(lower, __reduce_min_sync(0xffffffffu, entry[2 + level]));
     }
   }
-  const auto answer = [&](int token, float probability) {
-    p.tokens[at_row] = token;
-    if (p.probabilities) p.probabilities[at_row] = probability;
-  };
-  if (largest <= kNothing) {  // nothing to take
-    if (rank == 0 && thread == 0) answer(-1, 0.0f);
-    return;
-  }
+  if (largest <= kNothing) return;  // nothing to take
   const float most = value_of(largest);
   if (!sampled) {  // the best: the lowest index that has it, of the first CTA that has one
     bool before = false;
@@ -1504,7 +1502,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     row.scale = octave / degrees;
     row.scale32 = static_cast<float>(row.scale);
     row.largest = most;
-    const bool ordinary = (capped ? p.softcap > 1e-30f && p.softcap <= kMostCap * temperature : fabsf(most) < 1e30f) && temperature > 1e-30f && temperature < 1e30f;
+    const PlainRange plain = plain_range(most, degrees);
+    const bool ordinary = (capped ? p.softcap > 1e-30f && p.softcap <= kMostCap * temperature : plain.fits) && temperature > 1e-30f && temperature < 1e30f;
     row.top = static_cast<double>(most);
     row.top32 = most;
     if (capped && ordinary) {
@@ -1514,9 +1513,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     } else if (capped) {
       row.top = softened_any(most, row.cap, sh.table);
     }
-    row.cut = fmaxf(__double2float_rd(static_cast<double>(most) - kShareOctaves * 0.69314718055994530942 * degrees), -3.402823466e38f);
+    row.cut = plain.cut;
     // (sizes at which 32 bits hold the whole part of every share that there is)
-    row.form = !ordinary ? kAny : capped ? kCapped : row.cut > -1e30f ? kPlain : kAny;
+    row.form = !ordinary ? kAny : capped ? kCapped : kPlain;
   }
   __syncthreads();
 

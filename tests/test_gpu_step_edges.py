@@ -1,0 +1,44 @@
+"""Tokens from logits and plans at the edges of what their calls take, against the plain forms of tests/step_ref.py (see test_gpu_step.py for how near is equal)."""
+import pytest
+import torch
+
+from gevva_b200 import step
+from tests.test_gpu_step import DEV, compare, generator, ints
+
+pytestmark = pytest.mark.gpu
+
+
+def f32(values):
+    return torch.tensor(values, dtype=torch.float32, device=DEV)
+
+
+# ---- low temperatures, no cap
+
+def rows_with_ties(gen, vocabulary, dtype):
+    """Largest values of several sizes, some several times, some with the next floats below beside them, and a bulk further down."""
+    largest = [10.0, 10.0, 20.0, 0.1, -20.0, 17.3, 1000.0, 0.0]
+    x = torch.randn(len(largest), vocabulary, generator=gen, device=DEV) * 2.5
+    for r, most in enumerate(largest):
+        x[r] = most - 1.0 - x[r].abs() * max(1.0, abs(most) / 16)
+        at = torch.randperm(vocabulary, generator=gen, device=DEV)
+        top = torch.tensor(most, dtype=dtype, device=DEV)
+        x[r, at[:r % 4 + 1]] = top.float()
+        if r % 2:
+            x[r, at[8:11]] = torch.nextafter(top, torch.full_like(top, -1e9)).float()
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("vocabulary", [100, 9000, 70001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-4, 1e-6, 1e-7, 1e-8, 3e-9, 1e-9, 1e-10, 1e-12, 1e-15, 1e-20, 1e-29])
+def test_low_temperatures(vocabulary, dtype, temperature):
+    """A step of 32 bits is many temperatures there: what is next to the largest has next to no share, and the largest ones have equal ones."""
+    gen = generator(vocabulary + 11)
+    logits = rows_with_ties(gen, vocabulary, dtype)
+    rows = len(logits)
+    cold = torch.full((rows,), temperature, device=DEV)
+    for rules in ({}, dict(top_p=f32([0.35] * rows)), dict(top_p=f32([0.999] * rows)), dict(top_k=ints([2] * rows)), dict(top_k=ints([400] * rows)),
+                  dict(min_p=f32([0.1] * rows)), dict(top_k=ints([400] * rows), top_p=f32([0.6] * rows), min_p=f32([0.01] * rows)),
+                  dict(top_p=f32([-1.0] * rows))):
+        for _ in range(2):
+            compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(rules, temperature=cold))
