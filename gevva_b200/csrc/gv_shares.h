@@ -170,4 +170,11 @@ GV_SHARES_HD float value_of(uint32_t order) {
 #endif
 }
 
+// How many of `count` bins of equal width one has, for bins that reach over `extent`.  A number of 32 bits: of an extent so small that they
+// would be more, fewer bins are in use.  (With infinitely many the largest, at a distance of zero, would be none of them.)
+GV_SHARES_HD float bins_for_one(int count, float extent) { return fminf(static_cast<float>(count - 1) / extent, 3.402823466e38f); }
+// Which one a distance is in, its count a power of two; of no number, or one beyond the bins, any.
+GV_SHARES_HD int bin_at(float distance, float per, int count) { return static_cast<int>(share_whole(distance, per) & static_cast<uint32_t>(count - 1)); }
+static_assert(kShareWhole % 4096 == 0, "the bits behind a whole number");
+
 }  // namespace gv

@@ -519,9 +519,8 @@ __device__ __noinline__ uint32_t first_index_of(float value) {
 }
 
 // (the whole number stands in the low bits; of ranges without an extent it means nothing: sums tell whether the border is where counts say)
-__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return share_whole(bins.high - x, bins.per) & (kBins - 1); }
-static_assert(kShareWhole % kBins == 0, "the bits behind a whole number");
-__device__ __forceinline__ Bins bins_between(float low, float high) { return {low, high, static_cast<float>(kBins - 1) / (high - low)}; }
+__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return bin_at(bins.high - x, bins.per, kBins); }
+__device__ __forceinline__ Bins bins_between(float low, float high) { return {low, high, bins_for_one(kBins, high - low)}; }
 
 template <int kThreads>
 __device__ __forceinline__ void clear_bins() {
@@ -839,8 +838,8 @@ __device__ __noinline__ int prune(int count, int ranks, float highest) {
   uint32_t least = sh.warp_index[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) least = min(least, sh.warp_index[w]);
-  const float per = static_cast<float>(kFewBins - 1) / (highest - value_of(least));
-  const auto bin = [&](unsigned long long entry) { return static_cast<int>((share_whole(highest - ranked_value(entry), per) - kShareWhole) & (kFewBins - 1)); };
+  const float per = bins_for_one(kFewBins, highest - value_of(least));
+  const auto bin = [&](unsigned long long entry) { return bin_at(highest - ranked_value(entry), per, kFewBins); };
 #pragma unroll
   for (int j = 0; j < kEach; ++j)
     if (threadIdx.x + j * kThreads < count) atomicAdd(&sh.bins[bin(entries[j])], 1);
@@ -1575,9 +1574,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         which ^= 1;
         if (shares) target = rules.top_p * all;
       }
-      // (half a bin, and what 32 bits lose of it)
+      // (half a bin, which is wider than a part of the range where that is next to nothing, and what 32 bits lose of it)
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
-      const double off = shares ? (0.505 / (kBins - 1) * (static_cast<double>(bins.high) - bins.low) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
+      const double off = shares ? (0.505 / static_cast<double>(bins.per) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
       const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, surely, turn);
       if (window.says == kNotHere || low == high) break;
       if (window.says == kInList || window.says == kListHasAll) {

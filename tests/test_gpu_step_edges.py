@@ -42,3 +42,35 @@ def test_low_temperatures(vocabulary, dtype, temperature):
                   dict(top_p=f32([-1.0] * rows))):
         for _ in range(2):
             compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(rules, temperature=cold))
+
+
+# ---- values so near one another that bins of equal width between them are too narrow for numbers of 32 bits
+
+@pytest.mark.parametrize("vocabulary", [100, 500, 900, 5000, 70001])
+@pytest.mark.parametrize("spread", [1e-45, 1e-38, 1e-37, 3e-36, 1e-30])
+def test_first_of_a_narrow_range(vocabulary, spread):
+    gen = generator(vocabulary + 12)
+    rows = 7
+    one = torch.zeros(rows, vocabulary, device=DEV)
+    one[torch.arange(rows), torch.randint(0, vocabulary, (rows,), generator=gen, device=DEV)] = spread
+    some = torch.randint(0, 5, (rows, vocabulary), generator=gen, device=DEV).float() * spread
+    for logits in (one, some, some - 3 * spread):
+        for k in (1, 3, 70, 200, 300, 1000):
+            compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_k=ints([k] * rows)))
+        compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_p=f32([0.37, 0.811, 0.123, 0.59, 0.99, 0.9999, 0.001])))
+
+
+@pytest.mark.parametrize("temperature", [5e-38, 1e-37, 1e-36])
+@pytest.mark.parametrize("vocabulary", [5000, 7001])
+def test_borders_at_temperatures_next_to_nothing(temperature, vocabulary):
+    """By top_p far down: the many values 24.5 temperatures below the largest are together more than what it leaves out.  The largest is the vocabulary's
+    last, so that small random numbers find them.  (The plain form adds so many shares to one or less: each rounding is at most 2^-53.  The border
+    by top_p is 2.56e-12 from the next one, which 2^-40 and twice those of up to 7400 values stay below; of more no token could be told.)"""
+    gen = generator(vocabulary + 13)
+    u = f32([0.0, 1e-9, 1e-8, 3e-8, 4.5e-8, 5.5e-8, 8e-8, 1e-7, 0.5])
+    rows = len(u)
+    logits = torch.full((rows, vocabulary), -24.5 * temperature, device=DEV)
+    logits[:, torch.randint(0, vocabulary - 1, (2,), generator=gen, device=DEV)] = -20.0 * temperature
+    logits[:, -1] = 0.0
+    given = dict(temperature=torch.full((rows,), temperature, device=DEV), top_p=f32([1 - 2.0 ** -24] * rows))
+    compare(logits, u, given, off=vocabulary * 2.0 ** -53, most_near=0.6)
