@@ -170,6 +170,14 @@ GV_SHARES_HD float value_of(uint32_t order) {
 #endif
 }
 
+// Half of what `x` is below `high`.
+GV_SHARES_HD float half_distance(float high, float x) {
+#ifdef __CUDA_ARCH__
+  return __fmaf_rn(x, -0.5f, 0.5f * high);
+#else
+  return __builtin_fmaf(x, -0.5f, 0.5f * high);
+#endif
+}
 // How many of `count` bins of equal width one has, for bins that reach over `extent`.  A number of 32 bits: of an extent so small that they
 // would be more, fewer bins are in use.  (With infinitely many the largest, at a distance of zero, would be none of them.)
 GV_SHARES_HD float bins_for_one(int count, float extent) { return fminf(static_cast<float>(count - 1) / extent, 3.402823466e38f); }

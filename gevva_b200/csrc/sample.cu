@@ -52,9 +52,11 @@ struct BinWindow {
   BinsSay says;
   int sure_first, sure_last;  // what holds it in any case (kBins: that may be behind all bins)
 };
-// Bins of equal width from `high` (bin 0's middle) down to `low`; a bin's values are the nearest to its middle.
+// Bins of equal width from `high` (bin 0's middle) down to `low`; a bin's values are the nearest to its middle.  Half of a distance is a number of 32
+// bits wherever both ends are; infinite values are in the first bin, and `high` is the largest number then.
 struct Bins {
-  float low, high, per;  // bins for one
+  float low, high, per_two;  // bins for two
+  __device__ __forceinline__ float middle(float bin) const { return high - 2.0f * (bin / per_two); }
 };
 
 // How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values where cap and
@@ -519,8 +521,11 @@ __device__ __noinline__ uint32_t first_index_of(float value) {
 }
 
 // (the whole number stands in the low bits; of ranges without an extent it means nothing: sums tell whether the border is where counts say)
-__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return bin_at(bins.high - x, bins.per, kBins); }
-__device__ __forceinline__ Bins bins_between(float low, float high) { return {low, high, bins_for_one(kBins, high - low)}; }
+__device__ __forceinline__ int bin_of(const Bins& bins, float x) { return bin_at(half_distance(bins.high, x), bins.per_two, kBins); }
+__device__ __forceinline__ Bins bins_between(float low, float high) {
+  const float finite = fminf(high, 3.402823466e38f);
+  return {low, finite, bins_for_one(kBins, half_distance(finite, low))};
+}
 
 template <int kThreads>
 __device__ __forceinline__ void clear_bins() {
@@ -838,8 +843,8 @@ __device__ __noinline__ int prune(int count, int ranks, float highest) {
   uint32_t least = sh.warp_index[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) least = min(least, sh.warp_index[w]);
-  const float per = bins_for_one(kFewBins, highest - value_of(least));
-  const auto bin = [&](unsigned long long entry) { return bin_at(highest - ranked_value(entry), per, kFewBins); };
+  const float finite = fminf(highest, 3.402823466e38f), per_two = bins_for_one(kFewBins, half_distance(finite, value_of(least)));
+  const auto bin = [&](unsigned long long entry) { return bin_at(half_distance(finite, ranked_value(entry)), per_two, kFewBins); };
 #pragma unroll
   for (int j = 0; j < kEach; ++j)
     if (threadIdx.x + j * kThreads < count) atomicAdd(&sh.bins[bin(entries[j])], 1);
@@ -953,7 +958,7 @@ __device__ __noinline__ bool border_from_list(int count, bool shares, double abo
 __device__ __noinline__ uint32_t order_with(Bins bins, int bin, uint32_t low, uint32_t high) {
   const int lane = threadIdx.x & 31;
   if (low < high) {  // most often it is among the 32 numbers about the bin's edge
-    const uint32_t edge = order_of(bins.high - (static_cast<float>(bin) + 0.5f) / bins.per);
+    const uint32_t edge = order_of(bins.middle(static_cast<float>(bin) + 0.5f));
     const uint32_t begin = edge > low + 16 && edge < high ? edge - 16 : low, at = min(begin + lane, high);
     const uint32_t yes = __ballot_sync(0xffffffffu, at == high || bin_of(bins, value_of(at)) <= bin);
     if (yes != 0 && (yes & 1) == 0) return min(begin + __ffs(yes) - 1, high);
@@ -1009,7 +1014,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
 #pragma unroll
     for (int i = 0; i < kOf; ++i) {
       const int bin = threadIdx.x * kOf + i;
-      const float middle = fmaxf(bins.high - static_cast<float>(bin) / bins.per, bins.low);
+      const float middle = fmaxf(bins.middle(static_cast<float>(bin)), bins.low);
       mass[i] = 0.0f;
       if (shares && count[i] > 0) mass[i] = count[i] * (plain ? exp2f((middle - top32) * rate) : static_cast<float>(share<kThreads>(middle)));
       counted += count[i];
@@ -1576,7 +1581,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
       }
       // (half a bin, which is wider than a part of the range where that is next to nothing, and what 32 bits lose of it)
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
-      const double off = shares ? (0.505 / static_cast<double>(bins.per) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
+      const double off = shares ? (1.01 / static_cast<double>(bins.per_two) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
       const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, surely, turn);
       if (window.says == kNotHere || low == high) break;
       if (window.says == kInList || window.says == kListHasAll) {
@@ -1610,9 +1615,9 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
       const uint32_t next_low = order_with(bins, window.sure_last, low, high);
       const uint32_t next_high = window.sure_first > 0 ? order_below(order_with(bins, window.sure_first - 1, low, high)) : high;
       if (next_low == low && next_high == high) break;
-      const Bins closer = bins_between(value_of(next_low), value_of(next_high));
+      const float lowest = value_of(next_low), highest = value_of(next_high);
       clear_bins<kThreads>();
-      const Sifted sifted = sift_row<T, kThreads>(true, closer.low, closer.high, seen, true, shares, !known, closer);
+      const Sifted sifted = sift_row<T, kThreads>(true, lowest, highest, seen, true, shares, !known, bins_between(lowest, highest));
       const Three sums = cluster_sums<kThreads>(sifted.above, sifted.all, 0.0, which);
       which ^= 1;
       above_mine += sifted.above;
@@ -1622,7 +1627,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         target = rules.top_p * all;
         known = true;
       }
-      seen = closer.high;
+      seen = highest;
       sure_low = low = next_low;
       sure_high = high = next_high;
     }

@@ -74,3 +74,27 @@ def test_borders_at_temperatures_next_to_nothing(temperature, vocabulary):
     logits[:, -1] = 0.0
     given = dict(temperature=torch.full((rows,), temperature, device=DEV), top_p=f32([1 - 2.0 ** -24] * rows))
     compare(logits, u, given, off=vocabulary * 2.0 ** -53, most_near=0.6)
+
+
+# ---- many infinite values
+
+@pytest.mark.parametrize("vocabulary", [5000, 70001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("infinite", [3, 200, 1100, 3000])
+def test_many_infinite_values(vocabulary, dtype, infinite):
+    """Each has the same share and the others none, also where they are more than a top_k that is more than a list is made for."""
+    gen = generator(vocabulary + infinite)
+    rows = 4
+    logits = torch.randn(rows, vocabulary, generator=gen, device=DEV) * 2.5
+    logits[1] *= 1e37
+    logits[2, ::3] = torch.finfo(dtype).max
+    logits[3] = logits[3].round()
+    logits = logits.to(dtype)
+    for r in range(rows):
+        logits[r, torch.randperm(vocabulary, generator=gen, device=DEV)[:infinite]] = float("inf")
+    for k in (1, 2, 70, 150, 300, 1000, 1024, 2000, 4000):
+        compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_k=ints([k] * rows)), most_near=0.5)
+    for p in (0.37, 0.811):
+        compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_p=f32([p] * rows)), most_near=0.5)
+        compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_p=f32([p] * rows), top_k=ints([700] * rows)), most_near=0.5)
+    compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(min_p=f32([0.3] * rows)), most_near=0.5)
