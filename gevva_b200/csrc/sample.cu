@@ -259,6 +259,8 @@ __device__ __forceinline__ Softened softened(float x, const Cap& c, float cap32,
 // A cap of at most this many times the temperature is of ordinary size: y in 32 bits is off by cap * 2^-22, so that a distance's whole part is
 // by 2 * 128 * 46 * 2^-22 = 0.003 32nds, and y in 64 bits by cap * 2^-51.3, a share's exponent by 2^-43: no more than the series leaves.
 constexpr double kMostCap = 128.0;
+// So is a temperature of at least this many: zero and what is next to it come from wide_of off by up to 2^-126, 2^-46 of a temperature here.
+constexpr float kLeastCappedDegrees = 1e-24f;
 // By its distance from the largest in y, whose whole part needs 32 bits only: none beyond kShareOctaves.
 __device__ __forceinline__ double capped_share(float x, double scale, float scale32, double top, float top32, const Cap& cap, float cap32, const double* table) {
   const Softened it = softened(x, cap, cap32, table);
@@ -1507,7 +1509,8 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     row.scale32 = static_cast<float>(row.scale);
     row.largest = most;
     const PlainRange plain = plain_range(most, degrees);
-    const bool ordinary = (capped ? p.softcap > 1e-30f && p.softcap <= kMostCap * temperature : plain.fits) && temperature > 1e-30f && temperature < 1e30f;
+    const bool ordinary = (capped ? p.softcap > 1e-30f && p.softcap <= kMostCap * temperature && temperature >= kLeastCappedDegrees : plain.fits) &&
+                          temperature > 1e-30f && temperature < 1e30f;
     row.top = static_cast<double>(most);
     row.top32 = most;
     if (capped && ordinary) {

@@ -98,3 +98,33 @@ def test_many_infinite_values(vocabulary, dtype, infinite):
         compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_p=f32([p] * rows)), most_near=0.5)
         compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(top_p=f32([p] * rows), top_k=ints([700] * rows)), most_near=0.5)
     compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(min_p=f32([0.3] * rows)), most_near=0.5)
+
+
+# ---- caps and temperatures next to nothing
+
+@pytest.mark.parametrize("vocabulary", [4, 100, 5000])
+@pytest.mark.parametrize("temperature", [2e-30, 1e-29, 1e-28, 1e-27, 1e-24])
+def test_capped_values_next_to_zero(vocabulary, temperature):
+    """Values about the smallest normal number, zeros among them, at temperatures of which they are a part that counts: a random number of a half
+    falls into the second half of the row, whose shares' sum is larger by (2 * 2e-38 - 3.7e-38) / temperature of a quarter."""
+    x = torch.zeros(2, vocabulary, device=DEV)
+    quarter = vocabulary // 4
+    x[:, quarter:2 * quarter] = 3.7e-38
+    x[:, 2 * quarter:] = 2e-38
+    x[1] = -x[1]  # (and by as much into the first)
+    for cap in (temperature, 30 * temperature):
+        for rules in ({}, dict(top_k=ints([vocabulary - 1] * 2))):
+            compare(x, f32([0.5, 0.5]), dict(rules, temperature=f32([temperature] * 2)), softcap=cap, most_near=1.0 if temperature > 5e-28 else 0.0)
+
+
+@pytest.mark.parametrize("vocabulary", [5000, 70001])
+@pytest.mark.parametrize("softcap", [30.0, 1e4])
+def test_many_infinite_values_capped(vocabulary, softcap):
+    """An infinite value is capped to the cap, and ranks before others that are."""
+    gen = generator(vocabulary + 14)
+    logits = torch.randn(4, vocabulary, generator=gen, device=DEV) * torch.tensor([2.5, 1e37, 40.0, 1e4], device=DEV)[:, None]
+    for r, infinite in enumerate((3, 200, 1100, 3000)):
+        logits[r, torch.randperm(vocabulary, generator=gen, device=DEV)[:infinite]] = float("inf")
+    for rules in ({}, dict(top_k=ints([150] * 4)), dict(top_k=ints([1000] * 4)), dict(top_p=f32([0.37, 0.811, 0.937, 0.123])), dict(min_p=f32([0.3] * 4)),
+                  dict(top_k=ints([2000] * 4), top_p=f32([0.37, 0.811, 0.937, 0.123]))):
+        compare(logits, torch.rand(4, generator=gen, device=DEV), rules, softcap, off=2 * softcap * 2.0 ** -51, most_near=0.5)
