@@ -78,11 +78,12 @@ class PagePool:
 
 class StepPlan:
     """What plan_step says of a step: token_offsets [sequences + 1], lengths [sequences] with the new tokens counted, slots and positions
-    [tokens], taken [1] and the table that it was made for; all int32 on the GPU.  `batch` is what chunk_attention takes."""
+    [tokens], taken [1] and the table that it was made for; all int32 on the GPU.  `batch` is what chunk_attention takes: one handle, whose
+    tensors are the plan's."""
 
     def __init__(self, token_offsets, lengths, slots, positions, taken, table):
         self.token_offsets, self.lengths, self.slots, self.positions, self.taken, self.table = token_offsets, lengths, slots, positions, taken, table
-        self._batch = None
+        self._batch, self._goes_on = None, False
 
     @classmethod
     def empty(cls, sequences, table, tokens, lengths=None, taken=None):
@@ -92,14 +93,26 @@ class StepPlan:
 
     @classmethod
     def in_place(cls, lengths, table, pool, tokens):
-        """One whose lengths and count of pages are the state itself: the step goes on from what it has written."""
-        return cls.empty(lengths.shape[0], table, tokens, lengths, pool.taken)
+        """One whose lengths and count of pages are the state itself: the step goes on from what it has written.  That is the lengths and the
+        pool's count which plan_step is given with this plan, also where they are other tensors than before (what trim_step returned, for
+        instance); the plan's own follow, and a captured call keeps those that it was captured with."""
+        plan = cls.empty(lengths.shape[0], table, tokens, lengths, pool.taken)
+        plan._goes_on = True
+        return plan
 
     @property
     def batch(self):
-        if self._batch is None:
-            self._batch = PagedBatch(self.token_offsets, self.lengths, self.table)
-        return self._batch
+        batch = self._batch
+        if batch is None:
+            batch = self._batch = PagedBatch(self.token_offsets, self.lengths, self.table)
+        elif batch.token_offsets is not self.token_offsets or batch.lengths is not self.lengths or batch.table is not self.table:
+            batch._take(self.token_offsets, self.lengths, self.table)
+        return batch
+
+    def _follow(self, lengths, taken):
+        self.lengths, self.taken = lengths, taken
+        if self._batch is not None:
+            self.batch
 
 
 @dataclass
@@ -131,8 +144,8 @@ def plan_step(lengths, news, table, pool, page_size, tokens, shift=None, out=Non
     """Rows, pages and places of the step's new tokens, as a StepPlan: request s, which has lengths[s] tokens in the cache and the pages for
     them in its row of `table`, gets news[s] more.  The table is written with pages out of `pool`; `tokens` is how many rows the
     step's tensors have, and rows behind the last request's get slot -1.  `shift` [sequences] is added to the positions (not to the
-    places).  `out` takes the plan; its lengths may be `lengths` and its taken pool.taken (StepPlan.in_place), other outputs share
-    no memory with what is read.  Without it the pool's count stays as it was, and the plan has the new one.  Requests whose
+    places).  `out` takes the plan; one in place (StepPlan.in_place) writes its lengths to `lengths` and its count to pool.taken, other outputs
+    share no memory with what is read.  Without it the pool's count stays as it was, and the plan has the new one.  Requests whose
     numbers cannot be, too few pages or more tokens than rows leave everything as it was and no row a token; pool.check() reports them."""
     device, sequences, stride = _requests(lengths, news, "news", table, pool)
     if stream is not None:
@@ -146,13 +159,16 @@ def plan_step(lengths, news, table, pool, page_size, tokens, shift=None, out=Non
     else:
         if out.table is not table and (out.table.data_ptr() != table.data_ptr() or out.table.shape != table.shape or out.table.stride() != table.stride()):
             raise ValueError("out: a plan for another table")
-        addresses = (_at(out.token_offsets, i32, (sequences + 1,), device, "out.token_offsets"), _at(out.lengths, i32, (sequences,), device, "out.lengths"),
+        after, count = (lengths, pool.taken) if out._goes_on else (out.lengths, out.taken)
+        addresses = (_at(out.token_offsets, i32, (sequences + 1,), device, "out.token_offsets"), _at(after, i32, (sequences,), device, "out.lengths"),
                      _at(out.slots, i32, (tokens,), device, "out.slots"), _at(out.positions, i32, (tokens,), device, "out.positions"),
-                     _at(out.taken, i32, (1,), device, "out.taken"))
+                     _at(count, i32, (1,), device, "out.taken"))
     free, taken, status = pool._addresses
     args = _pack(_PLAN, lengths.data_ptr(), news.data_ptr(), _at(shift, i32, (sequences,), device, "shift"), table.data_ptr(), free, taken, *addresses, status,
                  sequences, table.shape[1], stride, pool.pages, page_size, tokens)
     _status(_enqueue(_lib().gevva_step_plan, device, None, args), "plan_step")
+    if out._goes_on and (out.lengths is not lengths or out.taken is not pool.taken):
+        out._follow(lengths, pool.taken)
     return out
 
 

@@ -128,3 +128,54 @@ def test_many_infinite_values_capped(vocabulary, softcap):
     for rules in ({}, dict(top_k=ints([150] * 4)), dict(top_k=ints([1000] * 4)), dict(top_p=f32([0.37, 0.811, 0.937, 0.123])), dict(min_p=f32([0.3] * 4)),
                   dict(top_k=ints([2000] * 4), top_p=f32([0.37, 0.811, 0.937, 0.123]))):
         compare(logits, torch.rand(4, generator=gen, device=DEV), rules, softcap, off=2 * softcap * 2.0 ** -51, most_near=0.5)
+
+
+# ---- plans in place
+
+def test_a_plan_in_place_goes_on_from_what_a_trim_returned():
+    """The lengths and the count that trim_step made take the place of those that the plan began with: no page is handed out twice."""
+    from tests import step_ref
+    from tests.test_gpu_step import requests
+    rng, lengths, table, free, taken = requests(4, 30, 16, 60, width=20)
+    pool, rows, state = step.PagePool(ints(free), ints([taken])), ints(table), ints(lengths)
+    plan = step.StepPlan.in_place(state, rows, pool, 300)
+    held, first, count = plan.batch, state, pool.taken
+    for turn in range(6):
+        news = [int(x) for x in rng.integers(0, 10, 30)]
+        want = step_ref.plan(lengths, news, table, free, taken, 16, 300)
+        assert step.plan_step(state, ints(news), rows, pool, 16, 300, out=plan) is plan
+        lengths, taken, table = want[1], want[4], want[5]
+        assert state.tolist() == lengths and pool.taken.tolist() == [taken] and rows.tolist() == table and plan.slots.tolist() == want[2]
+        assert plan.lengths is state and plan.taken is pool.taken and plan.batch is held and held.lengths is state
+        live = [row[i] for row, n in zip(table, lengths) for i in range(-(-n // 16))]
+        assert len(set(live)) == len(live)
+        if turn % 2 == 0:
+            keep = [max(0, n - int(rng.integers(0, 30))) for n in lengths]
+            lengths, free, taken = step_ref.trim(lengths, keep, table, free, taken, 16)
+            trimmed = step.trim_step(state, ints(keep), rows, pool, 16)
+            state, pool.taken = trimmed.lengths, trimmed.taken
+    pool.check()
+    assert first is not state and count is not pool.taken
+
+
+def test_a_captured_plan_in_place_keeps_its_tensors():
+    pool, table, state, news = step.PagePool.whole(20, DEV), torch.full((2, 5), -1, dtype=torch.int32, device=DEV), ints([0, 0]), ints([1, 20])
+    plan = step.StepPlan.in_place(state, table, pool, 30)
+    step.plan_step(state, news, table, pool, 16, 30, out=plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.plan_step(state, news, table, pool, 16, 30, out=plan)
+    count, pool.taken, other = pool.taken, ints([7]), ints([5, 5])
+    step.plan_step(other, news, table, pool, 16, 30, out=plan)
+    assert other.tolist() == [6, 25] and pool.taken.item() == 8 and state.tolist() == [1, 20] and plan.batch.lengths is other
+    graph.replay()
+    assert state.tolist() == [2, 40] and other.tolist() == [6, 25] and pool.taken.item() == 8 and count.item() == 4  # (1 + 2 pages, and one more)
+    pool.check()
+
+
+def test_the_batch_of_a_plan_has_the_plans_tensors():
+    pool, table = step.PagePool.whole(20, DEV), torch.full((2, 5), -1, dtype=torch.int32, device=DEV)
+    plan = step.plan_step(ints([0, 0]), ints([1, 20]), table, pool, 16, 21)
+    batch = plan.batch
+    plan.lengths, plan.table = plan.lengths.clone(), plan.table.clone()
+    assert plan.batch is batch and batch.lengths is plan.lengths and batch.table is plan.table
