@@ -380,5 +380,5 @@ class AttentionLayer:
         return self._behind(hidden, seen)
 
     def _behind(self, hidden, seen):
-        y = torch.mm(seen.view(hidden.shape[0], -1), self.out_w.t())
+        y = torch.mm(seen.view(hidden.shape[0], seen.shape[1] * seen.shape[2]), self.out_w.t())
         return block_norm_add(y, self.post, hidden, eps=self.eps)

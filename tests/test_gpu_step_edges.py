@@ -179,3 +179,19 @@ def test_the_batch_of_a_plan_has_the_plans_tensors():
     batch = plan.batch
     plan.lengths, plan.table = plan.lengths.clone(), plan.table.clone()
     assert plan.batch is batch and batch.lengths is plan.lengths and batch.table is plan.table
+
+
+# ---- layers
+
+@pytest.mark.parametrize("prompt", [False, True])
+def test_a_layer_of_no_rows(prompt):
+    from gevva_b200 import attention as attn
+    from tests.test_gpu_step import attention_layer
+    layer = attention_layer(generator(71))
+    pool, table = step.PagePool.whole(8, DEV), torch.full((2, 4), -1, dtype=torch.int32, device=DEV)
+    plan = step.plan_step(ints([0, 0]), ints([0, 0]), table, pool, 16, 0)
+    hidden = torch.zeros(0, 256, dtype=torch.bfloat16, device=DEV)
+    for batch in (plan, plan.batch, attn.PagedBatch(ints([0, 0, 0]), ints([5, 0]), ints([[0], [1]]))):
+        assert layer.forward(hidden, batch, prompt).shape == (0, 256)
+    pool.check()
+    layer.cache.check()
