@@ -231,8 +231,16 @@ class SyntheticStack:
 
     def decode(self, tokens, plan, uniforms, concurrent=True, **settings):
         """The next token of each row: int32 `tokens` of the step that `plan` (a step.StepPlan) places, through the layers and the head.  `settings` are
-        those of step.sample_tokens."""
+        those of step.sample_tokens.  A row below zero has no token (sample_tokens gives -1 where a mask leaves nothing): zeros go through the
+        layers in its place, and it gets none again.  A request that waits is better left out of the step, with no new token in the plan."""
         if self.head is None or self.attention is None:
             raise ValueError("a stack that decodes has attention and a vocabulary")
-        hidden = self.forward(self.head.rows[tokens.long()], concurrent, plan)
-        return self.head.forward(hidden, uniforms, **settings)
+        none = tokens < 0
+        hidden = self.forward(self.head.rows[tokens.clamp(min=0).long()].masked_fill_(none[:, None], 0.0), concurrent, plan)
+        chosen = self.head.forward(hidden, uniforms, **settings)
+        if settings.get("probability"):
+            chosen[0].masked_fill_(none, -1)
+            chosen[1].masked_fill_(none, 0.0)
+        else:
+            chosen.masked_fill_(none, -1)
+        return chosen

@@ -195,3 +195,20 @@ def test_a_layer_of_no_rows(prompt):
         assert layer.forward(hidden, batch, prompt).shape == (0, 256)
     pool.check()
     layer.cache.check()
+
+
+def test_a_stack_with_a_row_without_a_token():
+    """The other rows get what they get beside any token, and what the row leaves in the cache is finite."""
+    from gevva_b200.synthetic import SyntheticAttention, SyntheticStack
+    gen = generator(72)
+    stack = SyntheticStack(2, 16, DEV, distinct_experts=False, attention=SyntheticAttention(window=24, whole_every=2, pages=16, page_size=16), vocabulary=1201)
+    pool, table, lengths = step.PagePool.whole(16, DEV), torch.full((3, 4), -1, dtype=torch.int32, device=DEV), ints([0, 0, 0])
+    u = torch.rand(3, generator=gen, device=DEV)
+    got = []
+    for middle in (-1, 5):
+        plan = step.plan_step(lengths, ints([1, 1, 1]), table, pool, 16, 3)
+        got.append(stack.decode(ints([7, middle, 1200]), plan, u, probability=True))
+        for layer in stack.attention:
+            assert layer.cache.k.isfinite().all() and layer.cache.v.isfinite().all()
+    (without, shares), (beside, others) = got
+    assert without.tolist() == [beside[0], -1, beside[2]] and shares.tolist() == [others[0], 0, others[2]] and (beside >= 0).all()
