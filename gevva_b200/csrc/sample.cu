@@ -88,7 +88,8 @@ struct RowState {
 
 template <int kThreads>
 struct SampleShared {
-  static constexpr int kEach = kThreads >= 512 ? 2 : 4;  // a thread's entries of the list
+  static constexpr int kEach = 4;  // a thread's entries of the list
+  static_assert(kBins % (4 * kThreads) == 0, "a thread adds up its bins four at a time");
   static constexpr int kCap = kEach * kThreads;
   static constexpr int kWarps = kThreads / 32;
   static constexpr int kFew = 128;
