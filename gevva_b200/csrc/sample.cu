@@ -161,63 +161,63 @@ __device__ __forceinline__ uint32_t order_above(uint32_t order) { return order =
 static __constant__ double g_exp2_table[kExp2Entries] = GV_EXP2_TABLE_INIT;
 
 // One step of a bitonic sort between lanes, or between a lane's two values.
-  __device__ __forceinline__ void order_lanes(unsigned long long& x, int stride, bool up) {
-    const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, stride);
-    const bool lower = (threadIdx.x & stride) == 0;
-    x = (x < y) == (lower == up) ? x : y;
-  }
-  // Bitonic, ascending; entries from `count` on up to a power of two, at least 64, are made the largest.  Strides below 64 are between
-  // the lanes of a warp, two values each, the others in shared memory.
-  template <int kThreads>
+__device__ __forceinline__ void order_lanes(unsigned long long& x, int stride, bool up) {
+  const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, stride);
+  const bool lower = (threadIdx.x & stride) == 0;
+  x = (x < y) == (lower == up) ? x : y;
+}
+// Bitonic, ascending; entries from `count` on up to a power of two, at least 64, are made the largest.  Strides below 64 are between
+// the lanes of a warp, two values each, the others in shared memory.
+template <int kThreads>
 __device__ __noinline__ void sort_list(unsigned long long* list, int count) {
   constexpr int kWarps = kThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int whole = 64;
-    while (whole < count && whole < SampleShared<kThreads>::kCap) whole *= 2;
-    for (int i = count + threadIdx.x; i < whole; i += kThreads) list[i] = ~0ull;
-    __syncthreads();
-    for (int size = 64; size <= whole; size *= 2) {
-      for (int stride = size / 2; stride >= 64; stride /= 2) {
-        for (int i = threadIdx.x; i < whole / 2; i += kThreads) {
-          const int a = 2 * i - (i & (stride - 1)), b = a + stride;
-          const unsigned long long x = list[a], y = list[b];
-          if ((x > y) == ((a & size) == 0)) {
-            list[a] = y;
-            list[b] = x;
-          }
+  int whole = 64;
+  while (whole < count && whole < SampleShared<kThreads>::kCap) whole *= 2;
+  for (int i = count + threadIdx.x; i < whole; i += kThreads) list[i] = ~0ull;
+  __syncthreads();
+  for (int size = 64; size <= whole; size *= 2) {
+    for (int stride = size / 2; stride >= 64; stride /= 2) {
+      for (int i = threadIdx.x; i < whole / 2; i += kThreads) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const unsigned long long x = list[a], y = list[b];
+        if ((x > y) == ((a & size) == 0)) {
+          list[a] = y;
+          list[b] = x;
         }
-        __syncthreads();
-      }
-      for (int block = warp; block < whole / 64; block += kWarps) {
-        unsigned long long* const values = list + 64 * block;
-        unsigned long long x = values[lane], y = values[lane + 32];
-        if (size == 64) {
-#pragma unroll
-          for (int inner = 2; inner <= 32; inner *= 2) {
-#pragma unroll
-            for (int stride = inner / 2; stride > 0; stride /= 2) {
-              order_lanes(x, stride, (lane & inner) == 0);           // (at 32: x up, y down)
-              order_lanes(y, stride, inner == 32 ? false : (lane & inner) == 0);
-            }
-          }
-        }
-        const bool up = (64 * block & size) == 0;
-        if ((x > y) == up) {
-          const unsigned long long z = x;
-          x = y;
-          y = z;
-        }
-#pragma unroll
-        for (int stride = 16; stride > 0; stride /= 2) {
-          order_lanes(x, stride, up);
-          order_lanes(y, stride, up);
-        }
-        values[lane] = x;
-        values[lane + 32] = y;
       }
       __syncthreads();
     }
+    for (int block = warp; block < whole / 64; block += kWarps) {
+      unsigned long long* const values = list + 64 * block;
+      unsigned long long x = values[lane], y = values[lane + 32];
+      if (size == 64) {
+#pragma unroll
+        for (int inner = 2; inner <= 32; inner *= 2) {
+#pragma unroll
+          for (int stride = inner / 2; stride > 0; stride /= 2) {
+            order_lanes(x, stride, (lane & inner) == 0);           // (at 32: x up, y down)
+            order_lanes(y, stride, inner == 32 ? false : (lane & inner) == 0);
+          }
+        }
+      }
+      const bool up = (64 * block & size) == 0;
+      if ((x > y) == up) {
+        const unsigned long long z = x;
+        x = y;
+        y = z;
+      }
+#pragma unroll
+      for (int stride = 16; stride > 0; stride /= 2) {
+        order_lanes(x, stride, up);
+        order_lanes(y, stride, up);
+      }
+      values[lane] = x;
+      values[lane + 32] = y;
+    }
+    __syncthreads();
   }
+}
 
 __device__ __forceinline__ float ranked_value(unsigned long long entry) { return value_of(~static_cast<uint32_t>(entry >> 32)); }
 // What top_k and top_p leave: values above `value`, and those equal to it up to `index`.
