@@ -980,8 +980,8 @@ __device__ __noinline__ uint32_t order_with(Bins bins, int bin, uint32_t low, ui
   return low;
 }
 
-// Where the counts say that `target` is reached, with `above` in front of the bins.  Counts times the shares of their bins' middles are off by up to
-// `off` of themselves: the border lies between where they reach the target with that much more and with that much less.  Where
+// Where the counts say that `target` is reached, with `above` in front of the bins.  Counts times the shares of their bins' middles are off by a factor of
+// up to exp(off) either way: the border lies between where they reach the target with that much less and with that much more.  Where
 // that is more than the list holds, it is looked at with a quarter, a sixteenth or a 64th of it (errors of many bins cancel; sums will tell), or
 // closer.  `surely`: it is in the bins, whatever the counts say.  (With a sixteenth as the least 48 of 256 rows of 128000 by top_p were looked at again.)
 template <int kThreads>
@@ -1049,7 +1049,7 @@ __device__ __noinline__ BinWindow window_of_bins(Bins bins, bool shares, double 
     }
     // the target for counts' sums, by each edge: in which bin it is reached first
     const float rest = shares ? static_cast<float>(target - above) : static_cast<float>(ceil(target - above)), o = shares ? static_cast<float>(off) : 0.0f;
-    float edge[kEdges] = {__fdividef(rest, 1.0f + o), o < 1.0f ? __fdividef(rest, 1.0f - o) : INFINITY};
+    float edge[kEdges] = {rest * expf(-o), rest * expf(o)};  // (counts: the target itself)
     int hit[kEdges];
 #pragma unroll
     for (int e = 2; e < kEdges; e += 2) {
@@ -1583,7 +1583,11 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         which ^= 1;
         if (shares) target = rules.top_p * all;
       }
-      // (half a bin, which is wider than a part of the range where that is next to nothing, and what 32 bits lose of it)
+      // By how much, as an exponent, shares by middles are off.  A value is half a bin from its middle at most, and 0.005 for what the bin's number loses
+      // (three roundings of 2^-24 of up to 1023); the middle is off by up to three roundings of at most `size`; capped values in 32 bits by 5e-7
+      // of the cap each, the largest and another (an exponential off by 2^-22 of up to one, of which a softened value takes at most half, a reciprocal
+      // by 2^-23 and six roundings).  The rest is within 2.5e-5 of 1e-4: 259 additions of a lane and 21 of bins (2^-24 each: 1.7e-5), exponents of
+      // up to 24 temperatures from three roundings (4.3e-6, and on a row's average, which is ln of its size, 2.3e-6), exponentials (2^-22).
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
       const double off = shares ? (1.01 / static_cast<double>(bins.per_two) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
       const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, surely, turn);

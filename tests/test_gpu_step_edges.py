@@ -212,3 +212,19 @@ def test_a_stack_with_a_row_without_a_token():
             assert layer.cache.k.isfinite().all() and layer.cache.v.isfinite().all()
     (without, shares), (beside, others) = got
     assert without.tolist() == [beside[0], -1, beside[2]] and shares.tolist() == [others[0], 0, others[2]] and (beside >= 0).all()
+
+
+@pytest.mark.parametrize("temperature", [5e-38, 1e-37])
+def test_borders_of_wide_bins(temperature):
+    """At temperatures of which a bin is a part that counts: values at the upper ends of their bins, whose shares' sum is more than their middles say by
+    up to exp of half a bin.  The border is just in front of the last of a bin."""
+    width = 1.0 / 1.7014118e38  # of the bins in use, at most as many as a number of 32 bits says
+    at = torch.arange(1, 86, dtype=torch.float64).repeat_interleave(50)
+    row = torch.cat([torch.zeros(1, dtype=torch.float64), -(at - 0.499) * width])
+    row = row[torch.randperm(len(row), generator=torch.Generator().manual_seed(3))].float()
+    degrees = float(torch.tensor(temperature))
+    shares = torch.exp(row.double() / degrees).sort(descending=True).values.cumsum(0)
+    bins = torch.arange(24, 64)
+    p = shares[50 * bins] / shares[-1] * 0.9995
+    for u in (0.97, 0.73, 0.41):
+        compare(row.expand(len(bins), -1).to(DEV), f32([u] * len(bins)), dict(temperature=f32([temperature] * len(bins)), top_p=p.float().to(DEV)), off=1e-12)
