@@ -15,11 +15,14 @@
 // A list that has all that may be kept (most rows that are not flat) is cut by rank and walked over by index in the first CTA instead.
 // All sums are taken in an order that sizes alone give: the same inputs give the same token.
 //
-// Floors are a row's bytes, read once: 64 rows of 262144 in bf16 5.1 us, 256 of 50257 in f32 7.9, of 128000 20.  None of them bounds: a pass over values
-// in L2 takes 30 to 60 issue slots a value and warp for shares in 64 bits (8 for the largest value, about 10 cycles of the shared-memory atomics
-// a count in a bin).  In a graph over inputs larger than L2, f32 64 x 262144: the largest alone 18.8 us (3.6 TB/s), as they are 45, above a floor 68,
-// by count 87, by top_p 157; bf16 with settings of their own and a cap 114; 256 x 50257 as they are 38.6, 256 x 128000 by top_p 231; one row of 262144
-// 4.6, 13.9, by count 21, by top_p 34, of which about half is cluster barriers and the first CTA's work on lists and bins.  With borders found by
+// Floors are a row's bytes, read once: 64 rows of 262144 in bf16 5.1 us, 256 of 50257 in f32 7.9, of 128000 20.  None of them bounds, and no
+// pipe does: a pass over values in L2 takes 30 to 60 issue slots a value and warp for shares in 64 bits (8 for the largest value, about 10 cycles of
+// the shared-memory atomics a count in a bin), and an SM's 13 to 14 warps fill a quarter (best token) to a half (tokens as they are, top_p) of the slots
+// between waits for memory, fixed latencies and barriers.  For 22 (tokens as they are) to 57 % of the time (rows with settings of their own) an
+// SM has no CTA, since rows take different times.  In a graph over inputs larger than L2, f32 64 x 262144: the largest alone 18.9 us (3.6 TB/s), as they are 46, above a floor of 0.1 59 and of 0.01 86, by a
+// count of 50 49, of 300 89, of 1000 103, by top_p 155 to 163; bf16 with settings of their own and a cap 75 to 184 by what is drawn, 108 on most;
+// 256 x 50257 as they are 38.8, 256 x 128000 by top_p 220 to 260; one row of 262144 4.8, 14.0, by a count of 50 14, of 1000 34, by top_p 38, of which about
+// half is cluster barriers and the first CTA's work on lists and bins.  With borders found by
 // halving instead of bins, conversions of values where they are used and half the CTAs for rows with rules (the first form) the 64 rows with
 // settings of their own took 424 us, the 256 of 50257 70 and the 256 of 128000 720.
 //
@@ -1683,7 +1686,8 @@ cudaError_t launch_type(const SampleCall& call, int sm_count, cudaStream_t strea
   if (bytes <= 4096) return launch_threads<T, 128>(call, 1, stream);
   // Two CTAs an SM take as many rows as there are; where there are fewer, as many CTAs a row as that leaves, down to 8 KB each.  With rules to find
   // borders for, rows take up to five times as long as one another: twice as many CTAs then (64 rows of 262144, each with rules of its
-  // own, 243 -> 146 us when they took that; 256 rows of 128000 by top_p 300 -> 265; without rules 256 rows of 50257 would go 38 -> 47).
+  // own, 243 -> 146 us when they took that; 256 rows of 128000 by top_p 300 -> 265; without rules 256 rows of 50257 would go 38 -> 47, which a call
+  // pays whose settings are given and keep all: they are the device's to read).
   const long long ctas_at_once = (call.top_k || call.top_p || call.min_p ? 4ll : 2ll) * sm_count;
   int ctas = 1;
   while (ctas < kMostCtas && 2ll * ctas * call.rows <= ctas_at_once && bytes > 16384ll * ctas) ctas *= 2;

@@ -3,8 +3,9 @@
 // Two running sums over the requests, of their tokens and of their pages, say where each one's rows and pages begin; everything else follows
 // for each row and each page by itself.  A cluster does it in one launch: every CTA works out both sums for itself (up to 16384
 // requests in shared memory), takes its part of the rows and pages, and writes what a call may have been given as inputs too (lengths, the number
-// of pages handed out) behind a barrier of the cluster, when all have read them.  Nothing but latency bounds it: launch, two dependent
-// reads, the sums, the search of a row's request, two dependent reads, a write.  In a graph: 64 requests 3.4 us, four prompts of 4608 tokens 5.8, 1000
+// of pages handed out) behind a barrier of the cluster, when all have read them.  Latency bounds plans and small trims: launch, two dependent
+// reads, the sums, the search of a row's request, two dependent reads, a write.  Trims of large batches are bound by the cluster's eight SMs, through
+// which all their table entries go.  In a graph: 64 requests 3.4 us, four prompts of 4608 tokens 5.8, 1000
 // requests with drafts 7.4; trimmed, 64 requests 4.1, 1000 of which a third end 9.3 (15.8 with a search for each page instead of one for a
 // warp's pages).
 #include "gv_common.cuh"

@@ -239,7 +239,8 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
     largest.  The row's token is the first of the vocabulary up to which the kept shares' sum exceeds its random number times the whole sum.
     temperature, top_p and min_p are float32 [rows], top_k int32 [rows], each None for none; a temperature that is not above zero
     takes the best token, a top_k of zero or less, a top_p of one or more and a min_p of zero or less keep all.  Minus infinity and NaN are never
-    taken; a row of nothing else gives -1.  With `probability` also the token's share of the kept ones, float32 [rows].  `out` takes the
+    taken; a row of nothing else gives -1.  Shares are off by up to 2^-42.8 of themselves, with a softcap by 2^-50 of softcap / temperature more, and may
+    be none below 2^-200 of the largest.  With `probability` also the token's share of the kept ones, float32 [rows].  `out` takes the
     tokens."""
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"logits: expected CUDA float32 or bfloat16 (rows, vocabulary), got {logits.dtype} {tuple(logits.shape)} on {logits.device}")

@@ -570,7 +570,9 @@ int gevva_step_append(const gevva_step_append_args* args, gevva_stream_t stream)
  * and the row's token is the first of the vocabulary up to which the sum of kept shares exceeds uniforms[row] (0 <= u < 1) times the sum of
  * all kept ones.  A temperature that is not above zero takes the first by rank.  Minus infinity and NaN are never taken, a row of
  * nothing else gives token -1 and probability 0; of infinite logits each has the same share and the others none.  Shares and
- * sums are in 64 bits.  probabilities: the token's share of the kept ones' sum.  Settings are NULL or [rows]; row_stride may be
+ * sums are held in 64 bits and summed in an order that sizes give: a share is off by up to 2^-42.8 of itself, with a softcap by 2^-50 of
+ * softcap / temperature more, so that a token may be its neighbour's where a border lies as near as that to a random number or to a rule's;
+ * shares below 2^-200 of the largest may count as none.  probabilities: the token's share of the kept ones' sum.  Settings are NULL or [rows]; row_stride may be
  * zero (many tokens from one row).  logits are aligned to their type; up to 15 bytes in front of and behind a row are read, within the
  * 16-byte lines that its ends lie in.  vocabulary up to 524288; at most 2^27 - 1 rows. */
 typedef struct {
