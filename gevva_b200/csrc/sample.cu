@@ -1499,8 +1499,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
     return;
   }
   const bool capped = p.softcap > 0.0f;
-  // (the scale of a capped row's shares is a number of 32 bits too: below this temperature there are no shares but the largest's)
-  const double degrees = capped ? fmax(static_cast<double>(temperature), 1e-30) : static_cast<double>(temperature);
+  const double degrees = static_cast<double>(temperature);
   if (thread == 0) {
     RowState& row = sh.row;
     constexpr double octave = 1.4426950408889634074 * kExp2Entries;

@@ -228,3 +228,17 @@ def test_borders_of_wide_bins(temperature):
     p = shares[50 * bins] / shares[-1] * 0.9995
     for u in (0.97, 0.73, 0.41):
         compare(row.expand(len(bins), -1).to(DEV), f32([u] * len(bins)), dict(temperature=f32([temperature] * len(bins)), top_p=p.float().to(DEV)), off=1e-12)
+
+
+@pytest.mark.parametrize("vocabulary", [7, 300, 5000])
+@pytest.mark.parametrize("size", [1e-31, 1e-35, 1e-38])
+def test_capped_values_of_next_to_nothing(vocabulary, size):
+    """Logits, cap and temperature that are all below 1e-30: what counts is how large they are to one another.  (Subnormal temperatures are read as they are
+    on both sides; softened values are off by 2^-50 of the smaller of cap and value.)"""
+    gen = generator(vocabulary + 15)
+    for cap in f32([3 * size, 100 * size, 1e-6, 30.0]).tolist():  # (a call's cap is a number of 32 bits)
+        logits = torch.randn(5, vocabulary, generator=gen, device=DEV) * 2.5 * size
+        for part in (0.1, 1.0, 3.0):
+            for rules in ({}, dict(top_k=ints([4] * 5)), dict(top_p=f32([0.83] * 5)), dict(min_p=f32([0.05] * 5))):
+                given = dict(rules, temperature=f32([part * size] * 5))
+                compare(logits, torch.rand(5, generator=gen, device=DEV), given, cap, off=vocabulary * 2.0 ** -53 + 4 * 12 / part * 2.0 ** -50)
