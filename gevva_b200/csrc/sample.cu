@@ -265,11 +265,11 @@ __device__ __forceinline__ Softened softened(float x, const Cap& c, float cap32,
 constexpr double kMostCap = 128.0;
 // So is a temperature of at least this many: zero and what is next to it come from wide_of off by up to 2^-126, 2^-46 of a temperature here.
 constexpr float kLeastCappedDegrees = 1e-24f;
-// By its distance from the largest in y, whose whole part needs 32 bits only: none beyond kShareOctaves.
+// By its distance from the largest in y, at most two caps (12 thousand 32nds of an octave), whose whole part needs 32 bits only: none beyond kShareOctaves.
 __device__ __forceinline__ double capped_share(float x, double scale, float scale32, double top, float top32, const Cap& cap, float cap32, const double* table) {
   const Softened it = softened(x, cap, cap32, table);
   const float octaves = (it.y32 - top32) * scale32;
-  const double share = share_with(it.y - top, scale, share_whole(fmaxf(it.y32 - top32, -1e30f), scale32), table, kTableCopies);
+  const double share = share_with(it.y - top, scale, share_whole(it.y32 - top32, scale32), table, kTableCopies);
   return octaves > -kShareOctaves * kExp2Entries ? share : 0.0;
 }
 // cap * tanh(x / cap) for any cap, to a few steps of 64 bits: 1 - e keeps too little of a value that is small next to its cap.  There the series

@@ -242,3 +242,16 @@ def test_capped_values_of_next_to_nothing(vocabulary, size):
             for rules in ({}, dict(top_k=ints([4] * 5)), dict(top_p=f32([0.83] * 5)), dict(min_p=f32([0.05] * 5))):
                 given = dict(rules, temperature=f32([part * size] * 5))
                 compare(logits, torch.rand(5, generator=gen, device=DEV), given, cap, off=vocabulary * 2.0 ** -53 + 4 * 12 / part * 2.0 ** -50)
+
+
+@pytest.mark.parametrize("vocabulary", [7, 300, 5000])
+@pytest.mark.parametrize("cap", [4e29, 2e30, 1e31, 1e32])
+def test_large_caps(vocabulary, cap):
+    """Caps and temperatures far apart from ordinary ones, of which the cap is a few or many."""
+    gen = generator(vocabulary + 16)
+    cap = f32([cap]).item()
+    logits = torch.randn(5, vocabulary, generator=gen, device=DEV) * torch.tensor([0.3, 1.0, 5.0, 30.0, 300.0], device=DEV)[:, None] * cap
+    for parts in (1.5, 15.0, 110.0):
+        for rules in ({}, dict(top_k=ints([4] * 5)), dict(top_p=f32([0.83] * 5)), dict(top_p=f32([1 - 2.0 ** -23] * 5)), dict(min_p=f32([0.05] * 5))):
+            given = dict(rules, temperature=f32([cap / parts] * 5))
+            compare(logits, torch.rand(5, generator=gen, device=DEV), given, cap, off=vocabulary * 2.0 ** -53 + parts * 2.0 ** -50, most_near=0.4)
