@@ -59,7 +59,7 @@ struct BinWindow {
 // bits wherever both ends are; infinite values are in the first bin, and `high` is the largest number then.
 struct Bins {
   float low, high, per_two;  // bins for two
-  __device__ __forceinline__ float middle(float bin) const { return high - 2.0f * (bin / per_two); }
+  __device__ __forceinline__ float middle(float bin) const { return __fmaf_rn(bin / per_two, -2.0f, high); }  // (twice that may be more than a number says)
 };
 
 // How shares are worked out: from 32 bits' whole part where temperature and values are of ordinary size, of capped values where cap and
@@ -1586,12 +1586,13 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads) sample_kernel(const 
         if (shares) target = rules.top_p * all;
       }
       // By how much, as an exponent, shares by middles are off.  A value is half a bin from its middle at most, and 0.005 for what the bin's number loses
-      // (three roundings of 2^-24 of up to 1023); the middle is off by up to three roundings of at most `size`; capped values in 32 bits by 5e-7
-      // of the cap each, the largest and another (an exponential off by 2^-22 of up to one, of which a softened value takes at most half, a reciprocal
-      // by 2^-23 and six roundings).  The rest is within 2.5e-5 of 1e-4: 259 additions of a lane and 21 of bins (2^-24 each: 1.7e-5), exponents of
-      // up to 24 temperatures from three roundings (4.3e-6, and on a row's average, which is ln of its size, 2.3e-6), exponentials (2^-22).
+      // (three roundings of 2^-24 of up to 1023); the middle is off by up to three roundings of at most `size`, or of 2^-149 where that is subnormal;
+      // capped values in 32 bits by 5e-7 of the cap each, the largest and another (an exponential off by 2^-22 of up to one, of which a softened
+      // value takes at most half, a reciprocal by 2^-23 and six roundings).  The rest is within 2.5e-5 of 1e-4: 259 additions of a lane and 21 of bins
+      // (2^-24 each: 1.7e-5), exponents of up to 24 temperatures from three roundings (4.3e-6, and on a row's average, which is ln of its size,
+      // 2.3e-6), exponentials (2^-22).
       const double size = fmax(fabs(static_cast<double>(bins.high)), fabs(static_cast<double>(bins.low)));
-      const double off = shares ? (1.01 / static_cast<double>(bins.per_two) + 0x1p-22 * size + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
+      const double off = shares ? (1.01 / static_cast<double>(bins.per_two) + 0x1p-22 * size + 0x1p-147 + (capped ? 1e-6 * p.softcap : 0.0)) / degrees + 1e-4 : 0.0;
       const BinWindow window = window_of_bins<kThreads>(bins, shares, above, target, off, surely, turn);
       if (window.says == kNotHere || low == high) break;
       if (window.says == kInList || window.says == kListHasAll) {

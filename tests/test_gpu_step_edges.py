@@ -255,3 +255,19 @@ def test_large_caps(vocabulary, cap):
         for rules in ({}, dict(top_k=ints([4] * 5)), dict(top_p=f32([0.83] * 5)), dict(top_p=f32([1 - 2.0 ** -23] * 5)), dict(min_p=f32([0.05] * 5))):
             given = dict(rules, temperature=f32([cap / parts] * 5))
             compare(logits, torch.rand(5, generator=gen, device=DEV), given, cap, off=vocabulary * 2.0 ** -53 + parts * 2.0 ** -50, most_near=0.4)
+
+
+@pytest.mark.parametrize("vocabulary", [1810, 20001])
+@pytest.mark.parametrize("temperature", [3e36, 1e38, 3e38])
+def test_values_over_the_whole_range(vocabulary, temperature):
+    """From the lowest numbers to the largest, further apart than a number of 32 bits says, at temperatures at which all of them have a share."""
+    gen = generator(vocabulary + 17)
+    rows = 12
+    logits = (torch.randn(rows, vocabulary, generator=gen, device=DEV) * 1.4).clamp(-3.3, 3.3) * 1e38
+    logits[::3] = (logits[::3] / 4e36).round() * 4e36
+    for cap in f32([0.0, 1e38, 3e38]).tolist():
+        for _ in range(3):
+            given = dict(temperature=f32([temperature] * rows), top_p=torch.rand(rows, generator=gen, device=DEV))
+            off = vocabulary * 2.0 ** -53 + 4e38 / temperature * 2.0 ** -50
+            compare(logits, torch.rand(rows, generator=gen, device=DEV), given, cap, off=off, most_near=0.4)
+            compare(logits, torch.rand(rows, generator=gen, device=DEV), dict(given, top_k=ints([vocabulary // 2] * rows)), cap, off=off, most_near=0.4)
