@@ -19,6 +19,11 @@ int launched(cudaError_t e) {
   return e == cudaErrorInvalidValue ? GEVVA_MOE_BAD_ARGUMENT : GEVVA_MOE_CUDA_ERROR;
 }
 
+bool touch(const void* a, long long a_bytes, const void* b, long long b_bytes) {
+  const intptr_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
+  return a && b && x < y + b_bytes && y < x + a_bytes;
+}
+
 // What calls without a status word of their own report into, one of each device.  (In host code the name is only a handle.)
 static __device__ int g_attention_status;
 constexpr int kMaxDevices = 64;
@@ -45,6 +50,10 @@ namespace {
 
 constexpr int kMaxPositions = 1 << 30;
 constexpr int kMaxGroup = 128;
+
+using gv::launched;
+using gv::status_word;
+using gv::touch;
 
 bool aligned(const void* p) { return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool aligned_or_null(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -93,11 +102,6 @@ bool meets(const void* out, long long count, const gv::AttnRows& rows, int token
   return at < dim;
 }
 
-// Of the norms, whose rows and vectors are whole ranges: whether two of them share memory; none shares any with a null pointer.
-bool touch(const void* a, long long a_bytes, const void* b, long long b_bytes) {
-  const intptr_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
-  return a && b && x < y + b_bytes && y < x + a_bytes;
-}
 // A row is written when it has been read, not when others have: an output is an input, row for row, or lies apart from it, and apart from the vectors.
 bool norm_apart(const void* out, const gv::BlockNormCall& call) {
   const long long vector = 2ll * call.width, rows = call.rows * vector;
@@ -135,9 +139,6 @@ bool pages_ok(gv::AttnPages* out, const gevva_attn_cache* c, const gevva_attn_ba
   out->table_stride = b->table_stride;
   return true;
 }
-
-using gv::launched;
-using gv::status_word;
 
 // What both forms of the append have; the places of the tokens are the caller's to fill.
 template <class Args>

@@ -81,6 +81,8 @@ cudaError_t launch_block_norm(const BlockNormCall& call, int sm_count, cudaStrea
 
 // What an entry point returns for a launch's result.
 int launched(cudaError_t e);
+// Whether two ranges of memory share any of it; none shares any with a null pointer.
+bool touch(const void* a, long long a_bytes, const void* b, long long b_bytes);
 // A call's status word, or else the current device's.
 cudaError_t status_word(int* own, int** out);
 

@@ -19,10 +19,10 @@
 // pipe does: a pass over values in L2 takes 30 to 60 issue slots a value and warp for shares in 64 bits (8 for the largest value, about 10 cycles of
 // the shared-memory atomics a count in a bin), and an SM's 13 to 14 warps fill a quarter (best token) to a half (tokens as they are, top_p) of the slots
 // between waits for memory, fixed latencies and barriers.  For 22 (tokens as they are) to 57 % of the time (rows with settings of their own) an
-// SM has no CTA, since rows take different times.  In a graph over inputs larger than L2, f32 64 x 262144: the largest alone 18.9 us (3.6 TB/s), as they are 46, above a floor of 0.1 59 and of 0.01 86, by a
-// count of 50 49, of 300 89, of 1000 103, by top_p 155 to 163; bf16 with settings of their own and a cap 75 to 184 by what is drawn, 108 on most;
-// 256 x 50257 as they are 38.8, 256 x 128000 by top_p 220 to 260; one row of 262144 4.8, 14.0, by a count of 50 14, of 1000 34, by top_p 38, of which about
-// half is cluster barriers and the first CTA's work on lists and bins.  With borders found by
+// SM has no CTA, since rows take different times.  In a graph over inputs larger than L2, f32 64 x 262144: the largest alone 18.9 us (3.6 TB/s),
+// as they are 46, above a floor of 0.1 59 and of 0.01 86, by a count of 50 49, of 300 89, of 1000 103, by top_p 155 to 163; bf16 with settings of
+// their own and a cap 75 to 184 by what is drawn, 108 on most; 256 x 50257 as they are 38.8, 256 x 128000 by top_p 220 to 260; one row of 262144
+// 4.8, 14.0, by a count of 50 14, of 1000 34, by top_p 38, of which about half is cluster barriers and the first CTA's work on lists and bins.  With borders found by
 // halving instead of bins, conversions of values where they are used and half the CTAs for rows with rules (the first form) the 64 rows with
 // settings of their own took 424 us, the 256 of 50257 70 and the 256 of 128000 720.
 //
@@ -526,7 +526,7 @@ __device__ __noinline__ uint32_t first_index_of(float value) {
   return index;
 }
 
-// (the whole number stands in the low bits; of ranges without an extent it means nothing: sums tell whether the border is where counts say)
+// (of what is not in the range any: sums tell whether the border is where counts say)
 __device__ __forceinline__ int bin_of(const Bins& bins, float x) { return bin_at(half_distance(bins.high, x), bins.per_two, kBins); }
 __device__ __forceinline__ Bins bins_between(float low, float high) {
   const float finite = fminf(high, 3.402823466e38f);

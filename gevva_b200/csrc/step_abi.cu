@@ -17,10 +17,7 @@ struct Range {
   const void* at;
   long long bytes;
 };
-bool meet(const Range& a, const Range& b) {
-  const intptr_t x = reinterpret_cast<intptr_t>(a.at), y = reinterpret_cast<intptr_t>(b.at);
-  return a.at && b.at && x < y + b.bytes && y < x + a.bytes;
-}
+bool meet(const Range& a, const Range& b) { return gv::touch(a.at, a.bytes, b.at, b.bytes); }
 Range words(const int* p, long long count) { return {p, 4 * count}; }
 
 // Whether no output shares memory with another one or with what is read.
